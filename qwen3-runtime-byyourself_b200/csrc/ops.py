@@ -1347,6 +1347,139 @@ def attention_decode_flat_parts(d: int, group: int) -> int:
     return int(fn(group))
 
 
+# ------------------------------------------------------------------ a cache in 8 bits, steps with drafted tokens
+SCALE_BYTES = (-60 + 127, 60 + 127)      # the scales that a row of 8-bit codes can have: 2^-60 to 2^60
+
+
+class CachePages:
+    """A layer's pages of keys and values [pages, kv heads, PAGE_TOKENS, head size], both of one type: bfloat16, float32, or
+    float8_e4m3fn with a scale for each row (`key_scales`, `value_scales`: float8_e8m0fnu [pages, kv heads, PAGE_TOKENS], powers
+    of two).  A row in 8 bits stands for code * scale, exactly also in bfloat16."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor, key_scales: Optional[torch.Tensor] = None,
+                 value_scales: Optional[torch.Tensor] = None):
+        if keys.dim() != 4 or keys.shape[2] != PAGE_TOKENS or values.shape != keys.shape or values.dtype != keys.dtype:
+            raise KernelError(f"cache pages: keys and values are [pages, kv heads, {PAGE_TOKENS}, head size] of one type")
+        self.eight_bit = keys.dtype == torch.float8_e4m3fn
+        if not self.eight_bit and keys.dtype not in _SUFFIX:
+            raise KernelError(f"cache pages: element type {keys.dtype} is not supported (float32, bfloat16 or float8_e4m3fn)")
+        if self.eight_bit != (key_scales is not None) or self.eight_bit != (value_scales is not None):
+            raise KernelError("cache pages: pages in 8 bits have scales, others have none")
+        if self.eight_bit and (key_scales.shape != keys.shape[:3] or value_scales.shape != keys.shape[:3]):
+            raise KernelError("cache pages: the scales are [pages, kv heads, page tokens]")
+        if keys.shape[3] > 256:
+            raise KernelError(f"cache pages: head size {keys.shape[3]} (sizes up to 256)")
+        _dev(keys, "keys")
+        _dev(values, "values", keys.dtype)
+        _ptr(key_scales, "key_scales", torch.float8_e8m0fnu)
+        _ptr(value_scales, "value_scales", torch.float8_e8m0fnu)
+        self.keys, self.values, self.key_scales, self.value_scales = keys, values, key_scales, value_scales
+        self.n_pages, self.kv_heads, _, self.d = keys.shape
+
+    def pointers(self, dtype: torch.dtype, what: str):
+        """(keys, values, key scales, value scales) for a launch on rows of `dtype`."""
+        if not self.eight_bit and self.keys.dtype != dtype:
+            raise KernelError(f"{what}: pages of {self.keys.dtype} for rows of {dtype}")
+        scales = (self.key_scales.data_ptr(), self.value_scales.data_ptr()) if self.eight_bit else (None, None)
+        return (self.keys.data_ptr(), self.values.data_ptr()) + scales
+
+
+def cache_append(qkv: torch.Tensor, q_out: torch.Tensor, cache: CachePages, q_norm_w, k_norm_w, cos, sin, eps: float, token_seq,
+                 token_pos, token_place, page_table, nq: int, norm_once: bool = False) -> torch.Tensor:
+    """Per-head norm of q and k, rotation, and the write of k and v into the cache's pages, quantised where these are in 8 bits:
+    `qkv_prepare` for such a cache and for drafted tokens.  `token_pos` [tokens] is the position by which a token is rotated,
+    `token_place` its place in the sequence's cache (drafted tokens of a tree: several at one position, side by side in the cache).
+    A token whose place has no page is not written.  `norm_once`: a normed and rotated value is rounded once, when it is stored."""
+    s, n, d = _suffix(qkv), token_seq.numel(), cache.d
+    if qkv.dim() != 2 or qkv.shape[0] < n or qkv.shape[1] < (nq + 2 * cache.kv_heads) * d or nq <= 0 or page_table.dim() != 2 \
+            or token_pos.numel() < n or token_place.numel() < n or q_out.numel() < n * nq * d \
+            or any(w is not None and w.numel() != d for w in (q_norm_w, k_norm_w)) or (q_norm_w is None) != (k_norm_w is None):
+        raise KernelError("cache_append: shapes do not fit")
+    fn = _fn("cache_rows.cu", f"q3_cache_append_{s}",
+             [c_void_p] * 10 + [c_float] + [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64] + [c_int] * 5 + [c_void_p])
+    _check(fn(_dev(qkv, "qkv"), _dev(q_out, "q_out", qkv.dtype), *cache.pointers(qkv.dtype, "cache_append"),
+              _ptr(q_norm_w, "q_norm_w", torch.float32), _ptr(k_norm_w, "k_norm_w", torch.float32),
+              _ptr(cos, "cos", torch.float32), _ptr(sin, "sin", torch.float32), float(eps), _dev(token_seq, "token_seq", torch.int32),
+              _dev(token_pos, "token_pos", torch.int32), _dev(token_place, "token_place", torch.int32),
+              _dev(page_table, "page_table", torch.int32), page_table.shape[1], cache.n_pages, n, qkv.shape[1], nq, cache.kv_heads, d,
+              _rotary_dim(cos, sin, d), int(bool(norm_once)), _stream()), "cache_append")
+    return q_out
+
+
+def cache_read(cache: CachePages, page_table, seq_end, keys_out: torch.Tensor, values_out: torch.Tensor) -> None:
+    """The rows of an 8-bit cache as pages of bfloat16 or float32: page j of sequence s to keys_out[s, j] and values_out[s, j]
+    [sequences, pages, kv heads, PAGE_TOKENS, head size], for every page that holds one of the first seq_end[s] rows; rows behind
+    them in the last page are zeros, pages behind it stay as they are."""
+    if not cache.eight_bit:
+        raise KernelError("cache_read: the cache is not in 8 bits")
+    n = seq_end.numel()
+    if page_table.dim() != 2 or page_table.shape[0] < n or keys_out.dim() != 5 or keys_out.shape[0] < n or keys_out.shape[2:] != cache.keys.shape[1:] \
+            or values_out.shape != keys_out.shape or values_out.dtype != keys_out.dtype:
+        raise KernelError("cache_read: shapes do not fit")
+    fn = _fn("cache_rows.cu", f"q3_cache_read_{_suffix(keys_out)}",
+             [c_void_p] * 5 + [c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p] + [c_int] * 3 + [c_void_p])
+    _check(fn(*cache.pointers(keys_out.dtype, "cache_read"), _dev(page_table, "page_table", torch.int32), page_table.shape[1],
+              _dev(seq_end, "seq_end", torch.int32), n, cache.n_pages, _dev(keys_out, "keys_out"), _dev(values_out, "values_out"),
+              keys_out.shape[1], cache.kv_heads, cache.d, _stream()), "cache_read")
+
+
+def cache_keep(store: torch.Tensor, scales: Optional[torch.Tensor], page_table, seq_pos0, path) -> None:
+    """After a step with drafted tokens: the rows of those that stand move up behind the sequence's old end.  `path` int32
+    [sequences, n]: the numbers of these tokens among the sequence's new ones, ascending, -1 behind the last; row seq_pos0 + path[i]
+    goes to seq_pos0 + i.  `store` [..., pages, kv heads, PAGE_TOKENS, head size]: the keys and values of every layer of a
+    cache group, all moved alike; `scales` [..., pages, kv heads, PAGE_TOKENS] of a store in 8 bits."""
+    eight_bit = store.dtype == torch.float8_e4m3fn
+    if store.dim() < 4 or store.shape[-2] != PAGE_TOKENS or (not eight_bit and store.dtype not in _SUFFIX) or eight_bit != (scales is not None) \
+            or (eight_bit and scales.shape != store.shape[:-1]):
+        raise KernelError(f"cache_keep: the store is [..., pages, kv heads, {PAGE_TOKENS}, head size] of float32, bfloat16 or float8_e4m3fn, "
+                          "the latter with scales")
+    if path.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] < path.shape[0] or seq_pos0.numel() < path.shape[0]:
+        raise KernelError("cache_keep: shapes do not fit")
+    n_pages, nkv, _, d = store.shape[-4:]
+    areas = math.prod(store.shape[:-4])
+    fn = _fn("cache_rows.cu", "q3_cache_keep", [c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                                c_int, c_int, c_void_p])
+    _check(fn(_dev(store, "store"), _ptr(scales, "scales", torch.float8_e8m0fnu), areas, n_pages, nkv, d * store.element_size(),
+              _dev(page_table, "page_table", torch.int32), page_table.shape[1], _dev(seq_pos0, "seq_pos0", torch.int32),
+              _dev(path, "path", torch.int32), path.shape[1], path.shape[0], _stream()), "cache_keep")
+
+
+@dataclass
+class TreeScratch:
+    """Elements of the buffers that `attention_tree` needs: `parts` float32, `counters` int32 (zero when made, left zero)."""
+    parts: int
+    counters: int
+
+
+def attention_tree_scratch(n_seqs: int, max_new: int, nq: int, nkv: int, d: int, device) -> TreeScratch:
+    """The scratch of steps of up to `n_seqs` sequences with up to `max_new` new tokens each."""
+    return TreeScratch(1, 1)
+
+
+def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts: torch.Tensor, counters: torch.Tensor, seq_start, seq_pos0,
+                   page_table, max_new: int, nq: int, scale: float, tree: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens of every sequence - one, a run, or a tree of drafted ones - over the cache's pages, which hold
+    their keys and values already (`cache_append`).  Sequence s brings tokens seq_start[s] .. seq_start[s + 1] - 1 (at most `max_new`),
+    whose rows stand at places seq_pos0[s], seq_pos0[s] + 1, ... of its cache.  A token sees all earlier rows of its sequence
+    and, of the new ones, number n where bit n % 64 of tree[token, n // 64] is set (`tree` int64 [tokens, words]); without `tree`
+    those up to itself.  A token that sees nothing gets zeros.  q, out [tokens, nq * head size]; `parts` and `counters` as
+    `attention_tree_scratch` says."""
+    s, n, d, nkv = _suffix(q), q.shape[0], cache.d, cache.kv_heads
+    n_seqs = seq_pos0.numel()
+    if q.dim() != 2 or q.shape[1] != nq * d or out.shape != q.shape or nq <= 0 or nq % nkv or page_table.dim() != 2 \
+            or page_table.shape[0] < n_seqs or seq_start.numel() < n_seqs + 1 or max_new <= 0:
+        raise KernelError("attention_tree: shapes do not fit")
+    if tree is not None and (tree.dim() != 2 or tree.shape[0] < n or tree.shape[1] * 64 < max_new):
+        raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
+    fn = _fn("attention_tree.cu", f"q3_attention_tree_any_{s}",
+             [c_void_p] * 9 + [c_int, c_int64, c_int, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p])
+    _check(fn(_dev(q, "q"), *cache.pointers(q.dtype, "attention_tree"), _dev(out, "out", q.dtype), _dev(seq_start, "seq_start", torch.int32),
+              _dev(seq_pos0, "seq_pos0", torch.int32), _dev(page_table, "page_table", torch.int32), page_table.shape[1], cache.n_pages,
+              n_seqs, n, nq, nkv, d, float(scale), _ptr(tree, "tree", torch.int64), 0 if tree is None else tree.shape[1], _stream()),
+           "attention_tree")
+    return out
+
+
 # ------------------------------------------------------------------ bfloat16 weight-streaming product
 SKINNY_MAX_ROWS = 64
 
