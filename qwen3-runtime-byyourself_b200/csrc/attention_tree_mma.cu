@@ -1,0 +1,624 @@
+// Attention of a step's new tokens - one, a run or a tree of drafted ones a sequence - over the cache's pages in bfloat16 or in 8 bits, for
+// few rows (a row: a token and query head) a kv head: up to 32 at a time.  What a token sees and what comes out is said in attention_tree.cu.
+//
+// Few rows read many keys, so the floor is the time of the cached rows from memory: 2 (d + 1) bytes a token and kv head in 8 bits.
+//   - A block of four warps takes a range of the pages of all (sequence, kv head, tile of rows) in a row, two blocks an SM (tree_work.cuh).
+//   - A warp takes every fourth step of 32 (16) keys of the range, by itself: it copies the step's keys and values into shared memory with
+//     asynchronous copies two steps ahead, and every lane copies just what it will read, so that nothing but the row scales is
+//     shared between lanes, no barrier is met and no bank conflict arises.
+//   - Scores and weighted values are mma.m16n8k16 with the rows as the 16-row operand.  What a lane holds of keys and values are runs of 16
+//     bytes, which fixes the order in which the products walk a head's values and keys; the query is read in the same order.
+//   - 8 bits: a code is exact in half precision and becomes that in one conversion a pair; queries are divided by a power of two for
+//     each row, so that they fit, exactly, unless a value is below 2^-24 of its row's largest.  The key's scale multiplies the score.  The value's scale
+//     2^v is part of the weight: w = 2^(x + v - M), x the score in log2 units and M the running maximum of x + v, so the largest weight is of the order
+//     of 1 whatever the scales are, and what half precision drops is below 2^-24 of the largest term; the sum of the softmax is that of w 2^-v, in 32 bits.
+//   - The maximum is raised only when it is exceeded by more than 2^8.
+//   - A step with new tokens masks by bits; a value that is no number reaches only the rows that see it (a product of 0 and a NaN is a NaN:
+//     such values are taken out before the product and added to the rows that see them).
+#include "page8.cuh"
+#include "tree_work.cuh"
+
+#ifndef Q3_HEAD_DIM
+#error "compile with -DQ3_HEAD_DIM=<64 or 128>"
+#endif
+
+namespace {
+
+constexpr int D = Q3_HEAD_DIM, PAGE = Q3_PAGE_TOKENS;
+static_assert(D == 64 || D == 128, "head sizes 64 and 128");
+static_assert(PAGE == 64, "a page holds 64 tokens");
+constexpr int WARPS = 4, STAGES = 3, BLOCKS_PER_SM = 2;
+constexpr int LEAST_PAGES = 4;                      // of a block's range
+constexpr float RAISE = 8.0f;
+
+template <bool F8> struct Form {
+    static constexpr int KEYS = F8 || D == 64 ? 32 : 16;              // keys of a step
+    static constexpr int TILES = KEYS / 8, OWN = KEYS / 4;            // n-tiles of the scores; keys whose columns and values a lane holds
+    static constexpr int ROW = D * (F8 ? 1 : 2);                      // bytes of a cached row
+    static constexpr int K_RUNS = ROW / 64;                           // 16-byte runs of a key a lane holds
+    static constexpr int V_BYTES = ROW / 8;                           // bytes of a value a lane holds: in runs of V_RUN
+    static constexpr int V_RUN = V_BYTES < 16 ? V_BYTES : 16, V_RUNS = V_BYTES / V_RUN;
+    static constexpr int SPAN = V_RUN / (F8 ? 1 : 2);                 // values of a run: value columns c SPAN .. of a group of 8 SPAN
+    static constexpr int K_BYTES = TILES * K_RUNS * 512, STAGE = K_BYTES + OWN * V_RUNS * 32 * V_RUN;
+};
+
+template <bool F8, int MT> constexpr int smem_ring = WARPS* STAGES* Form<F8>::STAGE;
+constexpr int Q_PITCH = D * 2 + 8;
+template <int MT> constexpr int merge_bytes = WARPS * 16 * MT * D * 4;
+template <bool F8, int MT> constexpr int area = smem_ring<F8, MT> > merge_bytes<MT> ? smem_ring<F8, MT> : merge_bytes<MT>;
+template <bool F8, int MT> constexpr int smem_bytes =
+    area<F8, MT> + WARPS * STAGES * 64 + 16 * MT * Q_PITCH + 16 * MT * 4 + 2 * WARPS * 16 * MT * 4 + 64;
+
+struct Args {
+    TreeStep step;
+    const bf16* q;
+    bf16* out;
+    const unsigned char *keys, *values;
+    const uint8_t *key_scales, *value_scales;
+    float* parts;
+    int* counters;
+    float scale_log2;
+};
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int N> __device__ __forceinline__ void load_words(uint32_t* w, uint32_t at) {
+    if constexpr (N == 16) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    else asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+}
+
+template <bool F8> __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (F8)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool F8> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (F8) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+__device__ __forceinline__ uint32_t half2_bits(uint32_t codes) {
+    const __half2 v = q3_half2_of(codes);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The values of a word that are infinities or NaNs, each marked by all of its bits.
+template <bool F8> __device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
+    if constexpr (F8) return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+    else return ((((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+}
+
+// Where the float4 number f of a row lies in the buffer in which the warps' sums meet: lanes that write together do not meet in a bank.
+template <int SPAN> __device__ __forceinline__ int meet_at(int row, int f) {
+    if constexpr (SPAN == 16) return f ^ ((((f >> 3) & 3) << 1) | (row & 1));
+    else return f ^ (((f >> 3) & 1) | ((row & 1) << 1));
+}
+
+template <bool F8, int MT>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(const __grid_constant__ Args a) {
+    using F = Form<F8>;
+    constexpr int ROWS = 16 * MT, KEYS = F::KEYS, TILES = F::TILES, OWN = F::OWN, N_TILES = D / 8, K_STEPS = D / 16;
+    constexpr int PART = ROWS * (D + 2);
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char* const q_rows = smem + area<F8, MT> + WARPS * STAGES * 64;
+    float* const row_factor = reinterpret_cast<float*>(q_rows + ROWS * Q_PITCH);
+    float* const warp_max = row_factor + ROWS;                        // [WARPS][ROWS]
+    float* const warp_sum_of = warp_max + WARPS * ROWS;
+    long long* const shared_range = reinterpret_cast<long long*>(warp_sum_of + WARPS * ROWS);
+    pdl_launch_dependents();
+    pdl_wait();
+    const TreeStep& st = a.step;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = st.nq / st.nkv, per_tile = ROWS / group;
+
+    if (warp == 0) {
+        const TreeShare share = tree_share(st, per_tile, LEAST_PAGES);
+        int seq = 0, items = 0;
+        int64_t before = 0;
+        if (share.from < share.to) tree_find(st, per_tile, share.from, seq, before, items);
+        if (lane == 0) {
+            shared_range[0] = share.from;
+            shared_range[1] = share.to;
+            shared_range[2] = share.quota;
+            shared_range[3] = before;
+            shared_range[4] = ((long long)items << 32) | (unsigned)seq;
+        }
+    }
+    __syncthreads();
+    const int64_t from = shared_range[0], to = shared_range[1], quota = shared_range[2];
+    int64_t before = shared_range[3];
+    int seq = (int)(shared_range[4] & 0xffffffff), items_before = (int)(shared_range[4] >> 32);
+
+    const uint32_t ring = smem_at(smem) + warp * (STAGES * F::STAGE), scales = smem_at(smem) + area<F8, MT> + warp * (STAGES * 64);
+
+    for (int64_t at = from; at < to;) {
+        const TreePart part = tree_part(st, per_tile, at, to, seq, before, items_before);
+        const int t0 = st.seq_start[part.seq], n_new = tree_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
+        const int first = part.tile * per_tile, rows = min(per_tile, n_new - first) * group;
+        const int key_begin = part.begin * PAGE, key_end = min(part.end * PAGE, pos0 + n_new);
+        const int steps = (key_end - key_begin + KEYS - 1) / KEYS;
+        const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
+
+        // ---- copies of a step's rows; the page of the step after it is asked for meanwhile
+        auto page_of = [&](int s) {
+            if (s >= steps) return 0;
+            const int p = table[(key_begin + s * KEYS) / PAGE];
+            return p >= 0 && p < st.n_pages ? p : 0;                 // (a number that is no page: stay within the cache)
+        };
+        int next_page = page_of(warp);
+        auto issue = [&](int s, int stage) {
+            if (s < steps) {
+                const int64_t row0 = ((int64_t)next_page * st.nkv + part.head) * PAGE + ((key_begin + s * KEYS) & (PAGE - 1));
+                next_page = page_of(s + WARPS);
+                const unsigned char *k = a.keys + row0 * F::ROW, *v = a.values + row0 * F::ROW;
+                const uint32_t dst = ring + stage * F::STAGE;
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)
+#pragma unroll
+                    for (int h = 0; h < F::K_RUNS; ++h)
+                        copy_async<16>(dst + (j * F::K_RUNS + h) * 512 + lane * 16, k + (OWN * (g >> 1) + 2 * j + (g & 1)) * F::ROW + h * 64 + t * 16);
+#pragma unroll
+                for (int i = 0; i < OWN; ++i)
+#pragma unroll
+                    for (int h = 0; h < F::V_RUNS; ++h)
+                        copy_async<F::V_RUN>(dst + F::K_BYTES + ((i * F::V_RUNS + h) * 32 + lane) * F::V_RUN, v + (OWN * t + i) * F::ROW + h * 128 + g * F::V_RUN);
+                if constexpr (F8) {
+                    if (lane < 16) copy_async<4>(scales + stage * 64 + lane * 4, (lane < 8 ? a.key_scales : a.value_scales) + row0 + (lane & 7) * 4);
+                }
+            }
+            copy_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) issue(warp + i * WARPS, i);
+
+        // ---- the tile's queries, in half precision behind a power of two a row, or as they are
+        for (int r = warp; r < ROWS; r += WARPS) {
+            constexpr int PER = D / 32;
+            bf16 x[PER];
+            if (r < rows) {
+                const bf16* src = a.q + ((int64_t)(t0 + first + r / group) * st.nq + part.head * group + r % group) * D + lane * PER;
+#pragma unroll
+                for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(x + e) = *reinterpret_cast<const uint32_t*>(src + e);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) x[e] = __float2bfloat16_rn(0.0f);
+            }
+            uint32_t* dst = reinterpret_cast<uint32_t*>(q_rows + r * Q_PITCH + lane * PER * 2);
+            if constexpr (F8) {
+                float top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf(__bfloat162float(x[e])));
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                int e2 = (int)(__float_as_uint(top) >> 23) - 127;
+                e2 = e2 >= 128 ? 0 : min(max(e2, -100), 100);
+                const float down = q3_exp2i(-e2);
+#pragma unroll
+                for (int e = 0; e < PER; e += 2) dst[e / 2] = pack2<true>(__bfloat162float(x[e]) * down, __bfloat162float(x[e + 1]) * down);
+                if (lane == 0) row_factor[r] = a.scale_log2 * q3_exp2i(e2);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; e += 2) dst[e / 2] = *reinterpret_cast<uint32_t*>(x + e);
+                if (lane == 0) row_factor[r] = a.scale_log2;
+            }
+        }
+        __syncthreads();
+
+        const uint32_t q_at = smem_at(q_rows) + g * Q_PITCH + (F8 ? 32 : 16) * t;
+        auto load_q = [&](int mt, int ks, uint32_t* f) {
+            const uint32_t p = q_at + mt * 16 * Q_PITCH + (F8 ? (ks >> 2) * 128 + (ks & 3) * 8 : (ks >> 1) * 64 + (ks & 1) * 8);
+            uint32_t w[2];
+            load_words<8>(w, p);
+            f[0] = w[0]; f[2] = w[1];
+            load_words<8>(w, p + 8 * Q_PITCH);
+            f[1] = w[0]; f[3] = w[1];
+        };
+        uint32_t q_frag[MT == 1 ? K_STEPS : 1][4];
+        if constexpr (MT == 1) {
+#pragma unroll
+            for (int ks = 0; ks < K_STEPS; ++ks) load_q(0, ks, q_frag[ks]);
+        }
+        float factor[MT][2];
+        int own[MT][2];                                              // the token of a row, among the sequence's new ones
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = mt * 16 + r * 8 + g;
+                factor[mt][r] = row_factor[row];
+                own[mt][r] = first + min(row, rows - 1) / group;
+            }
+
+        float o[MT][N_TILES][4], m_run[MT][2], l_run[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int n = 0; n < N_TILES; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
+            m_run[mt][0] = m_run[mt][1] = -INFINITY;
+            l_run[mt][0] = l_run[mt][1] = 0.0f;
+        }
+
+        int stage = 0;
+        for (int s = warp; s < steps; s += WARPS) {
+            issue(s + (STAGES - 1) * WARPS, stage == 0 ? STAGES - 1 : stage - 1);
+            copy_wait<STAGES - 1>();
+            __syncwarp();
+            const uint32_t here = ring + stage * F::STAGE;
+            const int key0 = key_begin + s * KEYS;
+            const bool edge = key0 + KEYS > pos0;                    // some key of the step is a new token's, or behind the end
+
+            // ---- scores
+            float sc[MT][TILES][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[mt][j][e] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < F::K_RUNS; ++h) {
+                constexpr int INNER = F8 ? 4 : 2;
+                uint32_t w[TILES][4];
+#pragma unroll
+                for (int j = 0; j < TILES; ++j) load_words<16>(w[j], here + (j * F::K_RUNS + h) * 512 + lane * 16);
+#pragma unroll
+                for (int m = 0; m < INNER; ++m) {
+                    uint32_t b[TILES][2];
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j) {
+                        b[j][0] = F8 ? half2_bits(w[j][m]) : w[j][2 * (m & 1)];
+                        b[j][1] = F8 ? half2_bits(w[j][m] >> 16) : w[j][2 * (m & 1) + 1];
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        uint32_t f[4];
+                        const uint32_t* qf = f;
+                        if constexpr (MT == 1) qf = q_frag[h * INNER + m];
+                        else load_q(mt, h * INNER + m, f);
+#pragma unroll
+                        for (int j = 0; j < TILES; ++j) mma<F8>(sc[mt][j], qf, b[j][0], b[j][1]);
+                    }
+                }
+            }
+
+            // ---- in log2 units, with the scales of keys and values; what is not seen is minus infinity
+            float back[OWN];                                         // 2^-v
+            if constexpr (F8) {
+                uint32_t kw[2], vw[2];
+                load_words<8>(kw, scales + stage * 64 + t * 8);
+                load_words<8>(vw, scales + stage * 64 + 32 + t * 8);
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    const uint32_t kb = (kw[i >> 2] >> (8 * (i & 3))) & 0xffu, vb = (vw[i >> 2] >> (8 * (i & 3))) & 0xffu;
+                    const float ks = __uint_as_float(kb << 23), v = __uint_as_float(0x4b000000u | vb) - (8388608.0f + Q3_SCALE_BIAS);
+                    back[i] = __uint_as_float(0x7f000000u - (vb << 23));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float& x = sc[mt][i >> 1][2 * r + (i & 1)];
+                            x = fmaf(x * ks, factor[mt][r], v);
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[mt][j][e] *= a.scale_log2;
+            }
+            uint32_t seen[MT][2];                                    // of the step's keys, by row
+            if (edge) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own[mt][r]) * st.words : nullptr;
+                        seen[mt][r] = (uint32_t)tree_seen(mask, st.words, pos0, n_new, own[mt][r], key0);
+#pragma unroll
+                        for (int i = 0; i < OWN; ++i)
+                            if (!(seen[mt][r] >> (OWN * t + i) & 1u)) sc[mt][i >> 1][2 * r + (i & 1)] = -INFINITY;
+                    }
+                if constexpr (F8) {                                  // (the scale of a row that nobody wrote may be anything)
+#pragma unroll
+                    for (int i = 0; i < OWN; ++i)
+                        if (key0 + OWN * t + i >= pos0 + n_new) back[i] = 0.0f;
+                }
+            }
+
+            // ---- the running maximum
+            float top[MT][2];
+            bool raise = false;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x = fmaxf(sc[mt][0][2 * r], sc[mt][0][2 * r + 1]);
+#pragma unroll
+                    for (int j = 1; j < TILES; ++j) x = fmaxf(x, fmaxf(sc[mt][j][2 * r], sc[mt][j][2 * r + 1]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    top[mt][r] = x;
+                    raise |= x > m_run[mt][r] + RAISE;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        if (top[mt][r] > m_run[mt][r]) {
+                            const float alpha = ex2(m_run[mt][r] - top[mt][r]);
+                            m_run[mt][r] = top[mt][r];
+                            l_run[mt][r] *= alpha;
+#pragma unroll
+                            for (int n = 0; n < N_TILES; ++n) {
+                                o[mt][n][2 * r] *= alpha;
+                                o[mt][n][2 * r + 1] *= alpha;
+                            }
+                        }
+                    }
+            }
+
+            // ---- weights
+            uint32_t p[MT][TILES / 2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float m = m_run[mt][r] == -INFINITY ? 0.0f : m_run[mt][r];      // nothing seen so far
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j) {
+                        const float x = ex2(sc[mt][j][2 * r] - m), y = ex2(sc[mt][j][2 * r + 1] - m);
+                        if constexpr (F8) sum = fmaf(x, back[2 * j], fmaf(y, back[2 * j + 1], sum));
+                        else sum += x + y;
+                        p[mt][j >> 1][(j & 1) * 2 + r] = pack2<F8>(x, y);
+                    }
+                    l_run[mt][r] += sum;
+                }
+
+            // ---- weighted values
+            uint32_t odd = 0;                                        // some value of the step is no number
+#pragma unroll
+            for (int m = 0; m < TILES / 2; ++m)
+#pragma unroll
+                for (int h = 0; h < F::V_RUNS; ++h) {
+                    constexpr int W = F::V_RUN / 4;
+                    uint32_t w[4][W];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) load_words<F::V_RUN>(w[i], here + F::K_BYTES + (((4 * m + i) * F::V_RUNS + h) * 32 + lane) * F::V_RUN);
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool dead = key0 + OWN * t + 4 * m + i >= pos0 + n_new;
+#pragma unroll
+                            for (int k = 0; k < W; ++k) {
+                                if (dead) w[i][k] = 0u;
+                                const uint32_t bad = no_numbers<F8>(w[i][k]);
+                                odd |= bad;
+                                w[i][k] &= ~bad;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < W; ++k) {
+                        if constexpr (F8) {
+                            const uint32_t x0 = __byte_perm(w[0][k], w[1][k], 0x5140), x1 = __byte_perm(w[0][k], w[1][k], 0x7362);
+                            const uint32_t y0 = __byte_perm(w[2][k], w[3][k], 0x5140), y1 = __byte_perm(w[2][k], w[3][k], 0x7362);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t x = e < 2 ? x0 : x1, y = e < 2 ? y0 : y1;
+                                const uint32_t b0 = half2_bits(e & 1 ? x >> 16 : x), b1 = half2_bits(e & 1 ? y >> 16 : y);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<F8>(o[mt][h * F::SPAN + 4 * k + e], p[mt][m], b0, b1);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t sel = e ? 0x7632 : 0x5410;
+                                const uint32_t b0 = __byte_perm(w[0][k], w[1][k], sel), b1 = __byte_perm(w[2][k], w[3][k], sel);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) mma<F8>(o[mt][h * F::SPAN + 2 * k + e], p[mt][m], b0, b1);
+                            }
+                        }
+                    }
+                }
+            if (edge && __any_sync(0xffffffffu, odd != 0)) {
+                // the values that are no numbers, to the rows that see their keys
+#pragma unroll 1
+                for (int key = 0; key < KEYS; ++key) {
+                    if (key0 + key >= pos0 + n_new) break;
+                    const uint32_t src = here + F::K_BYTES;
+#pragma unroll
+                    for (int h = 0; h < F::V_RUNS; ++h)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            uint32_t w[F::V_RUN / 4];
+                            load_words<F::V_RUN>(w, src + (((key % OWN) * F::V_RUNS + h) * 32 + (2 * t + b) * 4 + key / OWN) * F::V_RUN);
+#pragma unroll
+                            for (int e = 0; e < F::SPAN; ++e) {
+                                float v;
+                                uint32_t bad;
+                                if constexpr (F8) {
+                                    bad = no_numbers<true>(w[e / 4]) >> (8 * (e & 3)) & 1u;
+                                    v = __uint_as_float(0x7fffffffu);
+                                } else {
+                                    bad = no_numbers<false>(w[e / 2]) >> (16 * (e & 1)) & 1u;
+                                    v = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+                                }
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                    for (int r = 0; r < 2; ++r)
+                                        if (bad && (seen[mt][r] >> key & 1u)) o[mt][h * F::SPAN + e][2 * r + b] += v;
+                            }
+                        }
+                }
+            }
+            __syncwarp();                                            // the stage is read: it may be copied over
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+        }
+        copy_wait<0>();
+        __syncthreads();                                             // every warp is done with the ring
+
+        // ---- the warps' sums meet
+        float* const meet = reinterpret_cast<float*>(smem);
+        const bool some = warp < steps;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = mt * 16 + r * 8 + g;
+                float l = l_run[mt][r];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                if (t == 0) {
+                    warp_max[warp * ROWS + row] = m_run[mt][r];
+                    warp_sum_of[warp * ROWS + row] = l;
+                }
+                if (some && row < rows) {
+#pragma unroll
+                    for (int h = 0; h < F::V_RUNS; ++h)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int q = 0; q < F::SPAN / 4; ++q) {
+                                const int f = (h * 64 + (2 * t + b) * F::SPAN) / 4 + q;
+                                float4 v;
+                                v.x = o[mt][h * F::SPAN + 4 * q][2 * r + b];
+                                v.y = o[mt][h * F::SPAN + 4 * q + 1][2 * r + b];
+                                v.z = o[mt][h * F::SPAN + 4 * q + 2][2 * r + b];
+                                v.w = o[mt][h * F::SPAN + 4 * q + 3][2 * r + b];
+                                reinterpret_cast<float4*>(meet)[(warp * ROWS + row) * (D / 4) + meet_at<F::SPAN>(row, f)] = v;
+                            }
+                }
+            }
+        __syncthreads();
+        const bool whole = part.begin == 0 && part.end == part.pages;
+        const int slot = 2 * (int)blockIdx.x + (at == from ? 0 : 1), met = min(WARPS, steps);
+        auto place = [&](int row, int f) { return a.out + ((int64_t)(t0 + first + row / group) * st.nq + part.head * group + row % group) * D + 4 * f; };
+        auto put = [&](int row, int f, float4 v, float l) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint2 w;
+            w.x = pack2<false>(v.x * inv, v.y * inv);
+            w.y = pack2<false>(v.z * inv, v.w * inv);
+            *reinterpret_cast<uint2*>(place(row, f)) = w;
+        };
+        for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+            const int row = i / (D / 4), f = i % (D / 4);
+            float m = -INFINITY, l = 0.0f;
+            for (int w = 0; w < met; ++w) m = fmaxf(m, warp_max[w * ROWS + row]);
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int w = 0; w < met; ++w) {
+                const float mw = warp_max[w * ROWS + row], alpha = mw == m ? 1.0f : ex2(mw - m);
+                const float4 u = reinterpret_cast<const float4*>(meet)[(w * ROWS + row) * (D / 4) + meet_at<F::SPAN>(row, f)];
+                l = fmaf(alpha, warp_sum_of[w * ROWS + row], l);
+                v.x = fmaf(alpha, u.x, v.x); v.y = fmaf(alpha, u.y, v.y); v.z = fmaf(alpha, u.z, v.z); v.w = fmaf(alpha, u.w, v.w);
+            }
+            if (whole) {
+                put(row, f, v, l);
+            } else {
+                float* dst = a.parts + (int64_t)slot * PART;
+                *reinterpret_cast<float4*>(dst + row * D + 4 * f) = v;
+                if (f == 0) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * row) = make_float2(m, l);
+            }
+        }
+        if (!whole) {
+            int* const last = reinterpret_cast<int*>(shared_range) + 12;
+            const int b0 = (int)(part.item_begin / quota), b1 = (int)((part.item_begin + part.pages - 1) / quota);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                *last = atomicAdd(a.counters + part.item, 1) == b1 - b0 ? 1 : 0;
+                if (*last) a.counters[part.item] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            if (*last) {
+                const int slot0 = 2 * b0 + ((int64_t)b0 * quota == part.item_begin ? 0 : 1);
+                for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+                    const int row = i / (D / 4), f = i % (D / 4);
+                    float m = -INFINITY, l = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int b = b0; b <= b1; ++b) {
+                        const float* src = a.parts + (int64_t)(b == b0 ? slot0 : 2 * b) * PART;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * D + 2 * row));
+                        const float4 u = __ldcg(reinterpret_cast<const float4*>(src + row * D + 4 * f));
+                        const float m2 = fmaxf(m, ml.x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml.x == m2 ? 1.0f : ex2(ml.x - m2);
+                        m = m2;
+                        l = fmaf(now, ml.y, l * was);
+                        v.x = fmaf(now, u.x, v.x * was); v.y = fmaf(now, u.y, v.y * was);
+                        v.z = fmaf(now, u.z, v.z * was); v.w = fmaf(now, u.w, v.w * was);
+                    }
+                    put(row, f, v, l);
+                }
+            }
+        }
+        __syncthreads();                                             // the buffers are free for the next part
+        at = part.item_begin + part.end;
+    }
+}
+
+template <bool F8, int MT> int launch(Args a, int max_new, int sm_count, cudaStream_t stream) {
+    static Q3PerDevice configured;
+    constexpr int bytes = smem_bytes<F8, MT>;
+    const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, MT>, bytes, configured);
+    if (e != cudaSuccess) return (int)e;
+    const int group = a.step.nq / a.step.nkv, per_tile = 16 * MT / group, tiles = (max_new + per_tile - 1) / per_tile;
+    const int64_t items = (int64_t)a.step.n_seqs * a.step.nkv * tiles;
+    if (items > 0x7fffffff) return Q3_ERR_TOO_LARGE;
+    const int64_t most = (items * a.step.pages_per_seq + LEAST_PAGES - 1) / LEAST_PAGES;
+    const int grid = (int)(most < BLOCKS_PER_SM * sm_count ? most : BLOCKS_PER_SM * sm_count);
+    return (int)q3_launch(tree_mma_kernel<F8, MT>, dim3(grid), dim3(WARPS * 32), (size_t)bytes, stream, a);
+}
+
+}  // namespace
+
+Q3_EXPORT int q3_attention_tree_mma_head_dim() { return D; }
+
+// Float32 values of `parts` for a launch (counters: one int32 for every sequence, kv head and tile of new tokens, at most one for each token).
+Q3_EXPORT int64_t q3_attention_tree_mma_parts(int max_new, int group) {
+    if (max_new <= 0 || group <= 0 || group > 32) return 0;
+    const int rows = max_new * group <= 16 ? 16 : 32;
+    return (int64_t)2 * BLOCKS_PER_SM * q3_device_sm_count() * rows * (D + 2);
+}
+
+Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
+                                         void* out, float* parts, int* counters, const int* seq_start, const int* seq_pos0,
+                                         const int* page_table, int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv,
+                                         float scale, const void* tree, int words, void* stream) {
+    if (n_seqs <= 0 || max_new <= 0) return 0;
+    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > 32 || n_pages <= 0 || pages_per_seq <= 0 || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
+        return Q3_ERR_BAD_SIZE;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
+        return Q3_ERR_MISALIGNED;
+    Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new}, (const bf16*)q, (bf16*)out,
+              (const unsigned char*)k_pages, (const unsigned char*)v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, parts, counters,
+              scale * 1.4426950408889634f};
+    const int sms = q3_device_sm_count();
+    const bool few = max_new * (nq / nkv) <= 16;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (k_scales != nullptr) return few ? launch<true, 1>(a, max_new, sms, s) : launch<true, 2>(a, max_new, sms, s);
+    return few ? launch<false, 1>(a, max_new, sms, s) : launch<false, 2>(a, max_new, sms, s);
+}

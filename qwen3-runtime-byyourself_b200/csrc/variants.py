@@ -11,6 +11,8 @@ def all_variants():
         ("sampling.cu", ()),
         ("cache_rows.cu", ()),
         ("attention_tree.cu", ()),
+        ("attention_tree_mma.cu", ("Q3_HEAD_DIM=128",)),
+        ("attention_tree_mma.cu", ("Q3_HEAD_DIM=64",)),
         ("attention_decode.cu", ("Q3_HEAD_DIM=128",)),
         ("attention_decode_flat.cu", ("Q3_HEAD_DIM=128",)),
         # of heads of 64 it is first asked for when a running server has many sequences: not the time to compile
