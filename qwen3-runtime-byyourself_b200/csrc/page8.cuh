@@ -25,11 +25,9 @@ __device__ __forceinline__ int q3_scale_exponent(float top) {
 }
 __device__ __forceinline__ float q3_exp2i(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }   // |k| <= 126
 
-// Two values, divided by the scale, as codes.
-__device__ __forceinline__ uint32_t q3_codes2(float a, float b, float inv_scale) {
-    const float nan = __uint_as_float(0x7fffffffu);
-    const float2 v = make_float2(q3_is_number(a) ? a * inv_scale : nan, q3_is_number(b) ? b * inv_scale : nan);
-    return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+// Two values, divided by the scale, as codes (NaN stays NaN; an infinity has to be one already).
+__device__ __forceinline__ uint32_t q3_codes2(float2 v, float inv_scale) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv_scale, v.y * inv_scale), __NV_SATFINITE, __NV_E4M3);
 }
 // Two codes (the low 16 bits) as the numbers they stand for, exact in half precision.
 __device__ __forceinline__ __half2 q3_half2_of(uint32_t codes) {

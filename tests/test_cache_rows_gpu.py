@@ -141,6 +141,30 @@ def test_rows_of_every_size_and_no_numbers(kind, d):
             assert torch.equal(x.isnan(), want.isnan()) and torch.equal(x.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
+@pytest.mark.parametrize("kind,eight_bit,d,kv,group", [("bf16", True, 128, 3, 3), ("bf16", False, 64, 1, 4), ("f32", True, 128, 2, 1), ("bf16", True, 80, 1, 5)])
+@pytest.mark.parametrize("once", [True, False])
+def test_a_prompt_is_what_its_tokens_are(kind, eight_bit, d, kv, group, once):
+    """So many rows that heads are taken several at a time give the same bits as a few."""
+    from qwen3_b200.csrc import ops
+    dtype, heads, n = TYPES[kind], kv * group, 5000
+    g = torch.Generator(device="cuda").manual_seed(d)
+    qkv = torch.randn(n, (heads + 2 * kv) * d, generator=g, device="cuda").to(dtype)
+    qw, kw = (1 + 0.3 * torch.randn(d, generator=g, device="cuda") for _ in range(2))
+    angle = torch.rand(n, d // 2, generator=g, device="cuda") * 6.3
+    table, n_pages = tc.pages_for([n], 1)
+    table, at = table.cuda(), torch.arange(n, dtype=torch.int32, device="cuda")
+    whole, few = blank(n_pages, kv, d, dtype, eight_bit), blank(n_pages, kv, d, dtype, eight_bit)
+    outs = [torch.empty(n, heads * d, dtype=dtype, device="cuda") for _ in range(2)]
+    seq = torch.zeros_like(at)
+    ops.cache_append(qkv, outs[0], whole, qw, kw, angle.cos(), angle.sin(), 1e-6, seq, at, at, table, heads, norm_once=once)
+    for i in range(0, n, 250):
+        s = slice(i, i + 250)
+        ops.cache_append(qkv[s], outs[1][s], few, qw, kw, angle.cos(), angle.sin(), 1e-6, seq[s], at[s], at[s], table, heads, norm_once=once)
+    assert torch.equal(*outs)
+    for name in ("keys", "values") + (("key_scales", "value_scales") if eight_bit else ()):
+        assert torch.equal(raw(getattr(whole, name)), raw(getattr(few, name)))
+
+
 def test_tokens_without_a_page_are_not_written():
     from qwen3_b200.csrc import ops
     for d, eight_bit in itertools.product((128, 40), (True, False)):
