@@ -127,32 +127,31 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
     pdl_wait();
     const TreeStep& st = a.step;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = st.nq / st.nkv, per_tile = ROWS / group;
+    using Work = TreeWork<PAGE, ROWS>;
+    const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const TreeShare share = tree_share(st, per_tile, LEAST_PAGES);
-        int seq = 0, items = 0;
-        int64_t before = 0;
-        if (share.from < share.to) tree_find(st, per_tile, share.from, seq, before, items);
+        const TreeShare share = Work::share(st, LEAST_PAGES, blockIdx.x, gridDim.x);
+        TreePlace place = {0, 0, 0};
+        if (share.from < share.to) place = Work::find(st, share.from);
         if (lane == 0) {
             shared_range[0] = share.from;
             shared_range[1] = share.to;
             shared_range[2] = share.quota;
-            shared_range[3] = before;
-            shared_range[4] = ((long long)items << 32) | (unsigned)seq;
+            shared_range[3] = place.before;
+            shared_range[4] = ((long long)place.items_before << 32) | (unsigned)place.seq;
         }
     }
     __syncthreads();
     const int64_t from = shared_range[0], to = shared_range[1], quota = shared_range[2];
-    int64_t before = shared_range[3];
-    int seq = (int)(shared_range[4] & 0xffffffff), items_before = (int)(shared_range[4] >> 32);
+    TreePlace walk = {shared_range[3], (int)(shared_range[4] >> 32), (int)(shared_range[4] & 0xffffffff)};
 
     const uint32_t ring = smem_at(smem) + warp * (STAGES * F::STAGE), scales = smem_at(smem) + area<F8, MT> + warp * (STAGES * 64);
 
     for (int64_t at = from; at < to;) {
-        const TreePart part = tree_part(st, per_tile, at, to, seq, before, items_before);
-        const int t0 = st.seq_start[part.seq], n_new = tree_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
-        const int first = part.tile * per_tile, rows = min(per_tile, n_new - first) * group;
+        const TreePart part = Work::part(st, at, to, walk);
+        const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
+        const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0);      // row i of the tile: token (row0 + i) / group, head (row0 + i) % group
         const int key_begin = part.begin * PAGE, key_end = min(part.end * PAGE, pos0 + n_new);
         const int steps = (key_end - key_begin + KEYS - 1) / KEYS;
         const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
@@ -166,9 +165,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
         int next_page = page_of(warp);
         auto issue = [&](int s, int stage) {
             if (s < steps) {
-                const int64_t row0 = ((int64_t)next_page * st.nkv + part.head) * PAGE + ((key_begin + s * KEYS) & (PAGE - 1));
+                const int64_t cell0 = ((int64_t)next_page * st.nkv + part.head) * PAGE + ((key_begin + s * KEYS) & (PAGE - 1));
                 next_page = page_of(s + WARPS);
-                const unsigned char *k = a.keys + row0 * F::ROW, *v = a.values + row0 * F::ROW;
+                const unsigned char *k = a.keys + cell0 * F::ROW, *v = a.values + cell0 * F::ROW;
                 const uint32_t dst = ring + stage * F::STAGE;
 #pragma unroll
                 for (int j = 0; j < TILES; ++j)
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
                     for (int h = 0; h < F::V_RUNS; ++h)
                         copy_async<F::V_RUN>(dst + F::K_BYTES + ((i * F::V_RUNS + h) * 32 + lane) * F::V_RUN, v + (OWN * t + i) * F::ROW + h * 128 + g * F::V_RUN);
                 if constexpr (F8) {
-                    if (lane < 16) copy_async<4>(scales + stage * 64 + lane * 4, (lane < 8 ? a.key_scales : a.value_scales) + row0 + (lane & 7) * 4);
+                    if (lane < 16) copy_async<4>(scales + stage * 64 + lane * 4, (lane < 8 ? a.key_scales : a.value_scales) + cell0 + (lane & 7) * 4);
                 }
             }
             copy_commit();
@@ -194,7 +193,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             constexpr int PER = D / 32;
             bf16 x[PER];
             if (r < rows) {
-                const bf16* src = a.q + ((int64_t)(t0 + first + r / group) * st.nq + part.head * group + r % group) * D + lane * PER;
+                const bf16* src = a.q + ((int64_t)(t0 + (row0 + r) / group) * st.nq + part.head * group + (row0 + r) % group) * D + lane * PER;
 #pragma unroll
                 for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(x + e) = *reinterpret_cast<const uint32_t*>(src + e);
             } else {
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             for (int r = 0; r < 2; ++r) {
                 const int row = mt * 16 + r * 8 + g;
                 factor[mt][r] = row_factor[row];
-                own[mt][r] = first + min(row, rows - 1) / group;
+                own[mt][r] = (row0 + min(row, rows - 1)) / group;
             }
 
         float o[MT][N_TILES][4], m_run[MT][2], l_run[MT][2];
@@ -515,9 +514,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
                 }
             }
         __syncthreads();
-        const bool whole = part.begin == 0 && part.end == part.pages;
+        const bool whole = part.begin == 0 && part.end == part.units;
         const int slot = 2 * (int)blockIdx.x + (at == from ? 0 : 1), met = min(WARPS, steps);
-        auto place = [&](int row, int f) { return a.out + ((int64_t)(t0 + first + row / group) * st.nq + part.head * group + row % group) * D + 4 * f; };
+        auto place = [&](int row, int f) { return a.out + ((int64_t)(t0 + (row0 + row) / group) * st.nq + part.head * group + (row0 + row) % group) * D + 4 * f; };
         auto put = [&](int row, int f, float4 v, float l) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             uint2 w;
@@ -546,7 +545,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
         }
         if (!whole) {
             int* const last = reinterpret_cast<int*>(shared_range) + 12;
-            const int b0 = (int)(part.item_begin / quota), b1 = (int)((part.item_begin + part.pages - 1) / quota);
+            const int b0 = (int)(part.item_begin / quota), b1 = (int)((part.item_begin + part.units - 1) / quota);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -585,8 +584,7 @@ template <bool F8, int MT> int launch(Args a, int max_new, int sm_count, cudaStr
     constexpr int bytes = smem_bytes<F8, MT>;
     const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, MT>, bytes, configured);
     if (e != cudaSuccess) return (int)e;
-    const int group = a.step.nq / a.step.nkv, per_tile = 16 * MT / group, tiles = (max_new + per_tile - 1) / per_tile;
-    const int64_t items = (int64_t)a.step.n_seqs * a.step.nkv * tiles;
+    const int64_t items = (int64_t)a.step.n_seqs * a.step.nkv * TreeWork<PAGE, 16 * MT>::tiles_of(max_new, a.step.nq / a.step.nkv);
     if (items > 0x7fffffff) return Q3_ERR_TOO_LARGE;
     const int64_t most = (items * a.step.pages_per_seq + LEAST_PAGES - 1) / LEAST_PAGES;
     const int grid = (int)(most < BLOCKS_PER_SM * sm_count ? most : BLOCKS_PER_SM * sm_count);
@@ -597,11 +595,10 @@ template <bool F8, int MT> int launch(Args a, int max_new, int sm_count, cudaStr
 
 Q3_EXPORT int q3_attention_tree_mma_head_dim() { return D; }
 
-// Float32 values of `parts` for a launch (counters: one int32 for every sequence, kv head and tile of new tokens, at most one for each token).
-Q3_EXPORT int64_t q3_attention_tree_mma_parts(int max_new, int group) {
-    if (max_new <= 0 || group <= 0 || group > 32) return 0;
-    const int rows = max_new * group <= 16 ? 16 : 32;
-    return (int64_t)2 * BLOCKS_PER_SM * q3_device_sm_count() * rows * (D + 2);
+// Float32 values of `parts` for a launch of up to so many rows (new tokens of a sequence x query heads a kv head); `counters`: one int32 for every
+// sequence, kv head and 16 rows.
+Q3_EXPORT int64_t q3_attention_tree_mma_parts(int rows) {
+    return (int64_t)2 * BLOCKS_PER_SM * q3_device_sm_count() * (rows <= 16 ? 16 : 32) * (D + 2);
 }
 
 Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
@@ -609,7 +606,7 @@ Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, con
                                          const int* page_table, int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv,
                                          float scale, const void* tree, int words, void* stream) {
     if (n_seqs <= 0 || max_new <= 0) return 0;
-    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > 32 || n_pages <= 0 || pages_per_seq <= 0 || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
+    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || n_pages <= 0 || pages_per_seq <= 0 || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
         return Q3_ERR_BAD_SIZE;
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
         return Q3_ERR_MISALIGNED;

@@ -1451,27 +1451,38 @@ class TreeScratch:
     counters: int
 
 
-def _tree_on_tensor_cores(dtype: torch.dtype, group: int, d: int) -> bool:
-    """Whether the tensor-core kernels take such a step: bfloat16 queries, head sizes 64 and 128, up to 32 query heads a kv head."""
-    return dtype == torch.bfloat16 and d in (64, 128) and group <= 32
-
-
+# Rows of a kv head (new tokens of a sequence x query heads a kv head) from which a step with drafted tokens goes to the tcgen05 kernel.
+tree_tc_rows = 33
 _tree_parts = {}
+
+
+def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int) -> str:
+    """Which kernel takes a step of `rows` rows a kv head at most, over a cache of so many places (pages x kv heads x PAGE_TOKENS): `tc` and `mma`
+    take bfloat16 queries and head sizes 64 and 128, `any` the others."""
+    if dtype != torch.bfloat16 or d not in (64, 128):
+        return "any"
+    return "tc" if rows >= tree_tc_rows and scale > 0 and places < 2 ** 31 else "mma"
+
+
+def _tree_parts_of(form: str, rows: int, d: int, device) -> int:
+    key = (device, form, rows <= 16, d)
+    parts = _tree_parts.get(key)
+    if parts is None:
+        if form == "tc":
+            fn = _fn_untimed("attention_tree_tc.cu", "q3_attention_tree_tc_parts", [], defines=(f"Q3_HEAD_DIM={d}",))
+        else:
+            fn = _fn_untimed("attention_tree_mma.cu", "q3_attention_tree_mma_parts", [c_int], defines=(f"Q3_HEAD_DIM={d}",))
+        fn.restype = c_int64
+        with torch.cuda.device(device):
+            parts = _tree_parts[key] = int(fn() if form == "tc" else fn(rows))
+    return parts
 
 
 def attention_tree_scratch(n_seqs: int, max_new: int, nq: int, nkv: int, d: int, device) -> TreeScratch:
     """The scratch of steps of up to `n_seqs` sequences with up to `max_new` new tokens each."""
-    group = nq // max(nkv, 1)
-    if not _tree_on_tensor_cores(torch.bfloat16, group, d):
-        return TreeScratch(0, 0)
-    key = (torch.device(device), max_new * group <= 16, d)
-    parts = _tree_parts.get(key)
-    if parts is None:
-        fn = _fn_untimed("attention_tree_mma.cu", "q3_attention_tree_mma_parts", [c_int, c_int], defines=(f"Q3_HEAD_DIM={d}",))
-        fn.restype = c_int64
-        with torch.cuda.device(key[0]):
-            parts = _tree_parts[key] = int(fn(max_new, group))
-    return TreeScratch(parts, n_seqs * nkv * max_new)
+    rows, device = max_new * (nq // max(nkv, 1)), torch.device(device)
+    forms = ([] if d not in (64, 128) else ["mma"] + (["tc"] if rows >= tree_tc_rows else []))
+    return TreeScratch(max([_tree_parts_of(form, rows, d, device) for form in forms], default=0), n_seqs * nkv * -(-rows // 16) if forms else 0)
 
 
 def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts: torch.Tensor, counters: torch.Tensor, seq_start, seq_pos0,
@@ -1490,22 +1501,31 @@ def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts:
     if tree is not None and (tree.dim() != 2 or tree.shape[0] < n or tree.shape[1] * 64 < max_new):
         raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
     words = 0 if tree is None else tree.shape[1]
-    rows = (_dev(q, "q"), *cache.pointers(q.dtype, "attention_tree"), _dev(out, "out", q.dtype))
+    tensors = (_dev(q, "q"), *cache.pointers(q.dtype, "attention_tree"), _dev(out, "out", q.dtype))
     lists = (_dev(seq_start, "seq_start", torch.int32), _dev(seq_pos0, "seq_pos0", torch.int32), _dev(page_table, "page_table", torch.int32),
              page_table.shape[1], cache.n_pages, n_seqs)
     masks = _ptr(tree, "tree", torch.int64)
-    if _tree_on_tensor_cores(q.dtype, nq // nkv, d):
-        need = attention_tree_scratch(n_seqs, max_new, nq, nkv, d, q.device)
-        if parts.numel() < need.parts or counters.numel() < need.counters:
+    rows = max_new * (nq // nkv)
+    form = _tree_form(q.dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS)
+    if form != "any":
+        if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 16):
             raise KernelError("attention_tree: parts or counters are too small (attention_tree_scratch)")
+        parts_at = _dev(parts, "parts", torch.float32)
+        if form == "tc":
+            fn = _fn("attention_tree_tc.cu", "q3_attention_tree_tc_bf16",
+                     [c_void_p] * 10 + [c_int, c_int64] + [c_int] * 4 + [c_float, c_void_p, c_int, c_void_p, c_void_p], defines=(f"Q3_HEAD_DIM={d}",))
+            _check(fn(*tensors, parts_at, *lists, max_new, nq, nkv, float(scale), masks, words, _status_word(q.device).data_ptr(), _stream()),
+                   "attention_tree")
+            _count_extra(1)
+            return out
         fn = _fn("attention_tree_mma.cu", "q3_attention_tree_mma_bf16",
                  [c_void_p] * 11 + [c_int, c_int64] + [c_int] * 4 + [c_float, c_void_p, c_int, c_void_p], defines=(f"Q3_HEAD_DIM={d}",))
-        _check(fn(*rows, _dev(parts, "parts", torch.float32), _dev(counters, "counters", torch.int32), *lists, max_new, nq, nkv, float(scale),
-                  masks, words, _stream()), "attention_tree")
+        _check(fn(*tensors, parts_at, _dev(counters, "counters", torch.int32), *lists, max_new, nq, nkv, float(scale), masks, words, _stream()),
+               "attention_tree")
         return out
     fn = _fn("attention_tree.cu", f"q3_attention_tree_any_{s}",
              [c_void_p] * 9 + [c_int, c_int64, c_int, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p])
-    _check(fn(*rows, *lists, n, nq, nkv, d, float(scale), masks, words, _stream()), "attention_tree")
+    _check(fn(*tensors, *lists, n, nq, nkv, d, float(scale), masks, words, _stream()), "attention_tree")
     return out
 
 

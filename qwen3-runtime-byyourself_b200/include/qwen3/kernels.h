@@ -527,14 +527,22 @@ int q3_attention_tree_any_bf16(const void* q, const void* k_pages, const void* v
                                const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq, int64_t n_pages,
                                int n_seqs, int64_t n_tokens, int nq, int nkv, int d, float scale, const void* tree, int words, void* stream);
 
-/* ---- attention_tree_mma.cu (-DQ3_HEAD_DIM=64 or 128): the same for bfloat16 queries with up to 32 query heads a kv head ---- */
+/* ---- attention_tree_mma.cu (-DQ3_HEAD_DIM=64 or 128): the same for bfloat16 queries, 32 rows (new tokens x query heads of a kv head) at a time ---- */
 int q3_attention_tree_mma_head_dim(void);
-/* float32 values of `parts`; `counters`: an int32, zero when made and left zero, for each sequence, kv head and new token */
-int64_t q3_attention_tree_mma_parts(int max_new, int group);
+/* float32 values of `parts` for so many rows a sequence; `counters`: an int32, zero when made and left zero, for each sequence, kv head and 16 rows */
+int64_t q3_attention_tree_mma_parts(int rows);
 int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
                                float* parts, int* counters, const int* seq_start, const int* seq_pos0, const int* page_table,
                                int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv, float scale, const void* tree,
                                int words, void* stream);
+
+/* ---- attention_tree_tc.cu (-DQ3_HEAD_DIM=64 or 128): the same on tcgen05, 256 rows at a time; scale > 0; two launches ---- */
+int q3_attention_tree_tc_head_dim(void);
+int64_t q3_attention_tree_tc_parts(void);
+int q3_attention_tree_tc_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
+                              float* parts, const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq,
+                              int64_t n_pages, int n_seqs, int max_new, int nq, int nkv, float scale, const void* tree, int words,
+                              int* status, void* stream);
 
 /* ---- sampling.cu ------------------------------------------------------------------------------------------ */
 /* out[r] = index of the highest logit among the first `valid` (lowest id among equals, NaN as -inf) */
