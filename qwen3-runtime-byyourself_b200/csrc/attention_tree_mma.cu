@@ -1,17 +1,19 @@
 // Attention of a step's new tokens - one, a run or a tree of drafted ones a sequence - over the cache's pages in bfloat16 or in 8 bits, for
-// few rows (a row: a token and query head) a kv head: up to 32 at a time.  What a token sees and what comes out is said in attention_tree.cu.
+// few rows (a row: a token and query head) a kv head: 8, 16 or 32 at a time.  What a token sees and what comes out is said in attention_tree.cu.
 //
 // Few rows read many keys, so the floor is the time of the cached rows from memory: 2 (d + 1) bytes a token and kv head in 8 bits.
-//   - A block of four warps takes a range of the pages of all (sequence, kv head, tile of rows) in a row, two blocks an SM (tree_work.cuh).
-//   - A warp takes every fourth step of 32 (16) keys of the range, by itself: it copies the step's keys and values into shared memory with
-//     asynchronous copies two steps ahead, and every lane copies just what it will read, so that nothing but the row scales is
+//   - A block of four warps takes an equal share of the pages of all (sequence, kv head, tile of rows) (tree_work.cuh), three blocks an SM.
+//   - A warp takes every fourth step of 32 (16) keys of its block's, by itself: it copies the step's keys and values into shared memory with
+//     asynchronous copies a step or two ahead, and every lane copies just what it will read, so that nothing but the row scales is
 //     shared between lanes, no barrier is met and no bank conflict arises.
-//   - Scores and weighted values are mma.m16n8k16 with the rows as the 16-row operand.  What a lane holds of keys and values are runs of 16
-//     bytes, which fixes the order in which the products walk a head's values and keys; the query is read in the same order.
-//   - 8 bits: a code is exact in half precision and becomes that in one conversion a pair; queries are divided by a power of two for
-//     each row, so that they fit, exactly, unless a value is below 2^-24 of its row's largest.  The key's scale multiplies the score.  The value's scale
-//     2^v is part of the weight: w = 2^(x + v - M), x the score in log2 units and M the running maximum of x + v, so the largest weight is of the order
-//     of 1 whatever the scales are, and what half precision drops is below 2^-24 of the largest term; the sum of the softmax is that of w 2^-v, in 32 bits.
+//   - Products are mma.m16n8k16 with keys, then values, as the 16-row operand and the rows as its eight columns: S^T = K Q^T and O^T = V^T P^T, so 8 rows
+//     cost 8, not 16.  What a lane holds of keys and values are runs of 16 bytes, which fixes the order in which the products walk a
+//     head's values and the keys; the query is read in the same order.  The weights change from rows to columns by movmatrix.
+//   - 8 bits: a code is exact in half precision and becomes that in one conversion a pair (products of codes themselves are put together from the same
+//     conversions on this architecture).  Queries are divided by a power of two for each row, so that they fit, exactly, unless a value is below 2^-24 of its
+//     row's largest.  The key's scale multiplies the score.  The value's scale 2^v is part of the weight: w = 2^(x + v - M), x the score in log2 units
+//     and M the running maximum of x + v, so the largest weight is of the order of 1 whatever the scales are, and what half precision drops is
+//     below 2^-24 of the largest term; the sum of the softmax is that of w 2^-v, in 32 bits.
 //   - The maximum is raised only when it is exceeded by more than 2^8.
 //   - A step with new tokens masks by bits; a value that is no number reaches only the rows that see it (a product of 0 and a NaN is a NaN:
 //     such values are taken out before the product and added to the rows that see them).
@@ -27,27 +29,30 @@ namespace {
 constexpr int D = Q3_HEAD_DIM, PAGE = Q3_PAGE_TOKENS;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 static_assert(PAGE == 64, "a page holds 64 tokens");
-constexpr int WARPS = 4, STAGES = 3, BLOCKS_PER_SM = 2;
+constexpr int WARPS = 4;
+// Blocks an SM and stages of a warp's ring, by tiles of eight rows (registers, shared memory).
+template <int NT> constexpr int blocks_per_sm = NT == 4 ? 2 : 3;
+template <int NT> constexpr int stages = NT == 4 ? 3 : 2;
 constexpr int LEAST_PAGES = 4;                      // of a block's range
 constexpr float RAISE = 8.0f;
 
 template <bool F8> struct Form {
     static constexpr int KEYS = F8 || D == 64 ? 32 : 16;              // keys of a step
-    static constexpr int TILES = KEYS / 8, OWN = KEYS / 4;            // n-tiles of the scores; keys whose columns and values a lane holds
+    static constexpr int TILES = KEYS / 16, MINE = KEYS / 8, OWN = KEYS / 4;   // tiles of 16 keys; keys and values of a step that a lane holds
     static constexpr int ROW = D * (F8 ? 1 : 2);                      // bytes of a cached row
     static constexpr int K_RUNS = ROW / 64;                           // 16-byte runs of a key a lane holds
     static constexpr int V_BYTES = ROW / 8;                           // bytes of a value a lane holds: in runs of V_RUN
     static constexpr int V_RUN = V_BYTES < 16 ? V_BYTES : 16, V_RUNS = V_BYTES / V_RUN;
-    static constexpr int SPAN = V_RUN / (F8 ? 1 : 2);                 // values of a run: value columns c SPAN .. of a group of 8 SPAN
-    static constexpr int K_BYTES = TILES * K_RUNS * 512, STAGE = K_BYTES + OWN * V_RUNS * 32 * V_RUN;
+    static constexpr int SPAN = V_RUN / (F8 ? 1 : 2);                 // values of a run: lanes g hold values g SPAN .. of a group of 8 SPAN
+    static constexpr int K_BYTES = MINE * K_RUNS * 512, STAGE = K_BYTES + OWN * V_RUNS * 32 * V_RUN;
 };
 
-template <bool F8, int MT> constexpr int smem_ring = WARPS* STAGES* Form<F8>::STAGE;
 constexpr int Q_PITCH = D * 2 + 8;
-template <int MT> constexpr int merge_bytes = WARPS * 16 * MT * D * 4;
-template <bool F8, int MT> constexpr int area = smem_ring<F8, MT> > merge_bytes<MT> ? smem_ring<F8, MT> : merge_bytes<MT>;
-template <bool F8, int MT> constexpr int smem_bytes =
-    area<F8, MT> + WARPS * STAGES * 64 + 16 * MT * Q_PITCH + 16 * MT * 4 + 2 * WARPS * 16 * MT * 4 + 64;
+template <bool F8, int NT> constexpr int smem_ring = WARPS * stages<NT> * Form<F8>::STAGE;
+template <int NT> constexpr int merge_bytes = WARPS * 8 * NT * D * 4;
+template <bool F8, int NT> constexpr int area = smem_ring<F8, NT> > merge_bytes<NT> ? smem_ring<F8, NT> : merge_bytes<NT>;
+template <bool F8, int NT> constexpr int smem_bytes =
+    area<F8, NT> + WARPS * stages<NT> * 64 + 8 * NT * Q_PITCH + 8 * NT * 4 + 2 * WARPS * 8 * NT * 4 + 64;
 
 struct Args {
     TreeStep step;
@@ -81,6 +86,12 @@ template <bool F8> __device__ __forceinline__ void mma(float* c, const uint32_t*
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// An 8 x 8 tile of 16-bit values, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 template <bool F8> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if constexpr (F8) {
         const __half2 v = __floats2half2_rn(lo, hi);
@@ -108,21 +119,22 @@ template <bool F8> __device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
 
 // Where the float4 number f of a row lies in the buffer in which the warps' sums meet: lanes that write together do not meet in a bank.
 template <int SPAN> __device__ __forceinline__ int meet_at(int row, int f) {
-    if constexpr (SPAN == 16) return f ^ ((((f >> 3) & 3) << 1) | (row & 1));
-    else return f ^ (((f >> 3) & 1) | ((row & 1) << 1));
+    if constexpr (SPAN == 16) return f ^ (row >> 1 & 3);
+    else return f ^ ((row >> 1 & 1) | (row >> 2 & 1) << 2);
 }
 
-template <bool F8, int MT>
-__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(const __grid_constant__ Args a) {
+template <bool F8, int NT>
+__global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel(const __grid_constant__ Args a) {
     using F = Form<F8>;
-    constexpr int ROWS = 16 * MT, KEYS = F::KEYS, TILES = F::TILES, OWN = F::OWN, N_TILES = D / 8, K_STEPS = D / 16;
-    constexpr int PART = ROWS * (D + 2);
+    constexpr int ROWS = 8 * NT, KEYS = F::KEYS, TILES = F::TILES, OWN = F::OWN, MINE = F::MINE, M_TILES = D / 16, K_STEPS = D / 16;
+    constexpr int PART = ROWS * (D + 2), STAGES = stages<NT>;
     extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char* const q_rows = smem + area<F8, MT> + WARPS * STAGES * 64;
+    unsigned char* const q_rows = smem + area<F8, NT> + WARPS * STAGES * 64;
     float* const row_factor = reinterpret_cast<float*>(q_rows + ROWS * Q_PITCH);
     float* const warp_max = row_factor + ROWS;                        // [WARPS][ROWS]
     float* const warp_sum_of = warp_max + WARPS * ROWS;
-    long long* const shared_range = reinterpret_cast<long long*>(warp_sum_of + WARPS * ROWS);
+    TreeShare* const shared_share = reinterpret_cast<TreeShare*>(warp_sum_of + WARPS * ROWS);
+    int* const shared_last = reinterpret_cast<int*>(shared_share + 1);
     pdl_launch_dependents();
     pdl_wait();
     const TreeStep& st = a.step;
@@ -131,25 +143,16 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const TreeShare share = Work::share(st, LEAST_PAGES, blockIdx.x, gridDim.x);
-        TreePlace place = {0, 0, 0};
-        if (share.from < share.to) place = Work::find(st, share.from);
-        if (lane == 0) {
-            shared_range[0] = share.from;
-            shared_range[1] = share.to;
-            shared_range[2] = share.quota;
-            shared_range[3] = place.before;
-            shared_range[4] = ((long long)place.items_before << 32) | (unsigned)place.seq;
-        }
+        const TreeShare found = Work::share(st, LEAST_PAGES, blockIdx.x, gridDim.x);
+        if (lane == 0) *shared_share = found;
     }
     __syncthreads();
-    const int64_t from = shared_range[0], to = shared_range[1], quota = shared_range[2];
-    TreePlace walk = {shared_range[3], (int)(shared_range[4] >> 32), (int)(shared_range[4] & 0xffffffff)};
+    TreeShare share = *shared_share;
 
-    const uint32_t ring = smem_at(smem) + warp * (STAGES * F::STAGE), scales = smem_at(smem) + area<F8, MT> + warp * (STAGES * 64);
+    const uint32_t ring = smem_at(smem) + warp * (STAGES * F::STAGE), scales = smem_at(smem) + area<F8, NT> + warp * (STAGES * 64);
 
-    for (int64_t at = from; at < to;) {
-        const TreePart part = Work::part(st, at, to, walk);
+    for (int at = share.from; at < share.to;) {
+        const TreePart part = Work::part(st, share, at, blockIdx.x);
         const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
         const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0);      // row i of the tile: token (row0 + i) / group, head (row0 + i) % group
         const int key_begin = part.begin * PAGE, key_end = min(part.end * PAGE, pos0 + n_new);
@@ -170,10 +173,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
                 const unsigned char *k = a.keys + cell0 * F::ROW, *v = a.values + cell0 * F::ROW;
                 const uint32_t dst = ring + stage * F::STAGE;
 #pragma unroll
-                for (int j = 0; j < TILES; ++j)
+                for (int j = 0; j < MINE; ++j)
 #pragma unroll
                     for (int h = 0; h < F::K_RUNS; ++h)
-                        copy_async<16>(dst + (j * F::K_RUNS + h) * 512 + lane * 16, k + (OWN * (g >> 1) + 2 * j + (g & 1)) * F::ROW + h * 64 + t * 16);
+                        copy_async<16>(dst + (j * F::K_RUNS + h) * 512 + lane * 16, k + (MINE * g + j) * F::ROW + h * 64 + t * 16);
 #pragma unroll
                 for (int i = 0; i < OWN; ++i)
 #pragma unroll
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 int e2 = (int)(__float_as_uint(top) >> 23) - 127;
-                e2 = e2 >= 128 ? 0 : min(max(e2, -100), 100);
+                e2 = e2 >= 128 ? 0 : min(max(e2, -60), 60);
                 const float down = q3_exp2i(-e2);
 #pragma unroll
                 for (int e = 0; e < PER; e += 2) dst[e / 2] = pack2<true>(__bfloat162float(x[e]) * down, __bfloat162float(x[e + 1]) * down);
@@ -216,45 +219,43 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             } else {
 #pragma unroll
                 for (int e = 0; e < PER; e += 2) dst[e / 2] = *reinterpret_cast<uint32_t*>(x + e);
-                if (lane == 0) row_factor[r] = a.scale_log2;
             }
         }
         __syncthreads();
 
+        // the columns' operand of product ks: 16 of a head's values, in the order in which a lane holds keys
         const uint32_t q_at = smem_at(q_rows) + g * Q_PITCH + (F8 ? 32 : 16) * t;
-        auto load_q = [&](int mt, int ks, uint32_t* f) {
-            const uint32_t p = q_at + mt * 16 * Q_PITCH + (F8 ? (ks >> 2) * 128 + (ks & 3) * 8 : (ks >> 1) * 64 + (ks & 1) * 8);
-            uint32_t w[2];
-            load_words<8>(w, p);
-            f[0] = w[0]; f[2] = w[1];
-            load_words<8>(w, p + 8 * Q_PITCH);
-            f[1] = w[0]; f[3] = w[1];
+        auto load_q = [&](int n, int ks, uint32_t* f) {
+            load_words<8>(f, q_at + n * 8 * Q_PITCH + (F8 ? (ks >> 2) * 128 + (ks & 3) * 8 : (ks >> 1) * 64 + (ks & 1) * 8));
         };
-        uint32_t q_frag[MT == 1 ? K_STEPS : 1][4];
-        if constexpr (MT == 1) {
+        constexpr bool KEEP_Q = NT <= 2;
+        uint32_t q_frag[KEEP_Q ? NT : 1][KEEP_Q ? K_STEPS : 1][2];
+        if constexpr (KEEP_Q) {
 #pragma unroll
-            for (int ks = 0; ks < K_STEPS; ++ks) load_q(0, ks, q_frag[ks]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int ks = 0; ks < K_STEPS; ++ks) load_q(n, ks, q_frag[n][ks]);
         }
-        float factor[MT][2];
-        int own[MT][2];                                              // the token of a row, among the sequence's new ones
+        float factor[NT][2];
+        int own[NT][2];                                              // the token of a column's row, among the sequence's new ones
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = mt * 16 + r * 8 + g;
-                factor[mt][r] = row_factor[row];
-                own[mt][r] = (row0 + min(row, rows - 1)) / group;
+            for (int b = 0; b < 2; ++b) {
+                const int row = n * 8 + 2 * t + b;
+                factor[n][b] = F8 ? row_factor[row] : a.scale_log2;
+                own[n][b] = (row0 + min(row, rows - 1)) / group;
             }
 
-        float o[MT][N_TILES][4], m_run[MT][2], l_run[MT][2];
+        float o[NT][M_TILES][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int n = 0; n < N_TILES; ++n)
+            for (int i = 0; i < M_TILES; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
-            m_run[mt][0] = m_run[mt][1] = -INFINITY;
-            l_run[mt][0] = l_run[mt][1] = 0.0f;
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.0f;
+            m_run[n][0] = m_run[n][1] = -INFINITY;
+            l_run[n][0] = l_run[n][1] = 0.0f;
         }
 
         int stage = 0;
@@ -266,151 +267,153 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             const int key0 = key_begin + s * KEYS;
             const bool edge = key0 + KEYS > pos0;                    // some key of the step is a new token's, or behind the end
 
-            // ---- scores
-            float sc[MT][TILES][4];
+            // ---- scores: this lane's are those of keys MINE g .. + MINE - 1 and columns 2 t, 2 t + 1 of every tile
+            float sc[NT][TILES][4];                                  // [key 2 j][column 0, 1], [key 2 j + 1][column 0, 1]
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < TILES; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[mt][j][e] = 0.0f;
+                    for (int e = 0; e < 4; ++e) sc[n][j][e] = 0.0f;
 #pragma unroll
             for (int h = 0; h < F::K_RUNS; ++h) {
-                constexpr int INNER = F8 ? 4 : 2;
-                uint32_t w[TILES][4];
+                constexpr int INNER = F8 ? 4 : 2;                    // products of a run
+                uint32_t w[MINE][4];
 #pragma unroll
-                for (int j = 0; j < TILES; ++j) load_words<16>(w[j], here + (j * F::K_RUNS + h) * 512 + lane * 16);
+                for (int j = 0; j < MINE; ++j) load_words<16>(w[j], here + (j * F::K_RUNS + h) * 512 + lane * 16);
 #pragma unroll
                 for (int m = 0; m < INNER; ++m) {
-                    uint32_t b[TILES][2];
+                    uint32_t k[TILES][4];
 #pragma unroll
-                    for (int j = 0; j < TILES; ++j) {
-                        b[j][0] = F8 ? half2_bits(w[j][m]) : w[j][2 * (m & 1)];
-                        b[j][1] = F8 ? half2_bits(w[j][m] >> 16) : w[j][2 * (m & 1) + 1];
-                    }
+                    for (int j = 0; j < TILES; ++j)
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t f[4];
-                        const uint32_t* qf = f;
-                        if constexpr (MT == 1) qf = q_frag[h * INNER + m];
-                        else load_q(mt, h * INNER + m, f);
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t* run = w[2 * j + e];
+                            k[j][e] = F8 ? half2_bits(run[m]) : run[2 * (m & 1)];
+                            k[j][2 + e] = F8 ? half2_bits(run[m] >> 16) : run[2 * (m & 1) + 1];
+                        }
 #pragma unroll
-                        for (int j = 0; j < TILES; ++j) mma<F8>(sc[mt][j], qf, b[j][0], b[j][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        uint32_t f[2];
+                        const uint32_t* q = f;
+                        if constexpr (KEEP_Q) q = q_frag[n][h * INNER + m];
+                        else load_q(n, h * INNER + m, f);
+#pragma unroll
+                        for (int j = 0; j < TILES; ++j) mma<F8>(sc[n][j], k[j], q[0], q[1]);
                     }
                 }
             }
 
             // ---- in log2 units, with the scales of keys and values; what is not seen is minus infinity
-            float back[OWN];                                         // 2^-v
+            float back[MINE];                                        // 2^-v
             if constexpr (F8) {
-                uint32_t kw[2], vw[2];
-                load_words<8>(kw, scales + stage * 64 + t * 8);
-                load_words<8>(vw, scales + stage * 64 + 32 + t * 8);
+                uint32_t kw, vw;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(kw) : "r"(scales + stage * 64 + g * MINE) : "memory");
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(vw) : "r"(scales + stage * 64 + 32 + g * MINE) : "memory");
 #pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    const uint32_t kb = (kw[i >> 2] >> (8 * (i & 3))) & 0xffu, vb = (vw[i >> 2] >> (8 * (i & 3))) & 0xffu;
+                for (int i = 0; i < MINE; ++i) {
+                    const uint32_t kb = (kw >> (8 * i)) & 0xffu, vb = (vw >> (8 * i)) & 0xffu;
                     const float ks = __uint_as_float(kb << 23), v = __uint_as_float(0x4b000000u | vb) - (8388608.0f + Q3_SCALE_BIAS);
                     back[i] = __uint_as_float(0x7f000000u - (vb << 23));
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float& x = sc[mt][i >> 1][2 * r + (i & 1)];
-                            x = fmaf(x * ks, factor[mt][r], v);
+                        for (int b = 0; b < 2; ++b) {
+                            float& x = sc[n][i >> 1][2 * (i & 1) + b];
+                            x = fmaf(x * ks, factor[n][b], v);
                         }
                 }
             } else {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int j = 0; j < TILES; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[mt][j][e] *= a.scale_log2;
+                        for (int e = 0; e < 4; ++e) sc[n][j][e] *= a.scale_log2;
             }
-            uint32_t seen[MT][2];                                    // of the step's keys, by row
+            uint32_t seen[NT][2];                                    // of the step's keys, by row
             if (edge) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own[mt][r]) * st.words : nullptr;
-                        seen[mt][r] = (uint32_t)tree_seen(mask, st.words, pos0, n_new, own[mt][r], key0);
+                    for (int b = 0; b < 2; ++b) {
+                        const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own[n][b]) * st.words : nullptr;
+                        seen[n][b] = (uint32_t)tree_seen(mask, st.words, pos0, n_new, own[n][b], key0);
 #pragma unroll
-                        for (int i = 0; i < OWN; ++i)
-                            if (!(seen[mt][r] >> (OWN * t + i) & 1u)) sc[mt][i >> 1][2 * r + (i & 1)] = -INFINITY;
+                        for (int i = 0; i < MINE; ++i)
+                            if (!(seen[n][b] >> (MINE * g + i) & 1u)) sc[n][i >> 1][2 * (i & 1) + b] = -INFINITY;
                     }
                 if constexpr (F8) {                                  // (the scale of a row that nobody wrote may be anything)
 #pragma unroll
-                    for (int i = 0; i < OWN; ++i)
-                        if (key0 + OWN * t + i >= pos0 + n_new) back[i] = 0.0f;
+                    for (int i = 0; i < MINE; ++i)
+                        if (key0 + MINE * g + i >= pos0 + n_new) back[i] = 0.0f;
                 }
             }
 
             // ---- the running maximum
-            float top[MT][2];
+            float top[NT][2];
             bool raise = false;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float x = fmaxf(sc[mt][0][2 * r], sc[mt][0][2 * r + 1]);
+                for (int b = 0; b < 2; ++b) {
+                    float x = fmaxf(sc[n][0][b], sc[n][0][2 + b]);
 #pragma unroll
-                    for (int j = 1; j < TILES; ++j) x = fmaxf(x, fmaxf(sc[mt][j][2 * r], sc[mt][j][2 * r + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    top[mt][r] = x;
-                    raise |= x > m_run[mt][r] + RAISE;
+                    for (int j = 1; j < TILES; ++j) x = fmaxf(x, fmaxf(sc[n][j][b], sc[n][j][2 + b]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    top[n][b] = x;
+                    raise |= x > m_run[n][b] + RAISE;
                 }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        if (top[mt][r] > m_run[mt][r]) {
-                            const float alpha = ex2(m_run[mt][r] - top[mt][r]);
-                            m_run[mt][r] = top[mt][r];
-                            l_run[mt][r] *= alpha;
+                    for (int b = 0; b < 2; ++b) {
+                        if (top[n][b] > m_run[n][b]) {
+                            const float alpha = ex2(m_run[n][b] - top[n][b]);
+                            m_run[n][b] = top[n][b];
+                            l_run[n][b] *= alpha;
 #pragma unroll
-                            for (int n = 0; n < N_TILES; ++n) {
-                                o[mt][n][2 * r] *= alpha;
-                                o[mt][n][2 * r + 1] *= alpha;
+                            for (int i = 0; i < M_TILES; ++i) {
+                                o[n][i][b] *= alpha;
+                                o[n][i][2 + b] *= alpha;
                             }
                         }
                     }
             }
 
-            // ---- weights
-            uint32_t p[MT][TILES / 2][4];
+            // ---- weights, as the columns' operand
+            uint32_t p[NT][TILES][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = m_run[n][0] == -INFINITY ? 0.0f : m_run[n][0], m1 = m_run[n][1] == -INFINITY ? 0.0f : m_run[n][1];      // nothing seen so far
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float m = m_run[mt][r] == -INFINITY ? 0.0f : m_run[mt][r];      // nothing seen so far
-                    float sum = 0.0f;
+                for (int j = 0; j < TILES; ++j)
 #pragma unroll
-                    for (int j = 0; j < TILES; ++j) {
-                        const float x = ex2(sc[mt][j][2 * r] - m), y = ex2(sc[mt][j][2 * r + 1] - m);
-                        if constexpr (F8) sum = fmaf(x, back[2 * j], fmaf(y, back[2 * j + 1], sum));
-                        else sum += x + y;
-                        p[mt][j >> 1][(j & 1) * 2 + r] = pack2<F8>(x, y);
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = ex2(sc[n][j][2 * e] - m0), y = ex2(sc[n][j][2 * e + 1] - m1);
+                        l_run[n][0] = F8 ? fmaf(x, back[2 * j + e], l_run[n][0]) : l_run[n][0] + x;
+                        l_run[n][1] = F8 ? fmaf(y, back[2 * j + e], l_run[n][1]) : l_run[n][1] + y;
+                        p[n][j][e] = transposed(pack2<F8>(x, y));
                     }
-                    l_run[mt][r] += sum;
-                }
+            }
 
-            // ---- weighted values
+            // ---- weighted values: tile j's products walk keys OWN t + {2 j, OWN / 2 + 2 j, 2 j + 1, OWN / 2 + 2 j + 1} of every lane
             uint32_t odd = 0;                                        // some value of the step is no number
 #pragma unroll
-            for (int m = 0; m < TILES / 2; ++m)
+            for (int j = 0; j < TILES; ++j)
 #pragma unroll
                 for (int h = 0; h < F::V_RUNS; ++h) {
                     constexpr int W = F::V_RUN / 4;
                     uint32_t w[4][W];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) load_words<F::V_RUN>(w[i], here + F::K_BYTES + (((4 * m + i) * F::V_RUNS + h) * 32 + lane) * F::V_RUN);
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool dead = key0 + OWN * t + 4 * m + i >= pos0 + n_new;
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = (i & 1) * (OWN / 2) + 2 * j + (i >> 1);
+                        load_words<F::V_RUN>(w[i], here + F::K_BYTES + ((key * F::V_RUNS + h) * 32 + lane) * F::V_RUN);
+                        if (edge) {
+                            const bool dead = key0 + OWN * t + key >= pos0 + n_new;
 #pragma unroll
                             for (int k = 0; k < W; ++k) {
                                 if (dead) w[i][k] = 0u;
@@ -423,23 +426,18 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
 #pragma unroll
                     for (int k = 0; k < W; ++k) {
                         if constexpr (F8) {
-                            const uint32_t x0 = __byte_perm(w[0][k], w[1][k], 0x5140), x1 = __byte_perm(w[0][k], w[1][k], 0x7362);
-                            const uint32_t y0 = __byte_perm(w[2][k], w[3][k], 0x5140), y1 = __byte_perm(w[2][k], w[3][k], 0x7362);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t x = e < 2 ? x0 : x1, y = e < 2 ? y0 : y1;
-                                const uint32_t b0 = half2_bits(e & 1 ? x >> 16 : x), b1 = half2_bits(e & 1 ? y >> 16 : y);
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) mma<F8>(o[mt][h * F::SPAN + 4 * k + e], p[mt][m], b0, b1);
-                            }
-                        } else {
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const uint32_t sel = e ? 0x7632 : 0x5410;
-                                const uint32_t b0 = __byte_perm(w[0][k], w[1][k], sel), b1 = __byte_perm(w[2][k], w[3][k], sel);
+                                const uint32_t x = __byte_perm(w[0][k], w[1][k], e ? 0x7362 : 0x5140), y = __byte_perm(w[2][k], w[3][k], e ? 0x7362 : 0x5140);
+                                const uint32_t v[4] = {half2_bits(x), half2_bits(x >> 16), half2_bits(y), half2_bits(y >> 16)};
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) mma<F8>(o[mt][h * F::SPAN + 2 * k + e], p[mt][m], b0, b1);
+                                for (int n = 0; n < NT; ++n) mma<true>(o[n][(h * F::SPAN + 4 * k) / 2 + e], v, p[n][j][0], p[n][j][1]);
                             }
+                        } else {
+                            const uint32_t v[4] = {__byte_perm(w[0][k], w[1][k], 0x5410), __byte_perm(w[0][k], w[1][k], 0x7632),
+                                                   __byte_perm(w[2][k], w[3][k], 0x5410), __byte_perm(w[2][k], w[3][k], 0x7632)};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma<false>(o[n][(h * F::SPAN + 2 * k) / 2], v, p[n][j][0], p[n][j][1]);
                         }
                     }
                 }
@@ -450,29 +448,27 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
                     if (key0 + key >= pos0 + n_new) break;
                     const uint32_t src = here + F::K_BYTES;
 #pragma unroll
-                    for (int h = 0; h < F::V_RUNS; ++h)
+                    for (int h = 0; h < F::V_RUNS; ++h) {
+                        uint32_t w[F::V_RUN / 4];
+                        load_words<F::V_RUN>(w, src + (((key % OWN) * F::V_RUNS + h) * 32 + g * 4 + key / OWN) * F::V_RUN);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            uint32_t w[F::V_RUN / 4];
-                            load_words<F::V_RUN>(w, src + (((key % OWN) * F::V_RUNS + h) * 32 + (2 * t + b) * 4 + key / OWN) * F::V_RUN);
-#pragma unroll
-                            for (int e = 0; e < F::SPAN; ++e) {
-                                float v;
-                                uint32_t bad;
-                                if constexpr (F8) {
-                                    bad = no_numbers<true>(w[e / 4]) >> (8 * (e & 3)) & 1u;
-                                    v = __uint_as_float(0x7fffffffu);
-                                } else {
-                                    bad = no_numbers<false>(w[e / 2]) >> (16 * (e & 1)) & 1u;
-                                    v = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-                                }
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                                    for (int r = 0; r < 2; ++r)
-                                        if (bad && (seen[mt][r] >> key & 1u)) o[mt][h * F::SPAN + e][2 * r + b] += v;
+                        for (int e = 0; e < F::SPAN; ++e) {
+                            float v;
+                            uint32_t bad;
+                            if constexpr (F8) {
+                                bad = no_numbers<true>(w[e / 4]) >> (8 * (e & 3)) & 1u;
+                                v = __uint_as_float(0x7fffffffu);
+                            } else {
+                                bad = no_numbers<false>(w[e / 2]) >> (16 * (e & 1)) & 1u;
+                                v = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
                             }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int b = 0; b < 2; ++b)
+                                    if (bad && (seen[n][b] >> key & 1u)) o[n][(h * F::SPAN + e) / 2][2 * (e & 1) + b] += v;
                         }
+                    }
                 }
             }
             __syncwarp();                                            // the stage is read: it may be copied over
@@ -485,37 +481,32 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
         float* const meet = reinterpret_cast<float*>(smem);
         const bool some = warp < steps;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = mt * 16 + r * 8 + g;
-                float l = l_run[mt][r];
-                l += __shfl_xor_sync(0xffffffffu, l, 1);
-                l += __shfl_xor_sync(0xffffffffu, l, 2);
-                if (t == 0) {
-                    warp_max[warp * ROWS + row] = m_run[mt][r];
+            for (int b = 0; b < 2; ++b) {
+                const int row = n * 8 + 2 * t + b;
+                float l = l_run[n][b];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                if (g == 0) {
+                    warp_max[warp * ROWS + row] = m_run[n][b];
                     warp_sum_of[warp * ROWS + row] = l;
                 }
                 if (some && row < rows) {
 #pragma unroll
                     for (int h = 0; h < F::V_RUNS; ++h)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
-#pragma unroll
-                            for (int q = 0; q < F::SPAN / 4; ++q) {
-                                const int f = (h * 64 + (2 * t + b) * F::SPAN) / 4 + q;
-                                float4 v;
-                                v.x = o[mt][h * F::SPAN + 4 * q][2 * r + b];
-                                v.y = o[mt][h * F::SPAN + 4 * q + 1][2 * r + b];
-                                v.z = o[mt][h * F::SPAN + 4 * q + 2][2 * r + b];
-                                v.w = o[mt][h * F::SPAN + 4 * q + 3][2 * r + b];
-                                reinterpret_cast<float4*>(meet)[(warp * ROWS + row) * (D / 4) + meet_at<F::SPAN>(row, f)] = v;
-                            }
+                        for (int q = 0; q < F::SPAN / 4; ++q) {
+                            const int f = (h * 64 + g * F::SPAN) / 4 + q, i = (h * F::SPAN + 4 * q) / 2;
+                            reinterpret_cast<float4*>(meet)[(warp * ROWS + row) * (D / 4) + meet_at<F::SPAN>(row, f)] =
+                                make_float4(o[n][i][b], o[n][i][2 + b], o[n][i + 1][b], o[n][i + 1][2 + b]);
+                        }
                 }
             }
         __syncthreads();
-        const bool whole = part.begin == 0 && part.end == part.units;
-        const int slot = 2 * (int)blockIdx.x + (at == from ? 0 : 1), met = min(WARPS, steps);
+        const bool whole = part.parts == 1;
+        const int met = min(WARPS, steps);
         auto place = [&](int row, int f) { return a.out + ((int64_t)(t0 + (row0 + row) / group) * st.nq + part.head * group + (row0 + row) % group) * D + 4 * f; };
         auto put = [&](int row, int f, float4 v, float l) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -538,30 +529,27 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             if (whole) {
                 put(row, f, v, l);
             } else {
-                float* dst = a.parts + (int64_t)slot * PART;
+                float* dst = a.parts + (int64_t)part.slot * PART;
                 *reinterpret_cast<float4*>(dst + row * D + 4 * f) = v;
                 if (f == 0) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * row) = make_float2(m, l);
             }
         }
         if (!whole) {
-            int* const last = reinterpret_cast<int*>(shared_range) + 12;
-            const int b0 = (int)(part.item_begin / quota), b1 = (int)((part.item_begin + part.units - 1) / quota);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
-                *last = atomicAdd(a.counters + part.item, 1) == b1 - b0 ? 1 : 0;
-                if (*last) a.counters[part.item] = 0;
+                *shared_last = atomicAdd(a.counters + part.item, 1) == part.parts - 1 ? 1 : 0;
+                if (*shared_last) a.counters[part.item] = 0;
                 __threadfence();
             }
             __syncthreads();
-            if (*last) {
-                const int slot0 = 2 * b0 + ((int64_t)b0 * quota == part.item_begin ? 0 : 1);
+            if (*shared_last) {
                 for (int i = threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
                     const int row = i / (D / 4), f = i % (D / 4);
                     float m = -INFINITY, l = 0.0f;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int b = b0; b <= b1; ++b) {
-                        const float* src = a.parts + (int64_t)(b == b0 ? slot0 : 2 * b) * PART;
+                    for (int b = 0; b < part.parts; ++b) {
+                        const float* src = a.parts + (int64_t)part.slot_of(b) * PART;
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * D + 2 * row));
                         const float4 u = __ldcg(reinterpret_cast<const float4*>(src + row * D + 4 * f));
                         const float m2 = fmaxf(m, ml.x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml.x == m2 ? 1.0f : ex2(ml.x - m2);
@@ -575,20 +563,25 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM) tree_mma_kernel(con
             }
         }
         __syncthreads();                                             // the buffers are free for the next part
-        at = part.item_begin + part.end;
+        at = Work::next(share, at, part);
     }
 }
 
-template <bool F8, int MT> int launch(Args a, int max_new, int sm_count, cudaStream_t stream) {
+template <bool F8, int NT> int launch(const Args& a, int sm_count, cudaStream_t stream) {
     static Q3PerDevice configured;
-    constexpr int bytes = smem_bytes<F8, MT>;
-    const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, MT>, bytes, configured);
+    constexpr int bytes = smem_bytes<F8, NT>;
+    static_assert(blocks_per_sm<NT> * (bytes + 1024) <= 228 * 1024, "shared memory of an SM");
+    const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, NT>, bytes, configured);
     if (e != cudaSuccess) return (int)e;
-    const int64_t items = (int64_t)a.step.n_seqs * a.step.nkv * TreeWork<PAGE, 16 * MT>::tiles_of(max_new, a.step.nq / a.step.nkv);
-    if (items > 0x7fffffff) return Q3_ERR_TOO_LARGE;
-    const int64_t most = (items * a.step.pages_per_seq + LEAST_PAGES - 1) / LEAST_PAGES;
-    const int grid = (int)(most < BLOCKS_PER_SM * sm_count ? most : BLOCKS_PER_SM * sm_count);
-    return (int)q3_launch(tree_mma_kernel<F8, MT>, dim3(grid), dim3(WARPS * 32), (size_t)bytes, stream, a);
+    using Work = TreeWork<PAGE, 8 * NT>;
+    const int64_t units = Work::most_units(a.step), most = (units + LEAST_PAGES - 1) / LEAST_PAGES + Work::most_items(a.step);
+    if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
+    const int resident = blocks_per_sm<NT> * sm_count, grid = (int)(most < resident ? most : resident);
+    return (int)q3_launch(tree_mma_kernel<F8, NT>, dim3(grid), dim3(WARPS * 32), (size_t)bytes, stream, a);
+}
+template <bool F8> int launch_rows(const Args& a, int64_t rows, cudaStream_t stream) {
+    const int sms = q3_device_sm_count();
+    return rows <= 8 ? launch<F8, 1>(a, sms, stream) : rows <= 16 ? launch<F8, 2>(a, sms, stream) : launch<F8, 4>(a, sms, stream);
 }
 
 }  // namespace
@@ -596,9 +589,10 @@ template <bool F8, int MT> int launch(Args a, int max_new, int sm_count, cudaStr
 Q3_EXPORT int q3_attention_tree_mma_head_dim() { return D; }
 
 // Float32 values of `parts` for a launch of up to so many rows (new tokens of a sequence x query heads a kv head); `counters`: one int32 for every
-// sequence, kv head and 16 rows.
+// sequence, kv head and 8 rows.
 Q3_EXPORT int64_t q3_attention_tree_mma_parts(int rows) {
-    return (int64_t)2 * BLOCKS_PER_SM * q3_device_sm_count() * (rows <= 16 ? 16 : 32) * (D + 2);
+    const int each = rows <= 8 ? blocks_per_sm<1> * 8 : rows <= 16 ? blocks_per_sm<2> * 16 : blocks_per_sm<4> * 32;
+    return (int64_t)2 * q3_device_sm_count() * each * (D + 2);
 }
 
 Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
@@ -610,12 +604,9 @@ Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, con
         return Q3_ERR_BAD_SIZE;
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
         return Q3_ERR_MISALIGNED;
-    Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new}, (const bf16*)q, (bf16*)out,
+    const Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new}, (const bf16*)q, (bf16*)out,
               (const unsigned char*)k_pages, (const unsigned char*)v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, parts, counters,
               scale * 1.4426950408889634f};
-    const int sms = q3_device_sm_count();
-    const bool few = max_new * (nq / nkv) <= 16;
-    cudaStream_t s = (cudaStream_t)stream;
-    if (k_scales != nullptr) return few ? launch<true, 1>(a, max_new, sms, s) : launch<true, 2>(a, max_new, sms, s);
-    return few ? launch<false, 1>(a, max_new, sms, s) : launch<false, 2>(a, max_new, sms, s);
+    const int64_t rows = (int64_t)max_new * (nq / nkv);
+    return k_scales != nullptr ? launch_rows<true>(a, rows, (cudaStream_t)stream) : launch_rows<false>(a, rows, (cudaStream_t)stream);
 }

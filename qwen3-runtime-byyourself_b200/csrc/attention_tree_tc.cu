@@ -57,7 +57,7 @@ struct Note {                                             // what is noted of a 
 struct Shared {
     Note keys[NOTES], values[NOTES];
     float key_rest[NOTES][STRETCH], value_rest[NOTES][STRETCH];
-    long long range[5];
+    TreeShare share;
     unsigned long long bars[1 + 5 * STAGES + 6 + NOTES];
     uint32_t tmem;
 };
@@ -221,22 +221,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare share = Work::share(st, 1, blockIdx.x, gridDim.x);
-        TreePlace place = {0, 0, 0};
-        if (share.from < share.to) place = Work::find(st, share.from);
-        if (lane == 0) {
-            sh.range[0] = share.from;
-            sh.range[1] = share.to;
-            sh.range[3] = place.before;
-            sh.range[4] = ((long long)place.items_before << 32) | (unsigned)place.seq;
-        }
+        const TreeShare found = Work::share(st, 1, blockIdx.x, gridDim.x);
+        if (lane == 0) sh.share = found;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const int64_t from = sh.range[0], to = sh.range[1];
-    TreePlace walk = {sh.range[3], (int)(sh.range[4] >> 32), (int)(sh.range[4] & 0xffffffff)};
+    TreeShare share = sh.share;
     const int group = st.nq / st.nkv;
     auto failed = [&](int where) { if (lane == 0) atomicExch(a.status, where); };
 
@@ -248,8 +240,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         int stretch = 0;                                                             // of this block, over all parts
         uint32_t turn = 0, q_turn = 0;                                               // of this tile's barriers, of the parts
         bool ok = true;
-        for (int64_t at = from; at < to && ok;) {
-            const TreePart part = Work::part(st, at, to, walk);
+        for (int at = share.from; at < share.to && ok;) {
+            const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
             const int row0 = part.tile * ROWS, rows = n_new * group - row0 - x * BM;      // of this tile
             const int steps = part.end - part.begin;
@@ -294,7 +286,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (!ok) { failed(39); break; }
                 q_turn ^= 1u;
                 stretch += steps;
-                at = part.item_begin + part.end;
+                at = Work::next(share, at, part);
                 continue;
             }
 
@@ -445,9 +437,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             if (!ok) { failed(43); break; }
             tc_fence_after();
             // ---- the row, or its part of it
-            const bool whole = part.begin == 0 && part.end == part.units;
+            const bool whole = part.parts == 1;
             const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-            float* const dst = a.parts + ((int64_t)2 * blockIdx.x + (at == from ? 0 : 1)) * PART;
+            float* const dst = a.parts + (int64_t)part.slot * PART;
             const int pr = x * BM + r;                                               // the row among the part's
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -482,7 +474,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             if (!whole && r < rows) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * pr) = make_float2(m_run, l_run);
             tc_fence_before();
-            at = part.item_begin + part.end;
+            at = Work::next(share, at, part);
         }
     } else if (warp < MMA_WARP) {
         // ------------------------------------------------ the keys (warps 8-11) and the values (12-15)
@@ -492,8 +484,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const uint32_t tiles = is_v ? v_smem : k_smem, bar_full = is_v ? bar_v_full : bar_k_full, bar_empty = is_v ? bar_v_empty : bar_k_empty;
         int stretch = 0;
         bool ok = true;
-        for (int64_t at = from; at < to && ok;) {
-            const TreePart part = Work::part(st, at, to, walk);
+        for (int at = share.from; at < share.to && ok;) {
+            const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq], steps = part.end - part.begin;
             const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
             const int key_end = pos0 + n_new;
@@ -625,7 +617,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (lane == 0) mbar_arrive(bar_v_full + 8 * stage);
                 }
             }
-            at = part.item_begin + part.end;
+            at = Work::next(share, at, part);
         }
     } else {
         // ------------------------------------------------ the products: the whole warp walks and one elected thread issues
@@ -651,8 +643,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             __syncwarp();
         };
-        for (int64_t at = from; at < to && ok;) {
-            const TreePart part = Work::part(st, at, to, walk);
+        for (int at = share.from; at < share.to && ok;) {
+            const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int rows = Work::n_new(st, part.seq) * group - part.tile * ROWS, steps = part.end - part.begin, both = rows > BM ? 2 : 1;
             auto keys_here = [&](int number) { return mbar_wait_warp(bar_k_full + 8 * (number % STAGES), (uint32_t)(number / STAGES) & 1u); };
             ok = mbar_wait_warp(bar_q, q_turn) && keys_here(stretch);
@@ -691,7 +683,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (!ok) failed(49);
                 }
             }
-            at = part.item_begin + part.end;
+            at = Work::next(share, at, part);
         }
         }
     }
@@ -703,37 +695,27 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
 }
 
-// ---- the parts of the items that several blocks share, added up in their order: a block for the item that begins in one block's range and goes on behind it,
-// and 32 of its rows
+// ---- the parts of the items that several blocks share, added up in their order: for every block of the first kernel whose last part is the first one of such
+// an item, and for 32 of its rows, a block
 __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constant__ Args a, int blocks) {
-    __shared__ long long range[5];
+    __shared__ TreeShare shared_share;
     pdl_launch_dependents();
     pdl_wait();
     const TreeStep& st = a.step;
     const int b0 = blockIdx.x;
     if (threadIdx.x < 32) {
-        const TreeShare share = Work::share(st, 1, b0, blocks);
-        TreePlace place = {0, 0, 0};
-        if (share.from < share.to) place = Work::find(st, share.to - 1);
-        if (threadIdx.x == 0) {
-            range[0] = share.from;
-            range[1] = share.to;
-            range[2] = share.quota;
-            range[3] = place.before;
-            range[4] = place.seq;
-        }
+        const TreeShare found = Work::share(st, 1, b0, blocks);
+        if (threadIdx.x == 0) shared_share = found;
     }
     __syncthreads();
-    const int64_t from = range[0], to = range[1], quota = range[2];
-    if (from >= to) return;
-    TreePlace walk = {range[3], 0, (int)range[4]};
-    const TreePart part = Work::part(st, to - 1, to, walk);
-    const int64_t item_end = part.item_begin + part.units;
-    if (part.item_begin < from || item_end <= to) return;                            // begins before this range, or ends in it
+    TreeShare share = shared_share;
+    if (share.from >= share.to) return;
+    TreePart part;
+    for (int at = share.from; at < share.to; at = Work::next(share, at, part)) part = Work::part(st, share, at, b0);
+    if (part.parts == 1 || part.begin != 0) return;
     const int group = st.nq / st.nkv, t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq);
     const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0), first = blockIdx.y * 32;
     if (first >= rows) return;
-    const int last = (int)((item_end - 1) / quota), slot0 = 2 * b0 + (part.item_begin == from ? 0 : 1);
     const int r = first + (threadIdx.x & 31);
     if (r >= rows) return;
     bf16* const out = a.out + ((int64_t)(t0 + (row0 + r) / group) * st.nq + part.head * group + (row0 + r) % group) * D;
@@ -741,8 +723,8 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
         float m = -INFINITY, l = 0.0f, v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-        for (int b = b0; b <= last; ++b) {
-            const float* src = a.parts + (int64_t)(b == b0 ? slot0 : 2 * b) * PART;
+        for (int b = 0; b < part.parts; ++b) {
+            const float* src = a.parts + (int64_t)part.slot_of(b) * PART;
             const float2 ml = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * r);
             const float4 u0 = *reinterpret_cast<const float4*>(src + ((2 * c) * ROWS + r) * 4), u1 = *reinterpret_cast<const float4*>(src + ((2 * c + 1) * ROWS + r) * 4);
             const float m2 = fmaxf(m, ml.x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml.x == m2 ? 1.0f : ex2(ml.x - m2);
@@ -772,10 +754,9 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
     if (!F8 && (!q3_make_map_bf16(&map_k, a.keys, a.step.n_pages * a.step.nkv * PAGE, D, PAGE, 64, true) ||
                 !q3_make_map_bf16(&map_v, a.values, a.step.n_pages * a.step.nkv * PAGE, D, PAGE, 64, true)))
         return Q3_ERR_BAD_SIZE;
-    const int64_t items = (int64_t)a.step.n_seqs * a.step.nkv * Work::tiles_of(max_new, a.step.nq / a.step.nkv);
-    if (items > 0x7fffffff) return Q3_ERR_TOO_LARGE;
-    const int64_t most = items * ((a.step.pages_per_seq + 1) / 2);
-    const int sms = q3_device_sm_count(), blocks = (int)(most < sms ? most : sms);
+    const int64_t units = Work::most_units(a.step);
+    if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
+    const int sms = q3_device_sm_count(), blocks = (int)(units < sms ? units : sms);
     int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)SMEM_BYTES, stream, map_k, map_v, a);
     if (code != 0) return code;
     const int rows = (int64_t)max_new * (a.step.nq / a.step.nkv) < ROWS ? max_new * (a.step.nq / a.step.nkv) : ROWS;

@@ -1465,7 +1465,7 @@ def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int)
 
 
 def _tree_parts_of(form: str, rows: int, d: int, device) -> int:
-    key = (device, form, rows <= 16, d)
+    key = (device, form, -(-min(rows, 17) // 8), d)
     parts = _tree_parts.get(key)
     if parts is None:
         if form == "tc":
@@ -1482,7 +1482,7 @@ def attention_tree_scratch(n_seqs: int, max_new: int, nq: int, nkv: int, d: int,
     """The scratch of steps of up to `n_seqs` sequences with up to `max_new` new tokens each."""
     rows, device = max_new * (nq // max(nkv, 1)), torch.device(device)
     forms = ([] if d not in (64, 128) else ["mma"] + (["tc"] if rows >= tree_tc_rows else []))
-    return TreeScratch(max([_tree_parts_of(form, rows, d, device) for form in forms], default=0), n_seqs * nkv * -(-rows // 16) if forms else 0)
+    return TreeScratch(max([_tree_parts_of(form, rows, d, device) for form in forms], default=0), n_seqs * nkv * -(-rows // 8) if forms else 0)
 
 
 def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts: torch.Tensor, counters: torch.Tensor, seq_start, seq_pos0,
@@ -1508,7 +1508,7 @@ def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts:
     rows = max_new * (nq // nkv)
     form = _tree_form(q.dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS)
     if form != "any":
-        if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 16):
+        if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 8):
             raise KernelError("attention_tree: parts or counters are too small (attention_tree_scratch)")
         parts_at = _dev(parts, "parts", torch.float32)
         if form == "tc":

@@ -1,10 +1,14 @@
 // How the attention of a step over the paged cache is shared out over the blocks of a launch, and which of a sequence's new keys a token sees.
 //
 // The work is a list of items - (sequence, kv head, tile of rows; a row is a new token and a query head of the kv head's group) - of as
-// many stretches of UNIT keys as the sequence has.  The stretches of all items in a row are cut into ranges of equal length, one a
-// block, wherever they fall: contexts of unequal length take as long as equal ones of the same total, and a block has at most a part of an item, some whole
-// ones, and another part.  Which part of an item is whose, and so the order of a row's sums, hangs on the lengths of all sequences of the step and on
-// nothing else.
+// many stretches of UNIT keys as the sequence has.  It is shared out in one of two ways, whatever the sequences' lengths:
+//   pieces  every item is cut into equal pieces of at most `quota` stretches, and a block takes one piece.  `quota` is the best of four numbers between
+//           the even share and one at which the pieces are certainly no more than the blocks;
+//   ranges  the stretches of all items in a row are cut into ranges of equal length, one a block, wherever they fall: a block has at most a
+//           part of an item, some whole ones and another part.  Taken where pieces would leave blocks without work: many items a block, or so few blocks an
+//           item that equal pieces are half as long again.
+// Parts of an item are added up in their order.  Which part is whose, and so the order of a row's sums, hangs on the lengths of all sequences of the step
+// and on nothing else.
 #pragma once
 
 #include "common.cuh"
@@ -20,109 +24,142 @@ struct TreeStep {
 // A range of stretches [begin, end) of one item.
 struct TreePart {
     int seq, head, tile;                           // head: the kv head
-    int begin, end, units;                         // units: the item's in all
-    int64_t item_begin;                            // the item's first stretch in the list of all
-    int item;                                      // its number among the items
+    int begin, end, item;                          // item: its number among the items
+    int parts, slot, slot0, first_block;           // of the item: how many; this one's place in the scratch, the first one's, and the first one's block
+
+    // The place of the item's part i in the scratch (a block has two: of the part that it begins with, and of the one that it ends with).
+    __device__ __forceinline__ int slot_of(int i) const { return i == 0 ? slot0 : 2 * (first_block + i); }
 };
 
-// A block's range of the list, and the length of a range.
+// What a block has: in the way of ranges stretches [from, to) of the list (none: from >= to), else one piece.
 struct TreeShare {
-    int64_t from, to, quota;
-};
-
-// Where a walk through the list is: a sequence, and the stretches and items before it.
-struct TreePlace {
-    int64_t before;
-    int items_before, seq;
+    int from, to, quota;                           // quota: a range's length, or (`pieces`) the most stretches of a piece
+    int pieces;                                    // 1: pieces
+    int seq, before, items_before;                 // where `from` (a piece: the block's number) lies: its sequence, the stretches (pieces) and items before it
 };
 
 // UNIT: keys of a stretch; ROWS: rows of a tile.
 template <int UNIT, int ROWS> struct TreeWork {
-    static __device__ __forceinline__ int n_new(const TreeStep& a, int seq) { return min(a.seq_start[seq + 1] - a.seq_start[seq], a.max_new); }
-    static __device__ __forceinline__ int units(const TreeStep& a, int seq) {
-        const int n = n_new(a, seq);
-        return n <= 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT;
+    static __device__ __forceinline__ int n_new(const TreeStep& a, int seq) { return max(0, min(a.seq_start[seq + 1] - a.seq_start[seq], a.max_new)); }
+    static __device__ __forceinline__ int units(const TreeStep& a, int seq, int n) {
+        return n == 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT;
     }
-    static __host__ __device__ __forceinline__ int tiles_of(int n_new, int group) { return n_new <= 0 ? 0 : (int)(((int64_t)n_new * group + ROWS - 1) / ROWS); }
-    static __device__ __forceinline__ int tiles(const TreeStep& a, int seq) { return tiles_of(n_new(a, seq), a.nq / a.nkv); }
+    static __host__ __device__ __forceinline__ int tiles_of(int n_new, int group) { return (int)(((int64_t)n_new * group + ROWS - 1) / ROWS); }
 
-    // The range of block `block` of `blocks`, of at least `least` stretches.  Called by one whole warp.
-    static __device__ __forceinline__ TreeShare share(const TreeStep& a, int least, int block, int blocks) {
-        const int lane = threadIdx.x & 31;
-        long long total = 0;
-        for (int s = lane; s < a.n_seqs; s += 32) total += (long long)units(a, s) * tiles(a, s) * a.nkv;
+    // The most items and stretches that a step can have (the latter have to stay below 2^31).
+    static __host__ int64_t most_items(const TreeStep& a) { return (int64_t)a.n_seqs * a.nkv * tiles_of(a.max_new, a.nq / a.nkv); }
+    static __host__ int64_t most_units(const TreeStep& a) { return most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT); }
+
+    static __device__ __forceinline__ int warp_total(int v) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const long long even = (total + blocks - 1) / (long long)blocks;
-        TreeShare t;
-        t.quota = even > least ? even : least;
-        const long long from = (long long)block * t.quota;
-        t.from = from < total ? from : total;
-        t.to = t.from + t.quota < total ? t.from + t.quota : total;
-        return t;
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
     }
 
-    // The sequence in whose items stretch `at` lies.  Called by one whole warp.
-    static __device__ __forceinline__ TreePlace find(const TreeStep& a, int64_t at) {
-        const int lane = threadIdx.x & 31;
-        long long run = 0;
-        int items = 0;
-        TreePlace p;
+    // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more).
+    static __device__ TreeShare share(const TreeStep& a, int least, int block, int blocks) {
+        const int lane = threadIdx.x & 31, group = a.nq / a.nkv;
+        // of up to 32 sequences everything is read once
+        const bool few = a.n_seqs <= 32;
+        const int mine_new = few && lane < a.n_seqs ? n_new(a, lane) : 0, mine_units = few && lane < a.n_seqs ? units(a, lane, mine_new) : 0;
+        const int mine_items = mine_units > 0 ? tiles_of(mine_new, group) * a.nkv : 0;
+        auto each = [&](auto f) {                                        // sum over the sequences of f(units, items)
+            int sum = 0;
+            if (few) sum = f(mine_units, mine_items);
+            else
+                for (int s = lane; s < a.n_seqs; s += 32) {
+                    const int n = n_new(a, s), u = units(a, s, n);
+                    if (u > 0) sum += f(u, tiles_of(n, group) * a.nkv);
+                }
+            return warp_total(sum);
+        };
+        TreeShare t;
+        const int total = each([](int u, int n) { return u * n; }), items = each([](int, int n) { return n; });
+        const int even = max(least, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks));
+        t.pieces = 0;
+        t.quota = even;
+        if (items < blocks) {
+            // with pieces of `safe` stretches there are at most items + total / safe of them
+            const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + max(even / 2, 2);
+            for (int i = 0; i < 4 && !t.pieces; ++i) {
+                const int c = even + (min(safe, cap) - even) * i / 3;
+                if (each([c](int u, int n) { return u > 0 ? n * ((int)((unsigned)(u + c - 1) / (unsigned)c)) : 0; }) <= blocks) {
+                    t.pieces = 1;
+                    t.quota = c;
+                }
+            }
+        }
+        // where the block's range or piece begins
+        const int at = t.pieces ? block : (int)min((int64_t)total, (int64_t)block * t.quota);
+        t.from = at;
+        t.to = t.pieces ? at + 1 : min((int64_t)total, (int64_t)at + t.quota);
+        int run = 0, passed = 0;
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const int s = s0 + lane;
-            const int n = s < a.n_seqs ? tiles(a, s) * a.nkv : 0;
-            const long long mine = s < a.n_seqs ? (long long)units(a, s) * n : 0;
-            long long sum = mine;
-            int count = n;
+            const int n = few ? mine_new : s < a.n_seqs ? n_new(a, s) : 0, u = few ? mine_units : s < a.n_seqs ? units(a, s, n) : 0;
+            const int count = u > 0 ? tiles_of(n, group) * a.nkv : 0;
+            const int mine = u > 0 ? count * (t.pieces ? (int)((unsigned)(u + t.quota - 1) / (unsigned)t.quota) : u) : 0;
+            int sum = mine, counts = count;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-                const int c = __shfl_up_sync(0xffffffffu, count, o);
+                const int v = __shfl_up_sync(0xffffffffu, sum, o), c = __shfl_up_sync(0xffffffffu, counts, o);
                 if (lane >= o) {
                     sum += v;
-                    count += c;
+                    counts += c;
                 }
             }
             const unsigned hit = __ballot_sync(0xffffffffu, run + sum > at);
             if (hit != 0) {
                 const int first = __ffs(hit) - 1;
-                p.seq = s0 + first;
-                p.before = run + __shfl_sync(0xffffffffu, sum - mine, first);
-                p.items_before = items + __shfl_sync(0xffffffffu, count - n, first);
-                return p;
+                t.seq = s0 + first;
+                t.before = run + __shfl_sync(0xffffffffu, sum - mine, first);
+                t.items_before = passed + __shfl_sync(0xffffffffu, counts - count, first);
+                return t;
             }
             run += __shfl_sync(0xffffffffu, sum, 31);
-            items += __shfl_sync(0xffffffffu, count, 31);
+            passed += __shfl_sync(0xffffffffu, counts, 31);
         }
-        p.seq = a.n_seqs;
-        p.before = run;
-        p.items_before = items;
-        return p;
+        t.from = t.to = 0;                                               // nothing for this block
+        t.seq = t.before = t.items_before = 0;
+        return t;
     }
 
-    // The part of the range up to `to` that begins at stretch `at`, which lies in the list behind `place`; that moves on where it has to.
-    static __device__ __forceinline__ TreePart part(const TreeStep& a, int64_t at, int64_t to, TreePlace& place) {
+    // The part at `at` (t.from, then what `next` says) of a block's share; `t` is moved on to the sequence that holds it.
+    static __device__ __forceinline__ TreePart part(const TreeStep& a, TreeShare& t, int at, int block) {
         TreePart p;
         while (true) {
-            const int each = units(a, place.seq), per_head = tiles(a, place.seq), n = per_head * a.nkv;
-            const int64_t in = at - place.before;
-            if (in < (int64_t)each * n) {
-                const int i = (int)(in / each);
-                p.seq = place.seq;
-                p.head = i / per_head;
+            const int n = n_new(a, t.seq), u = units(a, t.seq, n), per_head = u > 0 ? tiles_of(n, a.nq / a.nkv) : 0, items = per_head * a.nkv;
+            const int cut = t.pieces && u > 0 ? (int)((unsigned)(u + t.quota - 1) / (unsigned)t.quota) : u;     // numbers that an item has in the list
+            const int in = at - t.before;
+            if (in < cut * items) {
+                const int i = (int)((unsigned)in / (unsigned)cut), off = in - i * cut, item_begin = t.before + i * cut;
+                p.seq = t.seq;
+                p.head = (int)((unsigned)i / (unsigned)per_head);
                 p.tile = i - p.head * per_head;
-                p.units = each;
-                p.begin = (int)(in - (int64_t)i * each);
-                p.item_begin = place.before + (int64_t)i * each;
-                p.end = to - p.item_begin < each ? (int)(to - p.item_begin) : each;
-                p.item = place.items_before + i;
+                p.item = t.items_before + i;
+                if (t.pieces) {
+                    p.begin = (int)((unsigned)(off * u) / (unsigned)cut);
+                    p.end = (int)((unsigned)((off + 1) * u) / (unsigned)cut);
+                    p.parts = cut;
+                    p.first_block = block - off;
+                    p.slot0 = 2 * p.first_block;
+                    p.slot = 2 * block;
+                } else {
+                    p.begin = off;
+                    p.end = min(u, t.to - item_begin);
+                    p.first_block = (int)((unsigned)item_begin / (unsigned)t.quota);
+                    p.parts = (int)((unsigned)(item_begin + u - 1) / (unsigned)t.quota) - p.first_block + 1;
+                    p.slot0 = 2 * p.first_block + (p.first_block * t.quota == item_begin ? 0 : 1);
+                    p.slot = 2 * block + (at == t.from ? 0 : 1);
+                }
                 return p;
             }
-            place.before += (int64_t)each * n;
-            place.items_before += n;
-            ++place.seq;
+            t.before += cut * items;
+            t.items_before += items;
+            ++t.seq;
         }
     }
+    static __device__ __forceinline__ int next(const TreeShare& t, int at, const TreePart& p) { return t.pieces ? at + 1 : at + (p.end - p.begin); }
 };
 
 // Bit i: the token sees key `key0 + i` of its sequence (i < 64), `own` being its number among the sequence's n_new new tokens.

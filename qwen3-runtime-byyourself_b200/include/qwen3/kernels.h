@@ -529,7 +529,7 @@ int q3_attention_tree_any_bf16(const void* q, const void* k_pages, const void* v
 
 /* ---- attention_tree_mma.cu (-DQ3_HEAD_DIM=64 or 128): the same for bfloat16 queries, 32 rows (new tokens x query heads of a kv head) at a time ---- */
 int q3_attention_tree_mma_head_dim(void);
-/* float32 values of `parts` for so many rows a sequence; `counters`: an int32, zero when made and left zero, for each sequence, kv head and 16 rows */
+/* float32 values of `parts` for so many rows a sequence; `counters`: an int32, zero when made and left zero, for each sequence, kv head and 8 rows */
 int64_t q3_attention_tree_mma_parts(int rows);
 int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
                                float* parts, int* counters, const int* seq_start, const int* seq_pos0, const int* page_table,
