@@ -4,8 +4,7 @@
 // Few rows read many keys, so the floor is the time of the cached rows from memory: 2 (d + 1) bytes a token and kv head in 8 bits.
 //   - A block of four warps takes an equal share of the pages of all (sequence, kv head, tile of rows) (tree_work.cuh), three blocks an SM.
 //   - A warp takes every fourth step of 32 (16) keys of its block's, by itself: it copies the step's keys and values into shared memory with
-//     asynchronous copies a step or two ahead, and every lane copies just what it will read, so that nothing but the row scales is
-//     shared between lanes, no barrier is met and no bank conflict arises.
+//     asynchronous copies a step or two ahead, laid so that a lane reads runs of 16 bytes without bank conflicts; no barrier is met.
 //   - Products are mma.m16n8k16 with keys, then values, as the 16-row operand and the rows as its eight columns: S^T = K Q^T and O^T = V^T P^T, so 8 rows
 //     cost 8, not 16.  What a lane holds of keys and values are runs of 16 bytes, which fixes the order in which the products walk a
 //     head's values and the keys; the query is read in the same order.  The weights change from rows to columns by movmatrix.
@@ -44,6 +43,9 @@ template <bool F8> struct Form {
     static constexpr int V_BYTES = ROW / 8;                           // bytes of a value a lane holds: in runs of V_RUN
     static constexpr int V_RUN = V_BYTES < 16 ? V_BYTES : 16, V_RUNS = V_BYTES / V_RUN;
     static constexpr int SPAN = V_RUN / (F8 ? 1 : 2);                 // values of a run: lanes g hold values g SPAN .. of a group of 8 SPAN
+    // Where the run of lane (g, t) lies among 32: a row's runs side by side, which is how eight lanes copy them (four rows' runs of a lane's neighbours are
+    // half sectors: 24 sectors a copy instead of 16), turned so that lanes that read together do not meet in a bank.
+    static __device__ __forceinline__ uint32_t value_at(int g, int t) { return (t * 8 + (g ^ (V_RUN == 16 ? 2 * t : 4 * (t >> 1)))) * V_RUN; }
     static constexpr int K_BYTES = MINE * K_RUNS * 512, STAGE = K_BYTES + OWN * V_RUNS * 32 * V_RUN;
 };
 
@@ -181,7 +183,8 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
                 for (int i = 0; i < OWN; ++i)
 #pragma unroll
                     for (int h = 0; h < F::V_RUNS; ++h)
-                        copy_async<F::V_RUN>(dst + F::K_BYTES + ((i * F::V_RUNS + h) * 32 + lane) * F::V_RUN, v + (OWN * t + i) * F::ROW + h * 128 + g * F::V_RUN);
+                        copy_async<F::V_RUN>(dst + F::K_BYTES + (i * F::V_RUNS + h) * 32 * F::V_RUN + F::value_at(lane & 7, lane >> 3),
+                                             v + (OWN * (lane >> 3) + i) * F::ROW + h * 128 + (lane & 7) * F::V_RUN);
                 if constexpr (F8) {
                     if (lane < 16) copy_async<4>(scales + stage * 64 + lane * 4, (lane < 8 ? a.key_scales : a.value_scales) + cell0 + (lane & 7) * 4);
                 }
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int key = (i & 1) * (OWN / 2) + 2 * j + (i >> 1);
-                        load_words<F::V_RUN>(w[i], here + F::K_BYTES + ((key * F::V_RUNS + h) * 32 + lane) * F::V_RUN);
+                        load_words<F::V_RUN>(w[i], here + F::K_BYTES + (key * F::V_RUNS + h) * 32 * F::V_RUN + F::value_at(g, t));
                         if (edge) {
                             const bool dead = key0 + OWN * t + key >= pos0 + n_new;
 #pragma unroll
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
 #pragma unroll
                     for (int h = 0; h < F::V_RUNS; ++h) {
                         uint32_t w[F::V_RUN / 4];
-                        load_words<F::V_RUN>(w, src + (((key % OWN) * F::V_RUNS + h) * 32 + g * 4 + key / OWN) * F::V_RUN);
+                        load_words<F::V_RUN>(w, src + ((key % OWN) * F::V_RUNS + h) * 32 * F::V_RUN + F::value_at(g, key / OWN));
 #pragma unroll
                         for (int e = 0; e < F::SPAN; ++e) {
                             float v;
