@@ -1,24 +1,28 @@
 // Attention of a step's new tokens over the cache's pages in bfloat16 or in 8 bits on the 5th-generation tensor cores, for trees (or runs) whose
 // rows - a row is a token and a query head - fill tiles of 128.  What a token sees and what comes out is said in attention_tree.cu.
 //
-// S = Q K^T and O += P V are tcgen05.mma of 128 rows and 128 keys with their accumulators in tensor memory.  A block (one an SM) takes two
-// tiles of 128 rows of one kv head at a time, so that a stretch of 128 keys is brought in once for both and the products of one tile run
-// under the softmax of the other; the stretches of all items are shared out evenly over the blocks (tree_work.cuh).
-//   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It reads its scores twice, for the maximum and for the
-//                weights, 32 at a time, so that 120 registers do; writes the weights over the scores, and rescales O when the maximum is raised by
-//                more than 2^8.  At the end of a part it writes the row, or its share of it for the second kernel to add up.
-//   warps 8-11   bring in the keys, warps 12-15 the values.  bfloat16: by TMA; 8 bits: a warp loads codes a stretch ahead into registers, turns
-//                them into half precision, which holds them exactly, and stores them where TMA would have put them.
-//   warp 16      issues the products, one elected thread.  (Warps 17-19 make its group of four whole, which registers are handed out to.)
+// S = Q K^T and O += P V are tcgen05.mma with the queries, the weights and the accumulators in tensor memory and a page of 64 keys or values in shared
+// memory.  (With the queries in shared memory a product of 128 x 128 x 16 took 130 cycles instead of 64: both operands together are what the tensor core can
+// read of shared memory in its whole time.)  A block, one an SM, works on two tiles side by side, so that the products of one run under the softmax of the other:
+//   more than 128 rows   two tiles of 128 rows, which take the same pages;
+//   up to 128 rows       twice the same rows, one tile with the pages of even number and one with those of odd number; their sums meet at the end.
+// The pages of all items are shared out evenly over the blocks (tree_work.cuh).
+//   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It puts its query there, reads its 64 scores, writes the weights over them, and
+//                rescales O when the maximum is raised by more than 2^8.  At the end of a part it writes the row, or its share of it for the second
+//                kernel to add up.
+//   warps 8-15   8 bits: turn the codes of keys (8-11) and values (12-15) into half precision, which holds them exactly, where TMA would have put them.
+//   warp 16      issues the products, one elected thread: whatever is ready, of either tile.
+//   warps 17, 18 copy keys and values: bfloat16 by TMA where the products read them, 8 bits as they lie, some pages ahead.
+//   (Warp 19 makes its group of four whole, which registers are handed out to.)
 //
-// 8 bits.  A stretch's keys are brought to one scale, that of its first row, 2^k0, by folding 2^(k - k0) into the half-precision numbers, which is exact
-// for k - k0 in -15 .. 7; so are its values.  Scores are then multiplied by 2^k0 with the softmax's own scale; v0 is added to the scores in log2 units, so
-// that a weight is w = 2^(x + v0 - M) with M the running maximum of x + v0 and the sum of the softmax that of w 2^-v0.  Where some row of a stretch has a scale outside that
+// 8 bits.  A page's keys are brought to one scale, that of its first row, 2^k0, by folding 2^(k - k0) into the half-precision numbers, which is exact
+// for k - k0 in -14 .. 7; so are its values.  Scores are then multiplied by 2^k0 with the softmax's own scale; v0 is added to the scores in log2 units, so
+// that a weight is w = 2^(x + v0 - M) with M the running maximum of x + v0 and the sum of the softmax that of w 2^-v0.  Where some row of a page has a scale outside that
 // range, what is missing (`rest`) is added score by score, in a path of its own.  Queries are brought into half precision as in attention_tree_mma.cu.
 //
-// A value that is no number (infinity, NaN) in a stretch that some row does not see in whole is taken out before the product, and put into the
+// A value that is no number (infinity, NaN) in a page that some row does not see in whole is taken out before the product, and put into the
 // outputs of the rows that see it: 0 times a NaN would reach the others.
-// What bounds it: a stretch of 128 keys and 256 rows is 2,048 cycles of the tensor pipe and as many of the special-function unit (an exponential a score).
+// What bounds it: a page and 256 rows are 1,024 cycles of the tensor pipe and as many of the special-function unit (an exponential a score).
 // Every mbarrier wait is bounded and reports into `status`.
 #include <cuda.h>
 
@@ -35,34 +39,47 @@ namespace {
 
 constexpr int D = Q3_HEAD_DIM, PAGE = Q3_PAGE_TOKENS;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
-static_assert(PAGE == 64, "a stretch is two pages of 64 keys");
-constexpr int BM = 128, ROWS = 2 * BM, STRETCH = 2 * PAGE, HALVES = D / 64;
-constexpr int SOFTMAX_WARPS = 8, BRING_WARPS = 4, V_WARP = 12, MMA_WARP = 16, THREADS = 20 * 32;
+static_assert(PAGE == 64, "a product takes a page of 64 keys");
+constexpr int BM = 128, ROWS = 2 * BM, HALVES = D / 64;
+constexpr int SOFTMAX_WARPS = 8, TURN_WARPS = 4, V_WARP = 12, MMA_WARP = 16, K_COPY_WARP = 17, V_COPY_WARP = 18, THREADS = 20 * 32;
 // Registers of a thread by role: 256 x 144 + 256 x 80 + 128 x 32 = 640 x 96, what the block is launched with.
-constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, BRING_REGS = 80, MMA_REGS = 32;
-static_assert(8 * 32 * SOFTMAX_REGS + 8 * 32 * BRING_REGS + 4 * 32 * MMA_REGS <= THREADS * LAUNCH_REGS, "shares of the launch's registers");
-constexpr int STAGES = 2, NOTES = 4;                      // stretches of keys and of values in shared memory; what is noted of a stretch lives longer
-constexpr int HALF_BYTES = BM * 128, TILE_BYTES = HALVES * HALF_BYTES;                     // 128 rows of 128 bytes; a tile of queries, keys or values
-constexpr int PANEL_BYTES = PAGE * 128;                   // a page's 64 rows of 128 bytes
-constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;   // S (and P over it) of tile x at x * 128, O at 256 + x * 128
+constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, TURN_REGS = 72, MMA_REGS = 48;
+static_assert(8 * 32 * SOFTMAX_REGS + 8 * 32 * TURN_REGS + 4 * 32 * MMA_REGS <= THREADS * LAUNCH_REGS, "shares of the launch's registers");
+constexpr int NOTES = 8;                                  // pages whose notes are kept: more than lie between the copies and the softmax
+constexpr int PANEL_BYTES = PAGE * 128, TILE_BYTES = HALVES * PANEL_BYTES;                 // 64 rows of 128 bytes; a page's keys or values in 16 bits
+constexpr int CODE_BYTES = PAGE * D;
+constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, COL_S = 0, COL_Q = 64, COL_O = 128;   // of tile x, from x * 256 on; P lies over S
 constexpr float RAISE = 8.0f;
-constexpr int FOLD_LOW = -15, FOLD_HIGH = 7;
+constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
 
-struct Note {                                             // what is noted of a stretch in 8 bits
-    float scale;                                          // 2^k0 (values: v0)
-    uint32_t flags[BRING_WARPS];                          // bit 0: some scale is out of range; bit 1: some value is no number
+struct Note {                                             // what is noted of a page
+    float scale;                                          // 8 bits: 2^k0 (values: v0)
+    uint32_t flags[TURN_WARPS];                           // bit 0: some scale is out of range; bit 1: some value is no number
     uint32_t pad[3];
 };
-struct Shared {
+template <bool F8> struct Layout {
+    static constexpr int STAGES = F8 ? 3 : 4;             // pages of keys and of values that the products can read
+    static constexpr int CODES = F8 ? 3 : 0;              // pages of codes of either on their way
+    static constexpr int K = 0, V = STAGES * TILE_BYTES, K_CODES = 2 * STAGES * TILE_BYTES, V_CODES = K_CODES + CODES * CODE_BYTES;
+    static constexpr int MEET = V_CODES + CODES * CODE_BYTES, REST = MEET + BM * D * 4;
+    // barriers: one word of 8 bytes each
+    static constexpr int Q = 0, S_FULL = 1, P_FULL = 3, PV_DONE = 5, NOTED = 7, K_FULL = NOTED + NOTES, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES;
+    static constexpr int V_EMPTY = V_FULL + STAGES, V_HERE = V_EMPTY + STAGES;             // V_HERE: TMA's values, before they are looked through
+    static constexpr int KC_FULL = V_HERE + STAGES, KC_EMPTY = KC_FULL + CODES, VC_FULL = KC_EMPTY + CODES, VC_EMPTY = VC_FULL + CODES;
+    static constexpr int MET = VC_EMPTY + CODES, MET_FREE = MET + 1, BARS = MET + 2;       // the sums of odd pages lie in MEET; they are read
+};
+template <bool F8> struct Shared {
+    uint8_t code_scales[2][F8 ? Layout<F8>::CODES : 1][PAGE];
     Note keys[NOTES], values[NOTES];
-    float key_rest[NOTES][STRETCH], value_rest[NOTES][STRETCH];
+    float key_rest[NOTES][PAGE], value_rest[NOTES][PAGE];
+    float2 meet[BM];                                      // (maximum, sum) of a tile of odd pages
     TreeShare share;
-    unsigned long long bars[1 + 5 * STAGES + 6 + NOTES];
+    unsigned long long bars[Layout<F8>::BARS];
     uint32_t tmem;
 };
-constexpr int SMEM_BYTES = 2 * TILE_BYTES + 2 * STAGES * TILE_BYTES + (int)sizeof(Shared);
-static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a block");
+template <bool F8> constexpr int smem_bytes = Layout<F8>::REST + (int)sizeof(Shared<F8>);
+static_assert(smem_bytes<true> <= 227 * 1024 && smem_bytes<false> <= 227 * 1024, "shared memory of a block");
 
 struct Args {
     TreeStep step;
@@ -75,7 +92,7 @@ struct Args {
     float scale_log2;
 };
 
-using Work = TreeWork<STRETCH, ROWS>;
+using Work = TreeWork<PAGE, ROWS>;
 
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile(
@@ -95,13 +112,6 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
           "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
           "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 // kind::f16 instruction descriptor: float32 accumulator, operands both half precision or both bfloat16; bit 16 = B is MN-major.
@@ -149,18 +159,33 @@ __device__ __forceinline__ int64_t page_of(const TreeStep& st, const int* table,
     return p >= 0 && p < st.n_pages ? p : 0;
 }
 
+// Whether a phase is complete, for a whole converged warp; does not wait.
+__device__ __forceinline__ bool mbar_passed_warp(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, done);
+}
+// Bytes from global memory as they lie (all a multiple of 16).
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // Where the values of an output row are that are no numbers: bit d of `plus` for +infinity, of `minus` for -infinity, of both for NaN.
 struct Odd {
     uint32_t plus[D / 32], minus[D / 32];
     bool any;
 };
 
-// The values of stretch `s` that are no numbers, of the keys that the row sees (bits lo: the first 64, hi: the others).
+// The values of page `s` that are no numbers, of the keys that the row sees.
 template <bool F8>
-__device__ __noinline__ void find_odd(const Args& a, const int* table, int head, int s, unsigned long long lo, unsigned long long hi, Odd& odd) {
-    for (int key = 0; key < STRETCH; ++key) {
-        if (!((key < 64 ? lo >> key : hi >> (key - 64)) & 1)) continue;
-        const int64_t cell = (page_of(a.step, table, 2 * s + (key >> 6)) * a.step.nkv + head) * PAGE + (key & 63);
+__device__ __noinline__ void find_odd(const Args& a, const int* table, int head, int s, unsigned long long seen, Odd& odd) {
+    for (int key = 0; key < PAGE; ++key) {
+        if (!(seen >> key & 1)) continue;
+        const int64_t cell = (page_of(a.step, table, s) * a.step.nkv + head) * PAGE + key;
         constexpr int WORDS = D * (F8 ? 1 : 2) / 4, EACH = F8 ? 4 : 2, BITS = F8 ? 8 : 16;
         const uint32_t* row = reinterpret_cast<const uint32_t*>(a.values + cell * (D * (F8 ? 1 : 2)));
         for (int w = 0; w < WORDS; ++w) {
@@ -182,36 +207,41 @@ __device__ __noinline__ void find_odd(const Args& a, const int* table, int head,
 template <bool F8>
 __global__ void __launch_bounds__(THREADS, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args a) {
+    using L = Layout<F8>;
     extern __shared__ unsigned char smem[];
     pdl_launch_dependents();
     const uint32_t base = smem_u32(smem);
-    const uint32_t q_smem = base, k_smem = base + 2 * TILE_BYTES, v_smem = k_smem + STAGES * TILE_BYTES;
-    Shared& sh = *reinterpret_cast<Shared*>(smem + 2 * TILE_BYTES + 2 * STAGES * TILE_BYTES);
+    Shared<F8>& sh = *reinterpret_cast<Shared<F8>*>(smem + L::REST);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bars = smem_u32(sh.bars);
-    const uint32_t bar_q = bars, bar_k_full = bars + 8, bar_k_empty = bar_k_full + 8 * STAGES, bar_v_full = bar_k_empty + 8 * STAGES;
-    const uint32_t bar_v_empty = bar_v_full + 8 * STAGES, bar_v_here = bar_v_empty + 8 * STAGES;      // v_here: TMA's values, before they are looked through
-    const uint32_t bar_s_full = bar_v_here + 8 * STAGES, bar_p_full = bar_s_full + 16, bar_pv_done = bar_p_full + 16;   // one a tile
-    const uint32_t bar_noted = bar_pv_done + 16;         // what is noted of a stretch's keys can be read
+    auto bar = [&](int which, int i) { return bars + 8 * (which + i); };
     if (base & 1023u) {                                  // the swizzled tiles need 1024-byte alignment
         if (threadIdx.x == 0) atomicExch(a.status, 40);
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(bar_q, SOFTMAX_WARPS);
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(bar_k_full + 8 * s, F8 ? BRING_WARPS : 1);
-            mbar_init(bar_k_empty + 8 * s, 1);
-            mbar_init(bar_v_full + 8 * s, BRING_WARPS);
-            mbar_init(bar_v_empty + 8 * s, 1);
-            mbar_init(bar_v_here + 8 * s, 1);
-        }
+        mbar_init(bar(L::Q, 0), SOFTMAX_WARPS);
+        mbar_init(bar(L::MET, 0), 4);
+        mbar_init(bar(L::MET_FREE, 0), 4);
         for (int x = 0; x < 2; ++x) {
-            mbar_init(bar_s_full + 8 * x, 1);
-            mbar_init(bar_p_full + 8 * x, 4);
-            mbar_init(bar_pv_done + 8 * x, 1);
+            mbar_init(bar(L::S_FULL, x), 1);
+            mbar_init(bar(L::P_FULL, x), 4);
+            mbar_init(bar(L::PV_DONE, x), 1);
         }
-        for (int n = 0; n < NOTES; ++n) mbar_init(bar_noted + 8 * n, BRING_WARPS);
+        for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), F8 ? 2 * TURN_WARPS : TURN_WARPS);
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(bar(L::K_FULL, s), F8 ? TURN_WARPS : 1);
+            mbar_init(bar(L::K_EMPTY, s), 1);
+            mbar_init(bar(L::V_FULL, s), TURN_WARPS);
+            mbar_init(bar(L::V_EMPTY, s), 1);
+            mbar_init(bar(L::V_HERE, s), 1);
+        }
+        for (int s = 0; s < L::CODES; ++s) {
+            mbar_init(bar(L::KC_FULL, s), 1);
+            mbar_init(bar(L::KC_EMPTY, s), TURN_WARPS);
+            mbar_init(bar(L::VC_FULL, s), 1);
+            mbar_init(bar(L::VC_EMPTY, s), TURN_WARPS);
+        }
         mbar_init_fence();
     }
     if (warp == MMA_WARP) {
@@ -221,7 +251,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 1, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, 2, blockIdx.x, gridDim.x);
         if (lane == 0) sh.share = found;
     }
     tc_fence_before();
@@ -231,31 +261,33 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     TreeShare share = sh.share;
     const int group = st.nq / st.nkv;
     auto failed = [&](int where) { if (lane == 0) atomicExch(a.status, where); };
+    // The turn of a barrier whose phases are pages, `number` of them in a ring of `size`.
+    auto turn_of = [](int number, int size) { return (uint32_t)(number / size) & 1u; };
 
     if (warp < SOFTMAX_WARPS) {
         // ------------------------------------------------ softmax: thread = row
-        const int x = warp >> 2, r = (warp & 3) * 32 + lane;                         // tile, row of it
-        const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = t_row + COL_S + x * 128, t_o = t_row + COL_O + x * 128;
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-        int stretch = 0;                                                             // of this block, over all parts
-        uint32_t turn = 0, q_turn = 0;                                               // of this tile's barriers, of the parts
+        const int x = warp >> 2, r = (warp & 3) * 32 + lane;                         // tile, row of it
+        const uint32_t t_tile = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * TILE_COLS;
+        int page0 = 0;                                                               // pages of this block before the part
+        uint32_t turn = 0, q_turn = 0, met_turn = 0;                                 // of this tile's barriers, of the parts, of those in which the tiles meet
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
-            const int row0 = part.tile * ROWS, rows = n_new * group - row0 - x * BM;      // of this tile
-            const int steps = part.end - part.begin;
-            const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
-            // ---- this row's query
-            const int row = row0 + x * BM + r, own = min(row / group, n_new - 1);
-            bf16* const out = a.out + ((int64_t)(t0 + own) * st.nq + part.head * group + row % group) * D;
+            const int all_rows = n_new * group - part.tile * ROWS, steps = part.end - part.begin;
+            const bool split = all_rows <= BM;                                       // one tile of rows: every other page
+            const int first = split ? x : 0, stride = split ? 2 : 1;
+            const int rows = split ? all_rows : all_rows - x * BM, row = part.tile * ROWS + (split ? 0 : x * BM) + r, own = min(row / group, n_new - 1);
+            const int64_t row_at = ((int64_t)(t0 + own) * st.nq + part.head * group + row % group) * D;
+            // ---- this row's query, into tensor memory
             float factor = a.scale_log2;
-            if (rows > 0) {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((int64_t)(t0 + own) * st.nq + part.head * group + row % group) * D);
-                const uint32_t dst = q_smem + x * TILE_BYTES;
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
                 float down = 1.0f;
                 if constexpr (F8) {
                     uint32_t top = 0;
+#pragma unroll
                     for (int c = 0; c < D / 8; ++c) {
                         const uint4 w = src[c];
                         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -267,49 +299,50 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     down = q3_exp2i(-e2);
                     factor *= q3_exp2i(e2);
                 }
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 w = src[c];
-                    if constexpr (F8) {
-                        uint32_t* v = &w.x;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
+                for (int c = 0; c < D / 64; ++c) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint4 w = src[8 * c + i];
+                        v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
                     }
-                    if (r >= rows) w = make_uint4(0, 0, 0, 0);
-                    st_shared_v4(dst + chunk_at(r, c, HALF_BYTES), w);
+                    if constexpr (F8) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
+                    }
+                    if (r >= rows) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = 0u;
+                    }
+                    __syncwarp();
+                    tc_st32(t_tile + COL_Q + 32 * c, v);
                 }
-                fence_proxy_async();
+                tc_wait_st();
+                tc_fence_before();
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_q);
-            if (rows <= 0) {                                                         // no second tile: on to the next part with the first tile's warps
-                ok = mbar_wait_warp(bar_q, q_turn);
-                if (!ok) { failed(39); break; }
-                q_turn ^= 1u;
-                stretch += steps;
-                at = Work::next(share, at, part);
-                continue;
-            }
-
-            q_turn ^= 1u;
+            if (lane == 0) mbar_arrive(bar(L::Q, 0));
 
             float m_run = -INFINITY, l_run = 0.0f;
-            const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own) * st.words : nullptr;
             Odd odd;
             odd.any = false;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) odd.plus[i] = odd.minus[i] = 0u;
-            for (int i = 0; i < steps; ++i, ++stretch) {
-                const int key0 = (part.begin + i) * STRETCH, note = stretch % NOTES;
-                const bool edge = key0 + STRETCH > pos0;                             // some key is a new token's, or behind the end
-                ok = mbar_wait_warp(bar_s_full + 8 * x, turn & 1u);
+            for (int n = first; n < steps; n += stride) {
+                const int key0 = (part.begin + n) * PAGE, number = page0 + n, note = number % NOTES;
+                const bool edge = key0 + PAGE > pos0;                                // some key is a new token's, or behind the end
+                ok = mbar_wait_warp(bar(L::S_FULL, x), turn);
                 if (!ok) { failed(41); break; }
-                if (F8 || edge) {                                                    // what is noted of the stretch
-                    ok = mbar_wait_warp(bar_v_full + 8 * (stretch % STAGES), (uint32_t)(stretch / STAGES) & 1u) &&
-                         (!F8 || mbar_wait_warp(bar_noted + 8 * note, (uint32_t)(stretch / NOTES) & 1u));
+                if (F8 || edge) {
+                    ok = mbar_wait_warp(bar(L::NOTED, note), turn_of(number, NOTES));
                     if (!ok) { failed(42); break; }
                 }
                 tc_fence_after();
-                // ---- of the stretch: score = dot * c1, in log2 units, and v0
+                uint32_t s[64];
+                tc_ld32(t_tile + COL_S, s);
+                tc_ld32(t_tile + COL_S + 32, s + 32);
+                // ---- of the page: score = dot * c1, in log2 units, and v0
                 float c1 = factor, v0 = 0.0f;
                 bool rests = false;
                 if constexpr (F8) {
@@ -317,54 +350,40 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     v0 = sh.values[note].scale;
                     uint32_t flags = 0;
 #pragma unroll
-                    for (int w = 0; w < BRING_WARPS; ++w) flags |= sh.keys[note].flags[w] | sh.values[note].flags[w];
+                    for (int w = 0; w < TURN_WARPS; ++w) flags |= sh.keys[note].flags[w] | sh.values[note].flags[w];
                     rests = flags & 1u;
                 }
-                uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+                tc_wait_ld();
                 if (edge) {
-                    const unsigned long long lo = tree_seen(mask, st.words, pos0, n_new, own, key0), hi = tree_seen(mask, st.words, pos0, n_new, own, key0 + 64);
-                    seen[0] = (uint32_t)lo;
-                    seen[1] = (uint32_t)(lo >> 32);
-                    seen[2] = (uint32_t)hi;
-                    seen[3] = (uint32_t)(hi >> 32);
+                    const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own) * st.words : nullptr;
+                    const unsigned long long seen = tree_seen(mask, st.words, pos0, n_new, own, key0);
                     uint32_t flags = 0;
 #pragma unroll
-                    for (int w = 0; w < BRING_WARPS; ++w) flags |= sh.values[note].flags[w];
-                    if (flags & 2u) find_odd<F8>(a, table, part.head, part.begin + i, lo, hi, odd);
+                    for (int w = 0; w < TURN_WARPS; ++w) flags |= sh.values[note].flags[w];
+                    if (flags & 2u) find_odd<F8>(a, st.page_table + (int64_t)part.seq * st.pages_per_seq, part.head, part.begin + n, seen, odd);
+                    const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (!(lo >> e & 1u)) s[e] = 0xff800000u;
+                        if (!(hi >> e & 1u)) s[e + 32] = 0xff800000u;
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 // ---- the maximum of x + v0 (and the rests)
-                float top = -INFINITY;
-                uint32_t s[2][32];
-                auto scores = [&](int c, uint32_t* v) {                              // 32 scores, those that are not seen minus infinity
-                    if (edge) {
+                float top;
+                if (F8 && rests) {
+                    top = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(seen[c] >> e & 1u)) v[e] = 0xff800000u;
-                    }
-                };
-                tc_ld32(t_s, s[0]);
+                    for (int e = 0; e < 64; ++e) top = fmaxf(top, fmaf(__uint_as_float(s[e]) * sh.key_rest[note][e], c1, sh.value_rest[note][e]));
+                } else {
+                    float mx[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tc_wait_ld();
-                    if (c < 3) tc_ld32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t* v = s[c & 1];
-                    scores(c, v);
-                    if (F8 && rests) {
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 4]));
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            top = fmaxf(top, fmaf(__uint_as_float(v[e]) * sh.key_rest[note][32 * c + e], c1, sh.value_rest[note][32 * c + e]));
-                    } else {
-                        float mx[4];
+                    for (int e = 8; e < 64; e += 8)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 4]));
-#pragma unroll
-                        for (int e = 8; e < 32; e += 8)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(v[e + k]), __uint_as_float(v[e + k + 4]));
-                        const float most = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                        top = fmaxf(top, most * c1);
-                    }
+                        for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(s[e + k]), __uint_as_float(s[e + k + 4]));
+                    top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c1;
                 }
                 top += v0;
                 const bool raise = top > m_run + RAISE;
@@ -374,317 +393,406 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     m_run = top;
                     l_run *= alpha;
                 }
-                __syncwarp();
-                if (i > 0 && __any_sync(0xffffffffu, raise)) {
-                    // (the products of the stretch before are done: this stretch's scores were asked for after them)
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        tc_ld32(t_o + c, s[0]);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * alpha);
-                        tc_st32(t_o + c, s[0]);
-                    }
-                }
                 // ---- weights, over the scores
                 const float shift = v0 - (m_run == -INFINITY ? 0.0f : m_run);
                 const float2 c2 = make_float2(c1, c1), shift2 = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                tc_ld32(t_s, s[0]);
+                uint32_t p[32];
+                if (F8 && rests) {
+                    // (where nothing is left by the folds, these are the other path's numbers to the bit: a row does not feel the scales of
+                    // keys that it does not see)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tc_wait_ld();
-                    if (c < 3) tc_ld32(t_s + 32 * (c + 1), s[(c + 1) & 1]);
-                    uint32_t* v = s[c & 1];
-                    scores(c, v);
-                    uint32_t p[16];
-                    if (F8 && rests) {
+                    for (int e = 0; e < 64; e += 2) {
+                        float w[2];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            // (where nothing is left by the folds, these are the other path's numbers to the bit: a row does not feel the scales of
-                            // keys that it does not see)
-                            float w[2];
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const float rest = sh.value_rest[note][32 * c + e + k];
-                                w[k] = ex2(fmaf(__uint_as_float(v[e + k]) * sh.key_rest[note][32 * c + e + k], c1, shift + rest));
-                                float& to_sum = k == 0 ? sum[(e >> 1) & 1].x : sum[(e >> 1) & 1].y;
-                                to_sum = fmaf(w[k], ex2(-rest), to_sum);
-                            }
-                            p[e / 2] = pack2<true>(w[0], w[1]);
+                        for (int k = 0; k < 2; ++k) {
+                            const float rest = sh.value_rest[note][e + k];
+                            w[k] = ex2(fmaf(__uint_as_float(s[e + k]) * sh.key_rest[note][e + k], c1, shift + rest));
+                            float& to_sum = k == 0 ? sum[(e >> 1) & 1].x : sum[(e >> 1) & 1].y;
+                            to_sum = fmaf(w[k], ex2(-rest), to_sum);
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float2 t = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), c2, shift2);
-                            const float2 w = make_float2(ex2(t.x), ex2(t.y));
-                            sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], w);
-                            p[e / 2] = pack2<F8>(w.x, w.y);
-                        }
+                        p[e / 2] = pack2<true>(w[0], w[1]);
                     }
-                    tc_st16(t_s + 16 * c, p);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 64; e += 2) {
+                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, shift2);
+                        const float2 w = make_float2(ex2(z.x), ex2(z.y));
+                        sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], w);
+                        p[e / 2] = pack2<F8>(w.x, w.y);
+                    }
                 }
                 const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 l_run += F8 ? total * ex2(-v0) : total;
+                __syncwarp();
+                tc_st32(t_tile + COL_S, p);
+                if (n > first && __any_sync(0xffffffffu, raise)) {
+                    // (the products of the page before are done: this page's scores were asked for after them)
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 64) {
+                        tc_ld32(t_tile + COL_O + c, s);
+                        tc_ld32(t_tile + COL_O + c + 32, s + 32);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * alpha);
+                        tc_st32(t_tile + COL_O + c, s);
+                        tc_st32(t_tile + COL_O + c + 32, s + 32);
+                    }
+                }
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_p_full + 8 * x);
+                if (lane == 0) mbar_arrive(bar(L::P_FULL, x));
                 turn ^= 1u;
             }
             if (!ok) break;
-            ok = mbar_wait_warp(bar_pv_done + 8 * x, turn ^ 1u);                      // the part's last products (turn: as many as there were stretches)
+            // the part's last products (turn: as many as there were pages); a tile without pages goes on with the other one's warps, not ahead of them
+            ok = first < steps ? mbar_wait_warp(bar(L::PV_DONE, x), turn ^ 1u) : mbar_wait_warp(bar(L::Q, 0), q_turn);
+            q_turn ^= 1u;
             if (!ok) { failed(43); break; }
             tc_fence_after();
             // ---- the row, or its part of it
             const bool whole = part.parts == 1;
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
             float* const dst = a.parts + (int64_t)part.slot * PART;
-            const int pr = x * BM + r;                                               // the row among the part's
+            const int part_row = split ? r : x * BM + r;
+            float mine = 1.0f, other = 0.0f;                                         // factors of the two tiles' sums
+            float4* const meet = reinterpret_cast<float4*>(smem + L::MEET);          // [D / 4][BM]
+            if (split) {
+                if (x == 1) {
+                    ok = mbar_wait_warp(bar(L::MET_FREE, 0), met_turn ^ 1u);
+                    if (!ok) { failed(39); break; }
+                    sh.meet[r] = make_float2(m_run, l_run);
+                    if (steps > 1 && (warp & 3) * 32 < rows) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                tc_ld32(t_o + c, o);
-                tc_wait_ld();
-                if (odd.any) {
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            __syncwarp();
+                            tc_ld32(t_tile + COL_O + c, o);
+                            tc_wait_ld();
+                            if (odd.any) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
-                        if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
+                                for (int e = 0; e < 32; ++e) {
+                                    if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
+                                    if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                meet[(c + e) / 4 * BM + r] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                        }
                     }
                 }
-                if (r < rows) {
-                    if (whole) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 v;
-                            v.x = pack2<false>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                            v.y = pack2<false>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                            v.z = pack2<false>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                            v.w = pack2<false>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                            *reinterpret_cast<uint4*>(out + c + e) = v;
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4*>(dst + ((c + e) / 4 * ROWS + pr) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                    }
+                if (x == 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(L::MET, 0));
+                } else {
+                    ok = mbar_wait_warp(bar(L::MET, 0), met_turn);
+                    if (!ok) { failed(38); break; }
+                    const float2 ml = sh.meet[r];
+                    const float m = fmaxf(m_run, ml.x);
+                    mine = m_run == m ? 1.0f : ex2(m_run - m);
+                    other = ml.x == m ? 1.0f : ex2(ml.x - m);
+                    m_run = m;
+                    l_run = fmaf(ml.y, other, l_run * mine);
                 }
             }
-            if (!whole && r < rows) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * pr) = make_float2(m_run, l_run);
+            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+            if (!(split && x == 1) && (warp & 3) * 32 < rows) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tc_ld32(t_tile + COL_O + c, o);
+                    tc_wait_ld();
+                    if (odd.any) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
+                            if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
+                        }
+                    }
+                    if (split && steps > 1) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 u = meet[(c + e) / 4 * BM + r];
+                            o[e] = __float_as_uint(fmaf(u.x, other, __uint_as_float(o[e]) * mine));
+                            o[e + 1] = __float_as_uint(fmaf(u.y, other, __uint_as_float(o[e + 1]) * mine));
+                            o[e + 2] = __float_as_uint(fmaf(u.z, other, __uint_as_float(o[e + 2]) * mine));
+                            o[e + 3] = __float_as_uint(fmaf(u.w, other, __uint_as_float(o[e + 3]) * mine));
+                        }
+                    }
+                    if (r < rows) {
+                        if (whole) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint4 v;
+                                v.x = pack2<false>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                                v.y = pack2<false>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                                v.z = pack2<false>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+                                v.w = pack2<false>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+                                *reinterpret_cast<uint4*>(a.out + row_at + c + e) = v;
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                *reinterpret_cast<uint4*>(dst + ((c + e) / 4 * ROWS + part_row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
+                    }
+                }
+                if (!whole && r < rows) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * part_row) = make_float2(m_run, l_run);
+            }
             tc_fence_before();
+            if (split) {
+                __syncwarp();
+                if (x == 0 && lane == 0) mbar_arrive(bar(L::MET_FREE, 0));
+                met_turn ^= 1u;
+            }
+            page0 += steps;
             at = Work::next(share, at, part);
         }
     } else if (warp < MMA_WARP) {
-        // ------------------------------------------------ the keys (warps 8-11) and the values (12-15)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BRING_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TURN_REGS));
         const bool is_v = warp >= V_WARP;
         const int w4 = warp & 3;
-        const uint32_t tiles = is_v ? v_smem : k_smem, bar_full = is_v ? bar_v_full : bar_k_full, bar_empty = is_v ? bar_v_empty : bar_k_empty;
-        int stretch = 0;
+        int number = 0;
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
-            const int n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq], steps = part.end - part.begin;
-            const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
-            const int key_end = pos0 + n_new;
+            const int pos0 = st.seq_pos0[part.seq], key_end = pos0 + Work::n_new(st, part.seq), steps = part.end - part.begin;
             if constexpr (F8) {
-                // a row is D / 16 lanes' sixteen codes; a warp has 32 rows of a stretch, all of one page
-                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = PER_ROW;
-                const unsigned char* const source = is_v ? a.values : a.keys;
-                const uint8_t* const scale_source = is_v ? a.value_scales : a.key_scales;
+                // ------------------------------------------------ codes to half precision: 16 rows of a page a warp, D / 16 lanes a row
+                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = 16 / AT_ONCE;
                 const int c = lane % PER_ROW, r_in = lane / PER_ROW;
-                uint4 codes[TURNS];
-                uint8_t scale[TURNS], scale0 = 0;
-                auto load = [&](int s) {
-                    const int64_t first = (page_of(st, table, 2 * s) * st.nkv + part.head) * PAGE;
-                    const int64_t cell = (page_of(st, table, 2 * s + (w4 >> 1)) * st.nkv + part.head) * PAGE + (w4 & 1) * 32 + r_in;
-                    scale0 = scale_source[first];
-#pragma unroll
-                    for (int i = 0; i < TURNS; ++i) {
-                        codes[i] = *reinterpret_cast<const uint4*>(source + (cell + i * AT_ONCE) * D + c * 16);
-                        scale[i] = scale_source[cell + i * AT_ONCE];
-                    }
-                };
-                load(part.begin);
-                for (int n = 0; n < steps; ++n, ++stretch) {
-                    const int stage = stretch % STAGES, note = stretch % NOTES, key0 = (part.begin + n) * STRETCH;
-                    const bool edge = key0 + STRETCH > pos0;
-                    ok = mbar_wait_warp(bar_empty + 8 * stage, ((uint32_t)(stretch / STAGES) & 1u) ^ 1u);
+                const int full = is_v ? L::V_FULL : L::K_FULL, empty = is_v ? L::V_EMPTY : L::K_EMPTY;
+                const int c_full = is_v ? L::VC_FULL : L::KC_FULL, c_empty = is_v ? L::VC_EMPTY : L::KC_EMPTY;
+                // the lanes of a row's second half (64 values) store their second chunk first: eight lanes, eight banks
+                const int swap = HALVES == 2 ? c >> 2 : 0;
+                for (int n = 0; n < steps; ++n, ++number) {
+                    const int stage = number % L::STAGES, slot = number % L::CODES, note = number % NOTES, key0 = (part.begin + n) * PAGE;
+                    const bool edge = key0 + PAGE > pos0;
+                    ok = mbar_wait_warp(bar(c_full, slot), turn_of(number, L::CODES)) && mbar_wait_warp(bar(empty, stage), turn_of(number, L::STAGES) ^ 1u);
                     if (!ok) { failed(is_v ? 45 : 44); break; }
-                    const uint32_t dst = tiles + stage * TILE_BYTES + (is_v ? (w4 >> 1) * (HALVES * PANEL_BYTES) : (w4 >> 1) * PANEL_BYTES);
+                    const uint32_t src = base + (is_v ? L::V_CODES : L::K_CODES) + slot * CODE_BYTES, dst = base + (is_v ? L::V : L::K) + stage * TILE_BYTES;
+                    const uint8_t* const scales = sh.code_scales[is_v][slot];
+                    const int scale0 = scales[0];
                     uint32_t flags = 0;
+                    uint4 codes[TURNS];
+                    int e[TURNS];
 #pragma unroll
                     for (int i = 0; i < TURNS; ++i) {
-                        const int row = (w4 & 1) * 32 + i * AT_ONCE + r_in, key = key0 + (w4 >> 1) * 64 + row;      // row of the page
-                        uint32_t* v = &codes[i].x;
-                        const int e = (int)scale[i] - (int)scale0, fold = min(max(e, FOLD_LOW), FOLD_HIGH);
-                        const bool live = key < key_end;
-                        if (edge && is_v) {
+                        const int row = w4 * 16 + i * AT_ONCE + r_in;
+                        codes[i] = ld_shared_v4(src + row * D + c * 16);
+                        e[i] = (int)scales[row] - scale0;
+                    }
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                if (!live) v[k] = 0u;
-                                const uint32_t bad = no_numbers<true>(v[k]);
-                                if (bad) flags |= 2u;
-                                v[k] &= ~bad;
+                    for (int i = 0; i < TURNS; ++i) {
+                        const int row = w4 * 16 + i * AT_ONCE + r_in;
+                        uint32_t* v = &codes[i].x;
+                        const int fold = min(max(e[i], FOLD_LOW), FOLD_HIGH);
+                        if (edge) {
+                            const bool live = key0 + row < key_end;                  // (the scale of a row that nobody wrote may be anything)
+                            if (!live) e[i] = fold;
+                            if (is_v) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    if (!live) v[k] = 0u;
+                                    const uint32_t bad = no_numbers<true>(v[k]);
+                                    if (bad) flags |= 2u;
+                                    v[k] &= ~bad;
+                                }
                             }
                         }
-                        if (live && e != fold) flags |= 1u;
-                        const __half2 by = __float2half2_rn(q3_exp2i(fold));
+                        if (e[i] != fold) flags |= 1u;
+                        const uint32_t one = (uint32_t)(fold + 15) << 10, both = one | one << 16;          // 2^fold, twice
+                        const __half2 by = *reinterpret_cast<const __half2*>(&both);
                         uint32_t h[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const __half2 z = __hmul2(q3_half2_of(v[k >> 1] >> (16 * (k & 1))), by);
                             h[k] = *reinterpret_cast<const uint32_t*>(&z);
                         }
-                        // the lanes of a row's second half (64 values) store their second chunk first: eight lanes, eight banks
-                        const int swap = HALVES == 2 ? c >> 2 : 0;
                         const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-                        const int half_bytes = is_v ? PANEL_BYTES : HALF_BYTES;
-                        st_shared_v4(dst + chunk_at(row, 2 * c + swap, half_bytes), swap ? hi : lo);
-                        st_shared_v4(dst + chunk_at(row, 2 * c + 1 - swap, half_bytes), swap ? lo : hi);
+                        st_shared_v4(dst + chunk_at(row, 2 * c + swap, PANEL_BYTES), swap ? hi : lo);
+                        st_shared_v4(dst + chunk_at(row, 2 * c + 1 - swap, PANEL_BYTES), swap ? lo : hi);
                     }
                     flags = __reduce_or_sync(0xffffffffu, flags);
-                    // what the fold leaves, as a factor of the key's score or in log2 units: read only where a flag says so, which any warp of either kind may
+                    // what the folds leave, as a factor of the key's score or in log2 units: read only where a flag says so, which any warp of either kind may
                     if (c == 0) {
 #pragma unroll
                         for (int i = 0; i < TURNS; ++i) {
-                            const int row = w4 * 32 + i * AT_ONCE + r_in, e = (int)scale[i] - (int)scale0, rest = e - min(max(e, FOLD_LOW), FOLD_HIGH);
-                            const bool live = key0 + row < key_end;                  // (the scale of a row that nobody wrote may be anything)
-                            if (is_v) sh.value_rest[note][row] = live ? (float)rest : 0.0f;
-                            else sh.key_rest[note][row] = live ? q3_exp2i(rest) : 1.0f;
+                            const int row = w4 * 16 + i * AT_ONCE + r_in, rest = e[i] - min(max(e[i], FOLD_LOW), FOLD_HIGH);
+                            if (is_v) sh.value_rest[note][row] = (float)rest;
+                            else sh.key_rest[note][row] = q3_exp2i(rest);
                         }
                     }
                     Note& to_note = is_v ? sh.values[note] : sh.keys[note];
                     if (lane == 0) {
                         to_note.flags[w4] = flags;
-                        if (w4 == 0) to_note.scale = is_v ? (float)((int)scale0 - Q3_SCALE_BIAS) : q3_exp2i((int)scale0 - Q3_SCALE_BIAS);
+                        if (w4 == 0) to_note.scale = is_v ? (float)(scale0 - Q3_SCALE_BIAS) : q3_exp2i(scale0 - Q3_SCALE_BIAS);
                     }
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        if (!is_v) mbar_arrive(bar_noted + 8 * note);
-                        mbar_arrive(bar_full + 8 * stage);
+                        mbar_arrive(bar(full, stage));
+                        mbar_arrive(bar(c_empty, slot));
+                        mbar_arrive(bar(L::NOTED, note));
                     }
-                    if (n + 1 < steps) load(part.begin + n + 1);
                 }
-            } else {
-                auto ask = [&](int n, int number) {                                  // the copies of a stretch, by one thread
-                    const int stage = number % STAGES;
-                    const uint32_t bar = (is_v ? bar_v_here : bar_k_full) + 8 * stage, dst = tiles + stage * TILE_BYTES;
-                    mbar_expect_tx(bar, TILE_BYTES);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const int row = (int)((page_of(st, table, 2 * (part.begin + n) + p) * st.nkv + part.head) * PAGE);
-#pragma unroll
-                        for (int h = 0; h < HALVES; ++h)
-                            tma_load_2d(is_v ? dst + p * (HALVES * PANEL_BYTES) + h * PANEL_BYTES : dst + h * HALF_BYTES + p * PANEL_BYTES, is_v ? &map_v : &map_k, bar,
-                                        h * 64, row);
-                    }
-                };
-                auto stage_free = [&](int number) { return mbar_wait_warp(bar_empty + 8 * (number % STAGES), ((uint32_t)(number / STAGES) & 1u) ^ 1u); };
-                for (int n = 0; n < steps && ok; ++n, ++stretch) {
-                    if (w4 == 0) {
-                        ok = stage_free(stretch);
-                        if (!ok) { failed(is_v ? 45 : 44); break; }
-                        if (lane == 0) ask(n, stretch);
-                        __syncwarp();
-                    }
-                    if (!is_v) continue;
-                    const int stage = stretch % STAGES, key0 = (part.begin + n) * STRETCH;
-                    ok = mbar_wait_warp(bar_v_here + 8 * stage, (uint32_t)(stretch / STAGES) & 1u);
+            } else if (is_v) {
+                // ------------------------------------------------ a look at the values of pages that some row does not see in whole
+                for (int n = 0; n < steps; ++n, ++number) {
+                    const int stage = number % L::STAGES, key0 = (part.begin + n) * PAGE;
+                    ok = mbar_wait_warp(bar(L::V_HERE, stage), turn_of(number, L::STAGES));
                     if (!ok) { failed(46); break; }
-                    if (key0 + STRETCH > pos0) {
-                        // values behind the end, and those that are no numbers, become zeros; a warp looks through 32 rows
+                    if (key0 + PAGE > pos0) {
+                        // values behind the end, and those that are no numbers, become zeros; a warp looks through 16 rows
                         uint32_t found = 0;
-                        const uint32_t page = v_smem + stage * TILE_BYTES + (w4 >> 1) * (HALVES * PANEL_BYTES);
-                        for (int i = lane; i < 32 * (D / 8); i += 32) {
-                            const int row = (w4 & 1) * 32 + i / (D / 8), key = key0 + (w4 >> 1) * 64 + row;
-                            const uint32_t at_chunk = page + chunk_at(row, i % (D / 8), PANEL_BYTES);
+                        for (int i = lane; i < 16 * (D / 8); i += 32) {
+                            const int row = w4 * 16 + i / (D / 8);
+                            const uint32_t at_chunk = base + L::V + stage * TILE_BYTES + chunk_at(row, i % (D / 8), PANEL_BYTES);
                             uint4 v = ld_shared_v4(at_chunk);
-                            if (key >= key_end) v = make_uint4(0, 0, 0, 0);
+                            const bool live = key0 + row < key_end;
+                            if (!live) v = make_uint4(0, 0, 0, 0);
                             const uint4 bad = make_uint4(no_numbers<false>(v.x), no_numbers<false>(v.y), no_numbers<false>(v.z), no_numbers<false>(v.w));
                             const uint32_t any = bad.x | bad.y | bad.z | bad.w;
                             found |= any;
-                            if (any != 0 || key >= key_end) st_shared_v4(at_chunk, make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w));
+                            if (any != 0 || !live) st_shared_v4(at_chunk, make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w));
                         }
                         found = __reduce_or_sync(0xffffffffu, found);
-                        if (lane == 0) sh.values[stretch % NOTES].flags[w4] = found != 0 ? 2u : 0u;
+                        if (lane == 0) sh.values[number % NOTES].flags[w4] = found != 0 ? 2u : 0u;
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    if (lane == 0) mbar_arrive(bar_v_full + 8 * stage);
+                    if (lane == 0) {
+                        mbar_arrive(bar(L::V_FULL, stage));
+                        mbar_arrive(bar(L::NOTED, number % NOTES));
+                    }
                 }
             }
             at = Work::next(share, at, part);
         }
     } else {
-        // ------------------------------------------------ the products: the whole warp walks and one elected thread issues
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MMA_REGS));
         if (warp == MMA_WARP) {
-        constexpr uint32_t idesc_s = idesc(F8, BM, STRETCH, false), idesc_pv = idesc(F8, BM, D, true);
-        const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint64_t q_desc = desc_k_major(q_smem), k_desc = desc_k_major(k_smem), v_desc = desc_mn_major(v_smem, PANEL_BYTES);
-        int stretch = 0;
-        uint32_t q_turn = 0, turn[2] = {0, 0}, done[2] = {0, 0};                    // parities: queries, weights of a tile, products of a tile
-        bool ok = true;
-        auto scores = [&](int x, int number, bool release) {
-            const uint32_t stage = (uint32_t)number % STAGES;
-            const uint64_t q_src = q_desc + (uint64_t)(x * (TILE_BYTES >> 4)), k_src = k_desc + (uint64_t)(stage * (TILE_BYTES >> 4));
-            if (elect_one()) {
+            // ------------------------------------------------ the products: the whole warp walks and one elected thread issues
+            constexpr uint32_t idesc_s = idesc(F8, BM, PAGE, false), idesc_pv = idesc(F8, BM, D, true);
+            const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t k_desc = desc_k_major(base + L::K), v_desc = desc_mn_major(base + L::V, PANEL_BYTES);
+            int page0 = 0;
+            uint32_t q_turn = 0, p_turn = 0, pv_turn = 0;                            // parities; of the tiles: bit x
+            bool ok = true;
+            for (int at = share.from; at < share.to && ok;) {
+                const TreePart part = Work::part(st, share, at, blockIdx.x);
+                const bool split = Work::n_new(st, part.seq) * group - part.tile * ROWS <= BM;
+                const int steps = part.end - part.begin, stride = split ? 2 : 1;
+                uint32_t k_used = 0, v_used = 0;                                     // stages that one of two tiles has read
+                int next[2] = {0, split ? 1 : 0};                                    // a tile's page: whose scores come next, or (waiting) whose weights do
+                uint32_t waits = 0;                                                  // bit x: tile x waits for its weights; bit 2 + x: for its products to end
+                ok = mbar_wait_warp(bar(L::Q, 0), q_turn);
+                q_turn ^= 1u;
+                if (!ok) { failed(47); break; }
+                tc_fence_after();
+                uint32_t idle = 0;
+                while ((next[0] < steps || next[1] < steps) && ok) {
+                    bool some = false;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-                    tc_mma_ss(acc + COL_S + x * 128, q_src + (uint64_t)(off >> 4), k_src + (uint64_t)(off >> 4), idesc_s, kk > 0 ? 1u : 0u);
-                }
-                tc_commit(bar_s_full + 8 * x);
-                if (release) tc_commit(bar_k_empty + 8 * stage);
-            }
-            __syncwarp();
-        };
-        for (int at = share.from; at < share.to && ok;) {
-            const TreePart part = Work::part(st, share, at, blockIdx.x);
-            const int rows = Work::n_new(st, part.seq) * group - part.tile * ROWS, steps = part.end - part.begin, both = rows > BM ? 2 : 1;
-            auto keys_here = [&](int number) { return mbar_wait_warp(bar_k_full + 8 * (number % STAGES), (uint32_t)(number / STAGES) & 1u); };
-            ok = mbar_wait_warp(bar_q, q_turn) && keys_here(stretch);
-            q_turn ^= 1u;
-            if (!ok) { failed(47); break; }
-            tc_fence_after();
-            for (int x = 0; x < both; ++x) scores(x, stretch, x == both - 1);
-            for (int i = 0; i < steps && ok; ++i, ++stretch) {
-                for (int x = 0; x < both && ok; ++x) {
-                    const uint32_t stage = (uint32_t)stretch % STAGES;
-                    ok = mbar_wait_warp(bar_p_full + 8 * x, turn[x]) && mbar_wait_warp(bar_v_full + 8 * stage, (uint32_t)(stretch / STAGES) & 1u);
-                    turn[x] ^= 1u;
-                    if (!ok) { failed(48); break; }
-                    tc_fence_after();
-                    const uint64_t v_src = v_desc + (uint64_t)(stage * (TILE_BYTES >> 4));
-                    if (elect_one()) {
+                    for (int x = 0; x < 2; ++x) {
+                        if (next[x] >= steps) continue;
+                        const int number = page0 + next[x];
+                        const uint32_t stage = (uint32_t)number % L::STAGES, turn = turn_of(number, L::STAGES);
+                        if (waits & (1u << x)) {
+                            if (!mbar_passed_warp(bar(L::P_FULL, x), p_turn >> x & 1u) || !mbar_passed_warp(bar(L::V_FULL, stage), turn)) continue;
+                            p_turn ^= 1u << x;
+                            const bool release = split || (v_used >> stage & 1u);
+                            v_used ^= split ? 0u : 1u << stage;
+                            tc_fence_after();
+                            if (elect_one()) {
 #pragma unroll
-                        for (int kk = 0; kk < STRETCH / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * (HALVES * PANEL_BYTES) + (kk & 3) * 16 * 128;
-                            tc_mma_ts(acc + COL_O + x * 128, acc + COL_S + x * 128 + kk * 8, v_src + (uint64_t)(off >> 4), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                                for (int kk = 0; kk < PAGE / 16; ++kk)
+                                    tc_mma_ts(acc + x * TILE_COLS + COL_O, acc + x * TILE_COLS + COL_S + kk * 8,
+                                              v_desc + (uint64_t)((stage * TILE_BYTES + kk * 16 * 128) >> 4), idesc_pv, (next[x] >= stride || kk > 0) ? 1u : 0u);
+                                tc_commit(bar(L::PV_DONE, x));
+                                if (release) tc_commit(bar(L::V_EMPTY, stage));
+                            }
+                            __syncwarp();
+                            waits ^= 5u << x;
+                            next[x] += stride;
+                            some = true;
+                            // the part's last products are nobody's to wait for here
+                            if (next[x] >= steps) {
+                                waits &= ~(4u << x);
+                                pv_turn ^= 1u << x;
+                            }
+                        } else {
+                            if (waits & (4u << x)) {
+                                // the next scores go where the weights were: once the products with them are done
+                                if (!mbar_passed_warp(bar(L::PV_DONE, x), pv_turn >> x & 1u)) continue;
+                                waits ^= 4u << x;
+                                pv_turn ^= 1u << x;
+                            }
+                            if (!mbar_passed_warp(bar(L::K_FULL, stage), turn)) continue;
+                            const bool release = split || (k_used >> stage & 1u);
+                            k_used ^= split ? 0u : 1u << stage;
+                            tc_fence_after();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int kk = 0; kk < D / 16; ++kk)
+                                    tc_mma_ts(acc + x * TILE_COLS + COL_S, acc + x * TILE_COLS + COL_Q + kk * 8,
+                                              k_desc + (uint64_t)((stage * TILE_BYTES + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+                                tc_commit(bar(L::S_FULL, x));
+                                if (release) tc_commit(bar(L::K_EMPTY, stage));
+                            }
+                            __syncwarp();
+                            waits |= 1u << x;
+                            some = true;
                         }
-                        tc_commit(bar_pv_done + 8 * x);
-                        if (x == both - 1) tc_commit(bar_v_empty + 8 * stage);
+                    }
+                    idle = some ? 0 : idle + 1;
+                    if (idle > Q3_WAIT_LIMIT) {
+                        ok = false;
+                        failed(48);
+                    }
+                }
+                page0 += steps;
+                at = Work::next(share, at, part);
+            }
+        } else if (warp == K_COPY_WARP || warp == V_COPY_WARP) {
+            // ------------------------------------------------ copies of the keys, of the values
+            const bool is_v = warp == V_COPY_WARP;
+            int number = 0;
+            bool ok = true;
+            for (int at = share.from; at < share.to && ok;) {
+                const TreePart part = Work::part(st, share, at, blockIdx.x);
+                const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
+                int64_t page = page_of(st, table, part.begin);
+                for (int i = part.begin; i < part.end; ++i, ++number) {
+                    const int64_t cell = (page * st.nkv + part.head) * PAGE;
+                    if (i + 1 < part.end) page = page_of(st, table, i + 1);
+                    if constexpr (F8) {
+                        const int slot = number % L::CODES;
+                        ok = mbar_wait_warp(bar(is_v ? L::VC_EMPTY : L::KC_EMPTY, slot), turn_of(number, L::CODES) ^ 1u);
+                        if (!ok) { failed(is_v ? 50 : 49); break; }
+                        if (lane == 0) {
+                            const uint32_t full = bar(is_v ? L::VC_FULL : L::KC_FULL, slot);
+                            mbar_expect_tx(full, CODE_BYTES + PAGE);
+                            copy_bulk(base + (is_v ? L::V_CODES : L::K_CODES) + slot * CODE_BYTES, (is_v ? a.values : a.keys) + cell * D, CODE_BYTES, full);
+                            copy_bulk(smem_u32(sh.code_scales[is_v][slot]), (is_v ? a.value_scales : a.key_scales) + cell, PAGE, full);
+                        }
+                    } else {
+                        const int stage = number % L::STAGES;
+                        ok = mbar_wait_warp(bar(is_v ? L::V_EMPTY : L::K_EMPTY, stage), turn_of(number, L::STAGES) ^ 1u);
+                        if (!ok) { failed(is_v ? 50 : 49); break; }
+                        if (lane == 0) {
+                            const uint32_t full = bar(is_v ? L::V_HERE : L::K_FULL, stage), dst = base + (is_v ? L::V : L::K) + stage * TILE_BYTES;
+                            mbar_expect_tx(full, TILE_BYTES);
+#pragma unroll
+                            for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * PANEL_BYTES, is_v ? &map_v : &map_k, full, h * 64, (int)cell);
+                        }
                     }
                     __syncwarp();
-                    // the next scores go where the weights were: once the products with them are done
-                    ok = mbar_wait_warp(bar_pv_done + 8 * x, done[x]);
-                    done[x] ^= 1u;
-                    if (ok && i + 1 < steps) {
-                        ok = keys_here(stretch + 1);
-                        if (ok) {
-                            tc_fence_after();
-                            scores(x, stretch + 1, x == both - 1);
-                        }
-                    }
-                    if (!ok) failed(49);
                 }
+                at = Work::next(share, at, part);
             }
-            at = Work::next(share, at, part);
-        }
         }
     }
     tc_fence_before();
@@ -704,7 +812,7 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
     const TreeStep& st = a.step;
     const int b0 = blockIdx.x;
     if (threadIdx.x < 32) {
-        const TreeShare found = Work::share(st, 1, b0, blocks);
+        const TreeShare found = Work::share(st, 2, b0, blocks);
         if (threadIdx.x == 0) shared_share = found;
     }
     __syncthreads();
@@ -748,7 +856,7 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
 
 template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
     static Q3PerDevice configured;
-    const cudaError_t e = q3_allow_shared_memory(tree_tc_kernel<F8>, SMEM_BYTES, configured);
+    const cudaError_t e = q3_allow_shared_memory(tree_tc_kernel<F8>, smem_bytes<F8>, configured);
     if (e != cudaSuccess) return (int)e;
     CUtensorMap map_k = {}, map_v = {};
     if (!F8 && (!q3_make_map_bf16(&map_k, a.keys, a.step.n_pages * a.step.nkv * PAGE, D, PAGE, 64, true) ||
@@ -756,8 +864,9 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
         return Q3_ERR_BAD_SIZE;
     const int64_t units = Work::most_units(a.step);
     if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
-    const int sms = q3_device_sm_count(), blocks = (int)(units < sms ? units : sms);
-    int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)SMEM_BYTES, stream, map_k, map_v, a);
+    const int64_t most = (units + 1) / 2 + Work::most_items(a.step);
+    const int sms = q3_device_sm_count(), blocks = (int)(most < sms ? most : sms);
+    int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)smem_bytes<F8>, stream, map_k, map_v, a);
     if (code != 0) return code;
     const int rows = (int64_t)max_new * (a.step.nq / a.step.nkv) < ROWS ? max_new * (a.step.nq / a.step.nkv) : ROWS;
     return (int)q3_launch(tree_tc_merge_kernel, dim3(blocks, (rows + 31) / 32), dim3(256), 0, stream, a, blocks);
@@ -778,7 +887,8 @@ Q3_EXPORT int q3_attention_tree_tc_bf16(const void* q, const void* k_pages, cons
     if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || n_pages <= 0 || pages_per_seq <= 0 || !(scale > 0.0f) || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
         return Q3_ERR_BAD_SIZE;                                                      // (the maximum is taken before the scale)
     if (n_pages * nkv * PAGE > 0x7fffffff) return Q3_ERR_TOO_LARGE;                  // a row's number is a coordinate of a copy
-    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts)) return Q3_ERR_MISALIGNED;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
+        return Q3_ERR_MISALIGNED;
     const Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new},
                     (const bf16*)q, (bf16*)out, (const unsigned char*)k_pages, (const unsigned char*)v_pages, (const uint8_t*)k_scales,
                     (const uint8_t*)v_scales, parts, status, scale * 1.4426950408889634f};
