@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     pdl_wait();
     const TreeStep& st = a.step;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    using Work = TreeWork<PAGE, ROWS>;
+    using Work = TreeWork<PAGE, ROWS, false>;
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
             }
         }
         __syncthreads();                                             // the buffers are free for the next part
-        at = Work::next(share, at, part);
+        at = Work::next(part);
     }
 }
 
@@ -576,7 +576,7 @@ template <bool F8, int NT> int launch(const Args& a, int sm_count, cudaStream_t 
     static_assert(blocks_per_sm<NT> * (bytes + 1024) <= 228 * 1024, "shared memory of an SM");
     const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, NT>, bytes, configured);
     if (e != cudaSuccess) return (int)e;
-    using Work = TreeWork<PAGE, 8 * NT>;
+    using Work = TreeWork<PAGE, 8 * NT, false>;
     const int64_t units = Work::most_units(a.step), most = (units + LEAST_PAGES - 1) / LEAST_PAGES + Work::most_items(a.step);
     if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
     const int resident = blocks_per_sm<NT> * sm_count, grid = (int)(most < resident ? most : resident);

@@ -1,19 +1,19 @@
 // Attention of a step's new tokens over the cache's pages in bfloat16 or in 8 bits on the 5th-generation tensor cores, for trees (or runs) whose
 // rows - a row is a token and a query head - fill tiles of 128.  What a token sees and what comes out is said in attention_tree.cu.
 //
-// S = Q K^T and O += P V are tcgen05.mma with the queries, the weights and the accumulators in tensor memory and a page of 64 keys or values in shared
-// memory.  (With the queries in shared memory a product of 128 x 128 x 16 took 130 cycles instead of 64: both operands together are what the tensor core can
-// read of shared memory in its whole time.)  A block, one an SM, works on two tiles side by side, so that the products of one run under the softmax of the other:
+// S = Q K^T and O += P V are tcgen05.mma over a page of 64 keys, with the accumulators and the weights in tensor memory.  A tile has two buffers of scores there, so
+// that a page's scores are made while the softmax is at the page before: its chain is then the softmax alone.  (With the queries in tensor memory, which leaves
+// room for one buffer, products of 128 x 64 x 16 take 33 cycles instead of 51, but scores wait for the products before them: 2,750 cycles a page.)
+// A block, one an SM, works on two tiles side by side, so that the products of one run under the softmax of the other:
 //   more than 128 rows   two tiles of 128 rows, which take the same pages;
 //   up to 128 rows       twice the same rows, one tile with the pages of even number and one with those of odd number; their sums meet at the end.
 // The pages of all items are shared out evenly over the blocks (tree_work.cuh).
-//   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It puts its query there, reads its 64 scores, writes the weights over them, and
+//   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It brings in its query, reads its 64 scores, writes the weights over them, and
 //                rescales O when the maximum is raised by more than 2^8.  At the end of a part it writes the row, or its share of it for the second
 //                kernel to add up.
 //   warps 8-15   8 bits: turn the codes of keys (8-11) and values (12-15) into half precision, which holds them exactly, where TMA would have put them.
-//   warp 16      issues the products, one elected thread: whatever is ready, of either tile.
+//   warps 16, 19 issue the products, one elected thread of each those of a tile.
 //   warps 17, 18 copy keys and values: bfloat16 by TMA where the products read them, 8 bits as they lie, some pages ahead.
-//   (Warp 19 makes its group of four whole, which registers are handed out to.)
 //
 // 8 bits.  A page's keys are brought to one scale, that of its first row, 2^k0, by folding 2^(k - k0) into the half-precision numbers, which is exact
 // for k - k0 in -14 .. 7; so are its values.  Scores are then multiplied by 2^k0 with the softmax's own scale; v0 is added to the scores in log2 units, so
@@ -48,7 +48,9 @@ static_assert(8 * 32 * SOFTMAX_REGS + 8 * 32 * TURN_REGS + 4 * 32 * MMA_REGS <= 
 constexpr int NOTES = 8;                                  // pages whose notes are kept: more than lie between the copies and the softmax
 constexpr int PANEL_BYTES = PAGE * 128, TILE_BYTES = HALVES * PANEL_BYTES;                 // 64 rows of 128 bytes; a page's keys or values in 16 bits
 constexpr int CODE_BYTES = PAGE * D;
-constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, COL_S = 0, COL_Q = 64, COL_O = 128;   // of tile x, from x * 256 on; P lies over S
+constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, COL_S = 0, COL_O = 128;              // of tile x, from x * 256 on; two buffers of S, P lies over S
+constexpr int Q_BYTES = HALVES * BM * 128, MEET_COLS = D / 2;                             // a tile's queries; columns of the sums that meet at a time
+static_assert(BM * MEET_COLS * 4 <= Q_BYTES, "they meet where the second tile's queries would be");
 constexpr float RAISE = 8.0f;
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
@@ -61,10 +63,10 @@ struct Note {                                             // what is noted of a 
 template <bool F8> struct Layout {
     static constexpr int STAGES = F8 ? 3 : 4;             // pages of keys and of values that the products can read
     static constexpr int CODES = F8 ? 3 : 0;              // pages of codes of either on their way
-    static constexpr int K = 0, V = STAGES * TILE_BYTES, K_CODES = 2 * STAGES * TILE_BYTES, V_CODES = K_CODES + CODES * CODE_BYTES;
-    static constexpr int MEET = V_CODES + CODES * CODE_BYTES, REST = MEET + BM * D * 4;
+    static constexpr int QUERIES = 0, MEET = Q_BYTES, K = 2 * Q_BYTES, V = K + STAGES * TILE_BYTES;
+    static constexpr int K_CODES = V + STAGES * TILE_BYTES, V_CODES = K_CODES + CODES * CODE_BYTES, REST = V_CODES + CODES * CODE_BYTES;
     // barriers: one word of 8 bytes each
-    static constexpr int Q = 0, S_FULL = 1, P_FULL = 3, PV_DONE = 5, NOTED = 7, K_FULL = NOTED + NOTES, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES;
+    static constexpr int Q = 0, S_FULL = 1, P_FULL = 5, PV_DONE = 9, NOTED = 11, K_FULL = NOTED + NOTES, K_EMPTY = K_FULL + STAGES, V_FULL = K_EMPTY + STAGES;
     static constexpr int V_EMPTY = V_FULL + STAGES, V_HERE = V_EMPTY + STAGES;             // V_HERE: TMA's values, before they are looked through
     static constexpr int KC_FULL = V_HERE + STAGES, KC_EMPTY = KC_FULL + CODES, VC_FULL = KC_EMPTY + CODES, VC_EMPTY = VC_FULL + CODES;
     static constexpr int MET = VC_EMPTY + CODES, MET_FREE = MET + 1, BARS = MET + 2;       // the sums of odd pages lie in MEET; they are read
@@ -92,7 +94,7 @@ struct Args {
     float scale_log2;
 };
 
-using Work = TreeWork<PAGE, ROWS>;
+using Work = TreeWork<PAGE, ROWS, true>;
 
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r) {
     asm volatile(
@@ -159,16 +161,6 @@ __device__ __forceinline__ int64_t page_of(const TreeStep& st, const int* table,
     return p >= 0 && p < st.n_pages ? p : 0;
 }
 
-// Whether a phase is complete, for a whole converged warp; does not wait.
-__device__ __forceinline__ bool mbar_passed_warp(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, done);
-}
 // Bytes from global memory as they lie (all a multiple of 16).
 __device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -220,20 +212,22 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(bar(L::Q, 0), SOFTMAX_WARPS);
+        mbar_init(bar(L::Q, 0), SOFTMAX_WARPS + 2);      // (with the warps that wait for it: it cannot be two parts ahead of them)
         mbar_init(bar(L::MET, 0), 4);
         mbar_init(bar(L::MET_FREE, 0), 4);
         for (int x = 0; x < 2; ++x) {
-            mbar_init(bar(L::S_FULL, x), 1);
-            mbar_init(bar(L::P_FULL, x), 4);
+            for (int b = 0; b < 2; ++b) {                // of a tile's two buffers
+                mbar_init(bar(L::S_FULL, 2 * x + b), 1);
+                mbar_init(bar(L::P_FULL, 2 * x + b), 4);
+            }
             mbar_init(bar(L::PV_DONE, x), 1);
         }
         for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), F8 ? 2 * TURN_WARPS : TURN_WARPS);
         for (int s = 0; s < L::STAGES; ++s) {
             mbar_init(bar(L::K_FULL, s), F8 ? TURN_WARPS : 1);
-            mbar_init(bar(L::K_EMPTY, s), 1);
+            mbar_init(bar(L::K_EMPTY, s), 2);
             mbar_init(bar(L::V_FULL, s), TURN_WARPS);
-            mbar_init(bar(L::V_EMPTY, s), 1);
+            mbar_init(bar(L::V_EMPTY, s), 2);
             mbar_init(bar(L::V_HERE, s), 1);
         }
         for (int s = 0; s < L::CODES; ++s) {
@@ -270,7 +264,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;                         // tile, row of it
         const uint32_t t_tile = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * TILE_COLS;
         int page0 = 0;                                                               // pages of this block before the part
-        uint32_t turn = 0, q_turn = 0, met_turn = 0;                                 // of this tile's barriers, of the parts, of those in which the tiles meet
+        uint32_t count = 0, q_turn = 0, met_turn = 0;                                // pages of this tile so far; parities of the parts, of the tiles' meetings
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
@@ -280,7 +274,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const int first = split ? x : 0, stride = split ? 2 : 1;
             const int rows = split ? all_rows : all_rows - x * BM, row = part.tile * ROWS + (split ? 0 : x * BM) + r, own = min(row / group, n_new - 1);
             const int64_t row_at = ((int64_t)(t0 + own) * st.nq + part.head * group + row % group) * D;
-            // ---- this row's query, into tensor memory
+            // ---- this row's query (twice the same rows: both tiles' products read the first one's)
             float factor = a.scale_log2;
             {
                 const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
@@ -299,27 +293,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     down = q3_exp2i(-e2);
                     factor *= q3_exp2i(e2);
                 }
+                if (!(split && x == 1)) {
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    uint32_t v[32];
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint4 w = src[c];
+                        if constexpr (F8) {
+                            uint32_t* v = &w.x;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint4 w = src[8 * c + i];
-                        v[4 * i] = w.x; v[4 * i + 1] = w.y; v[4 * i + 2] = w.z; v[4 * i + 3] = w.w;
+                            for (int e = 0; e < 4; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
+                        }
+                        if (r >= rows) w = make_uint4(0, 0, 0, 0);
+                        st_shared_v4(base + L::QUERIES + x * Q_BYTES + chunk_at(r, c, BM * 128), w);
                     }
-                    if constexpr (F8) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
-                    }
-                    if (r >= rows) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = 0u;
-                    }
-                    __syncwarp();
-                    tc_st32(t_tile + COL_Q + 32 * c, v);
+                    fence_proxy_async();
                 }
-                tc_wait_st();
-                tc_fence_before();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::Q, 0));
@@ -329,10 +316,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             odd.any = false;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) odd.plus[i] = odd.minus[i] = 0u;
-            for (int n = first; n < steps; n += stride) {
+            for (int n = first; n < steps; n += stride, ++count) {
                 const int key0 = (part.begin + n) * PAGE, number = page0 + n, note = number % NOTES;
+                const uint32_t buffer = count & 1u, turn = count >> 1 & 1u, t_s = t_tile + COL_S + buffer * 64;
                 const bool edge = key0 + PAGE > pos0;                                // some key is a new token's, or behind the end
-                ok = mbar_wait_warp(bar(L::S_FULL, x), turn);
+                ok = mbar_wait_warp(bar(L::S_FULL, 2 * x + buffer), turn);
                 if (!ok) { failed(41); break; }
                 if (F8 || edge) {
                     ok = mbar_wait_warp(bar(L::NOTED, note), turn_of(number, NOTES));
@@ -340,8 +328,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 }
                 tc_fence_after();
                 uint32_t s[64];
-                tc_ld32(t_tile + COL_S, s);
-                tc_ld32(t_tile + COL_S + 32, s + 32);
+                tc_ld32(t_s, s);
+                tc_ld32(t_s + 32, s + 32);
                 // ---- of the page: score = dot * c1, in log2 units, and v0
                 float c1 = factor, v0 = 0.0f;
                 bool rests = false;
@@ -425,9 +413,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 l_run += F8 ? total * ex2(-v0) : total;
                 __syncwarp();
-                tc_st32(t_tile + COL_S, p);
-                if (n > first && __any_sync(0xffffffffu, raise)) {
-                    // (the products of the page before are done: this page's scores were asked for after them)
+                tc_st32(t_s, p);
+                // the products of the page before have to be done where O is rescaled, and once the part ends: this page's are waited for then, and a
+                // parity tells a phase from the next one, not from the one after that
+                const bool rescale = n > first && __any_sync(0xffffffffu, raise);
+                if (rescale || (n > first && n + stride >= steps)) {
+                    ok = mbar_wait_warp(bar(L::PV_DONE, x), (count - 1) & 1u);
+                    if (!ok) { failed(37); break; }
+                    tc_fence_after();
+                }
+                if (rescale) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 64) {
                         tc_ld32(t_tile + COL_O + c, s);
@@ -442,12 +437,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(L::P_FULL, x));
-                turn ^= 1u;
+                if (lane == 0) mbar_arrive(bar(L::P_FULL, 2 * x + buffer));
             }
             if (!ok) break;
-            // the part's last products (turn: as many as there were pages); a tile without pages goes on with the other one's warps, not ahead of them
-            ok = first < steps ? mbar_wait_warp(bar(L::PV_DONE, x), turn ^ 1u) : mbar_wait_warp(bar(L::Q, 0), q_turn);
+            // the part's last products; a tile without pages goes on with the other one's warps, not ahead of them
+            ok = first < steps ? mbar_wait_warp(bar(L::PV_DONE, x), (count - 1) & 1u) : mbar_wait_warp(bar(L::Q, 0), q_turn);
             q_turn ^= 1u;
             if (!ok) { failed(43); break; }
             tc_fence_after();
@@ -456,99 +450,90 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             float* const dst = a.parts + (int64_t)part.slot * PART;
             const int part_row = split ? r : x * BM + r;
             float mine = 1.0f, other = 0.0f;                                         // factors of the two tiles' sums
-            float4* const meet = reinterpret_cast<float4*>(smem + L::MEET);          // [D / 4][BM]
-            if (split) {
-                if (x == 1) {
-                    ok = mbar_wait_warp(bar(L::MET_FREE, 0), met_turn ^ 1u);
-                    if (!ok) { failed(39); break; }
-                    sh.meet[r] = make_float2(m_run, l_run);
-                    if (steps > 1 && (warp & 3) * 32 < rows) {
+            float4* const meet = reinterpret_cast<float4*>(smem + L::MEET);          // [MEET_COLS / 4][BM]
+            if (split && x == 1) sh.meet[r] = make_float2(m_run, l_run);
+            const bool here = (warp & 3) * 32 < rows;                                // some row of the warp's is one
+            float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            __syncwarp();
-                            tc_ld32(t_tile + COL_O + c, o);
-                            tc_wait_ld();
-                            if (odd.any) {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) {
-                                    if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
-                                    if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
-                                }
-                            }
-#pragma unroll
-                            for (int e = 0; e < 32; e += 4)
-                                meet[(c + e) / 4 * BM + r] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
-                        }
-                    }
-                }
-                if (x == 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(L::MET, 0));
-                } else {
-                    ok = mbar_wait_warp(bar(L::MET, 0), met_turn);
+            for (int c0 = 0; c0 < D; c0 += MEET_COLS) {
+                if (split) {
+                    ok = x == 1 ? mbar_wait_warp(bar(L::MET_FREE, 0), met_turn ^ 1u) : mbar_wait_warp(bar(L::MET, 0), met_turn);
                     if (!ok) { failed(38); break; }
-                    const float2 ml = sh.meet[r];
-                    const float m = fmaxf(m_run, ml.x);
-                    mine = m_run == m ? 1.0f : ex2(m_run - m);
-                    other = ml.x == m ? 1.0f : ex2(ml.x - m);
-                    m_run = m;
-                    l_run = fmaf(ml.y, other, l_run * mine);
+                    if (x == 0 && c0 == 0) {
+                        const float2 ml = sh.meet[r];
+                        const float m = fmaxf(m_run, ml.x);
+                        mine = m_run == m ? 1.0f : ex2(m_run - m);
+                        other = ml.x == m ? 1.0f : ex2(ml.x - m);
+                        m_run = m;
+                        l_run = fmaf(ml.y, other, l_run * mine);
+                        inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+                    }
                 }
-            }
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-            if (!(split && x == 1) && (warp & 3) * 32 < rows) {
+                if (here && !(split && x == 1 && steps == 1)) {
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    __syncwarp();
-                    tc_ld32(t_tile + COL_O + c, o);
-                    tc_wait_ld();
-                    if (odd.any) {
+                    for (int c = c0; c < c0 + MEET_COLS; c += 32) {
+                        uint32_t o[32];
+                        __syncwarp();
+                        tc_ld32(t_tile + COL_O + c, o);
+                        tc_wait_ld();
+                        if (odd.any) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
-                            if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
-                        }
-                    }
-                    if (split && steps > 1) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            const float4 u = meet[(c + e) / 4 * BM + r];
-                            o[e] = __float_as_uint(fmaf(u.x, other, __uint_as_float(o[e]) * mine));
-                            o[e + 1] = __float_as_uint(fmaf(u.y, other, __uint_as_float(o[e + 1]) * mine));
-                            o[e + 2] = __float_as_uint(fmaf(u.z, other, __uint_as_float(o[e + 2]) * mine));
-                            o[e + 3] = __float_as_uint(fmaf(u.w, other, __uint_as_float(o[e + 3]) * mine));
-                        }
-                    }
-                    if (r < rows) {
-                        if (whole) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint4 v;
-                                v.x = pack2<false>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                                v.y = pack2<false>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                                v.z = pack2<false>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                                v.w = pack2<false>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                                *reinterpret_cast<uint4*>(a.out + row_at + c + e) = v;
+                            for (int e = 0; e < 32; ++e) {
+                                if (odd.plus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) + INFINITY);
+                                if (odd.minus[c / 32] >> e & 1u) o[e] = __float_as_uint(__uint_as_float(o[e]) - INFINITY);
                             }
-                        } else {
+                        }
+                        if (split && x == 1) {
 #pragma unroll
                             for (int e = 0; e < 32; e += 4)
-                                *reinterpret_cast<uint4*>(dst + ((c + e) / 4 * ROWS + part_row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                                meet[(c - c0 + e) / 4 * BM + r] =
+                                    make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                            continue;
+                        }
+                        if (split && steps > 1) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                const float4 u = meet[(c - c0 + e) / 4 * BM + r];
+                                o[e] = __float_as_uint(fmaf(u.x, other, __uint_as_float(o[e]) * mine));
+                                o[e + 1] = __float_as_uint(fmaf(u.y, other, __uint_as_float(o[e + 1]) * mine));
+                                o[e + 2] = __float_as_uint(fmaf(u.z, other, __uint_as_float(o[e + 2]) * mine));
+                                o[e + 3] = __float_as_uint(fmaf(u.w, other, __uint_as_float(o[e + 3]) * mine));
+                            }
+                        }
+                        if (r < rows) {
+                            if (whole) {
+#pragma unroll
+                                for (int e = 0; e < 32; e += 8) {
+                                    uint4 v;
+                                    v.x = pack2<false>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                                    v.y = pack2<false>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                                    v.z = pack2<false>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+                                    v.w = pack2<false>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+                                    *reinterpret_cast<uint4*>(a.out + row_at + c + e) = v;
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+                                    *reinterpret_cast<uint4*>(dst + ((c + e) / 4 * ROWS + part_row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            }
                         }
                     }
                 }
-                if (!whole && r < rows) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * part_row) = make_float2(m_run, l_run);
+                if (split) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(x == 1 ? L::MET : L::MET_FREE, 0));
+                    met_turn ^= 1u;
+                }
             }
+            if (!ok) break;
+            if (split && x == 1) {                                                   // all is read: queries may come here again
+                ok = mbar_wait_warp(bar(L::MET_FREE, 0), met_turn ^ 1u);
+                if (!ok) { failed(39); break; }
+            }
+            if (!whole && r < rows && !(split && x == 1)) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * part_row) = make_float2(m_run, l_run);
             tc_fence_before();
-            if (split) {
-                __syncwarp();
-                if (x == 0 && lane == 0) mbar_arrive(bar(L::MET_FREE, 0));
-                met_turn ^= 1u;
-            }
             page0 += steps;
-            at = Work::next(share, at, part);
+            at = Work::next(part);
         }
     } else if (warp < MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TURN_REGS));
@@ -669,92 +654,86 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
             }
-            at = Work::next(share, at, part);
+            at = Work::next(part);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MMA_REGS));
-        if (warp == MMA_WARP) {
-            // ------------------------------------------------ the products: the whole warp walks and one elected thread issues
+        if (warp == MMA_WARP || warp == MMA_WARP + 3) {
+            // ------------------------------------------------ the products of a tile: the whole warp walks and one elected thread issues
             constexpr uint32_t idesc_s = idesc(F8, BM, PAGE, false), idesc_pv = idesc(F8, BM, D, true);
-            const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint64_t k_desc = desc_k_major(base + L::K), v_desc = desc_mn_major(base + L::V, PANEL_BYTES);
-            int page0 = 0;
-            uint32_t q_turn = 0, p_turn = 0, pv_turn = 0;                            // parities; of the tiles: bit x
+            const int x = warp == MMA_WARP ? 0 : 1;
+            const uint32_t acc = __shfl_sync(0xffffffffu, tmem, 0) + x * TILE_COLS;
+            const uint64_t q_desc = desc_k_major(base + L::QUERIES), k_desc = desc_k_major(base + L::K), v_desc = desc_mn_major(base + L::V, PANEL_BYTES);
+            uint32_t q_turn = 0, count = 0;                                          // parity of the parts; this tile's pages so far
+            // the stage of a page and its turn, counted along
+            struct Place { uint32_t stage, turn; } k_at = {0, 0}, v_at = {0, 0};
+            auto step_on = [](Place& at, int by) {
+                at.stage += by;
+                while (at.stage >= L::STAGES) {
+                    at.stage -= L::STAGES;
+                    at.turn ^= 1u;
+                }
+            };
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
                 const TreePart part = Work::part(st, share, at, blockIdx.x);
                 const bool split = Work::n_new(st, part.seq) * group - part.tile * ROWS <= BM;
-                const int steps = part.end - part.begin, stride = split ? 2 : 1;
-                uint32_t k_used = 0, v_used = 0;                                     // stages that one of two tiles has read
-                int next[2] = {0, split ? 1 : 0};                                    // a tile's page: whose scores come next, or (waiting) whose weights do
-                uint32_t waits = 0;                                                  // bit x: tile x waits for its weights; bit 2 + x: for its products to end
+                const int steps = part.end - part.begin, first = split ? x : 0, stride = split ? 2 : 1;
+                auto scores = [&](uint32_t buffer) {                                 // of the page at k_at
+                    if (!mbar_wait_warp(bar(L::K_FULL, k_at.stage), k_at.turn)) return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t q_src = q_desc + (uint64_t)((split ? 0 : x) * (Q_BYTES >> 4)), k_src = k_desc + (uint64_t)(k_at.stage * (TILE_BYTES >> 4));
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            tc_mma_ss(acc + COL_S + buffer * 64, q_src + (uint64_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+                                      k_src + (uint64_t)(((kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+                        tc_commit(bar(L::S_FULL, 2 * x + buffer));
+                        tc_commit(bar(L::K_EMPTY, k_at.stage));                      // (both tiles' have to be done, or this one's twice)
+                        if (split) tc_commit(bar(L::K_EMPTY, k_at.stage));
+                    }
+                    __syncwarp();
+                    step_on(k_at, stride);
+                    return true;
+                };
+                Place k_next = k_at, v_next = v_at;                                  // behind this part
+                step_on(k_next, steps % (2 * L::STAGES));
+                step_on(v_next, steps % (2 * L::STAGES));
+                step_on(k_at, first);
+                step_on(v_at, first);
+                if (lane == 0) mbar_arrive(bar(L::Q, 0));
                 ok = mbar_wait_warp(bar(L::Q, 0), q_turn);
                 q_turn ^= 1u;
-                if (!ok) { failed(47); break; }
                 tc_fence_after();
-                uint32_t idle = 0;
-                while ((next[0] < steps || next[1] < steps) && ok) {
-                    bool some = false;
+                for (int b = 0; b < 2 && ok; ++b)
+                    if (first + b * stride < steps) ok = scores((count + b) & 1u);
+                if (!ok) { failed(47); break; }
+                for (int n = first; n < steps; n += stride, ++count) {
+                    const uint32_t buffer = count & 1u;
+                    // what is there long before is waited for first
+                    ok = mbar_wait_warp(bar(L::V_FULL, v_at.stage), v_at.turn) && mbar_wait_warp(bar(L::P_FULL, 2 * x + buffer), count >> 1 & 1u);
+                    if (!ok) { failed(48); break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t v_src = v_desc + (uint64_t)(v_at.stage * (TILE_BYTES >> 4));
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        if (next[x] >= steps) continue;
-                        const int number = page0 + next[x];
-                        const uint32_t stage = (uint32_t)number % L::STAGES, turn = turn_of(number, L::STAGES);
-                        if (waits & (1u << x)) {
-                            if (!mbar_passed_warp(bar(L::P_FULL, x), p_turn >> x & 1u) || !mbar_passed_warp(bar(L::V_FULL, stage), turn)) continue;
-                            p_turn ^= 1u << x;
-                            const bool release = split || (v_used >> stage & 1u);
-                            v_used ^= split ? 0u : 1u << stage;
-                            tc_fence_after();
-                            if (elect_one()) {
-#pragma unroll
-                                for (int kk = 0; kk < PAGE / 16; ++kk)
-                                    tc_mma_ts(acc + x * TILE_COLS + COL_O, acc + x * TILE_COLS + COL_S + kk * 8,
-                                              v_desc + (uint64_t)((stage * TILE_BYTES + kk * 16 * 128) >> 4), idesc_pv, (next[x] >= stride || kk > 0) ? 1u : 0u);
-                                tc_commit(bar(L::PV_DONE, x));
-                                if (release) tc_commit(bar(L::V_EMPTY, stage));
-                            }
-                            __syncwarp();
-                            waits ^= 5u << x;
-                            next[x] += stride;
-                            some = true;
-                            // the part's last products are nobody's to wait for here
-                            if (next[x] >= steps) {
-                                waits &= ~(4u << x);
-                                pv_turn ^= 1u << x;
-                            }
-                        } else {
-                            if (waits & (4u << x)) {
-                                // the next scores go where the weights were: once the products with them are done
-                                if (!mbar_passed_warp(bar(L::PV_DONE, x), pv_turn >> x & 1u)) continue;
-                                waits ^= 4u << x;
-                                pv_turn ^= 1u << x;
-                            }
-                            if (!mbar_passed_warp(bar(L::K_FULL, stage), turn)) continue;
-                            const bool release = split || (k_used >> stage & 1u);
-                            k_used ^= split ? 0u : 1u << stage;
-                            tc_fence_after();
-                            if (elect_one()) {
-#pragma unroll
-                                for (int kk = 0; kk < D / 16; ++kk)
-                                    tc_mma_ts(acc + x * TILE_COLS + COL_S, acc + x * TILE_COLS + COL_Q + kk * 8,
-                                              k_desc + (uint64_t)((stage * TILE_BYTES + (kk >> 2) * PANEL_BYTES + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
-                                tc_commit(bar(L::S_FULL, x));
-                                if (release) tc_commit(bar(L::K_EMPTY, stage));
-                            }
-                            __syncwarp();
-                            waits |= 1u << x;
-                            some = true;
-                        }
+                        for (int kk = 0; kk < PAGE / 16; ++kk)
+                            tc_mma_ts(acc + COL_O, acc + COL_S + buffer * 64 + kk * 8, v_src + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv, (n >= stride || kk > 0) ? 1u : 0u);
+                        tc_commit(bar(L::PV_DONE, x));
+                        tc_commit(bar(L::V_EMPTY, v_at.stage));
+                        if (split) tc_commit(bar(L::V_EMPTY, v_at.stage));
                     }
-                    idle = some ? 0 : idle + 1;
-                    if (idle > Q3_WAIT_LIMIT) {
-                        ok = false;
-                        failed(48);
+                    __syncwarp();
+                    step_on(v_at, stride);
+                    if (n + 2 * stride < steps) {
+                        // the scores of the page after the next go where these weights were, once the products with them are done
+                        ok = mbar_wait_warp(bar(L::PV_DONE, x), count & 1u) && scores(buffer);
+                        if (!ok) { failed(51); break; }
                     }
                 }
-                page0 += steps;
-                at = Work::next(share, at, part);
+                k_at = k_next;
+                v_at = v_next;
+                at = Work::next(part);
             }
         } else if (warp == K_COPY_WARP || warp == V_COPY_WARP) {
             // ------------------------------------------------ copies of the keys, of the values
@@ -791,7 +770,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     __syncwarp();
                 }
-                at = Work::next(share, at, part);
+                at = Work::next(part);
             }
         }
     }
@@ -805,7 +784,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 
 // ---- the parts of the items that several blocks share, added up in their order: for every block of the first kernel whose last part is the first one of such
 // an item, and for 32 of its rows, a block
-__global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constant__ Args a, int blocks) {
+constexpr int MERGE_THREADS = D / 8 * 32;
+__global__ void __launch_bounds__(MERGE_THREADS) tree_tc_merge_kernel(const __grid_constant__ Args a, int blocks) {
     __shared__ TreeShare shared_share;
     pdl_launch_dependents();
     pdl_wait();
@@ -819,7 +799,7 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
     TreeShare share = shared_share;
     if (share.from >= share.to) return;
     TreePart part;
-    for (int at = share.from; at < share.to; at = Work::next(share, at, part)) part = Work::part(st, share, at, b0);
+    for (int at = share.from; at < share.to; at = Work::next(part)) part = Work::part(st, share, at, b0);
     if (part.parts == 1 || part.begin != 0) return;
     const int group = st.nq / st.nkv, t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq);
     const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0), first = blockIdx.y * 32;
@@ -827,31 +807,41 @@ __global__ void __launch_bounds__(256) tree_tc_merge_kernel(const __grid_constan
     const int r = first + (threadIdx.x & 31);
     if (r >= rows) return;
     bf16* const out = a.out + ((int64_t)(t0 + (row0 + r) / group) * st.nq + part.head * group + (row0 + r) % group) * D;
-    for (int c = threadIdx.x >> 5; c < D / 8; c += 8) {                              // eight values a turn
-        float m = -INFINITY, l = 0.0f, v[8];
+    const int c = threadIdx.x >> 5;                                                  // eight values a warp
+    float m = -INFINITY, l = 0.0f, v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-        for (int b = 0; b < part.parts; ++b) {
-            const float* src = a.parts + (int64_t)part.slot_of(b) * PART;
-            const float2 ml = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * r);
-            const float4 u0 = *reinterpret_cast<const float4*>(src + ((2 * c) * ROWS + r) * 4), u1 = *reinterpret_cast<const float4*>(src + ((2 * c + 1) * ROWS + r) * 4);
-            const float m2 = fmaxf(m, ml.x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml.x == m2 ? 1.0f : ex2(ml.x - m2);
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    constexpr int AT_ONCE = 4;                                                       // parts asked for together
+    for (int b0 = 0; b0 < part.parts; b0 += AT_ONCE) {
+        float2 ml[AT_ONCE];
+        float4 u[AT_ONCE][2];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const float* src = a.parts + (int64_t)part.slot_of(min(b0 + k, part.parts - 1)) * PART;
+            ml[k] = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * r);
+            u[k][0] = *reinterpret_cast<const float4*>(src + ((2 * c) * ROWS + r) * 4);
+            u[k][1] = *reinterpret_cast<const float4*>(src + ((2 * c + 1) * ROWS + r) * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (b0 + k >= part.parts) break;
+            const float m2 = fmaxf(m, ml[k].x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml[k].x == m2 ? 1.0f : ex2(ml[k].x - m2);
             m = m2;
-            l = fmaf(now, ml.y, l * was);
+            l = fmaf(now, ml[k].y, l * was);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = fmaf(now, (&u0.x)[e], v[e] * was);
-                v[e + 4] = fmaf(now, (&u1.x)[e], v[e + 4] * was);
+                v[e] = fmaf(now, (&u[k][0].x)[e], v[e] * was);
+                v[e + 4] = fmaf(now, (&u[k][1].x)[e], v[e + 4] * was);
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint4 w;
-        w.x = pack2<false>(v[0] * inv, v[1] * inv);
-        w.y = pack2<false>(v[2] * inv, v[3] * inv);
-        w.z = pack2<false>(v[4] * inv, v[5] * inv);
-        w.w = pack2<false>(v[6] * inv, v[7] * inv);
-        *reinterpret_cast<uint4*>(out + 8 * c) = w;
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint4 w;
+    w.x = pack2<false>(v[0] * inv, v[1] * inv);
+    w.y = pack2<false>(v[2] * inv, v[3] * inv);
+    w.z = pack2<false>(v[4] * inv, v[5] * inv);
+    w.w = pack2<false>(v[6] * inv, v[7] * inv);
+    *reinterpret_cast<uint4*>(out + 8 * c) = w;
 }
 
 template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
@@ -869,7 +859,7 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
     int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)smem_bytes<F8>, stream, map_k, map_v, a);
     if (code != 0) return code;
     const int rows = (int64_t)max_new * (a.step.nq / a.step.nkv) < ROWS ? max_new * (a.step.nq / a.step.nkv) : ROWS;
-    return (int)q3_launch(tree_tc_merge_kernel, dim3(blocks, (rows + 31) / 32), dim3(256), 0, stream, a, blocks);
+    return (int)q3_launch(tree_tc_merge_kernel, dim3(blocks, (rows + 31) / 32), dim3(MERGE_THREADS), 0, stream, a, blocks);
 }
 
 }  // namespace

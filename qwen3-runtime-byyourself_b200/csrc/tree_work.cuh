@@ -26,6 +26,7 @@ struct TreePart {
     int seq, head, tile;                           // head: the kv head
     int begin, end, item;                          // item: its number among the items
     int parts, slot, slot0, first_block;           // of the item: how many; this one's place in the scratch, the first one's, and the first one's block
+    int list_end;                                  // where the block's share goes on
 
     // The place of the item's part i in the scratch (a block has two: of the part that it begins with, and of the one that it ends with).
     __device__ __forceinline__ int slot_of(int i) const { return i == 0 ? slot0 : 2 * (first_block + i); }
@@ -38,17 +39,37 @@ struct TreeShare {
     int seq, before, items_before;                 // where `from` (a piece: the block's number) lies: its sequence, the stretches (pieces) and items before it
 };
 
-// UNIT: keys of a stretch; ROWS: rows of a tile.
-template <int UNIT, int ROWS> struct TreeWork {
-    static __device__ __forceinline__ int n_new(const TreeStep& a, int seq) { return max(0, min(a.seq_start[seq + 1] - a.seq_start[seq], a.max_new)); }
-    static __device__ __forceinline__ int units(const TreeStep& a, int seq, int n) {
-        return n == 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT;
-    }
-    static __host__ __device__ __forceinline__ int tiles_of(int n_new, int group) { return (int)(((int64_t)n_new * group + ROWS - 1) / ROWS); }
+// What of a sequence counts in the list: its items, in the order of their heads and tiles, of so many stretches each.  With LIGHT a stretch of a tile of at most
+// half the rows (the last one of a head) costs half of another's: lengths are then counted in halves, those of light items rounded up to whole ones.
+struct TreeItems {
+    int units, per_head, light;                    // stretches of an item, tiles of a head, whether the last one is light (0 or 1)
+    int full, lighter;                             // the lengths
 
-    // The most items and stretches that a step can have (the latter have to stay below 2^31).
+    __device__ __forceinline__ int cut(int length, int quota) const { return (int)((unsigned)(length + quota - 1) / (unsigned)quota); }
+    // A head's length, or its pieces of up to `quota`.
+    __device__ __forceinline__ int of_head() const { return (per_head - light) * full + light * lighter; }
+    __device__ __forceinline__ int pieces_of_head(int quota) const { return units == 0 ? 0 : (per_head - light) * cut(full, quota) + (light ? cut(lighter, quota) : 0); }
+};
+
+// UNIT: keys of a stretch; ROWS: rows of a tile.
+template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
+    static constexpr int COUNT = LIGHT ? 2 : 1;    // of a stretch
+    static __device__ __forceinline__ int n_new(const TreeStep& a, int seq) { return max(0, min(a.seq_start[seq + 1] - a.seq_start[seq], a.max_new)); }
+    static __host__ __device__ __forceinline__ int tiles_of(int n_new, int group) { return (int)(((int64_t)n_new * group + ROWS - 1) / ROWS); }
+    static __device__ __forceinline__ TreeItems items_of(const TreeStep& a, int seq) {
+        TreeItems t;
+        const int n = n_new(a, seq), group = a.nq / a.nkv;
+        t.units = n == 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT;
+        t.per_head = t.units > 0 ? tiles_of(n, group) : 0;
+        t.light = LIGHT && t.per_head > 0 && n * group - (t.per_head - 1) * ROWS <= ROWS / 2 ? 1 : 0;
+        t.full = t.units * COUNT;
+        t.lighter = (t.units + 1) & ~1;
+        return t;
+    }
+
+    // The most items and counted stretches that a step can have (the latter have to stay below 2^30).
     static __host__ int64_t most_items(const TreeStep& a) { return (int64_t)a.n_seqs * a.nkv * tiles_of(a.max_new, a.nq / a.nkv); }
-    static __host__ int64_t most_units(const TreeStep& a) { return most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT); }
+    static __host__ int64_t most_units(const TreeStep& a) { return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT); }
 
     static __device__ __forceinline__ int warp_total(int v) {
 #pragma unroll
@@ -58,32 +79,28 @@ template <int UNIT, int ROWS> struct TreeWork {
 
     // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more).
     static __device__ TreeShare share(const TreeStep& a, int least, int block, int blocks) {
-        const int lane = threadIdx.x & 31, group = a.nq / a.nkv;
+        const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
-        const int mine_new = few && lane < a.n_seqs ? n_new(a, lane) : 0, mine_units = few && lane < a.n_seqs ? units(a, lane, mine_new) : 0;
-        const int mine_items = mine_units > 0 ? tiles_of(mine_new, group) * a.nkv : 0;
-        auto each = [&](auto f) {                                        // sum over the sequences of f(units, items)
+        const TreeItems none = {0, 0, 0, 0, 0}, mine = few && lane < a.n_seqs ? items_of(a, lane) : none;
+        auto each = [&](auto f) {                                        // sum over the sequences, for a head
             int sum = 0;
-            if (few) sum = f(mine_units, mine_items);
+            if (few) sum = f(mine);
             else
-                for (int s = lane; s < a.n_seqs; s += 32) {
-                    const int n = n_new(a, s), u = units(a, s, n);
-                    if (u > 0) sum += f(u, tiles_of(n, group) * a.nkv);
-                }
-            return warp_total(sum);
+                for (int s = lane; s < a.n_seqs; s += 32) sum += f(items_of(a, s));
+            return warp_total(sum) * a.nkv;
         };
         TreeShare t;
-        const int total = each([](int u, int n) { return u * n; }), items = each([](int, int n) { return n; });
-        const int even = max(least, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks));
+        const int total = each([](const TreeItems& i) { return i.of_head(); }), items = each([](const TreeItems& i) { return i.per_head; });
+        const int even = (max(least * COUNT, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks)) + COUNT - 1) & ~(COUNT - 1);
         t.pieces = 0;
         t.quota = even;
         if (items < blocks) {
-            // with pieces of `safe` stretches there are at most items + total / safe of them
+            // with pieces of `safe` there are at most items + total / safe of them
             const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + max(even / 2, 2);
             for (int i = 0; i < 4 && !t.pieces; ++i) {
                 const int c = even + (min(safe, cap) - even) * i / 3;
-                if (each([c](int u, int n) { return u > 0 ? n * ((int)((unsigned)(u + c - 1) / (unsigned)c)) : 0; }) <= blocks) {
+                if (each([c](const TreeItems& i) { return i.pieces_of_head(c); }) <= blocks) {
                     t.pieces = 1;
                     t.quota = c;
                 }
@@ -92,14 +109,13 @@ template <int UNIT, int ROWS> struct TreeWork {
         // where the block's range or piece begins
         const int at = t.pieces ? block : (int)min((int64_t)total, (int64_t)block * t.quota);
         t.from = at;
-        t.to = t.pieces ? at + 1 : min((int64_t)total, (int64_t)at + t.quota);
+        t.to = t.pieces ? at + 1 : (int)min((int64_t)total, (int64_t)at + t.quota);
         int run = 0, passed = 0;
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const int s = s0 + lane;
-            const int n = few ? mine_new : s < a.n_seqs ? n_new(a, s) : 0, u = few ? mine_units : s < a.n_seqs ? units(a, s, n) : 0;
-            const int count = u > 0 ? tiles_of(n, group) * a.nkv : 0;
-            const int mine = u > 0 ? count * (t.pieces ? (int)((unsigned)(u + t.quota - 1) / (unsigned)t.quota) : u) : 0;
-            int sum = mine, counts = count;
+            const TreeItems here = few ? mine : s < a.n_seqs ? items_of(a, s) : none;
+            const int own = a.nkv * (t.pieces ? here.pieces_of_head(t.quota) : here.of_head()), count = a.nkv * here.per_head;
+            int sum = own, counts = count;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, sum, o), c = __shfl_up_sync(0xffffffffu, counts, o);
@@ -112,7 +128,7 @@ template <int UNIT, int ROWS> struct TreeWork {
             if (hit != 0) {
                 const int first = __ffs(hit) - 1;
                 t.seq = s0 + first;
-                t.before = run + __shfl_sync(0xffffffffu, sum - mine, first);
+                t.before = run + __shfl_sync(0xffffffffu, sum - own, first);
                 t.items_before = passed + __shfl_sync(0xffffffffu, counts - count, first);
                 return t;
             }
@@ -128,38 +144,42 @@ template <int UNIT, int ROWS> struct TreeWork {
     static __device__ __forceinline__ TreePart part(const TreeStep& a, TreeShare& t, int at, int block) {
         TreePart p;
         while (true) {
-            const int n = n_new(a, t.seq), u = units(a, t.seq, n), per_head = u > 0 ? tiles_of(n, a.nq / a.nkv) : 0, items = per_head * a.nkv;
-            const int cut = t.pieces && u > 0 ? (int)((unsigned)(u + t.quota - 1) / (unsigned)t.quota) : u;     // numbers that an item has in the list
-            const int in = at - t.before;
-            if (in < cut * items) {
-                const int i = (int)((unsigned)in / (unsigned)cut), off = in - i * cut, item_begin = t.before + i * cut;
+            const TreeItems i = items_of(a, t.seq);
+            const int head = t.pieces ? i.pieces_of_head(t.quota) : i.of_head(), in = at - t.before;
+            if (in < head * a.nkv) {
                 p.seq = t.seq;
-                p.head = (int)((unsigned)i / (unsigned)per_head);
-                p.tile = i - p.head * per_head;
-                p.item = t.items_before + i;
+                p.head = (int)((unsigned)in / (unsigned)head);
+                const int in_head = in - p.head * head, a_full = t.pieces ? i.cut(i.full, t.quota) : i.full;     // numbers that a tile that is not light has
+                p.tile = min((int)((unsigned)in_head / (unsigned)a_full), i.per_head - 1);
+                const int off = in_head - p.tile * a_full, light = i.light && p.tile == i.per_head - 1 ? 1 : 0;
+                const int length = light ? i.lighter : i.full, count = light ? 1 : COUNT;
+                p.item = t.items_before + p.head * i.per_head + p.tile;
                 if (t.pieces) {
-                    p.begin = (int)((unsigned)(off * u) / (unsigned)cut);
-                    p.end = (int)((unsigned)((off + 1) * u) / (unsigned)cut);
-                    p.parts = cut;
+                    p.parts = i.cut(length, t.quota);
+                    p.begin = (int)((unsigned)(off * i.units) / (unsigned)p.parts);
+                    p.end = (int)((unsigned)((off + 1) * i.units) / (unsigned)p.parts);
                     p.first_block = block - off;
                     p.slot0 = 2 * p.first_block;
                     p.slot = 2 * block;
+                    p.list_end = at + 1;
                 } else {
-                    p.begin = off;
-                    p.end = min(u, t.to - item_begin);
+                    const int item_begin = at - off, to = min(length, t.to - item_begin);
+                    p.begin = off / count;                               // (whole: ranges and items begin with whole stretches)
+                    p.end = min(i.units, to / count);
                     p.first_block = (int)((unsigned)item_begin / (unsigned)t.quota);
-                    p.parts = (int)((unsigned)(item_begin + u - 1) / (unsigned)t.quota) - p.first_block + 1;
+                    p.parts = (int)((unsigned)(item_begin + length - 1) / (unsigned)t.quota) - p.first_block + 1;
                     p.slot0 = 2 * p.first_block + (p.first_block * t.quota == item_begin ? 0 : 1);
                     p.slot = 2 * block + (at == t.from ? 0 : 1);
+                    p.list_end = item_begin + to;
                 }
                 return p;
             }
-            t.before += cut * items;
-            t.items_before += items;
+            t.before += head * a.nkv;
+            t.items_before += i.per_head * a.nkv;
             ++t.seq;
         }
     }
-    static __device__ __forceinline__ int next(const TreeShare& t, int at, const TreePart& p) { return t.pieces ? at + 1 : at + (p.end - p.begin); }
+    static __device__ __forceinline__ int next(const TreePart& p) { return p.list_end; }
 };
 
 // Bit i: the token sees key `key0 + i` of its sequence (i < 64), `own` being its number among the sequence's n_new new tokens.
