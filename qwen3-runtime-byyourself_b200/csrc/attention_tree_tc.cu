@@ -11,7 +11,8 @@
 //   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It brings in its query, reads its 64 scores, writes the weights over them, and
 //                rescales O when the maximum is raised by more than 2^8.  At the end of a part it writes the row, or its share of it for the second
 //                kernel to add up.
-//   warps 8-15   8 bits: turn the codes of keys (8-11) and values (12-15) into half precision, which holds them exactly, where TMA would have put them.
+//   warps 8-15   8 bits: turn the codes of keys (8-10) and values (12-14) into half precision, which holds them exactly, where TMA would have put them;
+//                bfloat16: 12-15 look through the values of the pages that some row does not see in whole.
 //   warps 16, 19 issue the products, one elected thread of each those of a tile.
 //   warps 17, 18 copy keys and values: bfloat16 by TMA where the products read them, 8 bits as they lie, some pages ahead.
 //
@@ -54,10 +55,15 @@ static_assert(BM * MEET_COLS * 4 <= Q_BYTES, "they meet where the second tile's 
 constexpr float RAISE = 8.0f;
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
+// An item of several parts, the first of which is a block's last: noted behind all parts, a note a block, for the second kernel (parts 0: there is none).
+struct MergeNote {
+    int parts, slot0, first_block, rows, first_row, t0, head, pad;
+};
+static_assert(sizeof(MergeNote) == 32, "eight words");
 
 struct Note {                                             // what is noted of a page
     float scale;                                          // 8 bits: 2^k0 (values: v0)
-    uint32_t flags[TURN_WARPS];                           // bit 0: some scale is out of range; bit 1: some value is no number
+    uint32_t flags[TURN_WARPS];                           // bit 0: some scale is out of range; bit 1: some value is no number (8 bits: the first word alone)
     uint32_t pad[3];
 };
 template <bool F8> struct Layout {
@@ -152,6 +158,9 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ void load_words2(uint32_t* w, uint32_t at) {
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+}
 // 16-byte chunk `c` (of D / 8) of row r of a tile whose halves of 64 columns are `half_bytes` apart, as TMA's 128-byte swizzle lays it.
 __device__ __forceinline__ uint32_t chunk_at(int r, int c, int half_bytes) { return (uint32_t)((c >> 3) * half_bytes + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
@@ -222,19 +231,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             mbar_init(bar(L::PV_DONE, x), 1);
         }
-        for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), F8 ? 2 * TURN_WARPS : TURN_WARPS);
+        for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), F8 ? 2 : TURN_WARPS);
         for (int s = 0; s < L::STAGES; ++s) {
-            mbar_init(bar(L::K_FULL, s), F8 ? TURN_WARPS : 1);
+            mbar_init(bar(L::K_FULL, s), 1);
             mbar_init(bar(L::K_EMPTY, s), 2);
-            mbar_init(bar(L::V_FULL, s), TURN_WARPS);
+            mbar_init(bar(L::V_FULL, s), F8 ? 1 : TURN_WARPS);
             mbar_init(bar(L::V_EMPTY, s), 2);
             mbar_init(bar(L::V_HERE, s), 1);
         }
         for (int s = 0; s < L::CODES; ++s) {
             mbar_init(bar(L::KC_FULL, s), 1);
-            mbar_init(bar(L::KC_EMPTY, s), TURN_WARPS);
+            mbar_init(bar(L::KC_EMPTY, s), 1);
             mbar_init(bar(L::VC_FULL, s), 1);
-            mbar_init(bar(L::VC_EMPTY, s), TURN_WARPS);
+            mbar_init(bar(L::VC_EMPTY, s), 1);
         }
         mbar_init_fence();
     }
@@ -264,6 +273,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int x = warp >> 2, r = (warp & 3) * 32 + lane;                         // tile, row of it
         const uint32_t t_tile = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * TILE_COLS;
         int page0 = 0;                                                               // pages of this block before the part
+        MergeNote merge = {};
         uint32_t count = 0, q_turn = 0, met_turn = 0;                                // pages of this tile so far; parities of the parts, of the tiles' meetings
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
@@ -336,18 +346,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if constexpr (F8) {
                     c1 = fmaxf(c1 * sh.keys[note].scale, 1.2e-38f);                  // (what is not seen stays minus infinity)
                     v0 = sh.values[note].scale;
-                    uint32_t flags = 0;
-#pragma unroll
-                    for (int w = 0; w < TURN_WARPS; ++w) flags |= sh.keys[note].flags[w] | sh.values[note].flags[w];
-                    rests = flags & 1u;
+                    rests = (sh.keys[note].flags[0] | sh.values[note].flags[0]) & 1u;
                 }
                 tc_wait_ld();
                 if (edge) {
                     const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own) * st.words : nullptr;
                     const unsigned long long seen = tree_seen(mask, st.words, pos0, n_new, own, key0);
-                    uint32_t flags = 0;
+                    uint32_t flags = sh.values[note].flags[0];
+                    if constexpr (!F8) {
 #pragma unroll
-                    for (int w = 0; w < TURN_WARPS; ++w) flags |= sh.values[note].flags[w];
+                        for (int w = 1; w < TURN_WARPS; ++w) flags |= sh.values[note].flags[w];
+                    }
                     if (flags & 2u) find_odd<F8>(a, st.page_table + (int64_t)part.seq * st.pages_per_seq, part.head, part.begin + n, seen, odd);
                     const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
@@ -532,101 +541,104 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             if (!whole && r < rows && !(split && x == 1)) *reinterpret_cast<float2*>(dst + ROWS * D + 2 * part_row) = make_float2(m_run, l_run);
             tc_fence_before();
+            if (!whole && part.begin == 0) merge = {part.parts, part.slot0, part.first_block, min(all_rows, ROWS), part.tile * ROWS, t0, part.head, 0};
             page0 += steps;
             at = Work::next(part);
         }
+        if (threadIdx.x == 0) reinterpret_cast<MergeNote*>(a.parts + (int64_t)2 * gridDim.x * PART)[blockIdx.x] = merge;
     } else if (warp < MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TURN_REGS));
         const bool is_v = warp >= V_WARP;
         const int w4 = warp & 3;
-        int number = 0;
+        int page0 = 0;                                                               // pages of this block before the part
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int pos0 = st.seq_pos0[part.seq], key_end = pos0 + Work::n_new(st, part.seq), steps = part.end - part.begin;
             if constexpr (F8) {
-                // ------------------------------------------------ codes to half precision: 16 rows of a page a warp, D / 16 lanes a row
-                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = 16 / AT_ONCE;
+                // ------------------------------------------------ codes to half precision, a page a warp, D / 16 lanes a row: 25 instructions for a lane's
+                // sixteen codes (four warps on one page wait for one another's stores: 1,500 cycles a page)
+                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = PAGE / AT_ONCE;
                 const int c = lane % PER_ROW, r_in = lane / PER_ROW;
                 const int full = is_v ? L::V_FULL : L::K_FULL, empty = is_v ? L::V_EMPTY : L::K_EMPTY;
                 const int c_full = is_v ? L::VC_FULL : L::KC_FULL, c_empty = is_v ? L::VC_EMPTY : L::KC_EMPTY;
-                // the lanes of a row's second half (64 values) store their second chunk first: eight lanes, eight banks
+                // the lanes of a row's second half (64 values) take their second eight codes first: eight lanes store to eight banks
                 const int swap = HALVES == 2 ? c >> 2 : 0;
-                for (int n = 0; n < steps; ++n, ++number) {
-                    const int stage = number % L::STAGES, slot = number % L::CODES, note = number % NOTES, key0 = (part.begin + n) * PAGE;
-                    const bool edge = key0 + PAGE > pos0;
-                    ok = mbar_wait_warp(bar(c_full, slot), turn_of(number, L::CODES)) && mbar_wait_warp(bar(empty, stage), turn_of(number, L::STAGES) ^ 1u);
-                    if (!ok) { failed(is_v ? 45 : 44); break; }
-                    const uint32_t src = base + (is_v ? L::V_CODES : L::K_CODES) + slot * CODE_BYTES, dst = base + (is_v ? L::V : L::K) + stage * TILE_BYTES;
-                    const uint8_t* const scales = sh.code_scales[is_v][slot];
-                    const int scale0 = scales[0];
-                    uint32_t flags = 0;
-                    uint4 codes[TURNS];
-                    int e[TURNS];
+                uint32_t to[2][2];                                                   // where a lane's chunks go, of rows r_in and r_in + AT_ONCE (they alternate)
 #pragma unroll
-                    for (int i = 0; i < TURNS; ++i) {
-                        const int row = w4 * 16 + i * AT_ONCE + r_in;
-                        codes[i] = ld_shared_v4(src + row * D + c * 16);
-                        e[i] = (int)scales[row] - scale0;
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) to[i][k] = chunk_at(i * AT_ONCE + r_in, 2 * c + (k ^ swap), PANEL_BYTES) - i * AT_ONCE * 128;
+                // A stage and its codes are always the same warp's: a barrier's parity would not tell another one how far the pages between are
+                static_assert(L::STAGES == L::CODES && L::STAGES < TURN_WARPS, "a warp a stage; the last one looks on");
+                for (int n = w4 < L::STAGES ? (w4 - page0 % L::STAGES + L::STAGES) % L::STAGES : steps; n < steps; n += L::STAGES) {
+                    const int number = page0 + n, note = number % NOTES, key0 = (part.begin + n) * PAGE;
+                    const uint32_t turn = turn_of(number, L::STAGES);
+                    const bool edge = key0 + PAGE > pos0;
+                    ok = mbar_wait_warp(bar(c_full, w4), turn) && mbar_wait_warp(bar(empty, w4), turn ^ 1u);
+                    if (!ok) { failed(is_v ? 45 : 44); break; }
+                    const uint32_t src = base + (is_v ? L::V_CODES : L::K_CODES) + w4 * CODE_BYTES + lane * 16, dst = base + (is_v ? L::V : L::K) + w4 * TILE_BYTES;
+                    // this lane has the scales of rows `lane` and `lane` + 32: 2^fold, twice in a word, and what the fold leaves - as a factor of the key's
+                    // score, or in log2 units - which is read only where a flag says so, of either kind
+                    const uint8_t* const scales = sh.code_scales[is_v][w4];
+                    const int scale0 = scales[0];
+                    uint32_t flags = 0, by[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = lane + 32 * i;
+                        const int e = key0 + row < key_end ? (int)scales[row] - scale0 : 0;       // (the scale of a row that nobody wrote may be anything)
+                        const int fold = min(max(e, FOLD_LOW), FOLD_HIGH);
+                        by[i] = (uint32_t)(fold + 15) * 0x04000400u;
+                        if (e != fold) flags = 1u;
+                        if (is_v) sh.value_rest[note][row] = (float)(e - fold);
+                        else sh.key_rest[note][row] = q3_exp2i(e - fold);
                     }
 #pragma unroll
                     for (int i = 0; i < TURNS; ++i) {
-                        const int row = w4 * 16 + i * AT_ONCE + r_in;
-                        uint32_t* v = &codes[i].x;
-                        const int fold = min(max(e[i], FOLD_LOW), FOLD_HIGH);
-                        if (edge) {
-                            const bool live = key0 + row < key_end;                  // (the scale of a row that nobody wrote may be anything)
-                            if (!live) e[i] = fold;
-                            if (is_v) {
+                        const int row = i * AT_ONCE + r_in;                          // of this lane
+                        uint32_t v[2][2];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    if (!live) v[k] = 0u;
-                                    const uint32_t bad = no_numbers<true>(v[k]);
-                                    if (bad) flags |= 2u;
-                                    v[k] &= ~bad;
-                                }
+                        for (int k = 0; k < 2; ++k) load_words2(v[k], src + i * AT_ONCE * D + 8 * (k ^ swap));
+                        if (edge && is_v) {
+                            const bool live = key0 + row < key_end;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint32_t& w = v[k >> 1][k & 1];
+                                if (!live) w = 0u;
+                                const uint32_t bad = no_numbers<true>(w);
+                                if (bad) flags |= 2u;
+                                w &= ~bad;
                             }
                         }
-                        if (e[i] != fold) flags |= 1u;
-                        const uint32_t one = (uint32_t)(fold + 15) << 10, both = one | one << 16;          // 2^fold, twice
-                        const __half2 by = *reinterpret_cast<const __half2*>(&both);
-                        uint32_t h[8];
+                        const uint32_t mine = __shfl_sync(0xffffffffu, by[i * AT_ONCE >= 32 ? 1 : 0], row & 31);
+                        const __half2 m = *reinterpret_cast<const __half2*>(&mine);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const __half2 z = __hmul2(q3_half2_of(v[k >> 1] >> (16 * (k & 1))), by);
-                            h[k] = *reinterpret_cast<const uint32_t*>(&z);
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __half2 z = __hmul2(q3_half2_of(v[k][j >> 1] >> (16 * (j & 1))), m);
+                                h[j] = *reinterpret_cast<const uint32_t*>(&z);
+                            }
+                            st_shared_v4(dst + to[i & 1][k] + i * AT_ONCE * 128, make_uint4(h[0], h[1], h[2], h[3]));
                         }
-                        const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-                        st_shared_v4(dst + chunk_at(row, 2 * c + swap, PANEL_BYTES), swap ? hi : lo);
-                        st_shared_v4(dst + chunk_at(row, 2 * c + 1 - swap, PANEL_BYTES), swap ? lo : hi);
                     }
                     flags = __reduce_or_sync(0xffffffffu, flags);
-                    // what the folds leave, as a factor of the key's score or in log2 units: read only where a flag says so, which any warp of either kind may
-                    if (c == 0) {
-#pragma unroll
-                        for (int i = 0; i < TURNS; ++i) {
-                            const int row = w4 * 16 + i * AT_ONCE + r_in, rest = e[i] - min(max(e[i], FOLD_LOW), FOLD_HIGH);
-                            if (is_v) sh.value_rest[note][row] = (float)rest;
-                            else sh.key_rest[note][row] = q3_exp2i(rest);
-                        }
-                    }
-                    Note& to_note = is_v ? sh.values[note] : sh.keys[note];
-                    if (lane == 0) {
-                        to_note.flags[w4] = flags;
-                        if (w4 == 0) to_note.scale = is_v ? (float)(scale0 - Q3_SCALE_BIAS) : q3_exp2i(scale0 - Q3_SCALE_BIAS);
-                    }
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(bar(full, stage));
-                        mbar_arrive(bar(c_empty, slot));
+                        Note& to_note = is_v ? sh.values[note] : sh.keys[note];
+                        to_note.flags[0] = flags;
+                        to_note.scale = is_v ? (float)(scale0 - Q3_SCALE_BIAS) : q3_exp2i(scale0 - Q3_SCALE_BIAS);
+                        mbar_arrive(bar(full, w4));
+                        mbar_arrive(bar(c_empty, w4));
                         mbar_arrive(bar(L::NOTED, note));
                     }
                 }
             } else if (is_v) {
                 // ------------------------------------------------ a look at the values of pages that some row does not see in whole
-                for (int n = 0; n < steps; ++n, ++number) {
-                    const int stage = number % L::STAGES, key0 = (part.begin + n) * PAGE;
+                for (int n = 0; n < steps; ++n) {
+                    const int number = page0 + n, stage = number % L::STAGES, key0 = (part.begin + n) * PAGE;
                     ok = mbar_wait_warp(bar(L::V_HERE, stage), turn_of(number, L::STAGES));
                     if (!ok) { failed(46); break; }
                     if (key0 + PAGE > pos0) {
@@ -654,6 +666,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
             }
+            page0 += steps;
             at = Work::next(part);
         }
     } else {
@@ -782,49 +795,36 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     }
 }
 
-// ---- the parts of the items that several blocks share, added up in their order: for every block of the first kernel whose last part is the first one of such
-// an item, and for 32 of its rows, a block
+// ---- the parts of the items that several blocks share, added up in their order: for every block of the first kernel that noted one, and for 32 of its rows, a block
 constexpr int MERGE_THREADS = D / 8 * 32;
 __global__ void __launch_bounds__(MERGE_THREADS) tree_tc_merge_kernel(const __grid_constant__ Args a, int blocks) {
-    __shared__ TreeShare shared_share;
     pdl_launch_dependents();
     pdl_wait();
-    const TreeStep& st = a.step;
-    const int b0 = blockIdx.x;
-    if (threadIdx.x < 32) {
-        const TreeShare found = Work::share(st, 2, b0, blocks);
-        if (threadIdx.x == 0) shared_share = found;
-    }
-    __syncthreads();
-    TreeShare share = shared_share;
-    if (share.from >= share.to) return;
-    TreePart part;
-    for (int at = share.from; at < share.to; at = Work::next(part)) part = Work::part(st, share, at, b0);
-    if (part.parts == 1 || part.begin != 0) return;
-    const int group = st.nq / st.nkv, t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq);
-    const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0), first = blockIdx.y * 32;
-    if (first >= rows) return;
-    const int r = first + (threadIdx.x & 31);
-    if (r >= rows) return;
-    bf16* const out = a.out + ((int64_t)(t0 + (row0 + r) / group) * st.nq + part.head * group + (row0 + r) % group) * D;
+    const int4* note = reinterpret_cast<const int4*>(a.parts + (int64_t)2 * blocks * PART) + 2 * blockIdx.x;
+    const int4 n0 = note[0], n1 = note[1];
+    const int parts = n0.x, slot0 = n0.y, first_block = n0.z, rows = n0.w, r = blockIdx.y * 32 + (threadIdx.x & 31);
+    if (parts == 0 || r >= rows) return;
+    const int group = a.step.nq / a.step.nkv, row = n1.x + r;
+    bf16* const out = a.out + ((int64_t)(n1.y + row / group) * a.step.nq + n1.z * group + row % group) * D;
     const int c = threadIdx.x >> 5;                                                  // eight values a warp
     float m = -INFINITY, l = 0.0f, v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
     constexpr int AT_ONCE = 4;                                                       // parts asked for together
-    for (int b0 = 0; b0 < part.parts; b0 += AT_ONCE) {
+    for (int b0 = 0; b0 < parts; b0 += AT_ONCE) {
         float2 ml[AT_ONCE];
         float4 u[AT_ONCE][2];
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
-            const float* src = a.parts + (int64_t)part.slot_of(min(b0 + k, part.parts - 1)) * PART;
+            const int i = min(b0 + k, parts - 1);
+            const float* src = a.parts + (int64_t)(i == 0 ? slot0 : 2 * (first_block + i)) * PART;
             ml[k] = *reinterpret_cast<const float2*>(src + ROWS * D + 2 * r);
             u[k][0] = *reinterpret_cast<const float4*>(src + ((2 * c) * ROWS + r) * 4);
             u[k][1] = *reinterpret_cast<const float4*>(src + ((2 * c + 1) * ROWS + r) * 4);
         }
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
-            if (b0 + k >= part.parts) break;
+            if (b0 + k >= parts) break;
             const float m2 = fmaxf(m, ml[k].x), was = m == m2 ? 1.0f : ex2(m - m2), now = ml[k].x == m2 ? 1.0f : ex2(ml[k].x - m2);
             m = m2;
             l = fmaf(now, ml[k].y, l * was);
@@ -867,7 +867,7 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
 Q3_EXPORT int q3_attention_tree_tc_head_dim() { return D; }
 
 // Float32 values of `parts` for a launch.
-Q3_EXPORT int64_t q3_attention_tree_tc_parts() { return (int64_t)2 * q3_device_sm_count() * PART; }
+Q3_EXPORT int64_t q3_attention_tree_tc_parts() { return q3_device_sm_count() * ((int64_t)2 * PART + sizeof(MergeNote) / sizeof(float)); }
 
 Q3_EXPORT int q3_attention_tree_tc_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
                                         void* out, float* parts, const int* seq_start, const int* seq_pos0, const int* page_table,

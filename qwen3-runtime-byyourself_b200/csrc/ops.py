@@ -37,7 +37,7 @@ class KernelError(RuntimeError):
 # own later waves need) and the decode attention, which asks for its first pages before it waits, gains 0.5 % at batch
 # 16 and 32 and loses 0.3 % at batch 64; its form for many sequences, which stands between such products, gains 1.5 % at batch 64
 # (1526 -> 1503 us a step of 12 layers).  QWEN3_B200_PDL=1 / =0 turns it on / off for all.
-PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu")
+PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu", "attention_tree_tc.cu")
 _pdl_override = {"1": True, "0": False}.get(os.environ.get("QWEN3_B200_PDL", ""))
 _libs = {}
 
