@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const TreeShare found = Work::share(st, LEAST_PAGES, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, LEAST_PAGES, 8, blockIdx.x, gridDim.x);
         if (lane == 0) *shared_share = found;
     }
     __syncthreads();

@@ -11,7 +11,7 @@
 //   warps 0-7    softmax: thread r of a tile's 128 owns row r (TMEM lane r).  It brings in its query, reads its 64 scores, writes the weights over them, and
 //                rescales O when the maximum is raised by more than 2^8.  At the end of a part it writes the row, or its share of it for the second
 //                kernel to add up.
-//   warps 8-15   8 bits: turn the codes of keys (8-10) and values (12-14) into half precision, which holds them exactly, where TMA would have put them;
+//   warps 8-15   8 bits: turn the codes of keys (8-11) and values (12-15) into half precision, which holds them exactly, where TMA would have put them;
 //                bfloat16: 12-15 look through the values of the pages that some row does not see in whole.
 //   warps 16, 19 issue the products, one elected thread of each those of a tile.
 //   warps 17, 18 copy keys and values: bfloat16 by TMA where the products read them, 8 bits as they lie, some pages ahead.
@@ -37,7 +37,6 @@
 #endif
 
 namespace {
-
 constexpr int D = Q3_HEAD_DIM, PAGE = Q3_PAGE_TOKENS;
 static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 static_assert(PAGE == 64, "a product takes a page of 64 keys");
@@ -63,12 +62,12 @@ static_assert(sizeof(MergeNote) == 32, "eight words");
 
 struct Note {                                             // what is noted of a page
     float scale;                                          // 8 bits: 2^k0 (values: v0)
-    uint32_t flags[TURN_WARPS];                           // bit 0: some scale is out of range; bit 1: some value is no number (8 bits: the first word alone)
+    uint32_t flags[TURN_WARPS];                           // bit 0: some scale is out of range; bit 1: some value is no number (8 bits: the first two words)
     uint32_t pad[3];
 };
 template <bool F8> struct Layout {
-    static constexpr int STAGES = F8 ? 3 : 4;             // pages of keys and of values that the products can read
-    static constexpr int CODES = F8 ? 3 : 0;              // pages of codes of either on their way
+    static constexpr int STAGES = F8 ? 2 : 4;             // pages of keys and of values that the products can read
+    static constexpr int CODES = F8 ? 4 : 0;              // pages of codes of either on their way: what a page's copy takes, some 3,500 cycles, has to go by
     static constexpr int QUERIES = 0, MEET = Q_BYTES, K = 2 * Q_BYTES, V = K + STAGES * TILE_BYTES;
     static constexpr int K_CODES = V + STAGES * TILE_BYTES, V_CODES = K_CODES + CODES * CODE_BYTES, REST = V_CODES + CODES * CODE_BYTES;
     // barriers: one word of 8 bytes each
@@ -231,19 +230,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             mbar_init(bar(L::PV_DONE, x), 1);
         }
-        for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), F8 ? 2 : TURN_WARPS);
+        for (int n = 0; n < NOTES; ++n) mbar_init(bar(L::NOTED, n), TURN_WARPS);
         for (int s = 0; s < L::STAGES; ++s) {
-            mbar_init(bar(L::K_FULL, s), 1);
+            mbar_init(bar(L::K_FULL, s), F8 ? 2 : 1);
             mbar_init(bar(L::K_EMPTY, s), 2);
-            mbar_init(bar(L::V_FULL, s), F8 ? 1 : TURN_WARPS);
+            mbar_init(bar(L::V_FULL, s), F8 ? 2 : TURN_WARPS);
             mbar_init(bar(L::V_EMPTY, s), 2);
             mbar_init(bar(L::V_HERE, s), 1);
         }
         for (int s = 0; s < L::CODES; ++s) {
             mbar_init(bar(L::KC_FULL, s), 1);
-            mbar_init(bar(L::KC_EMPTY, s), 1);
+            mbar_init(bar(L::KC_EMPTY, s), 2);
             mbar_init(bar(L::VC_FULL, s), 1);
-            mbar_init(bar(L::VC_EMPTY, s), 1);
+            mbar_init(bar(L::VC_EMPTY, s), 2);
         }
         mbar_init_fence();
     }
@@ -254,7 +253,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 2, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, 2, 10, blockIdx.x, gridDim.x);
         if (lane == 0) sh.share = found;
     }
     tc_fence_before();
@@ -346,17 +345,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if constexpr (F8) {
                     c1 = fmaxf(c1 * sh.keys[note].scale, 1.2e-38f);                  // (what is not seen stays minus infinity)
                     v0 = sh.values[note].scale;
-                    rests = (sh.keys[note].flags[0] | sh.values[note].flags[0]) & 1u;
+                    rests = (sh.keys[note].flags[0] | sh.keys[note].flags[1] | sh.values[note].flags[0] | sh.values[note].flags[1]) & 1u;
                 }
                 tc_wait_ld();
                 if (edge) {
                     const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own) * st.words : nullptr;
                     const unsigned long long seen = tree_seen(mask, st.words, pos0, n_new, own, key0);
-                    uint32_t flags = sh.values[note].flags[0];
-                    if constexpr (!F8) {
-#pragma unroll
-                        for (int w = 1; w < TURN_WARPS; ++w) flags |= sh.values[note].flags[w];
-                    }
+                    uint32_t flags = sh.values[note].flags[0] | sh.values[note].flags[1];
+                    if constexpr (!F8) flags |= sh.values[note].flags[2] | sh.values[note].flags[3];
                     if (flags & 2u) find_odd<F8>(a, st.page_table + (int64_t)part.seq * st.pages_per_seq, part.head, part.begin + n, seen, odd);
                     const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
@@ -556,10 +552,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const TreePart part = Work::part(st, share, at, blockIdx.x);
             const int pos0 = st.seq_pos0[part.seq], key_end = pos0 + Work::n_new(st, part.seq), steps = part.end - part.begin;
             if constexpr (F8) {
-                // ------------------------------------------------ codes to half precision, a page a warp, D / 16 lanes a row: 25 instructions for a lane's
-                // sixteen codes (four warps on one page wait for one another's stores: 1,500 cycles a page)
-                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = PAGE / AT_ONCE;
-                const int c = lane % PER_ROW, r_in = lane / PER_ROW;
+                // ------------------------------------------------ codes to half precision, a page two warps, each 32 rows of it, D / 16 lanes a row: 25
+                // instructions for a lane's sixteen codes
+                constexpr int PER_ROW = D / 16, AT_ONCE = 32 / PER_ROW, TURNS = 32 / AT_ONCE;
+                const int c = lane % PER_ROW, r_in = lane / PER_ROW, my_stage = w4 >> 1, half = w4 & 1;
                 const int full = is_v ? L::V_FULL : L::K_FULL, empty = is_v ? L::V_EMPTY : L::K_EMPTY;
                 const int c_full = is_v ? L::VC_FULL : L::KC_FULL, c_empty = is_v ? L::VC_EMPTY : L::KC_EMPTY;
                 // the lanes of a row's second half (64 values) take their second eight codes first: eight lanes store to eight banks
@@ -568,49 +564,64 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) to[i][k] = chunk_at(i * AT_ONCE + r_in, 2 * c + (k ^ swap), PANEL_BYTES) - i * AT_ONCE * 128;
-                // A stage and its codes are always the same warp's: a barrier's parity would not tell another one how far the pages between are
-                static_assert(L::STAGES == L::CODES && L::STAGES < TURN_WARPS, "a warp a stage; the last one looks on");
-                for (int n = w4 < L::STAGES ? (w4 - page0 % L::STAGES + L::STAGES) % L::STAGES : steps; n < steps; n += L::STAGES) {
-                    const int number = page0 + n, note = number % NOTES, key0 = (part.begin + n) * PAGE;
-                    const uint32_t turn = turn_of(number, L::STAGES);
+                    for (int k = 0; k < 2; ++k)
+                        to[i][k] = base + (is_v ? L::V : L::K) + my_stage * TILE_BYTES + half * 32 * 128 +
+                                   chunk_at(i * AT_ONCE + r_in, 2 * c + (k ^ swap), PANEL_BYTES) - i * AT_ONCE * 128;
+                // A stage, and so the slots of its codes, are always the same warps': a barrier's parity would not tell others how far the pages between are
+                static_assert(L::STAGES == 2 && L::CODES % 2 == 0 && TURN_WARPS == 4, "two warps a stage");
+                for (int n = (my_stage ^ page0) & 1; n < steps; n += 2) {
+                    const int number = page0 + n, slot = number % L::CODES, note = number % NOTES, key0 = (part.begin + n) * PAGE;
                     const bool edge = key0 + PAGE > pos0;
-                    ok = mbar_wait_warp(bar(c_full, w4), turn) && mbar_wait_warp(bar(empty, w4), turn ^ 1u);
+                    // The notes of values are there before their stage is: the softmax of a page does not wait for the products of two pages before.
+                    // (Those of keys could then be written over ones that are still read.)
+                    ok = mbar_wait_warp(bar(c_full, slot), turn_of(number, L::CODES)) && (is_v || mbar_wait_warp(bar(empty, my_stage), turn_of(number, L::STAGES) ^ 1u));
                     if (!ok) { failed(is_v ? 45 : 44); break; }
-                    const uint32_t src = base + (is_v ? L::V_CODES : L::K_CODES) + w4 * CODE_BYTES + lane * 16, dst = base + (is_v ? L::V : L::K) + w4 * TILE_BYTES;
-                    // this lane has the scales of rows `lane` and `lane` + 32: 2^fold, twice in a word, and what the fold leaves - as a factor of the key's
-                    // score, or in log2 units - which is read only where a flag says so, of either kind
-                    const uint8_t* const scales = sh.code_scales[is_v][w4];
-                    const int scale0 = scales[0];
-                    uint32_t flags = 0, by[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int row = lane + 32 * i;
-                        const int e = key0 + row < key_end ? (int)scales[row] - scale0 : 0;       // (the scale of a row that nobody wrote may be anything)
-                        const int fold = min(max(e, FOLD_LOW), FOLD_HIGH);
-                        by[i] = (uint32_t)(fold + 15) * 0x04000400u;
-                        if (e != fold) flags = 1u;
-                        if (is_v) sh.value_rest[note][row] = (float)(e - fold);
-                        else sh.key_rest[note][row] = q3_exp2i(e - fold);
+                    const uint32_t src = base + (is_v ? L::V_CODES : L::K_CODES) + slot * CODE_BYTES + half * 32 * D + lane * 16;
+                    // this lane has the scale of a row: 2^fold, twice in a word, and what the fold leaves - as a factor of the key's score, or in log2
+                    // units - which is read only where a flag says so, of either kind
+                    const uint8_t* const scales = sh.code_scales[is_v][slot];
+                    const int scale0 = scales[0], my_row = half * 32 + lane;
+                    const int e = key0 + my_row < key_end ? (int)scales[my_row] - scale0 : 0;     // (the scale of a row that nobody wrote may be anything)
+                    const int fold = min(max(e, FOLD_LOW), FOLD_HIGH);
+                    const uint32_t by = (uint32_t)(fold + 15) * 0x04000400u;
+                    uint32_t flags = e != fold ? 1u : 0u;
+                    if (is_v) sh.value_rest[note][my_row] = (float)(e - fold);
+                    else sh.key_rest[note][my_row] = q3_exp2i(e - fold);
+                    if (edge && is_v) {
+#pragma unroll 1
+                        for (int i = 0; i < TURNS; ++i) {
+                            const uint4 w = ld_shared_v4(src + i * AT_ONCE * D);
+                            if (key0 + half * 32 + i * AT_ONCE + r_in < key_end && (no_numbers<true>(w.x) | no_numbers<true>(w.y) | no_numbers<true>(w.z) | no_numbers<true>(w.w)) != 0)
+                                flags |= 2u;
+                        }
                     }
-#pragma unroll
+                    flags = __reduce_or_sync(0xffffffffu, flags);
+                    __syncwarp();
+                    if (lane == 0) {
+                        Note& to_note = is_v ? sh.values[note] : sh.keys[note];
+                        to_note.flags[half] = flags;
+                        if (half == 0) to_note.scale = is_v ? (float)(scale0 - Q3_SCALE_BIAS) : q3_exp2i(scale0 - Q3_SCALE_BIAS);
+                        mbar_arrive(bar(L::NOTED, note));
+                    }
+                    if (is_v) {
+                        ok = mbar_wait_warp(bar(empty, my_stage), turn_of(number, L::STAGES) ^ 1u);
+                        if (!ok) { failed(36); break; }
+                    }
+                    // (few turns a round: the loops of all roles share an instruction cache; with twice as many everything took 1.05 times as long)
+#pragma unroll 4
                     for (int i = 0; i < TURNS; ++i) {
-                        const int row = i * AT_ONCE + r_in;                          // of this lane
                         uint32_t v[2][2];
 #pragma unroll
                         for (int k = 0; k < 2; ++k) load_words2(v[k], src + i * AT_ONCE * D + 8 * (k ^ swap));
                         if (edge && is_v) {
-                            const bool live = key0 + row < key_end;
+                            const bool live = key0 + half * 32 + i * AT_ONCE + r_in < key_end;
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 uint32_t& w = v[k >> 1][k & 1];
-                                if (!live) w = 0u;
-                                const uint32_t bad = no_numbers<true>(w);
-                                if (bad) flags |= 2u;
-                                w &= ~bad;
+                                w = live ? w & ~no_numbers<true>(w) : 0u;
                             }
                         }
-                        const uint32_t mine = __shfl_sync(0xffffffffu, by[i * AT_ONCE >= 32 ? 1 : 0], row & 31);
+                        const uint32_t mine = __shfl_sync(0xffffffffu, by, i * AT_ONCE + r_in);
                         const __half2 m = *reinterpret_cast<const __half2*>(&mine);
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
@@ -620,19 +631,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                                 const __half2 z = __hmul2(q3_half2_of(v[k][j >> 1] >> (16 * (j & 1))), m);
                                 h[j] = *reinterpret_cast<const uint32_t*>(&z);
                             }
-                            st_shared_v4(dst + to[i & 1][k] + i * AT_ONCE * 128, make_uint4(h[0], h[1], h[2], h[3]));
+                            st_shared_v4((i & 1 ? to[1][k] : to[0][k]) + i * AT_ONCE * 128, make_uint4(h[0], h[1], h[2], h[3]));
                         }
                     }
-                    flags = __reduce_or_sync(0xffffffffu, flags);
                     fence_proxy_async();
                     __syncwarp();
                     if (lane == 0) {
-                        Note& to_note = is_v ? sh.values[note] : sh.keys[note];
-                        to_note.flags[0] = flags;
-                        to_note.scale = is_v ? (float)(scale0 - Q3_SCALE_BIAS) : q3_exp2i(scale0 - Q3_SCALE_BIAS);
-                        mbar_arrive(bar(full, w4));
-                        mbar_arrive(bar(c_empty, w4));
-                        mbar_arrive(bar(L::NOTED, note));
+                        mbar_arrive(bar(full, my_stage));
+                        mbar_arrive(bar(c_empty, slot));
                     }
                 }
             } else if (is_v) {

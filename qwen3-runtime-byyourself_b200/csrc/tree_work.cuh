@@ -3,10 +3,9 @@
 // The work is a list of items - (sequence, kv head, tile of rows; a row is a new token and a query head of the kv head's group) - of as
 // many stretches of UNIT keys as the sequence has.  It is shared out in one of two ways, whatever the sequences' lengths:
 //   pieces  every item is cut into equal pieces of at most `quota` stretches, and a block takes one piece.  `quota` is the best of four numbers between
-//           the even share and one at which the pieces are certainly no more than the blocks;
+//           the even share and one at which the pieces are certainly no more than the blocks, or that is longer by what a second part would cost a block;
 //   ranges  the stretches of all items in a row are cut into ranges of equal length, one a block, wherever they fall: a block has at most a
-//           part of an item, some whole ones and another part.  Taken where pieces would leave blocks without work: many items a block, or so few blocks an
-//           item that equal pieces are half as long again.
+//           part of an item, some whole ones and another part.  Taken where there are no such pieces.
 // Parts of an item are added up in their order.  Which part is whose, and so the order of a row's sums, hangs on the lengths of all sequences of the step
 // and on nothing else.
 #pragma once
@@ -77,8 +76,9 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         return v;
     }
 
-    // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more).
-    static __device__ TreeShare share(const TreeStep& a, int least, int block, int blocks) {
+    // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more);
+    // `spare`: so many stretches take about as long as beginning and ending a part.
+    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int block, int blocks) {
         const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
@@ -97,7 +97,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         t.quota = even;
         if (items < blocks) {
             // with pieces of `safe` there are at most items + total / safe of them
-            const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + max(even / 2, 2);
+            const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + spare * COUNT;
             for (int i = 0; i < 4 && !t.pieces; ++i) {
                 const int c = even + (min(safe, cap) - even) * i / 3;
                 if (each([c](const TreeItems& i) { return i.pieces_of_head(c); }) <= blocks) {
