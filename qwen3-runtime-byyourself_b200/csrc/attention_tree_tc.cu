@@ -253,7 +253,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 2, 10, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, 2, 20, blockIdx.x, gridDim.x);
         if (lane == 0) sh.share = found;
     }
     tc_fence_before();
@@ -283,39 +283,45 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const int first = split ? x : 0, stride = split ? 2 : 1;
             const int rows = split ? all_rows : all_rows - x * BM, row = part.tile * ROWS + (split ? 0 : x * BM) + r, own = min(row / group, n_new - 1);
             const int64_t row_at = ((int64_t)(t0 + own) * st.nq + part.head * group + row % group) * D;
-            // ---- this row's query (twice the same rows: both tiles' products read the first one's)
+            // ---- the warp's queries, D / 8 lanes a row, each 16 bytes (twice the same rows: both tiles' products read the first one's, but the second one's
+            // warps want the rows' factors too).  In loops that are not unrolled: this is run once a part, from instructions that have left the caches by then.
             float factor = a.scale_log2;
             {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
-                float down = 1.0f;
+                constexpr int PER_ROW = D / 8, AT_ONCE = 32 / PER_ROW, TURNS = 32 / AT_ONCE;
+                const int c = lane % PER_ROW;
+                const uint32_t queries = base + L::QUERIES + x * Q_BYTES;
+                __syncwarp();
+#pragma unroll 1
+                for (int i = 0; i < TURNS; ++i) {
+                    const int of = i * AT_ONCE + lane / PER_ROW, to_row = (warp & 3) * 32 + of;       // the lane whose row this is
+                    const int64_t from = __shfl_sync(0xffffffffu, row_at, of);
+                    const uint32_t dst = queries + chunk_at(to_row, c, BM * 128);
+                    if (to_row < rows) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(a.q + from + 8 * c) : "memory");
+                    else st_shared_v4(dst, make_uint4(0, 0, 0, 0));
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 if constexpr (F8) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        const uint4 w = src[c];
-                        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll 4
+                    for (int i = 0; i < TURNS; ++i) {
+                        const uint32_t at_chunk = queries + chunk_at((warp & 3) * 32 + i * AT_ONCE + lane / PER_ROW, c, BM * 128);
+                        uint4 w = ld_shared_v4(at_chunk);
+                        uint32_t* v = &w.x;
+                        uint32_t top = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, v[e] >> 16 & 0x7fffu));
-                    }
-                    int e2 = (int)(top >> 7) - 127;
-                    e2 = e2 >= 128 ? 0 : min(max(e2, -60), 60);
-                    down = q3_exp2i(-e2);
-                    factor *= q3_exp2i(e2);
-                }
-                if (!(split && x == 1)) {
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        uint4 w = src[c];
-                        if constexpr (F8) {
-                            uint32_t* v = &w.x;
+                        for (int o = PER_ROW / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        int e2 = (int)(top >> 7) - 127;
+                        e2 = e2 >= 128 ? 0 : min(max(e2, -60), 60);
+                        const float down = q3_exp2i(-e2);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
-                        }
-                        if (r >= rows) w = make_uint4(0, 0, 0, 0);
-                        st_shared_v4(base + L::QUERIES + x * Q_BYTES + chunk_at(r, c, BM * 128), w);
+                        for (int e = 0; e < 4; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
+                        st_shared_v4(at_chunk, w);
+                        const float up = __shfl_sync(0xffffffffu, q3_exp2i(e2), (lane % AT_ONCE) * PER_ROW);   // of row i AT_ONCE + lane % AT_ONCE
+                        if (lane / AT_ONCE == i) factor = a.scale_log2 * up;
                     }
-                    fence_proxy_async();
                 }
+                fence_proxy_async();
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(L::Q, 0));
