@@ -7,6 +7,7 @@
 // of the query's type or codes of 8 bits with a scale a row (page8.cuh).
 // A block a (token, query head): four warps take every fourth key, each with a running maximum and sum of its own, and meet at the
 // end.  A key that is not seen is not read.  Bound by the latency of its chain of keys: it is here for 32-bit queries and odd head sizes.
+#include "../include/qwen3/cache_args.h"
 #include "page8.cuh"
 
 namespace {
@@ -106,29 +107,20 @@ int launch(const TreeArgs& a, int64_t n_tokens, cudaStream_t stream) {
     return (int)q3_launch(tree_any_kernel<T, F8>, grid, dim3(WARPS * 32), 0, stream, a);
 }
 
-int attend(const TreeArgs& a, int64_t n_tokens, bool f32, void* stream) {
-    if (a.n_seqs <= 0 || n_tokens <= 0) return 0;
+int attend(const q3_attention_tree_args& x, bool f32) {
+    const TreeArgs a = {x.q, x.k_pages, x.v_pages, (const uint8_t*)x.k_scales, (const uint8_t*)x.v_scales, x.out, (const int*)x.seq_start,
+                        (const int*)x.seq_pos0, (const int*)x.page_table, (const unsigned long long*)x.tree, x.words, x.pages_per_seq, x.n_seqs, x.nq, x.nkv,
+                        x.d, x.n_pages, (float)x.scale};
+    if (a.n_seqs <= 0 || x.n_tokens <= 0) return 0;
     if (a.nq <= 0 || a.nkv <= 0 || a.nq % a.nkv != 0 || a.d <= 0 || a.d > 256 || (a.tree != nullptr && a.words <= 0)) return Q3_ERR_BAD_SIZE;
-    if (n_tokens > (int64_t)65535 * 65535) return Q3_ERR_TOO_LARGE;
+    if (x.n_tokens > (int64_t)65535 * 65535) return Q3_ERR_TOO_LARGE;
     const bool f8 = a.k_scales != nullptr;
-    cudaStream_t s = (cudaStream_t)stream;
-    if (f32) return f8 ? launch<float, true>(a, n_tokens, s) : launch<float, false>(a, n_tokens, s);
-    return f8 ? launch<bf16, true>(a, n_tokens, s) : launch<bf16, false>(a, n_tokens, s);
+    cudaStream_t s = (cudaStream_t)x.stream;
+    if (f32) return f8 ? launch<float, true>(a, x.n_tokens, s) : launch<float, false>(a, x.n_tokens, s);
+    return f8 ? launch<bf16, true>(a, x.n_tokens, s) : launch<bf16, false>(a, x.n_tokens, s);
 }
 
 }  // namespace
 
-Q3_EXPORT int q3_attention_tree_any_f32(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
-                                        void* out, const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq,
-                                        int64_t n_pages, int n_seqs, int64_t n_tokens, int nq, int nkv, int d, float scale, const void* tree,
-                                        int words, void* stream) {
-    return attend({q, k_pages, v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, out, seq_start, seq_pos0, page_table,
-                   (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, d, n_pages, scale}, n_tokens, true, stream);
-}
-Q3_EXPORT int q3_attention_tree_any_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
-                                         void* out, const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq,
-                                         int64_t n_pages, int n_seqs, int64_t n_tokens, int nq, int nkv, int d, float scale, const void* tree,
-                                         int words, void* stream) {
-    return attend({q, k_pages, v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, out, seq_start, seq_pos0, page_table,
-                   (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, d, n_pages, scale}, n_tokens, false, stream);
-}
+Q3_EXPORT int q3_attention_tree_any_f32(const q3_attention_tree_args* a) { return attend(*a, true); }
+Q3_EXPORT int q3_attention_tree_any_bf16(const q3_attention_tree_args* a) { return attend(*a, false); }

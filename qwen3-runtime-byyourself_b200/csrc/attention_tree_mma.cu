@@ -598,18 +598,12 @@ Q3_EXPORT int64_t q3_attention_tree_mma_parts(int rows) {
     return (int64_t)2 * q3_device_sm_count() * each * (D + 2);
 }
 
-Q3_EXPORT int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
-                                         void* out, float* parts, int* counters, const int* seq_start, const int* seq_pos0,
-                                         const int* page_table, int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv,
-                                         float scale, const void* tree, int words, void* stream) {
-    if (n_seqs <= 0 || max_new <= 0) return 0;
-    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || n_pages <= 0 || pages_per_seq <= 0 || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
-        return Q3_ERR_BAD_SIZE;
-    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
-        return Q3_ERR_MISALIGNED;
-    const Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new}, (const bf16*)q, (bf16*)out,
-              (const unsigned char*)k_pages, (const unsigned char*)v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, parts, counters,
-              scale * 1.4426950408889634f};
-    const int64_t rows = (int64_t)max_new * (nq / nkv);
-    return k_scales != nullptr ? launch_rows<true>(a, rows, (cudaStream_t)stream) : launch_rows<false>(a, rows, (cudaStream_t)stream);
+Q3_EXPORT int q3_attention_tree_mma_bf16(const q3_attention_tree_args* x) {
+    if (x->n_seqs <= 0 || x->max_new <= 0) return 0;
+    const int refused = tree_refused(*x, D);
+    if (refused != 0) return refused;
+    const Args a = {tree_step(*x), (const bf16*)x->q, (bf16*)x->out, (const unsigned char*)x->k_pages, (const unsigned char*)x->v_pages,
+                    (const uint8_t*)x->k_scales, (const uint8_t*)x->v_scales, (float*)x->parts, (int*)x->counters, (float)x->scale * 1.4426950408889634f};
+    const int64_t rows = (int64_t)x->max_new * (x->nq / x->nkv);
+    return x->k_scales != nullptr ? launch_rows<true>(a, rows, (cudaStream_t)x->stream) : launch_rows<false>(a, rows, (cudaStream_t)x->stream);
 }

@@ -881,18 +881,13 @@ Q3_EXPORT int q3_attention_tree_tc_head_dim() { return D; }
 // Float32 values of `parts` for a launch.
 Q3_EXPORT int64_t q3_attention_tree_tc_parts() { return q3_device_sm_count() * ((int64_t)2 * PART + sizeof(MergeNote) / sizeof(float)); }
 
-Q3_EXPORT int q3_attention_tree_tc_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales,
-                                        void* out, float* parts, const int* seq_start, const int* seq_pos0, const int* page_table,
-                                        int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv, float scale,
-                                        const void* tree, int words, int* status, void* stream) {
-    if (n_seqs <= 0 || max_new <= 0) return 0;
-    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || n_pages <= 0 || pages_per_seq <= 0 || !(scale > 0.0f) || (tree != nullptr && (words <= 0 || words * 64 < max_new)))
-        return Q3_ERR_BAD_SIZE;                                                      // (the maximum is taken before the scale)
-    if (n_pages * nkv * PAGE > 0x7fffffff) return Q3_ERR_TOO_LARGE;                  // a row's number is a coordinate of a copy
-    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) || !aligned16(parts) || (k_scales != nullptr && (!aligned16(k_scales) || !aligned16(v_scales))))
-        return Q3_ERR_MISALIGNED;
-    const Args a = {{seq_start, seq_pos0, page_table, (const unsigned long long*)tree, words, pages_per_seq, n_seqs, nq, nkv, n_pages, max_new},
-                    (const bf16*)q, (bf16*)out, (const unsigned char*)k_pages, (const unsigned char*)v_pages, (const uint8_t*)k_scales,
-                    (const uint8_t*)v_scales, parts, status, scale * 1.4426950408889634f};
-    return k_scales != nullptr ? launch<true>(a, max_new, (cudaStream_t)stream) : launch<false>(a, max_new, (cudaStream_t)stream);
+Q3_EXPORT int q3_attention_tree_tc_bf16(const q3_attention_tree_args* x) {
+    if (x->n_seqs <= 0 || x->max_new <= 0) return 0;
+    const int refused = tree_refused(*x, D);
+    if (refused != 0) return refused;
+    if (!(x->scale > 0.0)) return Q3_ERR_BAD_SIZE;                                   // the maximum is taken before the scale
+    if (x->n_pages * x->nkv * PAGE > 0x7fffffff) return Q3_ERR_TOO_LARGE;            // a row's number is a coordinate of a copy
+    const Args a = {tree_step(*x), (const bf16*)x->q, (bf16*)x->out, (const unsigned char*)x->k_pages, (const unsigned char*)x->v_pages,
+                    (const uint8_t*)x->k_scales, (const uint8_t*)x->v_scales, (float*)x->parts, (int*)x->status, (float)x->scale * 1.4426950408889634f};
+    return x->k_scales != nullptr ? launch<true>(a, x->max_new, (cudaStream_t)x->stream) : launch<false>(a, x->max_new, (cudaStream_t)x->stream);
 }

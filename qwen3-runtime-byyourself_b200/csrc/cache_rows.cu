@@ -8,6 +8,7 @@
 // Norm and rotation as in attention.cu's qkv_prepare (src/model/self_attention.cpp:122-152): y = x / sqrt(mean(x^2) + eps) w
 // over a head, values i and i + r/2 of the first r turned by the angle of the token's position.  A token's place in the
 // cache is given beside its position: drafted tokens of a tree stand side by side at places of their own, several at one position.
+#include "../include/qwen3/cache_args.h"
 #include "page8.cuh"
 
 namespace {
@@ -394,63 +395,42 @@ keep_kernel(unsigned char* __restrict__ store, uint8_t* __restrict__ scales, int
     }
 }
 
-int append(AppendArgs a, bool f32, bool f8, void* stream) {
+int append(const q3_cache_append_args& x, bool f32) {
+    const AppendArgs a = {x.qkv, x.q_out, x.k_pages, x.v_pages, (uint8_t*)x.k_scales, (uint8_t*)x.v_scales, (const float*)x.q_norm, (const float*)x.k_norm,
+                          (const float*)x.cos_tab, (const float*)x.sin_tab, (const int*)x.token_seq, (const int*)x.token_pos, (const int*)x.token_place,
+                          (const int*)x.page_table, x.pages_per_seq, x.nq, x.nkv, x.d, x.rotary_dim, x.norm_once, x.n_pages, x.n_tokens, x.row, (float)x.eps};
     if (a.n_tokens <= 0) return 0;
     if (a.nq <= 0 || a.nkv <= 0 || a.d <= 0 || a.d > 256 || a.rot < 0 || a.rot > a.d || (a.rot & 1) || a.row < (int64_t)(a.nq + 2 * a.nkv) * a.d)
         return Q3_ERR_BAD_SIZE;
-    cudaStream_t s = (cudaStream_t)stream;
+    cudaStream_t s = (cudaStream_t)x.stream;
+    const bool f8 = a.k_scales != nullptr;
     if (f32) return f8 ? launch_append<float, true>(a, s) : launch_append<float, false>(a, s);
     return f8 ? launch_append<bf16, true>(a, s) : launch_append<bf16, false>(a, s);
 }
 
-template <typename T>
-int read(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, const int* page_table, int pages_per_seq,
-         const int* seq_end, int n_seqs, int64_t n_pages, void* k_out, void* v_out, int out_pages, int nkv, int d, void* stream) {
-    if (n_seqs <= 0 || out_pages <= 0) return 0;
-    if (nkv <= 0 || d <= 0 || d > 256) return Q3_ERR_BAD_SIZE;
-    if (n_seqs > 65535 || nkv > 65535) return Q3_ERR_TOO_LARGE;
-    return (int)q3_launch(read_kernel<T>, dim3(out_pages, nkv, n_seqs), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)k_pages,
-                          (const uint8_t*)v_pages, (const uint8_t*)k_scales, (const uint8_t*)v_scales, page_table, pages_per_seq, seq_end,
-                          n_pages, (T*)k_out, (T*)v_out, out_pages, nkv, d,
-                          d % 8 == 0 && aligned16(k_pages) && aligned16(v_pages) && aligned16(k_out) && aligned16(v_out));
+template <typename T> int read(const q3_cache_read_args& x) {
+    if (x.n_seqs <= 0 || x.out_pages <= 0) return 0;
+    if (x.nkv <= 0 || x.d <= 0 || x.d > 256) return Q3_ERR_BAD_SIZE;
+    if (x.n_seqs > 65535 || x.nkv > 65535) return Q3_ERR_TOO_LARGE;
+    return (int)q3_launch(read_kernel<T>, dim3(x.out_pages, x.nkv, x.n_seqs), dim3(256), 0, (cudaStream_t)x.stream, (const uint8_t*)x.k_pages,
+                          (const uint8_t*)x.v_pages, (const uint8_t*)x.k_scales, (const uint8_t*)x.v_scales, (const int*)x.page_table, x.pages_per_seq,
+                          (const int*)x.seq_end, x.n_pages, (T*)x.k_out, (T*)x.v_out, x.out_pages, x.nkv, x.d,
+                          x.d % 8 == 0 && aligned16(x.k_pages) && aligned16(x.v_pages) && aligned16(x.k_out) && aligned16(x.v_out));
 }
 
 }  // namespace
 
-Q3_EXPORT int q3_cache_append_f32(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_scales, void* v_scales, const float* q_norm,
-                                  const float* k_norm, const float* cos_tab, const float* sin_tab, float eps, const int* token_seq,
-                                  const int* token_pos, const int* token_place, const int* page_table, int pages_per_seq, int64_t n_pages,
-                                  int64_t n_tokens, int64_t row, int nq, int nkv, int d, int rotary_dim, int norm_once, void* stream) {
-    return append({qkv, q_out, k_pages, v_pages, (uint8_t*)k_scales, (uint8_t*)v_scales, q_norm, k_norm, cos_tab, sin_tab, token_seq, token_pos,
-                   token_place, page_table, pages_per_seq, nq, nkv, d, rotary_dim, norm_once, n_pages, n_tokens, row, eps},
-                  true, k_scales != nullptr, stream);
-}
-Q3_EXPORT int q3_cache_append_bf16(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_scales, void* v_scales, const float* q_norm,
-                                   const float* k_norm, const float* cos_tab, const float* sin_tab, float eps, const int* token_seq,
-                                   const int* token_pos, const int* token_place, const int* page_table, int pages_per_seq, int64_t n_pages,
-                                   int64_t n_tokens, int64_t row, int nq, int nkv, int d, int rotary_dim, int norm_once, void* stream) {
-    return append({qkv, q_out, k_pages, v_pages, (uint8_t*)k_scales, (uint8_t*)v_scales, q_norm, k_norm, cos_tab, sin_tab, token_seq, token_pos,
-                   token_place, page_table, pages_per_seq, nq, nkv, d, rotary_dim, norm_once, n_pages, n_tokens, row, eps},
-                  false, k_scales != nullptr, stream);
-}
+Q3_EXPORT int q3_cache_append_f32(const q3_cache_append_args* a) { return append(*a, true); }
+Q3_EXPORT int q3_cache_append_bf16(const q3_cache_append_args* a) { return append(*a, false); }
+Q3_EXPORT int q3_cache_read_f32(const q3_cache_read_args* a) { return read<float>(*a); }
+Q3_EXPORT int q3_cache_read_bf16(const q3_cache_read_args* a) { return read<bf16>(*a); }
 
-Q3_EXPORT int q3_cache_read_f32(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, const int* page_table,
-                                int pages_per_seq, const int* seq_end, int n_seqs, int64_t n_pages, void* k_out, void* v_out, int out_pages,
-                                int nkv, int d, void* stream) {
-    return read<float>(k_pages, v_pages, k_scales, v_scales, page_table, pages_per_seq, seq_end, n_seqs, n_pages, k_out, v_out, out_pages, nkv, d, stream);
-}
-Q3_EXPORT int q3_cache_read_bf16(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, const int* page_table,
-                                 int pages_per_seq, const int* seq_end, int n_seqs, int64_t n_pages, void* k_out, void* v_out, int out_pages,
-                                 int nkv, int d, void* stream) {
-    return read<bf16>(k_pages, v_pages, k_scales, v_scales, page_table, pages_per_seq, seq_end, n_seqs, n_pages, k_out, v_out, out_pages, nkv, d, stream);
-}
-
-Q3_EXPORT int q3_cache_keep(void* store, void* scales, int64_t n_areas, int64_t n_pages, int nkv, int row_bytes, const int* page_table,
-                            int pages_per_seq, const int* seq_pos0, const int* path, int path_len, int n_seqs, void* stream) {
-    if (n_areas <= 0 || n_seqs <= 0 || path_len <= 0) return 0;
-    if (nkv <= 0 || row_bytes <= 0) return Q3_ERR_BAD_SIZE;
-    if (n_seqs > 65535 || n_areas > 0x7fffffff) return Q3_ERR_TOO_LARGE;
-    if (row_bytes % 16 != 0 || !aligned16(store)) return Q3_ERR_MISALIGNED;
-    return (int)q3_launch(keep_kernel, dim3((unsigned)n_areas, n_seqs), dim3(256), 0, (cudaStream_t)stream, (unsigned char*)store,
-                          (uint8_t*)scales, n_pages, nkv, row_bytes, page_table, pages_per_seq, seq_pos0, path, path_len);
+Q3_EXPORT int q3_cache_keep(const q3_cache_keep_args* a) {
+    if (a->n_areas <= 0 || a->n_seqs <= 0 || a->path_len <= 0) return 0;
+    if (a->nkv <= 0 || a->row_bytes <= 0) return Q3_ERR_BAD_SIZE;
+    if (a->n_seqs > 65535 || a->n_areas > 0x7fffffff) return Q3_ERR_TOO_LARGE;
+    if (a->row_bytes % 16 != 0 || !aligned16(a->store)) return Q3_ERR_MISALIGNED;
+    return (int)q3_launch(keep_kernel, dim3((unsigned)a->n_areas, a->n_seqs), dim3(256), 0, (cudaStream_t)a->stream, (unsigned char*)a->store,
+                          (uint8_t*)a->scales, a->n_pages, a->nkv, a->row_bytes, (const int*)a->page_table, a->pages_per_seq, (const int*)a->seq_pos0,
+                          (const int*)a->path, a->path_len);
 }

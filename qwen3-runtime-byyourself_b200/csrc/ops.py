@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from dataclasses import dataclass
 from ctypes import c_float, c_int, c_int64, c_uint64, c_void_p
 from typing import Optional
@@ -1348,7 +1349,37 @@ def attention_decode_flat_parts(d: int, group: int) -> int:
 
 
 # ------------------------------------------------------------------ a cache in 8 bits, steps with drafted tokens
-SCALE_BYTES = (-60 + 127, 60 + 127)      # the scales that a row of 8-bit codes can have: 2^-60 to 2^60
+# Arguments go to these kernels as a structure (include/qwen3/cache_args.h): packed in half a microsecond, where two dozen arguments through ctypes take
+# two.  A call from Python is as long as the kernels of a small step: attention of one sequence took 12.9 us of the host, the kernel 7.8.
+_APPEND_ARGS, _READ_ARGS, _KEEP_ARGS = struct.Struct("@15q3qd6i"), struct.Struct("@9qq6i"), struct.Struct("@6q2q6i")
+_TREE_ARGS = struct.Struct("@14q2qd8i")
+_packed_fns = {}
+
+
+def _call_packed(what: str, source: str, name: str, args: bytes, d: int = 0) -> None:
+    """Calls an entry point that takes a structure of arguments; `d`: the head size that its source is compiled for (0: any)."""
+    global _launches
+    fn = _packed_fns.get((name, d))
+    if fn is None:
+        fn = _packed_fns[name, d] = _fn_untimed(source, name, [ctypes.c_char_p], defines=(f"Q3_HEAD_DIM={d}",) if d else ())
+    code = fn(args) if _timer is None else _timer.run(name, fn, (args,))
+    if code:
+        _check(code, what)
+    _launches += 1
+
+
+def _at(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """Where a tensor lies, as `_dev`."""
+    if t.is_cuda and t.dtype is dtype and t.is_contiguous():
+        return t.data_ptr()
+    return _dev(t, name, dtype)
+
+
+def _here() -> int:
+    return _pinned_stream if _pinned_stream is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
 
 class CachePages:
@@ -1378,10 +1409,11 @@ class CachePages:
 
     def pointers(self, dtype: torch.dtype, what: str):
         """(keys, values, key scales, value scales) for a launch on rows of `dtype`."""
-        if not self.eight_bit and self.keys.dtype != dtype:
+        if self.eight_bit:
+            return self.keys.data_ptr(), self.values.data_ptr(), self.key_scales.data_ptr(), self.value_scales.data_ptr()
+        if self.keys.dtype != dtype:
             raise KernelError(f"{what}: pages of {self.keys.dtype} for rows of {dtype}")
-        scales = (self.key_scales.data_ptr(), self.value_scales.data_ptr()) if self.eight_bit else (None, None)
-        return (self.keys.data_ptr(), self.values.data_ptr()) + scales
+        return self.keys.data_ptr(), self.values.data_ptr(), 0, 0
 
 
 def cache_append(qkv: torch.Tensor, q_out: torch.Tensor, cache: CachePages, q_norm_w, k_norm_w, cos, sin, eps: float, token_seq,
@@ -1390,19 +1422,18 @@ def cache_append(qkv: torch.Tensor, q_out: torch.Tensor, cache: CachePages, q_no
     `qkv_prepare` for such a cache and for drafted tokens.  `token_pos` [tokens] is the position by which a token is rotated,
     `token_place` its place in the sequence's cache (drafted tokens of a tree: several at one position, side by side in the cache).
     A token whose place has no page is not written.  `norm_once`: a normed and rotated value is rounded once, when it is stored."""
-    s, n, d = _suffix(qkv), token_seq.numel(), cache.d
-    if qkv.dim() != 2 or qkv.shape[0] < n or qkv.shape[1] < (nq + 2 * cache.kv_heads) * d or nq <= 0 or page_table.dim() != 2 \
-            or token_pos.numel() < n or token_place.numel() < n or q_out.numel() < n * nq * d \
-            or any(w is not None and w.numel() != d for w in (q_norm_w, k_norm_w)) or (q_norm_w is None) != (k_norm_w is None):
+    s, n, d, dtype, shape, row_of = _suffix(qkv), token_seq.numel(), cache.d, qkv.dtype, qkv.shape, page_table.shape
+    if len(shape) != 2 or shape[0] < n or shape[1] < (nq + 2 * cache.kv_heads) * d or nq <= 0 or len(row_of) != 2 \
+            or token_pos.numel() < n or token_place.numel() < n or q_out.numel() < n * nq * d or (q_norm_w is None) != (k_norm_w is None) \
+            or (q_norm_w is not None and (q_norm_w.numel() != d or k_norm_w.numel() != d)):
         raise KernelError("cache_append: shapes do not fit")
-    fn = _fn("cache_rows.cu", f"q3_cache_append_{s}",
-             [c_void_p] * 10 + [c_float] + [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64] + [c_int] * 5 + [c_void_p])
-    _check(fn(_dev(qkv, "qkv"), _dev(q_out, "q_out", qkv.dtype), *cache.pointers(qkv.dtype, "cache_append"),
-              _ptr(q_norm_w, "q_norm_w", torch.float32), _ptr(k_norm_w, "k_norm_w", torch.float32),
-              _ptr(cos, "cos", torch.float32), _ptr(sin, "sin", torch.float32), float(eps), _dev(token_seq, "token_seq", torch.int32),
-              _dev(token_pos, "token_pos", torch.int32), _dev(token_place, "token_place", torch.int32),
-              _dev(page_table, "page_table", torch.int32), page_table.shape[1], cache.n_pages, n, qkv.shape[1], nq, cache.kv_heads, d,
-              _rotary_dim(cos, sin, d), int(bool(norm_once)), _stream()), "cache_append")
+    norms = (_at(q_norm_w, "q_norm_w", _F32), _at(k_norm_w, "k_norm_w", _F32)) if q_norm_w is not None else (0, 0)
+    rotary = _rotary_dim(cos, sin, d)
+    angles = (_at(cos, "cos", _F32), _at(sin, "sin", _F32)) if cos is not None else (0, 0)
+    _call_packed("cache_append", "cache_rows.cu", "q3_cache_append_" + s, _APPEND_ARGS.pack(
+        _at(qkv, "qkv", dtype), _at(q_out, "q_out", dtype), *cache.pointers(dtype, "cache_append"), *norms, *angles,
+        _at(token_seq, "token_seq", _I32), _at(token_pos, "token_pos", _I32), _at(token_place, "token_place", _I32), _at(page_table, "page_table", _I32), _here(),
+        cache.n_pages, n, shape[1], float(eps), row_of[1], nq, cache.kv_heads, d, rotary, 1 if norm_once else 0))
     return q_out
 
 
@@ -1412,15 +1443,13 @@ def cache_read(cache: CachePages, page_table, seq_end, keys_out: torch.Tensor, v
     them in the last page are zeros, pages behind it stay as they are."""
     if not cache.eight_bit:
         raise KernelError("cache_read: the cache is not in 8 bits")
-    n = seq_end.numel()
-    if page_table.dim() != 2 or page_table.shape[0] < n or keys_out.dim() != 5 or keys_out.shape[0] < n or keys_out.shape[2:] != cache.keys.shape[1:] \
-            or values_out.shape != keys_out.shape or values_out.dtype != keys_out.dtype:
+    n, out, row_of = seq_end.numel(), keys_out.shape, page_table.shape
+    if len(row_of) != 2 or row_of[0] < n or len(out) != 5 or out[0] < n or out[2:] != cache.keys.shape[1:] or values_out.shape != out:
         raise KernelError("cache_read: shapes do not fit")
-    fn = _fn("cache_rows.cu", f"q3_cache_read_{_suffix(keys_out)}",
-             [c_void_p] * 5 + [c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p] + [c_int] * 3 + [c_void_p])
-    _check(fn(*cache.pointers(keys_out.dtype, "cache_read"), _dev(page_table, "page_table", torch.int32), page_table.shape[1],
-              _dev(seq_end, "seq_end", torch.int32), n, cache.n_pages, _dev(keys_out, "keys_out"), _dev(values_out, "values_out"),
-              keys_out.shape[1], cache.kv_heads, cache.d, _stream()), "cache_read")
+    s, dtype = _suffix(keys_out), keys_out.dtype
+    _call_packed("cache_read", "cache_rows.cu", "q3_cache_read_" + s, _READ_ARGS.pack(
+        *cache.pointers(dtype, "cache_read"), _at(page_table, "page_table", _I32), _at(seq_end, "seq_end", _I32), _at(keys_out, "keys_out", dtype),
+        _at(values_out, "values_out", dtype), _here(), cache.n_pages, row_of[1], n, out[1], cache.kv_heads, cache.d, 0))
 
 
 def cache_keep(store: torch.Tensor, scales: Optional[torch.Tensor], page_table, seq_pos0, path) -> None:
@@ -1428,20 +1457,19 @@ def cache_keep(store: torch.Tensor, scales: Optional[torch.Tensor], page_table, 
     [sequences, n]: the numbers of these tokens among the sequence's new ones, ascending, -1 behind the last; row seq_pos0 + path[i]
     goes to seq_pos0 + i.  `store` [..., pages, kv heads, PAGE_TOKENS, head size]: the keys and values of every layer of a
     cache group, all moved alike; `scales` [..., pages, kv heads, PAGE_TOKENS] of a store in 8 bits."""
-    eight_bit = store.dtype == torch.float8_e4m3fn
-    if store.dim() < 4 or store.shape[-2] != PAGE_TOKENS or (not eight_bit and store.dtype not in _SUFFIX) or eight_bit != (scales is not None) \
-            or (eight_bit and scales.shape != store.shape[:-1]):
+    shape, dtype, row_of, steps = store.shape, store.dtype, page_table.shape, path.shape
+    eight_bit = dtype == torch.float8_e4m3fn
+    if len(shape) < 4 or shape[-2] != PAGE_TOKENS or (not eight_bit and dtype not in _SUFFIX) or eight_bit != (scales is not None) \
+            or (eight_bit and scales.shape != shape[:-1]):
         raise KernelError(f"cache_keep: the store is [..., pages, kv heads, {PAGE_TOKENS}, head size] of float32, bfloat16 or float8_e4m3fn, "
                           "the latter with scales")
-    if path.dim() != 2 or page_table.dim() != 2 or page_table.shape[0] < path.shape[0] or seq_pos0.numel() < path.shape[0]:
+    if len(steps) != 2 or len(row_of) != 2 or row_of[0] < steps[0] or seq_pos0.numel() < steps[0]:
         raise KernelError("cache_keep: shapes do not fit")
-    n_pages, nkv, _, d = store.shape[-4:]
-    areas = math.prod(store.shape[:-4])
-    fn = _fn("cache_rows.cu", "q3_cache_keep", [c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                                                c_int, c_int, c_void_p])
-    _check(fn(_dev(store, "store"), _ptr(scales, "scales", torch.float8_e8m0fnu), areas, n_pages, nkv, d * store.element_size(),
-              _dev(page_table, "page_table", torch.int32), page_table.shape[1], _dev(seq_pos0, "seq_pos0", torch.int32),
-              _dev(path, "path", torch.int32), path.shape[1], path.shape[0], _stream()), "cache_keep")
+    n_pages, nkv, _, d = shape[-4:]
+    _call_packed("cache_keep", "cache_rows.cu", "q3_cache_keep", _KEEP_ARGS.pack(
+        _at(store, "store", dtype), _at(scales, "scales", torch.float8_e8m0fnu) if eight_bit else 0, _at(page_table, "page_table", _I32),
+        _at(seq_pos0, "seq_pos0", _I32), _at(path, "path", _I32), _here(), math.prod(shape[:-4]), n_pages, nkv, d * store.element_size(), row_of[1], steps[1],
+        steps[0], 0))
 
 
 @dataclass
@@ -1454,6 +1482,9 @@ class TreeScratch:
 # Rows of a kv head (new tokens of a sequence x query heads a kv head) from which a step with drafted tokens goes to the tcgen05 kernel.
 tree_tc_rows = 33
 _tree_parts = {}
+# source, entry point, whether it is compiled for a head size
+_TREE_FORMS = {"any": ("attention_tree.cu", "q3_attention_tree_any_", False), "mma": ("attention_tree_mma.cu", "q3_attention_tree_mma_", True),
+               "tc": ("attention_tree_tc.cu", "q3_attention_tree_tc_", True)}
 
 
 def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int) -> str:
@@ -1493,39 +1524,30 @@ def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts:
     and, of the new ones, number n where bit n % 64 of tree[token, n // 64] is set (`tree` int64 [tokens, words]); without `tree`
     those up to itself.  A token that sees nothing gets zeros.  q, out [tokens, nq * head size]; `parts` and `counters` as
     `attention_tree_scratch` says."""
-    s, n, d, nkv = _suffix(q), q.shape[0], cache.d, cache.kv_heads
-    n_seqs = seq_pos0.numel()
-    if q.dim() != 2 or q.shape[1] != nq * d or out.shape != q.shape or nq <= 0 or nq % nkv or page_table.dim() != 2 \
-            or page_table.shape[0] < n_seqs or seq_start.numel() < n_seqs + 1 or max_new <= 0:
+    s, dtype, shape, d, nkv = _suffix(q), q.dtype, q.shape, cache.d, cache.kv_heads
+    n_seqs, row_of = seq_pos0.numel(), page_table.shape
+    if len(shape) != 2 or shape[1] != nq * d or out.shape != shape or nq <= 0 or nq % nkv or len(row_of) != 2 \
+            or row_of[0] < n_seqs or seq_start.numel() < n_seqs + 1 or max_new <= 0:
         raise KernelError("attention_tree: shapes do not fit")
-    if tree is not None and (tree.dim() != 2 or tree.shape[0] < n or tree.shape[1] * 64 < max_new):
-        raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
-    words = 0 if tree is None else tree.shape[1]
-    tensors = (_dev(q, "q"), *cache.pointers(q.dtype, "attention_tree"), _dev(out, "out", q.dtype))
-    lists = (_dev(seq_start, "seq_start", torch.int32), _dev(seq_pos0, "seq_pos0", torch.int32), _dev(page_table, "page_table", torch.int32),
-             page_table.shape[1], cache.n_pages, n_seqs)
-    masks = _ptr(tree, "tree", torch.int64)
-    rows = max_new * (nq // nkv)
-    form = _tree_form(q.dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS)
+    masks = words = 0
+    if tree is not None:
+        if tree.dim() != 2 or tree.shape[0] < shape[0] or tree.shape[1] * 64 < max_new:
+            raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
+        masks, words = _at(tree, "tree", torch.int64), tree.shape[1]
+    q_at, rows, parts_at, counters_at, status = _at(q, "q", dtype), max_new * (nq // nkv), 0, 0, 0
+    form = _tree_form(dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS)
     if form != "any":
         if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 8):
             raise KernelError("attention_tree: parts or counters are too small (attention_tree_scratch)")
-        parts_at = _dev(parts, "parts", torch.float32)
+        parts_at, counters_at = _at(parts, "parts", _F32), _at(counters, "counters", _I32)
         if form == "tc":
-            fn = _fn("attention_tree_tc.cu", "q3_attention_tree_tc_bf16",
-                     [c_void_p] * 10 + [c_int, c_int64] + [c_int] * 4 + [c_float, c_void_p, c_int, c_void_p, c_void_p], defines=(f"Q3_HEAD_DIM={d}",))
-            _check(fn(*tensors, parts_at, *lists, max_new, nq, nkv, float(scale), masks, words, _status_word(q.device).data_ptr(), _stream()),
-                   "attention_tree")
+            status = _status_word(q.device).data_ptr()
             _count_extra(1)
-            return out
-        fn = _fn("attention_tree_mma.cu", "q3_attention_tree_mma_bf16",
-                 [c_void_p] * 11 + [c_int, c_int64] + [c_int] * 4 + [c_float, c_void_p, c_int, c_void_p], defines=(f"Q3_HEAD_DIM={d}",))
-        _check(fn(*tensors, parts_at, _dev(counters, "counters", torch.int32), *lists, max_new, nq, nkv, float(scale), masks, words, _stream()),
-               "attention_tree")
-        return out
-    fn = _fn("attention_tree.cu", f"q3_attention_tree_any_{s}",
-             [c_void_p] * 9 + [c_int, c_int64, c_int, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_int, c_void_p])
-    _check(fn(*tensors, *lists, n, nq, nkv, d, float(scale), masks, words, _stream()), "attention_tree")
+    source, name, size = _TREE_FORMS[form]
+    _call_packed("attention_tree", source, name + s, _TREE_ARGS.pack(
+        q_at, *cache.pointers(dtype, "attention_tree"), _at(out, "out", dtype), parts_at, counters_at, _at(seq_start, "seq_start", _I32),
+        _at(seq_pos0, "seq_pos0", _I32), _at(page_table, "page_table", _I32), masks, status, _here(), cache.n_pages, shape[0], float(scale), row_of[1], n_seqs, max_new,
+        nq, nkv, d, words, 0), d if size else 0)
     return out
 
 

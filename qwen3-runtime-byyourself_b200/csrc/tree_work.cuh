@@ -10,6 +10,7 @@
 // and on nothing else.
 #pragma once
 
+#include "../include/qwen3/cache_args.h"
 #include "common.cuh"
 
 struct TreeStep {
@@ -19,6 +20,19 @@ struct TreeStep {
     int64_t n_pages;
     int max_new;                                   // no sequence brings more tokens (those that one brings beyond are left out)
 };
+static inline TreeStep tree_step(const q3_attention_tree_args& a) {
+    return {(const int*)a.seq_start, (const int*)a.seq_pos0, (const int*)a.page_table, (const unsigned long long*)a.tree, a.words, a.pages_per_seq, a.n_seqs, a.nq,
+            a.nkv, a.n_pages, a.max_new};
+}
+// What is wrong with the arguments of a tensor-core form (0: nothing).
+static inline int tree_refused(const q3_attention_tree_args& a, int d) {
+    if (a.nq <= 0 || a.nkv <= 0 || a.nq % a.nkv != 0 || a.d != d || a.n_pages <= 0 || a.pages_per_seq <= 0 ||
+        (a.tree != nullptr && (a.words <= 0 || (int64_t)a.words * 64 < a.max_new)))
+        return Q3_ERR_BAD_SIZE;
+    for (const void* p : {a.q, a.k_pages, a.v_pages, a.k_scales, a.v_scales, (const void*)a.out, (const void*)a.parts})
+        if (!aligned16(p)) return Q3_ERR_MISALIGNED;
+    return 0;
+}
 
 // A range of stretches [begin, end) of one item.
 struct TreePart {

@@ -23,6 +23,8 @@
 
 #include <stdint.h>
 
+#include "cache_args.h"
+
 #define Q3_ERR_BAD_SIZE 10001        /* a size the kernel does not take */
 #define Q3_ERR_TOO_LARGE 10002       /* more rows, heads or blocks than one launch takes */
 #define Q3_ERR_MISALIGNED 10003      /* a pointer or stride that is not 16-byte aligned */
@@ -493,56 +495,27 @@ int q3_ssd_prompt_bf16(const void* x, const void* B, const void* C_rows, int64_t
                        void* stream);
 int q3_ssd_segments(int n_seqs, int max_new, int heads);
 
-/* ---- cache_rows.cu: rows of the cache, in the compute type or as e4m3 codes with a scale of a power of two a row ---- */
-/* k_scales, v_scales [pages, kv heads, 64] (bytes: exponent + 127) or null: codes in k_pages, v_pages, or values of the compute type.
-   Per-head norm (weights may be null), rotation of the first rotary_dim values by the token's position (tables may be null), q to
-   q_out, k and v to the token's place in its sequence's cache (nowhere, if there is no page); norm_once: one rounding, at the end */
-int q3_cache_append_f32(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_scales, void* v_scales, const float* q_norm,
-                        const float* k_norm, const float* cos_tab, const float* sin_tab, float eps, const int* token_seq,
-                        const int* token_pos, const int* token_place, const int* page_table, int pages_per_seq, int64_t n_pages,
-                        int64_t n_tokens, int64_t row, int nq, int nkv, int d, int rotary_dim, int norm_once, void* stream);
-int q3_cache_append_bf16(const void* qkv, void* q_out, void* k_pages, void* v_pages, void* k_scales, void* v_scales, const float* q_norm,
-                         const float* k_norm, const float* cos_tab, const float* sin_tab, float eps, const int* token_seq,
-                         const int* token_pos, const int* token_place, const int* page_table, int pages_per_seq, int64_t n_pages,
-                         int64_t n_tokens, int64_t row, int nq, int nkv, int d, int rotary_dim, int norm_once, void* stream);
-/* pages of codes as pages of values: page j of sequence s to number s * out_pages + j, as far as it holds some of the first seq_end[s] rows */
-int q3_cache_read_f32(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, const int* page_table,
-                      int pages_per_seq, const int* seq_end, int n_seqs, int64_t n_pages, void* k_out, void* v_out, int out_pages, int nkv,
-                      int d, void* stream);
-int q3_cache_read_bf16(const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, const int* page_table,
-                       int pages_per_seq, const int* seq_end, int n_seqs, int64_t n_pages, void* k_out, void* v_out, int out_pages, int nkv,
-                       int d, void* stream);
-/* in each of n_areas areas [pages, kv heads, 64, row_bytes] (scales: a byte a row, or null): row seq_pos0 + path[i] to seq_pos0 + i; a path
-   ascends, -1 ends it */
-int q3_cache_keep(void* store, void* scales, int64_t n_areas, int64_t n_pages, int nkv, int row_bytes, const int* page_table,
-                  int pages_per_seq, const int* seq_pos0, const int* path, int path_len, int n_seqs, void* stream);
+/* ---- cache_rows.cu: rows of the cache, in the compute type or in 8 bits (arguments: cache_args.h, read before the call returns) ---- */
+int q3_cache_append_f32(const q3_cache_append_args* args);
+int q3_cache_append_bf16(const q3_cache_append_args* args);
+int q3_cache_read_f32(const q3_cache_read_args* args);
+int q3_cache_read_bf16(const q3_cache_read_args* args);
+int q3_cache_keep(const q3_cache_keep_args* args);
 
-/* ---- attention_tree.cu: new tokens - one, a run or a tree of drafted ones a sequence - over the cache's pages (any head size) ---- */
-/* a token sees the seq_pos0 earlier rows and, of the new ones, number n where bit n % 64 of tree[token][n / 64] is set (tree null:
-   those up to itself); k_scales, v_scales as above */
-int q3_attention_tree_any_f32(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
-                              const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq, int64_t n_pages,
-                              int n_seqs, int64_t n_tokens, int nq, int nkv, int d, float scale, const void* tree, int words, void* stream);
-int q3_attention_tree_any_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
-                               const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq, int64_t n_pages,
-                               int n_seqs, int64_t n_tokens, int nq, int nkv, int d, float scale, const void* tree, int words, void* stream);
+/* ---- attention_tree.cu: new tokens - one, a run or a tree of drafted ones a sequence - over the cache's pages (any head size up to 256) ---- */
+int q3_attention_tree_any_f32(const q3_attention_tree_args* args);
+int q3_attention_tree_any_bf16(const q3_attention_tree_args* args);
 
 /* ---- attention_tree_mma.cu (-DQ3_HEAD_DIM=64 or 128): the same for bfloat16 queries, 32 rows (new tokens x query heads of a kv head) at a time ---- */
 int q3_attention_tree_mma_head_dim(void);
-/* float32 values of `parts` for so many rows a sequence; `counters`: an int32, zero when made and left zero, for each sequence, kv head and 8 rows */
+/* float32 values of `parts` for so many rows a sequence; `counters`: one for each sequence, kv head and 8 rows */
 int64_t q3_attention_tree_mma_parts(int rows);
-int q3_attention_tree_mma_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
-                               float* parts, int* counters, const int* seq_start, const int* seq_pos0, const int* page_table,
-                               int pages_per_seq, int64_t n_pages, int n_seqs, int max_new, int nq, int nkv, float scale, const void* tree,
-                               int words, void* stream);
+int q3_attention_tree_mma_bf16(const q3_attention_tree_args* args);
 
 /* ---- attention_tree_tc.cu (-DQ3_HEAD_DIM=64 or 128): the same on tcgen05, 256 rows at a time; scale > 0; two launches ---- */
 int q3_attention_tree_tc_head_dim(void);
 int64_t q3_attention_tree_tc_parts(void);
-int q3_attention_tree_tc_bf16(const void* q, const void* k_pages, const void* v_pages, const void* k_scales, const void* v_scales, void* out,
-                              float* parts, const int* seq_start, const int* seq_pos0, const int* page_table, int pages_per_seq,
-                              int64_t n_pages, int n_seqs, int max_new, int nq, int nkv, float scale, const void* tree, int words,
-                              int* status, void* stream);
+int q3_attention_tree_tc_bf16(const q3_attention_tree_args* args);
 
 /* ---- sampling.cu ------------------------------------------------------------------------------------------ */
 /* out[r] = index of the highest logit among the first `valid` (lowest id among equals, NaN as -inf) */
