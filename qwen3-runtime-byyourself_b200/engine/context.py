@@ -7,7 +7,7 @@ below are views of it.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Tuple
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -96,3 +96,16 @@ class StepContext:
     host_slots: List[int] = field(default_factory=list)
     host_n_new: List[int] = field(default_factory=list)
     host_pos0: List[int] = field(default_factory=list)
+    # a step with drafted tokens (Engine.step_tree): token_pos is then the place in the tree, and the tokens stand side by side in the cache
+    token_place: Optional[torch.Tensor] = None    # [N] int32: the token's place in its sequence's cache (None: token_pos)
+    tree: Optional[torch.Tensor] = None           # [N, words] int64: bit n of a token's mask: it sees its sequence's new token n
+    _ends: Optional[tuple] = field(default=None, repr=False)
+
+    def read_back(self, pages: int):
+        """For caches in 8 bits that are read back for a step: the sequences' lengths after the step, and the table of `pages` pages
+        a sequence in their order (made once a step)."""
+        if self._ends is None:
+            ends = self.seq_pos0 + (self.seq_start[1:] - self.seq_start[:-1])
+            table = torch.arange(self.n_seqs * pages, dtype=torch.int32, device=self.device).view(self.n_seqs, pages)
+            self._ends = (ends, table)
+        return self._ends

@@ -42,6 +42,15 @@ class StepEntry:
     want: Sequence[int] = ()
 
 
+@dataclass
+class TreeEntry:
+    """One sequence's drafted tokens: its slot, the tokens and, for each, the number of the one it follows among them (an earlier one;
+    -1: the sequence's last cached token)."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
 class StepError(ValueError):
     """A step that cannot run: empty, out-of-vocabulary ids, a wanted place outside the tokens."""
 
@@ -207,17 +216,29 @@ class Engine:
     """Weights, cache, scratch and stream state of one model on one GPU."""
 
     def __init__(self, model: Model, config, max_tokens: int, max_seq_len: Optional[int] = None,
-                 n_slots: Optional[int] = None, use_graphs: bool = True, guard_scratch: bool = False):
-        """`guard_scratch` (tests): activation buffers of exact size between guard zones; see `scratch_violations`."""
+                 n_slots: Optional[int] = None, use_graphs: bool = True, guard_scratch: bool = False,
+                 cache_dtype: Optional[str] = None):
+        """`guard_scratch` (tests): activation buffers of exact size between guard zones; see `scratch_violations`.
+        `cache_dtype` "float8": keys and values are kept as 8-bit codes with a scale of a power of two for each row of a head (129 bytes
+        instead of 256 at head size 128), for models of plain attention over all keys; None: as they are computed."""
         if model.dtype is None:
             raise ValueError("the model has no weights bound")
         self.model, self.config, self.plan = model, config, model.plan
         self.dtype, self.device = model.dtype, model.device
         if self.device.type != "cuda":
             raise KernelBuildError("the engine runs on a CUDA device only; there is no CPU path")
+        if cache_dtype not in (None, "float8"):
+            raise ValueError(f"cache_dtype {cache_dtype!r}: None (as computed) or 'float8'")
+        # whether every layer takes rows at places of their own: a cache in 8 bits, steps with drafted tokens
+        self.takes_rows = not model.cache_sources() and all(getattr(b.mixer, "takes_rows", lambda: False)() for b in model.blocks)
+        if cache_dtype is not None and not self.takes_rows:
+            raise ValueError("a cache in 8 bits takes a model whose layers are all plain attention over all keys")
         max_seq_len = min(max_seq_len or self.plan.max_positions, self.plan.max_positions)
         self.cache = KVCache(model.cache_needs(), max_tokens, max_seq_len, self.dtype, self.device, n_slots,
-                             cache_from=model.cache_sources())
+                             cache_from=model.cache_sources(), eight_bit=cache_dtype is not None)
+        self._drafted = {}         # slot -> parents of the drafted tokens of the last `step_tree`, until `keep`
+        self._tree_meta = _MetaBuffer(self.device)
+        self._tree_ctx = None
         self.max_seq_len = self.cache.max_seq_len
         self.vocab_size = self.plan.vocab_size
         self.scratch = Scratch(self.device, guard=guard_scratch)
@@ -242,7 +263,7 @@ class Engine:
     @classmethod
     def from_folder(cls, folder: str, dtype=None, max_tokens: int = 4096, max_seq_len: Optional[int] = None,
                     device="cuda:0", n_slots: Optional[int] = None, use_graphs: bool = True,
-                    guard_scratch: bool = False) -> "Engine":
+                    guard_scratch: bool = False, cache_dtype: Optional[str] = None) -> "Engine":
         """Load config.json and the safetensors of `folder`; the model class is chosen by config.json."""
         config = load_config(folder)
         model = build_model(config.plan())
@@ -251,20 +272,20 @@ class Engine:
         source = open_upload(folder, model.weight_specs(), model.ignorable_names(), compute, device, model._warn_rounding)
         model.bind(source, compute, device)
         source.finish()
-        engine = cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch)
+        engine = cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
         engine.weights_arena = source.arena                    # the parts' tensors are views of it
         return engine
 
     @classmethod
     def from_random(cls, config, seed: int, dtype=None, max_tokens: int = 4096, max_seq_len: Optional[int] = None,
                     device="cuda:0", n_slots: Optional[int] = None, use_graphs: bool = True,
-                    guard_scratch: bool = False) -> "Engine":
+                    guard_scratch: bool = False, cache_dtype: Optional[str] = None) -> "Engine":
         """Seeded random weights drawn on the device (no folder is written)."""
         model = build_model(config.plan())
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
         weights = random_weights(model.weight_specs(), seed, dtype=compute, device=device)
         model.bind(weights, compute, device)
-        return cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch)
+        return cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
 
     # -- sequences
     def new_sequence(self) -> int:
@@ -272,7 +293,8 @@ class Engine:
         return self.cache.alloc_slot()
 
     def release(self, slot: int) -> None:
-        """The sequence is finished: its slot and pages are given back."""
+        """The sequence is finished: its slot and pages are given back (those of drafted tokens that were not kept, too)."""
+        self._drafted.pop(int(slot), None)
         self.cache.free_slot(slot)
 
     def length(self, slot: int) -> int:
@@ -298,6 +320,8 @@ class Engine:
         entries' own tokens only stand for the count."""
         if not entries:
             raise StepError("a step needs at least one sequence")
+        if self._drafted:
+            raise StepError("the drafted tokens of the last step wait for `keep`")
         slots, n_new, tokens, want_rows = [], [], [], []
         start = 0
         for e in entries:
@@ -336,6 +360,89 @@ class Engine:
             raise
         self.cache.commit(step)
         return logits
+
+    # -- drafted tokens
+    def step_tree(self, entries: Sequence[TreeEntry]) -> torch.Tensor:
+        """Run trees of drafted tokens, one for each entry, as one batch over the sequences' caches: every token sees the sequence, the
+        drafted tokens that it follows, and itself, and stands at the position that its depth gives.  Returns float32 logits [tokens, vocab] in
+        the order of the entries and their tokens (scratch: valid until the next step).  The sequences do not grow: `keep` says which of the
+        tokens stand, and comes before any other step."""
+        if not self.takes_rows:
+            raise StepError("drafted tokens take a model whose layers are all plain attention over all keys")
+        if self._drafted:
+            raise StepError("the drafted tokens of the last step wait for `keep`")
+        if not entries:
+            raise StepError("a step needs at least one sequence")
+        slots, n_new, tokens, depths, seen = [], [], [], [], []
+        words = -(-max(len(e.tokens) for e in entries) // 64)
+        for e in entries:
+            toks, parents = np.asarray(e.tokens, dtype=np.int64).reshape(-1), [int(p) for p in e.parents]
+            if toks.size == 0 or len(parents) != toks.size:
+                raise StepError(f"slot {e.slot}: a tree needs at least one token, and a parent for each")
+            if toks.min() < 0 or toks.max() >= self.vocab_size:
+                raise StepError(f"slot {e.slot}: token id outside the vocabulary [0, {self.vocab_size})")
+            if any(not -1 <= p < i for i, p in enumerate(parents)):
+                raise StepError(f"slot {e.slot}: a drafted token follows an earlier one of its tree, or (-1) the sequence")
+            depth, mask = [], []
+            for i, p in enumerate(parents):
+                depth.append(depth[p] + 1 if p >= 0 else 0)
+                mask.append((mask[p] if p >= 0 else 0) | 1 << i)
+            slots.append(int(e.slot)); n_new.append(int(toks.size)); tokens.append(toks)
+            depths.append(np.asarray(depth, dtype=np.int32))
+            seen.extend([m >> 64 * w & 0xFFFFFFFFFFFFFFFF for w in range(words)] for m in mask)
+        step, N = list(zip(slots, n_new)), sum(n_new)
+        self.cache.reserve(step)                            # raises before anything is launched
+        try:
+            from ..csrc import ops
+            before = ops.launch_count()
+            pos0 = [self.cache.length(s) for s in slots]
+            ctx = self._build_context(slots, n_new, pos0, np.concatenate(tokens), list(range(N)))
+            lead = -(-N // 2) * 2                           # the masks begin at a whole word
+            host = self._tree_meta.stage(lead + 2 * N * words)
+            host[:N] = np.concatenate([d + p for d, p in zip(depths, pos0)])
+            host[lead:].view(np.uint64)[:] = np.asarray(seen, dtype=np.uint64).reshape(-1)
+            self._tree_meta.upload(lead + 2 * N * words)
+            ctx.token_place, ctx.token_pos = ctx.token_pos, self._tree_meta.dev[:N]
+            ctx.tree = self._tree_meta.dev[lead:lead + 2 * N * words].view(torch.int64).view(N, words)
+            with ops.on_current_stream():
+                logits = self.model.forward(ctx, self.cache)
+            self.launches += ops.launch_count() - before
+        except BaseException:
+            self.cache.cancel(step)
+            raise
+        self._drafted = {e.slot: [int(p) for p in e.parents] for e in entries}
+        self._tree_ctx = ctx
+        return logits
+
+    def keep(self, paths) -> None:
+        """Which of the last `step_tree`'s tokens stand: for every slot of it the numbers of those tokens, each one following the one
+        before it (an empty list: none).  Their rows move up behind the sequences, which grow by them; the others' are given up."""
+        if not self._drafted:
+            raise StepError("no drafted tokens wait for `keep`")
+        if set(paths) != set(self._drafted):
+            raise StepError(f"`keep` names the slots {sorted(self._drafted)} of the last tree step, got {sorted(paths)}")
+        rows = {}
+        for slot, parents in self._drafted.items():
+            path = [int(i) for i in paths[slot]]
+            for before, i in zip([-1] + path, path):
+                if not 0 <= i < len(parents) or parents[i] != before:
+                    raise StepError(f"slot {slot}: {path} is no path of its tree")
+            rows[slot] = path
+        from ..csrc import ops
+        slots, ctx = list(self._drafted), self._tree_ctx
+        if any(path != list(range(len(path))) for path in rows.values()):
+            most = max(len(p) for p in rows.values())
+            in_step = [rows.get(s, []) for s in ctx.host_slots]       # (a sequence may have ended since: nothing of it moves)
+            moves = torch.tensor([p + [-1] * (most - len(p)) for p in in_step], dtype=torch.int32, device=self.device)
+            for store, scales, table in zip(self.cache.stores, self.cache.scales, ctx.page_tables):
+                ops.cache_keep(store, scales, table, ctx.seq_pos0, moves)
+        kept = [(s, len(rows[s])) for s in slots if rows[s]]
+        if kept:
+            self.cache.commit(kept)
+        given_up = [(s, len(self._drafted[s]) - len(rows[s])) for s in slots if len(rows[s]) < len(self._drafted[s])]
+        if given_up:
+            self.cache.cancel(given_up)                     # from the new lengths on
+        self._drafted, self._tree_ctx = {}, None
 
     def _step_captured(self, slots, pos0, token_ids, want_rows, device_tokens):
         rows = decode_bucket(len(slots))

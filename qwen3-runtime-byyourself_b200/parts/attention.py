@@ -42,6 +42,7 @@ values of its own (no tensors of them) and reads another layer's cache.
 """
 from __future__ import annotations
 
+import dataclasses
 import functools
 from fractions import Fraction
 from typing import List, Optional
@@ -311,6 +312,8 @@ class GQAAttention(Part):
         N = ctx.n_tokens
         table = ctx.page_tables[cache.group]
         attn = ctx.scratch.get("attn.ctx", (N, nq * vd), torch.float32 if self.out_float32 else ctx.dtype)
+        if cache.key_scales is not None or ctx.tree is not None:
+            return self.mix_rows(x, ctx, cache, attn, table)
         if self.shared_kv and not cache.shared:
             raise ops.KernelError("attention without keys of its own needs another layer's cache")
         norm_eps = self.q_norm.eps if self.q_norm is not None else 0.0
@@ -372,6 +375,44 @@ class GQAAttention(Part):
         if self.out_gate or self.value_position is not None:
             gate = qkv[:, self.projection_width() - nq * vd:] if self.out_gate else None
             ops.turn_back_gate(attn, v_cos, v_sin, ctx.token_pos, gate, nq, vd)
+        return attn
+
+    def takes_rows(self) -> bool:
+        """Whether a cache in 8 bits and steps with drafted tokens can be had of this layer: plain attention over all keys, with rotation
+        tables or no rotation."""
+        return (type(self).mix is GQAAttention.mix and self.plain and not self.window
+                and (self.position is None or getattr(self.position, "fused_tables", False)))
+
+    def mix_rows(self, x, ctx, cache, attn, table) -> torch.Tensor:
+        """`mix` over a cache in 8 bits, and for a step with drafted tokens over any: rows are appended at places of their own, and the few
+        new tokens of a sequence attend to the pages as they are.  Longer prompts over a cache in 8 bits read it back first, for the prompt kernels."""
+        if not self.takes_rows() or cache.shared:
+            raise ops.KernelError("this attention takes neither a cache in 8 bits nor drafted tokens")
+        nq, nkv, d, N = self.num_heads, self.num_kv_heads, self.head_dim, ctx.n_tokens
+        cos = sin = None
+        if self.position is not None:
+            self.position.prepare(ctx.max_positions, ctx.device)
+            cos, sin = self.position.cos, self.position.sin
+        qkv = linear(x, self.w_qkv, ctx.scratch.get("attn.qkv", (N, self.projection_width()), ctx.dtype))
+        q = ctx.scratch.get("attn.q", (N, nq * d), ctx.dtype)
+        pages, token_pos = cache.rows(), ctx.token_pos[:N]
+        norms = (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps) if self.q_norm is not None else (None, None, 0.0)
+        ops.cache_append(qkv, q, pages, norms[0], norms[1], cos, sin, norms[2], ctx.token_seq[:N], token_pos,
+                         token_pos if ctx.token_place is None else ctx.token_place, table, nq, norm_once=self.norm_once)
+        if ctx.tree is not None or ctx.max_new <= rows_at_once:
+            sizes = ops.attention_tree_scratch(ctx.n_seqs, ctx.max_new, nq, nkv, d, ctx.device)
+            parts = ctx.scratch.get("attn.tree_parts", (sizes.parts,), torch.float32)
+            counters = ctx.scratch.counters("attn.tree_counters", sizes.counters)
+            return ops.attention_tree(q, pages, attn, parts, counters, ctx.seq_start, ctx.seq_pos0, table, ctx.max_new, nq, self.scale,
+                                      tree=ctx.tree)
+        per_seq = -(-ctx.max_context // ops.PAGE_TOKENS)
+        shape = (ctx.n_seqs, per_seq, nkv, ops.PAGE_TOKENS, d)
+        keys, values = (ctx.scratch.get(name, shape, ctx.dtype) for name in ("attn.read_keys", "attn.read_values"))
+        ends, read_table = ctx.read_back(per_seq)
+        ops.cache_read(pages, table, ends, keys, values)
+        flat = (ctx.n_seqs * per_seq, nkv, ops.PAGE_TOKENS, d)
+        self.attend(q, dataclasses.replace(cache, keys=keys.view(flat), values=values.view(flat), key_scales=None, value_scales=None, _rows=None), attn, ctx,
+                    read_table)
         return attn
 
     def decodes_split(self, ctx) -> bool:
@@ -634,6 +675,9 @@ def _decode_capped_fused_kernel(part, qkv, cache, out, ctx, table, q_norm_w, k_n
     return True
 
 
+# Over a cache in 8 bits the sequences of a step that bring at most so many tokens attend to the pages as they are; with more the step reads its
+# sequences' pages back for the prompt kernels, which then share a head's keys among many tiles of rows.
+rows_at_once = 64
 long_context_keys = 4096  # a decode step whose sequences may be longer takes wider clusters (if they are few)
 # Rows (sequences x kv heads) an SM of a decode step beyond which its pages are shared out evenly: the other form has two blocks an SM,
 # so beyond as many rows as SMs it takes every row in one block.  The attention of 8 kv heads of 128 there / here, us: 19 sequences of 130
