@@ -121,6 +121,13 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 // kind::f16 instruction descriptor: float32 accumulator, operands both half precision or both bfloat16; bit 16 = B is MN-major.
 constexpr uint32_t idesc(bool half, int m, int n, bool b_mn_major) {
     return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -301,24 +308,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 if constexpr (F8) {
+                    // a row's numbers by one power of two into half precision, each thread its own row
+                    __syncwarp();
+                    uint32_t tops = 0;
 #pragma unroll 4
-                    for (int i = 0; i < TURNS; ++i) {
-                        const uint32_t at_chunk = queries + chunk_at((warp & 3) * 32 + i * AT_ONCE + lane / PER_ROW, c, BM * 128);
+                    for (int i = 0; i < PER_ROW; ++i) {
+                        const uint4 w = ld_shared_v4(queries + chunk_at(r, i, BM * 128));
+                        tops = __vmaxu2(tops, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+                    }
+                    int e2 = (int)(max(tops & 0xffffu, tops >> 16) >> 7) - 127;
+                    e2 = e2 >= 128 ? 0 : min(max(e2, -60), 60);
+                    const float down = q3_exp2i(-e2);
+                    factor *= q3_exp2i(e2);
+#pragma unroll 4
+                    for (int i = 0; i < PER_ROW; ++i) {
+                        const uint32_t at_chunk = queries + chunk_at(r, i, BM * 128);
                         uint4 w = ld_shared_v4(at_chunk);
                         uint32_t* v = &w.x;
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) top = max(top, max(v[e] & 0x7fffu, v[e] >> 16 & 0x7fffu));
-#pragma unroll
-                        for (int o = PER_ROW / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        int e2 = (int)(top >> 7) - 127;
-                        e2 = e2 >= 128 ? 0 : min(max(e2, -60), 60);
-                        const float down = q3_exp2i(-e2);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[e] = pack2<true>(__uint_as_float(v[e] << 16) * down, __uint_as_float(v[e] & 0xffff0000u) * down);
                         st_shared_v4(at_chunk, w);
-                        const float up = __shfl_sync(0xffffffffu, q3_exp2i(e2), (lane % AT_ONCE) * PER_ROW);   // of row i AT_ONCE + lane % AT_ONCE
-                        if (lane / AT_ONCE == i) factor = a.scale_log2 * up;
                     }
                 }
                 fence_proxy_async();
@@ -342,9 +351,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (!ok) { failed(42); break; }
                 }
                 tc_fence_after();
-                uint32_t s[64];
-                tc_ld32(t_s, s);
-                tc_ld32(t_s + 32, s + 32);
                 // ---- of the page: score = dot * c1, in log2 units, and v0
                 float c1 = factor, v0 = 0.0f;
                 bool rests = false;
@@ -353,28 +359,44 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     v0 = sh.values[note].scale;
                     rests = (sh.keys[note].flags[0] | sh.keys[note].flags[1] | sh.values[note].flags[0] | sh.values[note].flags[1]) & 1u;
                 }
-                tc_wait_ld();
                 if (edge) {
+                    // scores of keys that the row does not see become minus infinity where they lie
                     const unsigned long long* mask = st.tree != nullptr ? st.tree + (int64_t)(t0 + own) * st.words : nullptr;
                     const unsigned long long seen = tree_seen(mask, st.words, pos0, n_new, own, key0);
                     uint32_t flags = sh.values[note].flags[0] | sh.values[note].flags[1];
                     if constexpr (!F8) flags |= sh.values[note].flags[2] | sh.values[note].flags[3];
                     if (flags & 2u) find_odd<F8>(a, st.page_table + (int64_t)part.seq * st.pages_per_seq, part.head, part.begin + n, seen, odd);
-                    const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        if (!(lo >> e & 1u)) s[e] = 0xff800000u;
-                        if (!(hi >> e & 1u)) s[e + 32] = 0xff800000u;
-                    }
                     __syncwarp();
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t s[32];
+                        const uint32_t bits = (uint32_t)(seen >> (32 * h));
+                        tc_ld32(t_s + 32 * h, s);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(bits >> e & 1u)) s[e] = 0xff800000u;
+                        tc_st32(t_s + 32 * h, s);
+                    }
+                    tc_wait_st();
                 }
                 // ---- the maximum of x + v0 (and the rests)
                 float top;
                 if (F8 && rests) {
                     top = -INFINITY;
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t s[32];
+                        tc_ld32(t_s + 32 * h, s);
+                        tc_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) top = fmaxf(top, fmaf(__uint_as_float(s[e]) * sh.key_rest[note][e], c1, sh.value_rest[note][e]));
+                        for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaf(__uint_as_float(s[e]) * sh.key_rest[note][32 * h + e], c1, sh.value_rest[note][32 * h + e]));
+                    }
                 } else {
+                    uint32_t s[64];
+                    tc_ld32(t_s, s);
+                    tc_ld32(t_s + 32, s + 32);
+                    tc_wait_ld();
                     float mx[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 4]));
@@ -396,35 +418,41 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 const float shift = v0 - (m_run == -INFINITY ? 0.0f : m_run);
                 const float2 c2 = make_float2(c1, c1), shift2 = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                uint32_t p[32];
-                if (F8 && rests) {
-                    // (where nothing is left by the folds, these are the other path's numbers to the bit: a row does not feel the scales of
-                    // keys that it does not see)
+                __syncwarp();
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t s[32], p[16];
+                    tc_ld32(t_s + 32 * h, s);
+                    tc_wait_ld();
+                    if (F8 && rests) {
+                        // (where nothing is left by the folds, these are the other path's numbers to the bit: a row does not feel the scales of
+                        // keys that it does not see)
 #pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
-                        float w[2];
+                        for (int e = 0; e < 32; e += 2) {
+                            float w[2];
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float rest = sh.value_rest[note][e + k];
-                            w[k] = ex2(fmaf(__uint_as_float(s[e + k]) * sh.key_rest[note][e + k], c1, shift + rest));
-                            float& to_sum = k == 0 ? sum[(e >> 1) & 1].x : sum[(e >> 1) & 1].y;
-                            to_sum = fmaf(w[k], ex2(-rest), to_sum);
+                            for (int k = 0; k < 2; ++k) {
+                                const float rest = sh.value_rest[note][32 * h + e + k];
+                                w[k] = ex2(fmaf(__uint_as_float(s[e + k]) * sh.key_rest[note][32 * h + e + k], c1, shift + rest));
+                                float& to_sum = k == 0 ? sum[(e >> 1) & 1].x : sum[(e >> 1) & 1].y;
+                                to_sum = fmaf(w[k], ex2(-rest), to_sum);
+                            }
+                            p[e / 2] = pack2<true>(w[0], w[1]);
                         }
-                        p[e / 2] = pack2<true>(w[0], w[1]);
-                    }
-                } else {
+                        __syncwarp();
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 64; e += 2) {
-                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, shift2);
-                        const float2 w = make_float2(ex2(z.x), ex2(z.y));
-                        sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], w);
-                        p[e / 2] = pack2<F8>(w.x, w.y);
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), c2, shift2);
+                            const float2 w = make_float2(ex2(z.x), ex2(z.y));
+                            sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], w);
+                            p[e / 2] = pack2<F8>(w.x, w.y);
+                        }
                     }
+                    tc_st16(t_s + 16 * h, p);
                 }
                 const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 l_run += F8 ? total * ex2(-v0) : total;
-                __syncwarp();
-                tc_st32(t_s, p);
                 // the products of the page before have to be done where O is rescaled, and once the part ends: this page's are waited for then, and a
                 // parity tells a phase from the next one, not from the one after that
                 const bool rescale = n > first && __any_sync(0xffffffffu, raise);
@@ -436,6 +464,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (rescale) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 64) {
+                        uint32_t s[64];
                         tc_ld32(t_tile + COL_O + c, s);
                         tc_ld32(t_tile + COL_O + c + 32, s + 32);
                         tc_wait_ld();
