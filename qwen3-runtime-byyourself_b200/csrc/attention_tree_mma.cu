@@ -33,6 +33,9 @@ constexpr int WARPS = 4;
 template <int NT> constexpr int blocks_per_sm = NT == 4 ? 2 : 3;
 template <int NT> constexpr int stages = NT == 4 ? 3 : 2;
 constexpr int LEAST_PAGES = 4;                      // of a block's range
+// Pages that take about as long as beginning and ending a part.  0 / 4 / 8 / 12: 64 sequences of up to 2,000 keys and one new token (8 bits) 57 / 44 / 42 / 42 us,
+// of up to 9,000 123 / 113 / 113 / 110, with four new tokens 129 / 102 / 83 / 82, of 130 20 / 14.6 / 15.2 / 15.2.
+constexpr int PART_PAGES = 8;
 constexpr float RAISE = 8.0f;
 
 template <bool F8> struct Form {
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const TreeShare found = Work::share(st, LEAST_PAGES, 8, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, LEAST_PAGES, 8, PART_PAGES, blockIdx.x, gridDim.x);
         if (lane == 0) *shared_share = found;
     }
     __syncthreads();
@@ -155,6 +158,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
 
     for (int at = share.from; at < share.to;) {
         const TreePart part = Work::part(st, share, at, blockIdx.x);
+        if (part.begin >= part.end) break;
         const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
         const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0);      // row i of the tile: token (row0 + i) / group, head (row0 + i) % group
         const int key_begin = part.begin * PAGE, key_end = min(part.end * PAGE, pos0 + n_new);
@@ -577,8 +581,8 @@ template <bool F8, int NT> int launch(const Args& a, int sm_count, cudaStream_t 
     const cudaError_t e = q3_allow_shared_memory(tree_mma_kernel<F8, NT>, bytes, configured);
     if (e != cudaSuccess) return (int)e;
     using Work = TreeWork<PAGE, 8 * NT, false>;
-    const int64_t units = Work::most_units(a.step), most = (units + LEAST_PAGES - 1) / LEAST_PAGES + Work::most_items(a.step);
-    if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
+    const int64_t units = Work::most_units(a.step, 0), most = (units + LEAST_PAGES - 1) / LEAST_PAGES + Work::most_items(a.step);
+    if (Work::most_units(a.step, PART_PAGES) > 0x3fffffff) return Q3_ERR_TOO_LARGE;
     const int resident = blocks_per_sm<NT> * sm_count, grid = (int)(most < resident ? most : resident);
     return (int)q3_launch(tree_mma_kernel<F8, NT>, dim3(grid), dim3(WARPS * 32), (size_t)bytes, stream, a);
 }

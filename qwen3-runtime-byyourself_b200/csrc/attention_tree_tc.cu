@@ -51,6 +51,9 @@ constexpr int CODE_BYTES = PAGE * D;
 constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, COL_S = 0, COL_O = 128;              // of tile x, from x * 256 on; two buffers of S, P lies over S
 constexpr int Q_BYTES = HALVES * BM * 128, MEET_COLS = D / 2;                             // a tile's queries; columns of the sums that meet at a time
 static_assert(BM * MEET_COLS * 4 <= Q_BYTES, "they meet where the second tile's queries would be");
+// Pages that take about as long as beginning and ending a part.  0 / 3 / 6 / 9: 32 sequences of up to 4,000 keys and 32 new tokens (bfloat16) 129 / 93 / 78 /
+// 76 us, 8 of up to 8,000 and 64 (8 bits) 118 / 100 / 95 / 99.
+constexpr int PART_PAGES = 6;
 constexpr float RAISE = 8.0f;
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
@@ -260,7 +263,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 2, 20, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, 2, 20, PART_PAGES, blockIdx.x, gridDim.x);
         if (lane == 0) sh.share = found;
     }
     tc_fence_before();
@@ -284,6 +287,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
+            if (part.begin >= part.end) break;
             const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
             const int all_rows = n_new * group - part.tile * ROWS, steps = part.end - part.begin;
             const bool split = all_rows <= BM;                                       // one tile of rows: every other page
@@ -585,6 +589,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
             const TreePart part = Work::part(st, share, at, blockIdx.x);
+            if (part.begin >= part.end) break;
             const int pos0 = st.seq_pos0[part.seq], key_end = pos0 + Work::n_new(st, part.seq), steps = part.end - part.begin;
             if constexpr (F8) {
                 // ------------------------------------------------ codes to half precision, a page two warps, each 32 rows of it, D / 16 lanes a row: 25
@@ -731,6 +736,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
                 const TreePart part = Work::part(st, share, at, blockIdx.x);
+            if (part.begin >= part.end) break;
                 const bool split = Work::n_new(st, part.seq) * group - part.tile * ROWS <= BM;
                 const int steps = part.end - part.begin, first = split ? x : 0, stride = split ? 2 : 1;
                 auto scores = [&](uint32_t buffer) {                                 // of the page at k_at
@@ -796,6 +802,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
                 const TreePart part = Work::part(st, share, at, blockIdx.x);
+            if (part.begin >= part.end) break;
                 const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
                 int64_t page = page_of(st, table, part.begin);
                 for (int i = part.begin; i < part.end; ++i, ++number) {
@@ -893,9 +900,9 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
     if (!F8 && (!q3_make_map_bf16(&map_k, a.keys, a.step.n_pages * a.step.nkv * PAGE, D, PAGE, 64, true) ||
                 !q3_make_map_bf16(&map_v, a.values, a.step.n_pages * a.step.nkv * PAGE, D, PAGE, 64, true)))
         return Q3_ERR_BAD_SIZE;
-    const int64_t units = Work::most_units(a.step);
+    const int64_t units = Work::most_units(a.step, PART_PAGES);
     if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
-    const int64_t most = (units + 1) / 2 + Work::most_items(a.step);
+    const int64_t most = (Work::most_units(a.step, 0) + 1) / 2 + Work::most_items(a.step);
     const int sms = q3_device_sm_count(), blocks = (int)(most < sms ? most : sms);
     int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)smem_bytes<F8>, stream, map_k, map_v, a);
     if (code != 0) return code;

@@ -5,7 +5,8 @@
 //   pieces  every item is cut into equal pieces of at most `quota` stretches, and a block takes one piece.  `quota` is the best of four numbers between
 //           the even share and one at which the pieces are certainly no more than the blocks, or that is longer by what a second part would cost a block;
 //   ranges  the stretches of all items in a row are cut into ranges of equal length, one a block, wherever they fall: a block has at most a
-//           part of an item, some whole ones and another part.  Taken where there are no such pieces.
+//           part of an item, some whole ones and another part.  Taken where there are no such pieces.  In the row every item is longer by `pad` stretches
+//           before its first one, for the time that beginning and ending it takes: a block with five short items is not the last.
 // Parts of an item are added up in their order.  Which part is whose, and so the order of a row's sums, hangs on the lengths of all sequences of the step
 // and on nothing else.
 #pragma once
@@ -48,7 +49,7 @@ struct TreePart {
 // What a block has: in the way of ranges stretches [from, to) of the list (none: from >= to), else one piece.
 struct TreeShare {
     int from, to, quota;                           // quota: a range's length, or (`pieces`) the most stretches of a piece
-    int pieces;                                    // 1: pieces
+    int pieces, pad;                               // 1: pieces; what an item is longer by, counted as lengths are (pieces: 0)
     int seq, before, items_before;                 // where `from` (a piece: the block's number) lies: its sequence, the stretches (pieces) and items before it
 };
 
@@ -60,7 +61,7 @@ struct TreeItems {
 
     __device__ __forceinline__ int cut(int length, int quota) const { return (int)((unsigned)(length + quota - 1) / (unsigned)quota); }
     // A head's length, or its pieces of up to `quota`.
-    __device__ __forceinline__ int of_head() const { return (per_head - light) * full + light * lighter; }
+    __device__ __forceinline__ int of_head(int pad) const { return (per_head - light) * full + light * lighter + per_head * pad; }
     __device__ __forceinline__ int pieces_of_head(int quota) const { return units == 0 ? 0 : (per_head - light) * cut(full, quota) + (light ? cut(lighter, quota) : 0); }
 };
 
@@ -82,7 +83,9 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
 
     // The most items and counted stretches that a step can have (the latter have to stay below 2^30).
     static __host__ int64_t most_items(const TreeStep& a) { return (int64_t)a.n_seqs * a.nkv * tiles_of(a.max_new, a.nq / a.nkv); }
-    static __host__ int64_t most_units(const TreeStep& a) { return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT); }
+    static __host__ int64_t most_units(const TreeStep& a, int pad) {
+        return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT + pad);
+    }
 
     static __device__ __forceinline__ int warp_total(int v) {
 #pragma unroll
@@ -91,8 +94,8 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
     }
 
     // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more);
-    // `spare`: so many stretches take about as long as beginning and ending a part.
-    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int block, int blocks) {
+    // `spare`: a piece may be longer than the even share by so many, rather than that blocks have several parts; `pad`: see above.
+    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int pad, int block, int blocks) {
         const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
@@ -105,10 +108,11 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
             return warp_total(sum) * a.nkv;
         };
         TreeShare t;
-        const int total = each([](const TreeItems& i) { return i.of_head(); }), items = each([](const TreeItems& i) { return i.per_head; });
-        const int even = (max(least * COUNT, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks)) + COUNT - 1) & ~(COUNT - 1);
+        const int items = each([](const TreeItems& i) { return i.per_head; });
+        int total = each([](const TreeItems& i) { return i.of_head(0); });
+        auto even_of = [&] { return (max(least * COUNT, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks)) + COUNT - 1) & ~(COUNT - 1); };
+        const int even = even_of();
         t.pieces = 0;
-        t.quota = even;
         if (items < blocks) {
             // with pieces of `safe` there are at most items + total / safe of them
             const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + spare * COUNT;
@@ -120,6 +124,11 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                 }
             }
         }
+        t.pad = t.pieces ? 0 : pad * COUNT;
+        if (!t.pieces) {
+            total += items * t.pad;
+            t.quota = even_of();
+        }
         // where the block's range or piece begins
         const int at = t.pieces ? block : (int)min((int64_t)total, (int64_t)block * t.quota);
         t.from = at;
@@ -128,7 +137,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const int s = s0 + lane;
             const TreeItems here = few ? mine : s < a.n_seqs ? items_of(a, s) : none;
-            const int own = a.nkv * (t.pieces ? here.pieces_of_head(t.quota) : here.of_head()), count = a.nkv * here.per_head;
+            const int own = a.nkv * (t.pieces ? here.pieces_of_head(t.quota) : here.of_head(t.pad)), count = a.nkv * here.per_head;
             int sum = own, counts = count;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -154,19 +163,20 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         return t;
     }
 
-    // The part at `at` (t.from, then what `next` says) of a block's share; `t` is moved on to the sequence that holds it.
+    // The part at `at` (t.from, then what `next` says) of a block's share; `t` is moved on to the sequence that holds it.  The last part of a range may be
+    // empty (begin == end): the range ends before the item's first stretch.
     static __device__ __forceinline__ TreePart part(const TreeStep& a, TreeShare& t, int at, int block) {
         TreePart p;
         while (true) {
             const TreeItems i = items_of(a, t.seq);
-            const int head = t.pieces ? i.pieces_of_head(t.quota) : i.of_head(), in = at - t.before;
+            const int head = t.pieces ? i.pieces_of_head(t.quota) : i.of_head(t.pad), in = at - t.before;
             if (in < head * a.nkv) {
                 p.seq = t.seq;
                 p.head = (int)((unsigned)in / (unsigned)head);
-                const int in_head = in - p.head * head, a_full = t.pieces ? i.cut(i.full, t.quota) : i.full;     // numbers that a tile that is not light has
+                const int in_head = in - p.head * head, a_full = t.pieces ? i.cut(i.full, t.quota) : i.full + t.pad;     // numbers that a tile that is not light has
                 p.tile = min((int)((unsigned)in_head / (unsigned)a_full), i.per_head - 1);
                 const int off = in_head - p.tile * a_full, light = i.light && p.tile == i.per_head - 1 ? 1 : 0;
-                const int length = light ? i.lighter : i.full, count = light ? 1 : COUNT;
+                const int length = (light ? i.lighter : i.full) + t.pad, count = light ? 1 : COUNT;
                 p.item = t.items_before + p.head * i.per_head + p.tile;
                 if (t.pieces) {
                     p.parts = i.cut(length, t.quota);
@@ -178,11 +188,11 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                     p.list_end = at + 1;
                 } else {
                     const int item_begin = at - off, to = min(length, t.to - item_begin);
-                    p.begin = off / count;                               // (whole: ranges and items begin with whole stretches)
-                    p.end = min(i.units, to / count);
-                    p.first_block = (int)((unsigned)item_begin / (unsigned)t.quota);
+                    p.begin = max(0, off - t.pad) / count;               // (whole: ranges, items and their pads begin with whole stretches)
+                    p.end = min(i.units, max(0, to - t.pad) / count);
+                    p.first_block = (int)((unsigned)(item_begin + t.pad) / (unsigned)t.quota);
                     p.parts = (int)((unsigned)(item_begin + length - 1) / (unsigned)t.quota) - p.first_block + 1;
-                    p.slot0 = 2 * p.first_block + (p.first_block * t.quota == item_begin ? 0 : 1);
+                    p.slot0 = 2 * p.first_block + (p.first_block * t.quota >= item_begin ? 0 : 1);
                     p.slot = 2 * block + (at == t.from ? 0 : 1);
                     p.list_end = item_begin + to;
                 }
