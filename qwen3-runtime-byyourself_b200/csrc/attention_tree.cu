@@ -5,14 +5,17 @@
 // places pos0, pos0 + 1, ... of the cache), number n where bit n % 64 of word n / 64 of its mask is set; without masks those up to
 // itself.  out = sum_j p_j v_j, p = softmax over the keys it sees of scale q . k; a token that sees none gets zeros.  Keys and values are
 // of the query's type or codes of 8 bits with a scale a row (page8.cuh).
-// A block a (token, query head): four warps take every fourth key, each with a running maximum and sum of its own, and meet at the
-// end.  A key that is not seen is not read.  Bound by the latency of its chain of keys: it is here for 32-bit queries and odd head sizes.
+// A block a (token, query head): each of its warps takes every eighth stretch of 32 keys, with a running maximum and sum of its own, and they meet at the
+// end.  The stretch's scores are made eight keys at a time, so that many loads are on their way; then its maximum and its weights, a key a lane; then
+// its values are added up, eight at a time again.  A key that is not seen is not read.  It is here for 32-bit queries and odd head sizes, and bound by the
+// latency of its loads: one token of 32 heads over 8 and 2,000 keys, 32-bit, 110 us (one key after the other 443), 8 sequences of them and 8 tokens each 877 (1,598); rows
+// that share a head's keys read them from the L2 again.
 #include "../include/qwen3/cache_args.h"
 #include "page8.cuh"
 
 namespace {
 
-constexpr int PAGE = Q3_PAGE_TOKENS, WARPS = 4, PER = 8;              // values of a head a lane: up to 256 in all
+constexpr int PAGE = Q3_PAGE_TOKENS, WARPS = 8, KEYS = 8;                     // keys whose loads are on their way together
 
 struct TreeArgs {
     const void *q, *k_pages, *v_pages;
@@ -25,13 +28,18 @@ struct TreeArgs {
     float scale;
 };
 
+// Value i of a row, zero beyond its end (without a branch: loads of several rows go out together).
 template <typename T, bool F8>
 __device__ __forceinline__ float value_at(const void* pages, int64_t cell, int d, int i) {
-    if constexpr (F8) return __low2float(q3_half2_of(((const uint8_t*)pages)[cell * d + i]));
-    else return to_f32<T>(((const T*)pages)[cell * d + i]);
+    const int64_t at = cell * d + min(i, d - 1);
+    float v;
+    if constexpr (F8) v = __low2float(q3_half2_of(((const uint8_t*)pages)[at]));
+    else v = to_f32<T>(((const T*)pages)[at]);
+    return i < d ? v : 0.0f;
 }
 
-template <typename T, bool F8>
+// PER: values of a head a lane.
+template <typename T, bool F8, int PER>
 __global__ void __launch_bounds__(WARPS * 32) tree_any_kernel(const TreeArgs a) {
     __shared__ float s_max[WARPS], s_sum[WARPS], s_out[WARPS][256];
     pdl_launch_dependents();
@@ -55,29 +63,60 @@ __global__ void __launch_bounds__(WARPS * 32) tree_any_kernel(const TreeArgs a) 
         o[t] = 0.0f;
     }
     const int keys = pos0 + (mask != nullptr ? min(n_new, a.words * 64) : own + 1);
-    for (int j = warp; j < keys; j += WARPS) {
-        const int x = j - pos0;
-        if (x >= 0 && mask != nullptr && !(mask[x >> 6] >> (x & 63) & 1)) continue;
-        if (j / PAGE >= a.pages_per_seq) break;
-        const int64_t page = a.page_table[(int64_t)seq * a.pages_per_seq + j / PAGE];
+    for (int j0 = warp * 32; j0 < keys && j0 / PAGE < a.pages_per_seq; j0 += WARPS * 32) {
+        const int64_t page = a.page_table[(int64_t)seq * a.pages_per_seq + j0 / PAGE];
         if (page < 0 || page >= a.n_pages) continue;
-        const int64_t cell = (page * a.nkv + g) * PAGE + j % PAGE;
-        float s = 0.0f;
-#pragma unroll
-        for (int t = 0; t < PER; ++t)
-            if (lane + 32 * t < d) s += q[t] * value_at<T, F8>(a.k_pages, cell, d, lane + 32 * t);
-        s = warp_sum(s) * a.scale;
-        float vs = 1.0f;
-        if constexpr (F8) {
-            s *= q3_exp2i((int)a.k_scales[cell] - Q3_SCALE_BIAS);
-            vs = q3_exp2i((int)a.v_scales[cell] - Q3_SCALE_BIAS);
+        const int64_t cell0 = (page * a.nkv + g) * PAGE + j0 % PAGE;
+        const int x = j0 + lane - pos0;
+        const bool sees = j0 + lane < keys && (x < 0 || mask == nullptr || (mask[x >> 6] >> (x & 63) & 1));
+        const unsigned seen = __ballot_sync(0xffffffffu, sees);
+        if (seen == 0) continue;
+        const int some = __ffs(seen) - 1;          // stands in for keys that are not seen
+        float factor = a.scale, vs = 1.0f, s = -INFINITY;
+        if (F8 && sees) {
+            factor = q3_exp2i((int)a.k_scales[cell0 + lane] - Q3_SCALE_BIAS);
+            vs = q3_exp2i((int)a.v_scales[cell0 + lane] - Q3_SCALE_BIAS);
         }
-        const float m_new = fmaxf(m, s), old = m_new == m ? 1.0f : expf(m - m_new), p = s == -INFINITY ? 0.0f : expf(s - m_new);
-        m = m_new;
-        l = l * old + p;
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += KEYS) {
+            if ((seen >> k0 & ((1u << KEYS) - 1u)) == 0) continue;
+            float dot[KEYS];
 #pragma unroll
-        for (int t = 0; t < PER; ++t)
-            if (lane + 32 * t < d) o[t] = o[t] * old + p * (vs * value_at<T, F8>(a.v_pages, cell, d, lane + 32 * t));
+            for (int k = 0; k < KEYS; ++k) {
+                const int64_t cell = cell0 + (seen >> (k0 + k) & 1u ? k0 + k : some);
+                dot[k] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < PER; ++t) dot[k] += q[t] * value_at<T, F8>(a.k_pages, cell, d, lane + 32 * t);
+            }
+#pragma unroll
+            for (int k = 0; k < KEYS; ++k) {
+                const float sum = warp_sum(dot[k]);
+                if (lane == k0 + k) s = sum;
+            }
+        }
+        if (F8) s *= a.scale;
+        s = sees ? s * factor : -INFINITY;
+        const float m_new = fmaxf(m, warp_max(s)), old = m_new == m ? 1.0f : expf(m - m_new), p = s == -INFINITY ? 0.0f : expf(s - m_new);
+        m = m_new;
+        l = l * old + warp_sum(p);
+        const float pv = p * vs;
+#pragma unroll
+        for (int t = 0; t < PER; ++t) o[t] *= old;
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += KEYS) {
+            if ((seen >> k0 & ((1u << KEYS) - 1u)) == 0) continue;
+#pragma unroll
+            for (int k = 0; k < KEYS; ++k) {
+                const bool here = seen >> (k0 + k) & 1u;
+                const int64_t cell = cell0 + (here ? k0 + k : some);
+                const float w = __shfl_sync(0xffffffffu, pv, k0 + k);
+#pragma unroll
+                for (int t = 0; t < PER; ++t) {
+                    const float v = value_at<T, F8>(a.v_pages, cell, d, lane + 32 * t);
+                    o[t] = here ? fmaf(w, v, o[t]) : o[t];
+                }
+            }
+        }
     }
 #pragma unroll
     for (int t = 0; t < PER; ++t)
@@ -104,7 +143,10 @@ __global__ void __launch_bounds__(WARPS * 32) tree_any_kernel(const TreeArgs a) 
 template <typename T, bool F8>
 int launch(const TreeArgs& a, int64_t n_tokens, cudaStream_t stream) {
     const dim3 grid(a.nq, (unsigned)(n_tokens < 65535 ? n_tokens : 65535), (unsigned)((n_tokens + 65534) / 65535));
-    return (int)q3_launch(tree_any_kernel<T, F8>, grid, dim3(WARPS * 32), 0, stream, a);
+    const dim3 block(WARPS * 32);
+    return (int)(a.d <= 64    ? q3_launch(tree_any_kernel<T, F8, 2>, grid, block, 0, stream, a)
+                 : a.d <= 128 ? q3_launch(tree_any_kernel<T, F8, 4>, grid, block, 0, stream, a)
+                              : q3_launch(tree_any_kernel<T, F8, 8>, grid, block, 0, stream, a));
 }
 
 int attend(const q3_attention_tree_args& x, bool f32) {

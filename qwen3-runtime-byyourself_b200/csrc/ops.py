@@ -1491,10 +1491,15 @@ _TREE_FORMS = {"any": ("attention_tree.cu", "q3_attention_tree_any_", False), "m
                "tc": ("attention_tree_tc.cu", "q3_attention_tree_tc_", True)}
 
 
+def attention_tree_tiled(dtype: torch.dtype, d: int) -> bool:
+    """Whether the tensor-core kernels take such queries; the others go to the general kernel, which is slow."""
+    return dtype == torch.bfloat16 and d in (64, 128)
+
+
 def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int, pages: int) -> str:
     """Which kernel takes a step of `rows` rows a kv head at most, over a cache of so many places (pages x kv heads x PAGE_TOKENS): `tc` and `mma`
     take bfloat16 queries and head sizes 64 and 128, `any` the others.  `pages`: an 8-bit cache's that the step can read at most, else 0."""
-    if dtype != torch.bfloat16 or d not in (64, 128):
+    if not attention_tree_tiled(dtype, d):
         return "any"
     return "tc" if rows >= tree_tc_rows and (rows > 32 or pages <= tree_tc_pages) and scale > 0 and places < 2 ** 31 else "mma"
 

@@ -384,8 +384,8 @@ class GQAAttention(Part):
                 and (self.position is None or getattr(self.position, "fused_tables", False)))
 
     def mix_rows(self, x, ctx, cache, attn, table) -> torch.Tensor:
-        """`mix` over a cache in 8 bits, and for a step with drafted tokens over any: rows are appended at places of their own, and the few
-        new tokens of a sequence attend to the pages as they are.  Longer prompts over a cache in 8 bits read it back first, for the prompt kernels."""
+        """`mix` over a cache in 8 bits, and for a step with drafted tokens over any: rows are appended at places of their own, and the
+        new tokens of a sequence attend to the pages as they are.  Long prompts over a cache in 8 bits read it back first, for the prompt kernels."""
         if not self.takes_rows() or cache.shared:
             raise ops.KernelError("this attention takes neither a cache in 8 bits nor drafted tokens")
         nq, nkv, d, N = self.num_heads, self.num_kv_heads, self.head_dim, ctx.n_tokens
@@ -399,7 +399,7 @@ class GQAAttention(Part):
         norms = (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps) if self.q_norm is not None else (None, None, 0.0)
         ops.cache_append(qkv, q, pages, norms[0], norms[1], cos, sin, norms[2], ctx.token_seq[:N], token_pos,
                          token_pos if ctx.token_place is None else ctx.token_place, table, nq, norm_once=self.norm_once)
-        if ctx.tree is not None or ctx.max_new <= rows_at_once:
+        if ctx.tree is not None or ctx.max_new <= (rows_at_once if ops.attention_tree_tiled(ctx.dtype, d) else 1):
             sizes = ops.attention_tree_scratch(ctx.n_seqs, ctx.max_new, nq, nkv, d, ctx.device)
             parts = ctx.scratch.get("attn.tree_parts", (sizes.parts,), torch.float32)
             counters = ctx.scratch.counters("attn.tree_counters", sizes.counters)
@@ -676,8 +676,10 @@ def _decode_capped_fused_kernel(part, qkv, cache, out, ctx, table, q_norm_w, k_n
 
 
 # Over a cache in 8 bits the sequences of a step that bring at most so many tokens attend to the pages as they are; with more the step reads its
-# sequences' pages back for the prompt kernels, which then share a head's keys among many tiles of rows.
-rows_at_once = 64
+# sequences' pages back for the prompt kernels, which then share a head's keys among many tiles of rows.  A small layer with 32 heads of 128 over
+# 8, as they are / read back: 1 sequence of 2,000 tokens and 64 new ones 164 / 229 us, of 16,000 158 / 703; 8 of 4,000 and 64 197 / 395, 256 394 / 399, 512
+# 957 / 1,019, 1,024 2,420 / 2,362.  The general kernel (32-bit queries, other head sizes) is behind from two new tokens on (1 of 2,000: 329 / 237).
+rows_at_once = 512
 long_context_keys = 4096  # a decode step whose sequences may be longer takes wider clusters (if they are few)
 # Rows (sequences x kv heads) an SM of a decode step beyond which its pages are shared out evenly: the other form has two blocks an SM,
 # so beyond as many rows as SMs it takes every row in one block.  The attention of 8 kv heads of 128 there / here, us: 19 sequences of 130

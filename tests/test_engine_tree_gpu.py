@@ -93,6 +93,24 @@ def test_a_cache_in_8_bits_is_near_the_other(tmp_path, name, dtype):
     assert 0 < float(off) < 0.1, float(off)
 
 
+@pytest.mark.parametrize("name", ["C", "D"])
+def test_a_prompt_attends_to_pages_read_back_as_to_the_pages(tmp_path, monkeypatch, name):
+    """The same codes and scales, read by the tree's attention or read back for the prompt kernels: only roundings of the compute type differ."""
+    import qwen3_b200 as q
+    from qwen3_b200.parts import attention
+    engine = engine_of(tmp_path, name, "bfloat16", "float8", seed=4)
+    prompt = random_tokens(np.random.default_rng(3), 150, engine.vocab_size)
+    outs = []
+    for limit in (512, 64):
+        monkeypatch.setattr(attention, "rows_at_once", limit)
+        slot = engine.new_sequence()
+        engine.step([q.StepEntry(slot, prompt[:70])])
+        outs.append(engine.step([q.StepEntry(slot, prompt[70:], want=[0, 40, 79])]).clone())
+        engine.release(slot)
+    # a layer's keys and values move by roundings of 2^-9, and those can move a code by one of its steps of 2^-4 at most
+    assert float((outs[0] - outs[1]).abs().max()) <= 0.06 * float(outs[0].abs().max())
+
+
 @pytest.mark.parametrize("cache_dtype", [None, "float8"])
 def test_speculative_generation_is_greedy_generation(tmp_path, cache_dtype):
     import qwen3_b200 as q
