@@ -3,7 +3,7 @@
 //
 // S = Q K^T and O += P V are tcgen05.mma over a page of 64 keys, with the accumulators and the weights in tensor memory.  A tile has two buffers of scores there, so
 // that a page's scores are made while the softmax is at the page before: its chain is then the softmax alone.  (With the queries in tensor memory, which leaves
-// room for one buffer, products of 128 x 64 x 16 take 33 cycles instead of 51, but scores wait for the products before them: 2,750 cycles a page.)
+// room for one buffer, products of 128 x 64 x 16 take 33 cycles instead of 51, but scores wait for the products before them: 2,750 cycles a page against 2,200.)
 // A block, one an SM, works on two tiles side by side, so that the products of one run under the softmax of the other:
 //   more than 128 rows   two tiles of 128 rows, which take the same pages;
 //   up to 128 rows       twice the same rows, one tile with the pages of even number and one with those of odd number; their sums meet at the end.
@@ -23,7 +23,11 @@
 //
 // A value that is no number (infinity, NaN) in a page that some row does not see in whole is taken out before the product, and put into the
 // outputs of the rows that see it: 0 times a NaN would reach the others.
-// What bounds it: a page and 256 rows are 1,024 cycles of the tensor pipe and as many of the special-function unit (an exponential a score).
+// What bounds it: a page and 256 rows are 1,340 cycles of the tensor pipe (products of 128 x 64 x 16 from shared memory take 51 cycles, those with the weights
+// 65) and 1,024 of the special-function unit (an exponential a score), but the steps from product to softmax to product take 2,200 in bfloat16 and 3,000 in 8 bits:
+// 19 of them a page and tile, each of a hundred cycles or two, since the roles push one another's instructions out of the first cache (without any exponential it
+// takes 5 % less, without any product 15 %).  Beginning and ending a part are 18,000 cycles.  1 sequence of 32,000 keys, 33 tokens and 64 heads over 8
+// (bfloat16) 70 us, the floor being 21; 8 of up to 8,000, 64 and 40 (8 bits) 95 (22); 8 of up to 3,000, 7 and 32 (bfloat16) 28 (11).
 // Every mbarrier wait is bounded and reports into `status`.
 #include <cuda.h>
 
@@ -42,7 +46,7 @@ static_assert(D == 64 || D == 128, "head sizes 64 and 128");
 static_assert(PAGE == 64, "a product takes a page of 64 keys");
 constexpr int BM = 128, ROWS = 2 * BM, HALVES = D / 64;
 constexpr int SOFTMAX_WARPS = 8, TURN_WARPS = 4, V_WARP = 12, MMA_WARP = 16, K_COPY_WARP = 17, V_COPY_WARP = 18, THREADS = 20 * 32;
-// Registers of a thread by role: 256 x 144 + 256 x 80 + 128 x 32 = 640 x 96, what the block is launched with.
+// Registers of a thread by role: 256 x 144 + 256 x 72 + 128 x 48 = 640 x 96, what the block is launched with.
 constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, TURN_REGS = 72, MMA_REGS = 48;
 static_assert(8 * 32 * SOFTMAX_REGS + 8 * 32 * TURN_REGS + 4 * 32 * MMA_REGS <= THREADS * LAUNCH_REGS, "shares of the launch's registers");
 constexpr int NOTES = 8;                                  // pages whose notes are kept: more than lie between the copies and the softmax
@@ -52,7 +56,7 @@ constexpr uint32_t TMEM_COLS = 512, TILE_COLS = 256, COL_S = 0, COL_O = 128;    
 constexpr int Q_BYTES = HALVES * BM * 128, MEET_COLS = D / 2;                             // a tile's queries; columns of the sums that meet at a time
 static_assert(BM * MEET_COLS * 4 <= Q_BYTES, "they meet where the second tile's queries would be");
 // Pages that take about as long as beginning and ending a part.  0 / 3 / 6 / 9: 32 sequences of up to 4,000 keys and 32 new tokens (bfloat16) 129 / 93 / 78 /
-// 76 us, 8 of up to 8,000 and 64 (8 bits) 118 / 100 / 95 / 99.
+// 76 us, 8 of up to 8,000 and 64 (8 bits) 118 / 100 / 95 / 99; as much longer a piece may be: 12 of up to 5,000 and 12 (bfloat16) 45 with 6, 57 with 40.
 constexpr int PART_PAGES = 6;
 constexpr float RAISE = 8.0f;
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
@@ -263,7 +267,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 2, 20, PART_PAGES, blockIdx.x, gridDim.x);
+        const TreeShare found = Work::share(st, 2, PART_PAGES, blockIdx.x, gridDim.x);
         if (lane == 0) sh.share = found;
     }
     tc_fence_before();

@@ -5,7 +5,7 @@
 //   pieces  every item is cut into equal pieces of at most `quota` stretches, and a block takes one piece.  `quota` is the best of four numbers between
 //           the even share and one at which the pieces are certainly no more than the blocks, or that is longer by what a second part would cost a block;
 //   ranges  the stretches of all items in a row are cut into ranges of equal length, one a block, wherever they fall: a block has at most a
-//           part of an item, some whole ones and another part.  Taken where there are no such pieces.  In the row every item is longer by `pad` stretches
+//           part of an item, some whole ones and another part.  Taken where there are no such pieces.  In the row every item is longer by some stretches
 //           before its first one, for the time that beginning and ending it takes: a block with five short items is not the last.
 // Parts of an item are added up in their order.  Which part is whose, and so the order of a row's sums, hangs on the lengths of all sequences of the step
 // and on nothing else.
@@ -83,8 +83,8 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
 
     // The most items and counted stretches that a step can have (the latter have to stay below 2^30).
     static __host__ int64_t most_items(const TreeStep& a) { return (int64_t)a.n_seqs * a.nkv * tiles_of(a.max_new, a.nq / a.nkv); }
-    static __host__ int64_t most_units(const TreeStep& a, int pad) {
-        return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT + pad);
+    static __host__ int64_t most_units(const TreeStep& a, int spare) {
+        return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT + spare);
     }
 
     static __device__ __forceinline__ int warp_total(int v) {
@@ -94,8 +94,9 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
     }
 
     // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more);
-    // `spare`: a piece may be longer than the even share by so many, rather than that blocks have several parts; `pad`: see above.
-    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int pad, int block, int blocks) {
+    // `spare`: so many stretches take about as long as beginning and ending a part: a piece may be longer than the even share by them, rather than that
+    // blocks have several parts, and items count as longer by them.
+    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int block, int blocks) {
         const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
@@ -124,7 +125,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                 }
             }
         }
-        t.pad = t.pieces ? 0 : pad * COUNT;
+        t.pad = t.pieces ? 0 : spare * COUNT;
         if (!t.pieces) {
             total += items * t.pad;
             t.quota = even_of();
