@@ -24,10 +24,11 @@
 // A value that is no number (infinity, NaN) in a page that some row does not see in whole is taken out before the product, and put into the
 // outputs of the rows that see it: 0 times a NaN would reach the others.
 // What bounds it: a page and 256 rows are 1,340 cycles of the tensor pipe (products of 128 x 64 x 16 from shared memory take 51 cycles, those with the weights
-// 65) and 1,024 of the special-function unit (an exponential a score), but the steps from product to softmax to product take 2,200 in bfloat16 and 3,000 in 8 bits:
-// 19 of them a page and tile, each of a hundred cycles or two, since the roles push one another's instructions out of the first cache (without any exponential it
-// takes 5 % less, without any product 15 %).  Beginning and ending a part are 18,000 cycles.  1 sequence of 32,000 keys, 33 tokens and 64 heads over 8
-// (bfloat16) 70 us, the floor being 21; 8 of up to 8,000, 64 and 40 (8 bits) 95 (22); 8 of up to 3,000, 7 and 32 (bfloat16) 28 (11).
+// 65) and 1,024 of the special-function unit (an exponential a score), but 2,200 pass in bfloat16 and 3,000 in 8 bits: the softmax's chain of a page and that of
+// the products' warp are each as long, seven waits of 130 to 160 cycles and what lies between.  (Without any exponential it takes 5 % less, with an eighth of
+// the products 15 %; two sets of softmax warps that take turns, or products of keys and of values by warps of their own: within 3 %.)  Beginning and ending a
+// part are 18,000 cycles.  1 sequence of 32,000 keys, 33 tokens and 64 heads over 8 (bfloat16) 70 us, the floor being 21; 8 of up to 8,000, 64 and 40 (8 bits)
+// 95 (22); 8 of up to 3,000, 7 and 32 (bfloat16) 28 (11).
 // Every mbarrier wait is bounded and reports into `status`.
 #include <cuda.h>
 
@@ -740,7 +741,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
                 const TreePart part = Work::part(st, share, at, blockIdx.x);
-            if (part.begin >= part.end) break;
+                if (part.begin >= part.end) break;
                 const bool split = Work::n_new(st, part.seq) * group - part.tile * ROWS <= BM;
                 const int steps = part.end - part.begin, first = split ? x : 0, stride = split ? 2 : 1;
                 auto scores = [&](uint32_t buffer) {                                 // of the page at k_at
@@ -806,7 +807,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
                 const TreePart part = Work::part(st, share, at, blockIdx.x);
-            if (part.begin >= part.end) break;
+                if (part.begin >= part.end) break;
                 const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
                 int64_t page = page_of(st, table, part.begin);
                 for (int i = part.begin; i < part.end; ++i, ++number) {
