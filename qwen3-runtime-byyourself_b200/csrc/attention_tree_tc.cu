@@ -838,6 +838,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 }
                 at = Work::next(part);
             }
+            // its last copies have landed before the block goes, also where another role has given up
+            constexpr int RING = F8 ? L::CODES : L::STAGES;
+            for (int i = max(0, number - RING); i < number; ++i)
+                mbar_wait_warp(bar(F8 ? (is_v ? L::VC_FULL : L::KC_FULL) : is_v ? L::V_HERE : L::K_FULL, i % RING), turn_of(i, RING));
         }
     }
     tc_fence_before();
