@@ -174,6 +174,16 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
             return p >= 0 && p < st.n_pages ? p : 0;                 // (a number that is no page: stay within the cache)
         };
         int next_page = page_of(warp);
+        // the warp's rows of queries are asked for before the copies, which wait for the page table
+        constexpr int PER = D / 32, MY_ROWS = ROWS / WARPS;
+        uint32_t q_raw[MY_ROWS][PER / 2];
+#pragma unroll
+        for (int i = 0; i < MY_ROWS; ++i) {
+            const int r = warp + i * WARPS;
+            const bf16* src = a.q + ((int64_t)(t0 + (row0 + min(r, rows - 1)) / group) * st.nq + part.head * group + (row0 + min(r, rows - 1)) % group) * D + lane * PER;
+#pragma unroll
+            for (int e = 0; e < PER / 2; ++e) q_raw[i][e] = r < rows ? reinterpret_cast<const uint32_t*>(src)[e] : 0u;
+        }
         auto issue = [&](int s, int stage) {
             if (s < steps) {
                 const int64_t cell0 = ((int64_t)next_page * st.nkv + part.head) * PAGE + ((key_begin + s * KEYS) & (PAGE - 1));
@@ -201,17 +211,10 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
         for (int i = 0; i < STAGES - 1; ++i) issue(warp + i * WARPS, i);
 
         // ---- the tile's queries, in half precision behind a power of two a row, or as they are
-        for (int r = warp; r < ROWS; r += WARPS) {
-            constexpr int PER = D / 32;
-            bf16 x[PER];
-            if (r < rows) {
-                const bf16* src = a.q + ((int64_t)(t0 + (row0 + r) / group) * st.nq + part.head * group + (row0 + r) % group) * D + lane * PER;
 #pragma unroll
-                for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(x + e) = *reinterpret_cast<const uint32_t*>(src + e);
-            } else {
-#pragma unroll
-                for (int e = 0; e < PER; ++e) x[e] = __float2bfloat16_rn(0.0f);
-            }
+        for (int i = 0; i < MY_ROWS; ++i) {
+            const int r = warp + i * WARPS;
+            const bf16* x = reinterpret_cast<const bf16*>(q_raw[i]);
             uint32_t* dst = reinterpret_cast<uint32_t*>(q_rows + r * Q_PITCH + lane * PER * 2);
             if constexpr (F8) {
                 float top = 0.0f;
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
                 if (lane == 0) row_factor[r] = a.scale_log2 * q3_exp2i(e2);
             } else {
 #pragma unroll
-                for (int e = 0; e < PER; e += 2) dst[e / 2] = *reinterpret_cast<uint32_t*>(x + e);
+                for (int e = 0; e < PER / 2; ++e) dst[e] = q_raw[i][e];
             }
         }
         __syncthreads();
@@ -544,9 +547,9 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
             }
         }
         if (!whole) {
-            __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
+                __threadfence();                                     // (of the block's writes, which the barrier has put before it)
                 *shared_last = atomicAdd(a.counters + part.item, 1) == part.parts - 1 ? 1 : 0;
                 if (*shared_last) a.counters[part.item] = 0;
                 __threadfence();

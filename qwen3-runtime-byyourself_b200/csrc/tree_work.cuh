@@ -46,23 +46,18 @@ struct TreePart {
     __device__ __forceinline__ int slot_of(int i) const { return i == 0 ? slot0 : 2 * (first_block + i); }
 };
 
+// What of a sequence counts in the list: its items, in the order of their heads and tiles, of so many stretches each.  With LIGHT a stretch of a tile of at most
+// half the rows (the last one of a head) costs half of another's: lengths are then counted in halves, those of light items rounded up to whole ones.
+struct TreeItems {
+    int units, tiles;                              // stretches of an item; twice the tiles of a head, and 1 if the last one is light
+};
+
 // What a block has: in the way of ranges stretches [from, to) of the list (none: from >= to), else one piece.
 struct TreeShare {
     int from, to, quota;                           // quota: a range's length, or (`pieces`) the most stretches of a piece
     int pieces, pad;                               // 1: pieces; what an item is longer by, counted as lengths are (pieces: 0)
     int seq, before, items_before;                 // where `from` (a piece: the block's number) lies: its sequence, the stretches (pieces) and items before it
-};
-
-// What of a sequence counts in the list: its items, in the order of their heads and tiles, of so many stretches each.  With LIGHT a stretch of a tile of at most
-// half the rows (the last one of a head) costs half of another's: lengths are then counted in halves, those of light items rounded up to whole ones.
-struct TreeItems {
-    int units, per_head, light;                    // stretches of an item, tiles of a head, whether the last one is light (0 or 1)
-    int full, lighter;                             // the lengths
-
-    __device__ __forceinline__ int cut(int length, int quota) const { return (int)((unsigned)(length + quota - 1) / (unsigned)quota); }
-    // A head's length, or its pieces of up to `quota`.
-    __device__ __forceinline__ int of_head(int pad) const { return (per_head - light) * full + light * lighter + per_head * pad; }
-    __device__ __forceinline__ int pieces_of_head(int quota) const { return units == 0 ? 0 : (per_head - light) * cut(full, quota) + (light ? cut(lighter, quota) : 0); }
+    TreeItems items;                               // the sequence's
 };
 
 // UNIT: keys of a stretch; ROWS: rows of a tile.
@@ -71,26 +66,28 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
     static __device__ __forceinline__ int n_new(const TreeStep& a, int seq) { return max(0, min(a.seq_start[seq + 1] - a.seq_start[seq], a.max_new)); }
     static __host__ __device__ __forceinline__ int tiles_of(int n_new, int group) { return (int)(((int64_t)n_new * group + ROWS - 1) / ROWS); }
     static __device__ __forceinline__ TreeItems items_of(const TreeStep& a, int seq) {
-        TreeItems t;
         const int n = n_new(a, seq), group = a.nq / a.nkv;
-        t.units = n == 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT;
-        t.per_head = t.units > 0 ? tiles_of(n, group) : 0;
-        t.light = LIGHT && t.per_head > 0 && n * group - (t.per_head - 1) * ROWS <= ROWS / 2 ? 1 : 0;
-        t.full = t.units * COUNT;
-        t.lighter = (t.units + 1) & ~1;
-        return t;
+        const int units = n == 0 ? 0 : (min(a.seq_pos0[seq] + n, a.pages_per_seq * Q3_PAGE_TOKENS) + UNIT - 1) / UNIT, tiles = units > 0 ? tiles_of(n, group) : 0;
+        return {units, 2 * tiles + (LIGHT && tiles > 0 && n * group - (tiles - 1) * ROWS <= ROWS / 2 ? 1 : 0)};
+    }
+    // Tiles of a head, whether the last one is light (0 or 1), the lengths of the others and of a light one.
+    static __device__ __forceinline__ int per_head(const TreeItems& i) { return i.tiles >> 1; }
+    static __device__ __forceinline__ int light(const TreeItems& i) { return i.tiles & 1; }
+    static __device__ __forceinline__ int full(const TreeItems& i) { return i.units * COUNT; }
+    static __device__ __forceinline__ int lighter(const TreeItems& i) { return (i.units + 1) & ~1; }
+    static __device__ __forceinline__ int cut(int length, int quota) { return (int)((unsigned)(length + quota - 1) / (unsigned)quota); }
+    // A head's length, or its pieces of up to `quota`.
+    static __device__ __forceinline__ int of_head(const TreeItems& i, int pad) {
+        return (per_head(i) - light(i)) * full(i) + light(i) * lighter(i) + per_head(i) * pad;
+    }
+    static __device__ __forceinline__ int pieces_of_head(const TreeItems& i, int quota) {
+        return i.units == 0 ? 0 : (per_head(i) - light(i)) * cut(full(i), quota) + (light(i) ? cut(lighter(i), quota) : 0);
     }
 
     // The most items and counted stretches that a step can have (the latter have to stay below 2^30).
     static __host__ int64_t most_items(const TreeStep& a) { return (int64_t)a.n_seqs * a.nkv * tiles_of(a.max_new, a.nq / a.nkv); }
     static __host__ int64_t most_units(const TreeStep& a, int spare) {
         return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT + spare);
-    }
-
-    static __device__ __forceinline__ int warp_total(int v) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
     }
 
     // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more);
@@ -100,29 +97,39 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
-        const TreeItems none = {0, 0, 0, 0, 0}, mine = few && lane < a.n_seqs ? items_of(a, lane) : none;
+        const TreeItems none = {0, 0}, mine = few && lane < a.n_seqs ? items_of(a, lane) : none;
         auto each = [&](auto f) {                                        // sum over the sequences, for a head
             int sum = 0;
             if (few) sum = f(mine);
             else
                 for (int s = lane; s < a.n_seqs; s += 32) sum += f(items_of(a, s));
-            return warp_total(sum) * a.nkv;
+            return __reduce_add_sync(0xffffffffu, sum) * a.nkv;
         };
         TreeShare t;
-        const int items = each([](const TreeItems& i) { return i.per_head; });
-        int total = each([](const TreeItems& i) { return i.of_head(0); });
+        const int items = each([](const TreeItems& i) { return per_head(i); });
+        int total = each([](const TreeItems& i) { return of_head(i, 0); });
         auto even_of = [&] { return (max(least * COUNT, (int)(((unsigned)total + blocks - 1) / (unsigned)blocks)) + COUNT - 1) & ~(COUNT - 1); };
         const int even = even_of();
         t.pieces = 0;
         if (items < blocks) {
             // with pieces of `safe` there are at most items + total / safe of them
             const int safe = max(even, (total + blocks - items - 1) / (blocks - items)), cap = even + spare * COUNT;
-            for (int i = 0; i < 4 && !t.pieces; ++i) {
-                const int c = even + (min(safe, cap) - even) * i / 3;
-                if (each([c](const TreeItems& i) { return i.pieces_of_head(c); }) <= blocks) {
-                    t.pieces = 1;
-                    t.quota = c;
-                }
+            // four numbers at once, eight lanes each
+            const int quota = even + (min(safe, cap) - even) * (lane >> 3) / 3;
+            int sum = 0;
+            for (int s0 = 0; s0 < a.n_seqs; s0 += 8) {
+                const int s = s0 + (lane & 7);
+                TreeItems i = none;
+                if (few) i = {__shfl_sync(0xffffffffu, mine.units, s & 31), __shfl_sync(0xffffffffu, mine.tiles, s & 31)};
+                else if (s < a.n_seqs) i = items_of(a, s);
+                sum += pieces_of_head(i, quota);
+            }
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const unsigned fits = __ballot_sync(0xffffffffu, sum * a.nkv <= blocks);
+            if (fits != 0) {
+                t.pieces = 1;
+                t.quota = __shfl_sync(0xffffffffu, quota, __ffs(fits) - 1);
             }
         }
         t.pad = t.pieces ? 0 : spare * COUNT;
@@ -138,7 +145,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const int s = s0 + lane;
             const TreeItems here = few ? mine : s < a.n_seqs ? items_of(a, s) : none;
-            const int own = a.nkv * (t.pieces ? here.pieces_of_head(t.quota) : here.of_head(t.pad)), count = a.nkv * here.per_head;
+            const int own = a.nkv * (t.pieces ? pieces_of_head(here, t.quota) : of_head(here, t.pad)), count = a.nkv * per_head(here);
             int sum = own, counts = count;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -154,6 +161,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                 t.seq = s0 + first;
                 t.before = run + __shfl_sync(0xffffffffu, sum - own, first);
                 t.items_before = passed + __shfl_sync(0xffffffffu, counts - count, first);
+                t.items = {__shfl_sync(0xffffffffu, here.units, first), __shfl_sync(0xffffffffu, here.tiles, first)};
                 return t;
             }
             run += __shfl_sync(0xffffffffu, sum, 31);
@@ -161,6 +169,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         }
         t.from = t.to = 0;                                               // nothing for this block
         t.seq = t.before = t.items_before = 0;
+        t.items = none;
         return t;
     }
 
@@ -169,18 +178,18 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
     static __device__ __forceinline__ TreePart part(const TreeStep& a, TreeShare& t, int at, int block) {
         TreePart p;
         while (true) {
-            const TreeItems i = items_of(a, t.seq);
-            const int head = t.pieces ? i.pieces_of_head(t.quota) : i.of_head(t.pad), in = at - t.before;
+            const TreeItems& i = t.items;
+            const int head = t.pieces ? pieces_of_head(i, t.quota) : of_head(i, t.pad), in = at - t.before;
             if (in < head * a.nkv) {
                 p.seq = t.seq;
                 p.head = (int)((unsigned)in / (unsigned)head);
-                const int in_head = in - p.head * head, a_full = t.pieces ? i.cut(i.full, t.quota) : i.full + t.pad;     // numbers that a tile that is not light has
-                p.tile = min((int)((unsigned)in_head / (unsigned)a_full), i.per_head - 1);
-                const int off = in_head - p.tile * a_full, light = i.light && p.tile == i.per_head - 1 ? 1 : 0;
-                const int length = (light ? i.lighter : i.full) + t.pad, count = light ? 1 : COUNT;
-                p.item = t.items_before + p.head * i.per_head + p.tile;
+                const int in_head = in - p.head * head, a_full = t.pieces ? cut(full(i), t.quota) : full(i) + t.pad;     // numbers that a tile that is not light has
+                p.tile = min((int)((unsigned)in_head / (unsigned)a_full), per_head(i) - 1);
+                const int off = in_head - p.tile * a_full, light_tile = light(i) && p.tile == per_head(i) - 1 ? 1 : 0;
+                const int length = (light_tile ? lighter(i) : full(i)) + t.pad, count = light_tile ? 1 : COUNT;
+                p.item = t.items_before + p.head * per_head(i) + p.tile;
                 if (t.pieces) {
-                    p.parts = i.cut(length, t.quota);
+                    p.parts = cut(length, t.quota);
                     p.begin = (int)((unsigned)(off * i.units) / (unsigned)p.parts);
                     p.end = (int)((unsigned)((off + 1) * i.units) / (unsigned)p.parts);
                     p.first_block = block - off;
@@ -200,8 +209,8 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                 return p;
             }
             t.before += head * a.nkv;
-            t.items_before += i.per_head * a.nkv;
-            ++t.seq;
+            t.items_before += per_head(i) * a.nkv;
+            t.items = items_of(a, ++t.seq);
         }
     }
     static __device__ __forceinline__ int next(const TreePart& p) { return p.list_end; }
