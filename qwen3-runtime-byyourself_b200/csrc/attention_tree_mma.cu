@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
                     const int row = i / (D / 4), f = i % (D / 4);
                     float m = -INFINITY, l = 0.0f;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int b = 0; b < part.parts; ++b) {
+                    auto add = [&](int b) {
                         const float* src = a.parts + (int64_t)part.slot_of(b) * PART;
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + ROWS * D + 2 * row));
                         const float4 u = __ldcg(reinterpret_cast<const float4*>(src + row * D + 4 * f));
@@ -569,7 +569,16 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
                         l = fmaf(now, ml.y, l * was);
                         v.x = fmaf(now, u.x, v.x * was); v.y = fmaf(now, u.y, v.y * was);
                         v.z = fmaf(now, u.z, v.z * was); v.w = fmaf(now, u.w, v.w * was);
-                    }
+                    };
+                    int b = 0;
+                    // (eight at once where there are many: one token of 32 heads over 32,000 keys has 51, 28.3 -> 26.3 us)
+                    if constexpr (NT == 1)
+#pragma unroll 1
+                        for (; b + 16 <= part.parts; b += 8)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) add(b + k);
+#pragma unroll 4
+                    for (; b < part.parts; ++b) add(b);
                     put(row, f, v, l);
                 }
             }
