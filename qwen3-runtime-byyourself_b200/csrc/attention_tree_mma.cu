@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     for (int at = share.from; at < share.to;) {
         const TreePart part = Work::part(st, share, at, blockIdx.x);
         if (part.begin >= part.end) break;
-        const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
+        const int t0 = part.t0, n_new = part.n_new, pos0 = part.pos0;
         const int row0 = part.tile * ROWS, rows = min(ROWS, n_new * group - row0);      // row i of the tile: token (row0 + i) / group, head (row0 + i) % group
         const int key_begin = part.begin * PAGE, key_end = min(part.end * PAGE, pos0 + n_new);
         const int steps = (key_end - key_begin + KEYS - 1) / KEYS;

@@ -90,6 +90,7 @@ template <bool F8> struct Shared {
     float key_rest[NOTES][PAGE], value_rest[NOTES][PAGE];
     float2 meet[BM];                                      // (maximum, sum) of a tile of odd pages
     TreeShare share;
+    TreePart part;
     unsigned long long bars[Layout<F8>::BARS];
     uint32_t tmem;
 };
@@ -268,8 +269,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     pdl_wait();
     const TreeStep& st = a.step;
     if (warp == 0) {
-        const TreeShare found = Work::share(st, 2, PART_PAGES, blockIdx.x, gridDim.x);
-        if (lane == 0) sh.share = found;
+        // the first part is found by this warp for all (most blocks have no other): 4,000 cycles for each role by itself
+        TreeShare found = Work::share(st, 2, PART_PAGES, blockIdx.x, gridDim.x);
+        TreePart first = {};
+        if (found.from < found.to) first = Work::part(st, found, found.from, blockIdx.x);
+        if (lane == 0) {
+            sh.share = found;
+            sh.part = first;
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -291,9 +298,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         uint32_t count = 0, q_turn = 0, met_turn = 0;                                // pages of this tile so far; parities of the parts, of the tiles' meetings
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
-            const TreePart part = Work::part(st, share, at, blockIdx.x);
+            const TreePart part = at == share.from ? sh.part : Work::part(st, share, at, blockIdx.x);
             if (part.begin >= part.end) break;
-            const int t0 = st.seq_start[part.seq], n_new = Work::n_new(st, part.seq), pos0 = st.seq_pos0[part.seq];
+            const int t0 = part.t0, n_new = part.n_new, pos0 = part.pos0;
             const int all_rows = n_new * group - part.tile * ROWS, steps = part.end - part.begin;
             const bool split = all_rows <= BM;                                       // one tile of rows: every other page
             const int first = split ? x : 0, stride = split ? 2 : 1;
@@ -593,9 +600,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         int page0 = 0;                                                               // pages of this block before the part
         bool ok = true;
         for (int at = share.from; at < share.to && ok;) {
-            const TreePart part = Work::part(st, share, at, blockIdx.x);
+            const TreePart part = at == share.from ? sh.part : Work::part(st, share, at, blockIdx.x);
             if (part.begin >= part.end) break;
-            const int pos0 = st.seq_pos0[part.seq], key_end = pos0 + Work::n_new(st, part.seq), steps = part.end - part.begin;
+            const int pos0 = part.pos0, key_end = pos0 + part.n_new, steps = part.end - part.begin;
             if constexpr (F8) {
                 // ------------------------------------------------ codes to half precision, a page two warps, each 32 rows of it, D / 16 lanes a row: 25
                 // instructions for a lane's sixteen codes
@@ -740,9 +747,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             };
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
-                const TreePart part = Work::part(st, share, at, blockIdx.x);
+                const TreePart part = at == share.from ? sh.part : Work::part(st, share, at, blockIdx.x);
                 if (part.begin >= part.end) break;
-                const bool split = Work::n_new(st, part.seq) * group - part.tile * ROWS <= BM;
+                const bool split = part.n_new * group - part.tile * ROWS <= BM;
                 const int steps = part.end - part.begin, first = split ? x : 0, stride = split ? 2 : 1;
                 auto scores = [&](uint32_t buffer) {                                 // of the page at k_at
                     if (!mbar_wait_warp(bar(L::K_FULL, k_at.stage), k_at.turn)) return false;
@@ -806,7 +813,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             int number = 0;
             bool ok = true;
             for (int at = share.from; at < share.to && ok;) {
-                const TreePart part = Work::part(st, share, at, blockIdx.x);
+                const TreePart part = at == share.from ? sh.part : Work::part(st, share, at, blockIdx.x);
                 if (part.begin >= part.end) break;
                 const int* table = st.page_table + (int64_t)part.seq * st.pages_per_seq;
                 int64_t page = page_of(st, table, part.begin);

@@ -41,6 +41,7 @@ struct TreePart {
     int begin, end, item;                          // item: its number among the items
     int parts, slot, slot0, first_block;           // of the item: how many; this one's place in the scratch, the first one's, and the first one's block
     int list_end;                                  // where the block's share goes on
+    int t0, n_new, pos0;                           // of the sequence: its first token and how many of the step's, its earlier keys
 
     // The place of the item's part i in the scratch (a block has two: of the part that it begins with, and of the one that it ends with).
     __device__ __forceinline__ int slot_of(int i) const { return i == 0 ? slot0 : 2 * (first_block + i); }
@@ -182,6 +183,9 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
             const int head = t.pieces ? pieces_of_head(i, t.quota) : of_head(i, t.pad), in = at - t.before;
             if (in < head * a.nkv) {
                 p.seq = t.seq;
+                p.t0 = a.seq_start[t.seq];
+                p.n_new = n_new(a, t.seq);
+                p.pos0 = a.seq_pos0[t.seq];
                 p.head = (int)((unsigned)in / (unsigned)head);
                 const int in_head = in - p.head * head, a_full = t.pieces ? cut(full(i), t.quota) : full(i) + t.pad;     // numbers that a tile that is not light has
                 p.tile = min((int)((unsigned)in_head / (unsigned)a_full), per_head(i) - 1);
