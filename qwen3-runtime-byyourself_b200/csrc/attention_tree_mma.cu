@@ -34,7 +34,11 @@ constexpr int WARPS = 4;
 // Blocks an SM and stages of a warp's ring, by tiles of eight rows (registers, shared memory).
 template <int NT> constexpr int blocks_per_sm = NT == 4 ? 2 : 3;
 template <int NT> constexpr int stages = NT == 4 ? 3 : 2;
-constexpr int LEAST_PAGES = 4;                      // of a block's range
+// A block is given no fewer pages, and all of items of up to WHOLE_PAGES (130 keys whole 7.4 us, in two parts 8.2; 600 whole 11.0, in five 9.1); in the time of
+// how many pages a part is added up, for every 128 packets of its rows: 0 (and four pages at least) / 0.1 / 0.2 / 0.3 for 1 sequence of 32,000 keys of 2 kv heads, 4
+// tokens and 8 heads 65 / 34 / 32 / 34 us, 3 of up to 30,000 of one, 1 and 8 (bfloat16) 31 / 24 / 24 / 25, 1 of 8,000 of 4, 2 and 16 16.1 / 16.2 / 17.3 / 18.6.
+constexpr int LEAST_PAGES = 2, WHOLE_PAGES = 4;
+constexpr float JOIN_PAGES = 0.2f;
 // Pages that take about as long as beginning and ending a part.  0 / 4 / 8 / 12: 64 sequences of up to 2,000 keys and one new token (8 bits) 57 / 44 / 42 / 42 us,
 // of up to 9,000 123 / 113 / 113 / 110, with four new tokens 129 / 102 / 83 / 82, of 130 20 / 14.6 / 15.2 / 15.2.
 constexpr int PART_PAGES = 8;
@@ -150,7 +154,9 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const TreeShare found = Work::share(st, LEAST_PAGES, PART_PAGES, blockIdx.x, gridDim.x);
+        const int most_rows = min(ROWS, st.max_new * group);
+        const float join = JOIN_PAGES * (float)((most_rows * (D / 4) + WARPS * 32 - 1) / (WARPS * 32));
+        const TreeShare found = Work::share(st, LEAST_PAGES, WHOLE_PAGES, join, PART_PAGES, blockIdx.x, gridDim.x);
         if (lane == 0) *shared_share = found;
     }
     __syncthreads();

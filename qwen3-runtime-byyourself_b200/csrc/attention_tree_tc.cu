@@ -59,6 +59,10 @@ static_assert(BM * MEET_COLS * 4 <= Q_BYTES, "they meet where the second tile's 
 // Pages that take about as long as beginning and ending a part.  0 / 3 / 6 / 9: 32 sequences of up to 4,000 keys and 32 new tokens (bfloat16) 129 / 93 / 78 /
 // 76 us, 8 of up to 8,000 and 64 (8 bits) 118 / 100 / 95 / 99; as much longer a piece may be: 12 of up to 5,000 and 12 (bfloat16) 45 with 6, 57 with 40.
 constexpr int PART_PAGES = 6;
+// A block is given no fewer pages; in the time of how many pages a part is added up: 0 / 0.05 / 0.12 / 0.25 for 1 sequence of 32,000 keys of one kv head, 20 tokens
+// and 8 heads 55 / 50 / 43 / 40 us, 2 of up to 30,000 and 24 (8 bits) 57 / 53 / 48 / 45, of up to 3,000 of 8 kv heads and 8 18.7 / 18.5 / 18.5 / 19.3.
+constexpr int LEAST_PAGES = 2;
+constexpr float JOIN_PAGES = 0.2f;
 constexpr float RAISE = 8.0f;
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
@@ -270,7 +274,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     const TreeStep& st = a.step;
     if (warp == 0) {
         // the first part is found by this warp for all (most blocks have no other): 4,000 cycles for each role by itself
-        TreeShare found = Work::share(st, 2, PART_PAGES, blockIdx.x, gridDim.x);
+        TreeShare found = Work::share(st, LEAST_PAGES, LEAST_PAGES, JOIN_PAGES, PART_PAGES, blockIdx.x, gridDim.x);
         TreePart first = {};
         if (found.from < found.to) first = Work::part(st, found, found.from, blockIdx.x);
         if (lane == 0) {
@@ -918,7 +922,7 @@ template <bool F8> int launch(const Args& a, int max_new, cudaStream_t stream) {
         return Q3_ERR_BAD_SIZE;
     const int64_t units = Work::most_units(a.step, PART_PAGES);
     if (units > 0x3fffffff) return Q3_ERR_TOO_LARGE;
-    const int64_t most = (Work::most_units(a.step, 0) + 1) / 2 + Work::most_items(a.step);
+    const int64_t most = (Work::most_units(a.step, 0) + LEAST_PAGES - 1) / LEAST_PAGES + Work::most_items(a.step);
     const int sms = q3_device_sm_count(), blocks = (int)(most < sms ? most : sms);
     int code = (int)q3_launch(tree_tc_kernel<F8>, dim3(blocks), dim3(THREADS), (size_t)smem_bytes<F8>, stream, map_k, map_v, a);
     if (code != 0) return code;

@@ -91,10 +91,12 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         return COUNT * most_items(a) * (((int64_t)a.pages_per_seq * Q3_PAGE_TOKENS + UNIT - 1) / UNIT + spare);
     }
 
-    // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more);
+    // What block `block` of `blocks` has.  Called by one whole warp; `least`: a block is not given fewer stretches (unless an item has no more), nor so few
+    // that adding up an item's parts would take longer than it saves: for an item of u stretches in pieces of q, where a part is added up in `join` times the
+    // time of a stretch, q + join u / q is least at q = sqrt(join u); `whole`: where no item has more stretches, none is cut;
     // `spare`: so many stretches take about as long as beginning and ending a part: a piece may be longer than the even share by them, rather than that
     // blocks have several parts, and items count as longer by them.
-    static __device__ TreeShare share(const TreeStep& a, int least, int spare, int block, int blocks) {
+    static __device__ TreeShare share(const TreeStep& a, int least, int whole, float join, int spare, int block, int blocks) {
         const int lane = threadIdx.x & 31;
         // of up to 32 sequences everything is read once
         const bool few = a.n_seqs <= 32;
@@ -106,6 +108,11 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
                 for (int s = lane; s < a.n_seqs; s += 32) sum += f(items_of(a, s));
             return __reduce_add_sync(0xffffffffu, sum) * a.nkv;
         };
+        int longest = mine.units;
+        if (!few)
+            for (int s = lane; s < a.n_seqs; s += 32) longest = max(longest, items_of(a, s).units);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        least = max(least, longest <= whole ? longest : __float2int_rn(sqrtf(join * (float)longest)));
         TreeShare t;
         const int items = each([](const TreeItems& i) { return per_head(i); });
         int total = each([](const TreeItems& i) { return of_head(i, 0); });
