@@ -98,17 +98,17 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
     // blocks have several parts, and items count as longer by them.
     static __device__ TreeShare share(const TreeStep& a, int least, int whole, float join, int spare, int block, int blocks) {
         const int lane = threadIdx.x & 31;
-        // of up to 32 sequences everything is read once
-        const bool few = a.n_seqs <= 32;
-        const TreeItems none = {0, 0}, mine = few && lane < a.n_seqs ? items_of(a, lane) : none;
+        // of up to 64 sequences everything is read once
+        const bool few = a.n_seqs <= 64;
+        const TreeItems none = {0, 0}, mine = few && lane < a.n_seqs ? items_of(a, lane) : none, mine2 = few && lane + 32 < a.n_seqs ? items_of(a, lane + 32) : none;
         auto each = [&](auto f) {                                        // sum over the sequences, for a head
             int sum = 0;
-            if (few) sum = f(mine);
+            if (few) sum = f(mine) + f(mine2);
             else
                 for (int s = lane; s < a.n_seqs; s += 32) sum += f(items_of(a, s));
             return __reduce_add_sync(0xffffffffu, sum) * a.nkv;
         };
-        int longest = mine.units;
+        int longest = max(mine.units, mine2.units);
         if (!few)
             for (int s = lane; s < a.n_seqs; s += 32) longest = max(longest, items_of(a, s).units);
         longest = __reduce_max_sync(0xffffffffu, longest);
@@ -128,7 +128,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
             for (int s0 = 0; s0 < a.n_seqs; s0 += 8) {
                 const int s = s0 + (lane & 7);
                 TreeItems i = none;
-                if (few) i = {__shfl_sync(0xffffffffu, mine.units, s & 31), __shfl_sync(0xffffffffu, mine.tiles, s & 31)};
+                if (few) i = {__shfl_sync(0xffffffffu, s0 < 32 ? mine.units : mine2.units, s & 31), __shfl_sync(0xffffffffu, s0 < 32 ? mine.tiles : mine2.tiles, s & 31)};
                 else if (s < a.n_seqs) i = items_of(a, s);
                 sum += pieces_of_head(i, quota);
             }
@@ -152,7 +152,7 @@ template <int UNIT, int ROWS, bool LIGHT> struct TreeWork {
         int run = 0, passed = 0;
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
             const int s = s0 + lane;
-            const TreeItems here = few ? mine : s < a.n_seqs ? items_of(a, s) : none;
+            const TreeItems here = few ? (s0 == 0 ? mine : mine2) : s < a.n_seqs ? items_of(a, s) : none;
             const int own = a.nkv * (t.pieces ? pieces_of_head(here, t.quota) : of_head(here, t.pad)), count = a.nkv * per_head(here);
             int sum = own, counts = count;
 #pragma unroll

@@ -89,7 +89,7 @@ def test_many_new_tokens(kind, store, d, kv, group, masks, spans):
 
 
 @pytest.mark.parametrize("kind,store", KINDS[:2])
-@pytest.mark.parametrize("spans", [[(9000, 1)], [(20000, 3)], [(9000, 40)], [(6000, 1)] * 3 + [(0, 1)] * 30, [(100 * i, 1 + i % 4) for i in range(40)],
+@pytest.mark.parametrize("spans", [[(9000, 1)], [(20000, 3)], [(9000, 40)], [(6000, 1)] * 3 + [(0, 1)] * 30, [(100 * i, 1 + i % 4) for i in range(40)], [(37 * (i % 9), 1 + i % 3) for i in range(70)],
                                    [(5000, 64), (1, 1)], [(900, 20)] * 9])
 def test_long_contexts(kind, store, spans):
     check(kind, store, 128, 1, 4, spans, "tree", seed=5)
