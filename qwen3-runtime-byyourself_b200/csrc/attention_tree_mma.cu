@@ -14,8 +14,9 @@
 //     and M the running maximum of x + v, so the largest weight is of the order of 1 whatever the scales are, and what half precision drops is
 //     below 2^-24 of the largest term; the sum of the softmax is that of w 2^-v, in 32 bits.
 //   - The maximum is raised only when it is exceeded by more than 2^8.
-//   - One new token, 32 heads over 8 (8 bits): 64 sequences of up to 9,000 keys (40 heads) 110 us, 5.6 TB/s of the 6.5 that a copy reaches; 8 of up to 4,000
-//     18.5 (the floor is 6.6: a block has six pages, and begins, meets and joins its parts for as long), one of 32,000 28.8, one of 130 7.9.
+//   - One new token, 32 heads over 8 (8 bits): 64 sequences of up to 9,000 keys (40 heads) 109 us, 5.6 TB/s of the 6.5 that a copy reaches; 8 of up to 4,000
+//     17.9 (the floor is 6.6: of 23,000 cycles 3,000 go by until a block knows its share, 3,500 until its copies are under way, 9,000 for its six pages, 1,500 until
+//     its warps' sums have met and 5,000 until the parts of a row have), one of 32,000 26.8, one of 130 7.4.
 //   - A step with new tokens masks by bits; a value that is no number reaches only the rows that see it (a product of 0 and a NaN is a NaN:
 //     such values are taken out before the product and added to the rows that see them).
 #include "page8.cuh"

@@ -27,8 +27,8 @@
 // 65) and 1,024 of the special-function unit (an exponential a score), but 2,200 pass in bfloat16 and 3,000 in 8 bits: the softmax's chain of a page and that of
 // the products' warp are each as long, seven waits of 130 to 160 cycles and what lies between.  (Without any exponential it takes 5 % less, with an eighth of
 // the products 15 %; two sets of softmax warps that take turns, or products of keys and of values by warps of their own: within 3 %.)  Beginning and ending a
-// part are 18,000 cycles.  1 sequence of 32,000 keys, 33 tokens and 64 heads over 8 (bfloat16) 70 us, the floor being 21; 8 of up to 8,000, 64 and 40 (8 bits)
-// 95 (22); 8 of up to 3,000, 7 and 32 (bfloat16) 28 (11).
+// part are 16,000 cycles.  1 sequence of 32,000 keys, 33 tokens and 64 heads over 8 (bfloat16) 70 us, the floor being 21; 8 of up to 8,000, 64 and 40 (8 bits)
+// 94 (22); 8 of up to 3,000, 7 and 32 (bfloat16) 27.5 (11).
 // Every mbarrier wait is bounded and reports into `status`.
 #include <cuda.h>
 
