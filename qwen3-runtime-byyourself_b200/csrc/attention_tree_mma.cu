@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_per_sm<NT>) tree_mma_kernel
     const int group = st.nq / st.nkv;
 
     if (warp == 0) {
-        const int most_rows = min(ROWS, st.max_new * group);
+        const int most_rows = (int)min((int64_t)ROWS, (int64_t)st.max_new * group);
         const float join = JOIN_PAGES * (float)((most_rows * (D / 4) + WARPS * 32 - 1) / (WARPS * 32));
         const TreeShare found = Work::share(st, LEAST_PAGES, WHOLE_PAGES, join, PART_PAGES, blockIdx.x, gridDim.x);
         if (lane == 0) *shared_share = found;
