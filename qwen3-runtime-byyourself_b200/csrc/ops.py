@@ -1479,12 +1479,14 @@ class TreeScratch:
     counters: int
 
 
-# Rows of a kv head (new tokens of a sequence x query heads a kv head) from which a step goes to the tcgen05 kernel, and for 8 bits up to 32 rows the most
-# pages (sequences x kv heads x pages of a sequence's table).  mma.sync / tcgen05 at 20 rows, 8 kv heads: bfloat16, 1 sequence of 500 tokens 20.7 / 14.3 us, of
-# 16,000 49.9 / 33.2, 8 of up to 4,000 38.2 / 29.2, of up to 16,000 71.0 / 64.3; 8 bits 19.9 / 16.8, 46.9 / 35.8, 35.9 / 33.9, but 70.0 / 97.2 (the codes of a page
-# take the tcgen05 kernel as long for 20 rows as for 128).  At 16 rows bfloat16 16.6 / 14.3, 47.4 / 29.9, 29.4 / 27.7, 70.1 / 68.7, 32 sequences of up to 2,000
-# tokens 39.7 / 46.6; 8 bits 27.8 / 37.0 for 8 of up to 4,000.
-tree_tc_rows, tree_tc_pages = 17, 8192
+# Rows of a kv head (new tokens of a sequence x query heads a kv head) from which a step goes to the tcgen05 kernel.  mma.sync / tcgen05 at 20 rows, 8 kv heads:
+# bfloat16, 1 sequence of 500 tokens 20.7 / 14.3 us, of 16,000 49.9 / 33.2, 8 of up to 4,000 38.2 / 29.2; 8 bits 19.9 / 16.8, 46.9 / 35.8, 35.9 / 33.9.  At 16 rows
+# bfloat16 16.6 / 14.3, 47.4 / 29.9, 29.4 / 27.7, 32 sequences of up to 2,000 tokens 39.7 / 46.6; 8 bits 27.8 / 37.0 for 8 of up to 4,000.
+# Up to 32 rows (a tile of the mma.sync kernel's) it has to have no more items (sequences x kv heads) than blocks: 28 rows, 20 sequences of up to 20 tokens
+# 13.1 / 16.8, of up to 250 21.9 / 20.9, 32 of them 20.1 / 25.4 - or, in bfloat16, page tables of more than `tree_tc_table` pages (32 of up to 1,000 tokens
+# 39.3 / 39.4, of up to 2,500 60.5 / 51.1; 8 bits 30.9 / 47.7, 55.8 / 70.0); and in 8 bits no more than `tree_tc_pages` pages in all (8 sequences of up to 16,000
+# 70.0 / 97.2, 12 of up to 6,000 44.0 / 52.1: the codes of a page take the tcgen05 kernel as long for 20 rows as for 128).
+tree_tc_rows, tree_tc_items, tree_tc_table, tree_tc_pages = 17, 148, 16, 4096
 _tree_parts = {}
 # source, entry point, whether it is compiled for a head size
 _TREE_FORMS = {"any": ("attention_tree.cu", "q3_attention_tree_any_", False), "mma": ("attention_tree_mma.cu", "q3_attention_tree_mma_", True),
@@ -1496,12 +1498,16 @@ def attention_tree_tiled(dtype: torch.dtype, d: int) -> bool:
     return dtype == torch.bfloat16 and d in (64, 128)
 
 
-def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int, pages: int) -> str:
-    """Which kernel takes a step of `rows` rows a kv head at most, over a cache of so many places (pages x kv heads x PAGE_TOKENS): `tc` and `mma`
-    take bfloat16 queries and head sizes 64 and 128, `any` the others.  `pages`: an 8-bit cache's that the step can read at most, else 0."""
+def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int, eight_bit: bool, items: int, table: int) -> str:
+    """Which kernel takes a step of `rows` rows a kv head at most and of so many items (sequences x kv heads), with page tables of `table` pages, over a
+    cache of so many places (pages x kv heads x PAGE_TOKENS): `tc` and `mma` take bfloat16 queries and head sizes 64 and 128, `any` the others."""
     if not attention_tree_tiled(dtype, d):
         return "any"
-    return "tc" if rows >= tree_tc_rows and (rows > 32 or pages <= tree_tc_pages) and scale > 0 and places < 2 ** 31 else "mma"
+    if rows < tree_tc_rows or scale <= 0 or places >= 2 ** 31:
+        return "mma"
+    if rows <= 32 and (items > tree_tc_items or items * table > tree_tc_pages if eight_bit else items > tree_tc_items and table <= tree_tc_table):
+        return "mma"
+    return "tc"
 
 
 def _tree_parts_of(form: str, rows: int, d: int, device) -> int:
@@ -1544,7 +1550,7 @@ def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts:
             raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
         masks, words = _at(tree, "tree", torch.int64), tree.shape[1]
     q_at, rows, parts_at, counters_at, status = _at(q, "q", dtype), max_new * (nq // nkv), 0, 0, 0
-    form = _tree_form(dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS, n_seqs * nkv * row_of[1] if cache.eight_bit else 0)
+    form = _tree_form(dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS, cache.eight_bit, n_seqs * nkv, row_of[1])
     if form != "any":
         if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 8):
             raise KernelError("attention_tree: parts or counters are too small (attention_tree_scratch)")
