@@ -17,8 +17,9 @@
 //   warps 17, 18 copy keys and values: bfloat16 by TMA where the products read them, 8 bits as they lie, some pages ahead.
 //
 // 8 bits.  A page's keys are brought to one scale, that of its first row, 2^k0, by folding 2^(k - k0) into the half-precision numbers, which is exact
-// for k - k0 in -14 .. 7; so are its values.  Scores are then multiplied by 2^k0 with the softmax's own scale; v0 is added to the scores in log2 units, so
-// that a weight is w = 2^(x + v0 - M) with M the running maximum of x + v0 and the sum of the softmax that of w 2^-v0.  Where some row of a page has a scale outside that
+// for k - k0 in -14 .. 7; so are its values, to the largest scale 2^v0 of its rows that all tokens see.  Scores are then multiplied by 2^k0 with the softmax's own scale; v0 is added to the scores
+// in log2 units, so that a weight is w = 2^(x + v0 - M) with M the running maximum of x + v0 and the sum of the softmax that of w 2^-v0.  The largest term's weight is not
+// below 2^-14 of M, since its value is folded by no more (2^-21 where a new token's scale is above 2^v0), and half precision drops what is below 2^-31 of M.  Where some row of a page has a scale outside that
 // range, what is missing (`rest`) is added score by score, in a path of its own.  Queries are brought into half precision as in attention_tree_mma.cu.
 //
 // A value that is no number (infinity, NaN) in a page that some row does not see in whole is taken out before the product, and put into the
@@ -63,7 +64,7 @@ constexpr int PART_PAGES = 6;
 // and 8 heads 55 / 50 / 43 / 40 us, 2 of up to 30,000 and 24 (8 bits) 57 / 53 / 48 / 45, of up to 3,000 of 8 kv heads and 8 18.7 / 18.5 / 18.5 / 19.3.
 constexpr int LEAST_PAGES = 2;
 constexpr float JOIN_PAGES = 0.2f;
-constexpr float RAISE = 8.0f;
+constexpr float RAISE = 8.0f, LIFT = 6.0f;                // 8 bits: weights are this much larger (in log2), up to 2^14, and lose nothing above 2^-20 of M
 constexpr int FOLD_LOW = -14, FOLD_HIGH = 7;
 constexpr int PART = ROWS * (D + 2);                      // float32 of a part: sums [D / 4][ROWS][4], then (maximum, sum) [ROWS][2]
 // An item of several parts, the first of which is a block's last: noted behind all parts, a note a block, for the second kernel (parts 0: there is none).
@@ -435,7 +436,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     l_run *= alpha;
                 }
                 // ---- weights, over the scores
-                const float shift = v0 - (m_run == -INFINITY ? 0.0f : m_run);
+                const float shift = v0 - (m_run == -INFINITY ? 0.0f : m_run) + (F8 ? LIFT : 0.0f);
                 const float2 c2 = make_float2(c1, c1), shift2 = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                 __syncwarp();
@@ -636,7 +637,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     // this lane has the scale of a row: 2^fold, twice in a word, and what the fold leaves - as a factor of the key's score, or in log2
                     // units - which is read only where a flag says so, of either kind
                     const uint8_t* const scales = sh.code_scales[is_v][slot];
-                    const int scale0 = scales[0], my_row = half * 32 + lane;
+                    const int my_row = half * 32 + lane;
+                    int scale0 = scales[0];
+                    if (is_v) {                                                      // the largest, of the rows that every token sees; 1 where there are none
+                        const int lo = key0 + lane < pos0 ? scales[lane] : 0, hi = key0 + 32 + lane < pos0 ? scales[32 + lane] : 0;
+                        scale0 = key0 < pos0 ? __reduce_max_sync(0xffffffffu, max(lo, hi)) : Q3_SCALE_BIAS;
+                    }
                     const int e = key0 + my_row < key_end ? (int)scales[my_row] - scale0 : 0;     // (the scale of a row that nobody wrote may be anything)
                     const int fold = min(max(e, FOLD_LOW), FOLD_HIGH);
                     const uint32_t by = (uint32_t)(fold + 15) * 0x04000400u;

@@ -220,3 +220,28 @@ def test_refusals():
             ops.attention_tree(*args, tree=bad)
     with pytest.raises(ops.KernelError):
         ops.attention_tree(*args[:8], 65, *args[9:], tree=tree)
+
+
+@pytest.mark.parametrize("store", ["bf16", "f8"])
+@pytest.mark.parametrize("d,kv,group", [(128, 2, 4), (64, 3, 3), (128, 1, 8)])
+@pytest.mark.parametrize("rows", [1, 10 ** 9])
+@pytest.mark.parametrize("spans,masks", [([(200, 3), (61, 9), (0, 1), (130, 5)], "tree"), ([(900, 4)], None), ([(40, 30), (3, 64), (700, 1)], "tree"),
+                                         ([(70 * (i % 5), 2 + i % 7) for i in range(45)], "tree")])
+def test_each_form_takes_any_number_of_rows(monkeypatch, store, d, kv, group, rows, spans, masks):
+    """The tcgen05 form where the mma.sync form would be taken, and the other way round: which is faster is all that the choice rests on."""
+    from qwen3_b200.csrc import ops
+    monkeypatch.setattr(ops, "tree_tc_rows", rows)
+    monkeypatch.setattr(ops, "tree_tc_items", 10 ** 9)
+    monkeypatch.setattr(ops, "tree_tc_pages", 10 ** 9)
+    check("bf16", store, d, kv, group, spans, masks, seed=11)
+
+
+def test_the_choice_of_a_form():
+    from qwen3_b200.csrc import ops
+
+    def form(rows, eight_bit=False, items=8, table=10, d=128, scale=0.1, dtype=torch.bfloat16, places=1000):
+        return ops._tree_form(dtype, rows, d, scale, places, eight_bit, items, table)
+    assert [form(r) for r in (1, 16, 17, 64)] == ["mma", "mma", "tc", "tc"]
+    assert [form(32, items=200), form(32, items=200, table=17), form(33, items=200)] == ["mma", "tc", "tc"]
+    assert [form(32, True, items=200, table=17), form(32, True, 100, 41), form(32, True, 100, 40), form(33, True, 200, 1000)] == ["mma", "mma", "tc", "tc"]
+    assert [form(64, d=80), form(64, dtype=torch.float32), form(64, scale=0.0), form(64, places=2 ** 31)] == ["any", "any", "mma", "mma"]
