@@ -379,8 +379,8 @@ class GQAAttention(Part):
 
     def takes_rows(self) -> bool:
         """Whether a cache in 8 bits and steps with drafted tokens can be had of this layer: plain attention over all keys, with rotation
-        tables or no rotation."""
-        return (type(self).mix is GQAAttention.mix and self.plain and not self.window
+        tables or no rotation.  (A short convolution makes a row from the rows before it in the step, and keeps the last ones as the sequence's state.)"""
+        return (type(self).mix is GQAAttention.mix and self.plain and not self.window and not self.conv_taps
                 and (self.position is None or getattr(self.position, "fused_tables", False)))
 
     def mix_rows(self, x, ctx, cache, attn, table) -> torch.Tensor:
