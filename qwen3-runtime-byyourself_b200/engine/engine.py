@@ -229,8 +229,7 @@ class Engine:
             raise KernelBuildError("the engine runs on a CUDA device only; there is no CPU path")
         if cache_dtype not in (None, "float8"):
             raise ValueError(f"cache_dtype {cache_dtype!r}: None (as computed) or 'float8'")
-        # whether every layer takes rows at places of their own: a cache in 8 bits, steps with drafted tokens
-        self.takes_rows = not model.cache_sources() and all(getattr(b.mixer, "takes_rows", lambda: False)() for b in model.blocks)
+        self.takes_rows, self.takes_trees = model.takes_rows(), model.takes_trees()      # a cache in 8 bits; steps with drafted tokens
         if cache_dtype is not None and not self.takes_rows:
             raise ValueError("a cache in 8 bits takes a model whose layers are all plain attention over all keys")
         max_seq_len = min(max_seq_len or self.plan.max_positions, self.plan.max_positions)
@@ -367,8 +366,8 @@ class Engine:
         drafted tokens that it follows, and itself, and stands at the position that its depth gives.  Returns float32 logits [tokens, vocab] in
         the order of the entries and their tokens (scratch: valid until the next step).  The sequences do not grow: `keep` says which of the
         tokens stand, and comes before any other step."""
-        if not self.takes_rows:
-            raise StepError("drafted tokens take a model whose layers are all plain attention over all keys")
+        if not self.takes_trees:
+            raise StepError("drafted tokens take a model whose layers are all plain attention over all keys, and whose blocks keep no state")
         if self._drafted:
             raise StepError("the drafted tokens of the last step wait for `keep`")
         if not entries:

@@ -101,6 +101,17 @@ class Model:
                 needs.append(dataclasses.replace(need, block_state=extra) if extra else need)
         return needs
 
+    def takes_rows(self) -> bool:
+        """Whether rows can be written at places of their own, as a cache in 8 bits asks for: every layer is plain attention over all keys
+        of a cache of its own, whose mixer keeps nothing else per sequence."""
+        return (not self.cache_sources() and all(getattr(b.mixer, "takes_rows", lambda: False)() for b in self.blocks)
+                and not any(n is not None and n.state_shape for n in self.cache_needs()))
+
+    def takes_trees(self) -> bool:
+        """Whether a step can bring drafted tokens, of which some stand beside each other and some are given up: nothing but cached rows is
+        kept per sequence.  (A block that mixes a row with the one before it would take another branch's, and keep it.)"""
+        return self.takes_rows() and not any(n is not None and n.block_state for n in self.cache_needs())
+
     def cache_sources(self) -> Dict[int, int]:
         return {i: spec.cache_from for i, spec in enumerate(self.plan.layers) if spec.cache_from is not None}
 

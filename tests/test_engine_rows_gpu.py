@@ -1,9 +1,9 @@
 """Engines over a cache in 8 bits and with drafted tokens: models that do not take them, and what a step may not leave behind."""
 import pytest
+import torch
 
 import qwen3_b200 as q
-from helpers import tiny
-from test_takes_rows import plan_with
+from test_takes_rows import plan_with, shifted_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,24 @@ def test_a_convolution_over_the_rows_is_refused(taps):
     with pytest.raises(q.StepError):
         engine.step_tree([q.TreeEntry(slot, [1], [-1])])
     assert engine.length(slot) == 3
+
+
+@pytest.mark.parametrize("cache_dtype", [None, "float8"])
+def test_blocks_that_keep_a_row_are_refused_drafted_tokens(cache_dtype):
+    """Their steps go over either cache: a sequence run whole is the sequence run in pieces and token by token."""
+    engine = q.Engine.from_random(Config(shifted_plan()), 2, dtype="float32", max_tokens=512, cache_dtype=cache_dtype)
+    tokens = [(7 * i) % 251 for i in range(80)]
+    outs = []
+    for cuts in ([80], [40, 30, 10], [76, 1, 1, 1, 1]):
+        slot, at = engine.new_sequence(), 0
+        for n in cuts:
+            last = engine.step([q.StepEntry(slot, tokens[at:at + n], want=[n - 1])])
+            at += n
+        outs.append(last.clone())
+        with pytest.raises(q.StepError):
+            engine.step_tree([q.TreeEntry(slot, [1, 2, 3], [-1, 0, 0])])
+        assert engine.length(slot) == 80
+        engine.release(slot)
+    # 32-bit sums in another order, and over 8 bits one rounding of a row that they turn
+    bound = (2e-4 if cache_dtype is None else 0.02) * float(outs[0].abs().max())
+    assert all(float((o - outs[0]).abs().max()) <= bound for o in outs)
