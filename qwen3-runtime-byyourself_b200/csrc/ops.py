@@ -1620,8 +1620,8 @@ def _status_word(device) -> torch.Tensor:
 
 
 def tcgen05_status(device) -> int:
-    """0, or where a bounded wait inside the tcgen05 product gave up (1 producer, 2 MMA, 3 epilogue);
-    reading it synchronises the device and clears it."""
+    """0, or where a bounded wait inside a tcgen05 kernel gave up (1 producer, 2 MMA, 3 epilogue, 4 accumulator of a product; 11 to 22 the
+    prompt attention; 36 to 51 the attention of drafted tokens); reading it synchronises the device and clears it."""
     word = _status_word(torch.device(device))
     value = int(word.item())
     if value:

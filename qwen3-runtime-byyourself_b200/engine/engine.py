@@ -305,8 +305,8 @@ class Engine:
         from ..csrc import ops
         where = ops.tcgen05_status(self.device)
         if where:
-            raise ops.KernelError(f"a wait inside the tcgen05 product ran out (stage {where}: 1 producer, 2 MMA, "
-                                  f"3 epilogue, 4 accumulator); its results are not valid")
+            raise ops.KernelError(f"a wait inside a tcgen05 kernel ran out (stage {where}: 1 to 4 a product - producer, MMA, epilogue, accumulator - "
+                                  f"or the decode attention, 11 to 22 the prompt attention, 36 to 51 the attention of drafted tokens); its results are not valid")
 
     # -- the step
     def step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:

@@ -87,8 +87,9 @@ def generate_speculative(engine: Engine, prompts: Sequence[Sequence[int]], max_n
         return -(-tokens // engine.cache.page_tokens)
 
     def choose(logits: torch.Tensor) -> List[int]:
-        ids = torch.empty(logits.shape[0], dtype=torch.int32, device=engine.device)
-        return ops.argmax(logits, ids).tolist()
+        ids = ops.argmax(logits, torch.empty(logits.shape[0], dtype=torch.int32, device=engine.device)).tolist()
+        engine.check_kernels()                               # the device has been waited for: nothing of a step that a kernel gave up on is taken
+        return ids
 
     for batch in plan_batches([len(p) for p in prompts], max_new_tokens, engine.cache.n_pages, engine.cache.n_slots, engine.cache.page_tokens,
                               batch_size):

@@ -51,3 +51,21 @@ def test_blocks_that_keep_a_row_are_refused_drafted_tokens(cache_dtype):
     # 32-bit sums in another order, and over 8 bits one rounding of a row that they turn
     bound = (2e-4 if cache_dtype is None else 0.02) * float(outs[0].abs().max())
     assert all(float((o - outs[0]).abs().max()) <= bound for o in outs)
+
+
+def test_a_kernel_that_gave_up_ends_the_generation():
+    """The word that a kernel sets when a wait runs out is set by hand, between steps: the tokens of that step are not returned, the slots and
+    pages go back, and the next generation runs."""
+    from qwen3_b200.csrc import ops
+    engine = q.Engine.from_random(Config(plan_with()), 3, dtype="float32", max_tokens=512)
+    calls = [0]
+
+    def draft(text):
+        calls[0] += 1
+        if calls[0] == 3:
+            ops._status_word(engine.device).fill_(47)
+        return [1, 2], [-1, 0]
+    with pytest.raises(ops.KernelError, match="47.*drafted"):
+        q.generate_speculative(engine, [[5, 6, 7]], 20, draft=draft)
+    assert engine.cache.pages_held() == 0 and calls[0] == 3
+    assert len(q.generate_speculative(engine, [[5, 6, 7]], 5, draft=draft)[0].token_ids) == 5
