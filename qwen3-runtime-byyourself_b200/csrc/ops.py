@@ -1613,6 +1613,9 @@ _tc_status = {}
 
 
 def _status_word(device) -> torch.Tensor:
+    """The device's word; one without a number is the current one, as tensors name it."""
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
     word = _tc_status.get(device)
     if word is None:
         word = _tc_status[device] = torch.zeros(1, dtype=torch.int32, device=device)

@@ -69,3 +69,16 @@ def test_a_kernel_that_gave_up_ends_the_generation():
         q.generate_speculative(engine, [[5, 6, 7]], 20, draft=draft)
     assert engine.cache.pages_held() == 0 and calls[0] == 3
     assert len(q.generate_speculative(engine, [[5, 6, 7]], 5, draft=draft)[0].token_ids) == 5
+
+
+def test_the_status_word_is_the_devices_however_it_is_named():
+    """Kernels write into the word of the device that their tensors name ("cuda:0"); an engine or a caller may have named it "cuda"."""
+    from qwen3_b200.csrc import ops
+    engine = q.Engine.from_random(Config(plan_with()), 3, dtype="float32", max_tokens=512, device="cuda")
+    engine.check_kernels()
+    for name in ("cuda", torch.device("cuda"), torch.device("cuda", torch.cuda.current_device())):
+        ops._status_word(torch.zeros(1, device="cuda").device).fill_(48)
+        assert ops.tcgen05_status(name) == 48 and ops.tcgen05_status(name) == 0
+    ops._status_word(torch.zeros(1, device="cuda").device).fill_(48)
+    with pytest.raises(ops.KernelError):
+        engine.check_kernels()
