@@ -1437,6 +1437,9 @@ def cache_append(qkv: torch.Tensor, q_out: torch.Tensor, cache: CachePages, q_no
     return q_out
 
 
+CACHE_READ_SEQS = 65535                # sequences of a call
+
+
 def cache_read(cache: CachePages, page_table, seq_end, keys_out: torch.Tensor, values_out: torch.Tensor) -> None:
     """The rows of an 8-bit cache as pages of bfloat16 or float32: page j of sequence s to keys_out[s, j] and values_out[s, j]
     [sequences, pages, kv heads, PAGE_TOKENS, head size], for every page that holds one of the first seq_end[s] rows; rows behind

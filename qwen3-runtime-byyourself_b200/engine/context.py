@@ -9,7 +9,10 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Tuple
 
+import numpy as np
 import torch
+
+from ..cache.book import PAGE_TOKENS
 
 
 class Scratch:
@@ -99,13 +102,25 @@ class StepContext:
     # a step with drafted tokens (Engine.step_tree): token_pos is then the place in the tree, and the tokens stand side by side in the cache
     token_place: Optional[torch.Tensor] = None    # [N] int32: the token's place in its sequence's cache (None: token_pos)
     tree: Optional[torch.Tensor] = None           # [N, words] int64: bit n of a token's mask: it sees its sequence's new token n
-    _ends: Optional[tuple] = field(default=None, repr=False)
+    _read: Dict[int, tuple] = field(default_factory=dict, repr=False)
 
-    def read_back(self, pages: int):
-        """For caches in 8 bits that are read back for a step: the sequences' lengths after the step, and the table of `pages` pages
-        a sequence in their order (made once a step)."""
-        if self._ends is None:
-            ends = self.seq_pos0 + (self.seq_start[1:] - self.seq_start[:-1])
-            table = torch.arange(self.n_seqs * pages, dtype=torch.int32, device=self.device).view(self.n_seqs, pages)
-            self._ends = (ends, table)
-        return self._ends
+    def read_back(self, group: int):
+        """For a cache in 8 bits that is read back for a step: the sequences' pages one after the other, as many as they hold.  Returns, for
+        a cache group, the page to read for each (int32 [pages, 1]), how many of its rows count (int32 [pages]) and the sequences' page table
+        over what was read (int32 [sequences, most pages of one]).  Made once a step."""
+        if not self._read:
+            lengths = np.asarray(self.host_pos0, dtype=np.int64) + np.asarray(self.host_n_new, dtype=np.int64)
+            counts = -(-lengths // PAGE_TOKENS)
+            first, total, most = np.cumsum(counts) - counts, int(counts.sum()), int(counts.max())
+            seq = np.repeat(np.arange(self.n_seqs), counts)
+            number = np.arange(total) - first[seq]
+            host = np.zeros(2 * total + self.n_seqs * most, dtype=np.int32)
+            host[:total] = seq * self.page_tables[group].shape[1] + number
+            host[total:2 * total] = np.minimum(lengths[seq] - PAGE_TOKENS * number, PAGE_TOKENS)
+            host[2 * total:].reshape(self.n_seqs, most)[seq, number] = np.arange(total)        # (behind a sequence's last page: any page that there is)
+            dev = torch.from_numpy(host).to(self.device)
+            self._read[-1] = dev[:total], dev[total:2 * total], dev[2 * total:].view(self.n_seqs, most)
+        where, rows, table = self._read[-1]
+        if group not in self._read:
+            self._read[group] = self.page_tables[group].reshape(-1).index_select(0, where).view(-1, 1), rows, table
+        return self._read[group]

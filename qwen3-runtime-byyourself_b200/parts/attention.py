@@ -385,7 +385,8 @@ class GQAAttention(Part):
 
     def mix_rows(self, x, ctx, cache, attn, table) -> torch.Tensor:
         """`mix` over a cache in 8 bits, and for a step with drafted tokens over any: rows are appended at places of their own, and the
-        new tokens of a sequence attend to the pages as they are.  Long prompts over a cache in 8 bits read it back first, for the prompt kernels."""
+        new tokens of a sequence attend to the pages as they are.  Long prompts over a cache in 8 bits read it back first, for the prompt kernels:
+        the pages that the step's sequences hold, in the compute type, into buffers that all layers share."""
         if not self.takes_rows() or cache.shared:
             raise ops.KernelError("this attention takes neither a cache in 8 bits nor drafted tokens")
         nq, nkv, d, N = self.num_heads, self.num_kv_heads, self.head_dim, ctx.n_tokens
@@ -405,14 +406,13 @@ class GQAAttention(Part):
             counters = ctx.scratch.counters("attn.tree_counters", sizes.counters)
             return ops.attention_tree(q, pages, attn, parts, counters, ctx.seq_start, ctx.seq_pos0, table, ctx.max_new, nq, self.scale,
                                       tree=ctx.tree)
-        per_seq = -(-ctx.max_context // ops.PAGE_TOKENS)
-        shape = (ctx.n_seqs, per_seq, nkv, ops.PAGE_TOKENS, d)
-        keys, values = (ctx.scratch.get(name, shape, ctx.dtype) for name in ("attn.read_keys", "attn.read_values"))
-        ends, read_table = ctx.read_back(per_seq)
-        ops.cache_read(pages, table, ends, keys, values)
-        flat = (ctx.n_seqs * per_seq, nkv, ops.PAGE_TOKENS, d)
-        self.attend(q, dataclasses.replace(cache, keys=keys.view(flat), values=values.view(flat), key_scales=None, value_scales=None, _rows=None), attn, ctx,
-                    read_table)
+        numbers, rows, read_table = ctx.read_back(cache.group)
+        n_pages = numbers.shape[0]
+        keys, values = (ctx.scratch.get(name, (n_pages, 1, nkv, ops.PAGE_TOKENS, d), ctx.dtype) for name in ("attn.read_keys", "attn.read_values"))
+        for i in range(0, n_pages, ops.CACHE_READ_SEQS):
+            some = slice(i, i + ops.CACHE_READ_SEQS)
+            ops.cache_read(pages, numbers[some], rows[some], keys[some], values[some])
+        self.attend(q, dataclasses.replace(cache, keys=keys[:, 0], values=values[:, 0], key_scales=None, value_scales=None, _rows=None), attn, ctx, read_table)
         return attn
 
     def decodes_split(self, ctx) -> bool:

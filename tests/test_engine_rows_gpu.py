@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import qwen3_b200 as q
+from helpers import tiny
 from test_takes_rows import plan_with, shifted_plan
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +83,31 @@ def test_the_status_word_is_the_devices_however_it_is_named():
     ops._status_word(torch.zeros(1, device="cuda").device).fill_(48)
     with pytest.raises(ops.KernelError):
         engine.check_kernels()
+
+
+@pytest.mark.parametrize("name,dtype", [("D", "bfloat16"), ("C", "bfloat16"), ("A", "float32")])
+def test_a_step_reads_back_the_pages_that_it_holds(monkeypatch, name, dtype):
+    """One prompt beside single tokens of sequences of very unequal length: the buffers hold the sequences' pages, not as many for each as the
+    longest has, and every token has the logits that it has where the prompt runs by itself and the others attend to the pages as they are."""
+    from qwen3_b200.parts import attention
+    monkeypatch.setattr(attention, "rows_at_once", 64)
+    config = q.config_from_dict(dict(tiny(name, max_position_embeddings=512), torch_dtype="bfloat16"))
+    lengths, outs = [400] + [5 + i for i in range(12)] + [64], []
+    prompt = [(5 * i) % 200 for i in range(90)]
+    for together in (True, False):
+        engine = q.Engine.from_random(config, 5, dtype=dtype, max_tokens=64 * 40, cache_dtype="float8", guard_scratch=True)
+        slots = [engine.new_sequence() for _ in lengths]
+        for s, n in zip(slots, lengths):                                  # (one by one: what is read back by then is small)
+            for at in range(0, n, 64):
+                engine.step([q.StepEntry(s, [(3 * i + s) % 200 for i in range(at, min(at + 64, n))])])
+        engine.scratch = type(engine.scratch)(engine.device, guard=True)
+        new = engine.new_sequence()
+        ones, run = [q.StepEntry(s, [9], want=[0]) for s in slots], [q.StepEntry(new, prompt, want=[0, 50, 89])]
+        outs.append(engine.step(ones + run).clone() if together else torch.cat([engine.step(ones).clone(), engine.step(run).clone()]))
+        assert engine.scratch_violations() == []
+        read = [t.numel() for k, t in engine.scratch._flat.items() if k[0] == "attn.read_keys"]
+        pages = (sum(-(-(n + 1) // 64) for n in lengths) if together else 0) + 2
+        assert read == [pages * 64 * config.num_key_value_heads * config.head_dim]
+    # as the bound of the two ways over one sequence: a rounding of a layer's rows to the compute type, which can move a code by one of its steps
+    bound = 0.06 if dtype == "bfloat16" else 0.02
+    assert float((outs[0] - outs[1]).abs().max()) <= bound * float(outs[0].abs().max())
