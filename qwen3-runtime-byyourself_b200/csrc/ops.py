@@ -1348,6 +1348,18 @@ def attention_decode_flat_parts(d: int, group: int) -> int:
     return int(fn(group))
 
 
+_sm_counts = {}
+
+
+def sm_count(device=None) -> int:
+    """The device's SMs (None: the current device's)."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    count = _sm_counts.get(device)
+    if count is None:
+        count = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return count
+
+
 # ------------------------------------------------------------------ a cache in 8 bits, steps with drafted tokens
 # Arguments go to these kernels as a structure (include/qwen3/cache_args.h): packed in half a microsecond, where two dozen arguments through ctypes take
 # two.  A call from Python is as long as the kernels of a small step: attention of one sequence took 12.9 us of the host, the kernel 7.8.
@@ -1485,11 +1497,12 @@ class TreeScratch:
 # Rows of a kv head (new tokens of a sequence x query heads a kv head) from which a step goes to the tcgen05 kernel.  mma.sync / tcgen05 at 20 rows, 8 kv heads:
 # bfloat16, 1 sequence of 500 tokens 20.7 / 14.3 us, of 16,000 49.9 / 33.2, 8 of up to 4,000 38.2 / 29.2; 8 bits 19.9 / 16.8, 46.9 / 35.8, 35.9 / 33.9.  At 16 rows
 # bfloat16 16.6 / 14.3, 47.4 / 29.9, 29.4 / 27.7, 32 sequences of up to 2,000 tokens 39.7 / 46.6; 8 bits 27.8 / 37.0 for 8 of up to 4,000.
-# Up to 32 rows (a tile of the mma.sync kernel's) it has to have no more items (sequences x kv heads) than blocks: 28 rows, 20 sequences of up to 20 tokens
-# 13.1 / 16.8, of up to 250 21.9 / 20.9, 32 of them 20.1 / 25.4 - or, in bfloat16, page tables of more than `tree_tc_table` pages (32 of up to 1,000 tokens
-# 39.3 / 39.4, of up to 2,500 60.5 / 51.1; 8 bits 30.9 / 47.7, 55.8 / 70.0); and in 8 bits no more than `tree_tc_pages` pages in all (8 sequences of up to 16,000
-# 70.0 / 97.2, 12 of up to 6,000 44.0 / 52.1: the codes of a page take the tcgen05 kernel as long for 20 rows as for 128).
-tree_tc_rows, tree_tc_items, tree_tc_table, tree_tc_pages = 17, 148, 16, 4096
+# Up to 32 rows (a tile of the mma.sync kernel's) it has to have no more items (sequences x kv heads) than blocks, of which it has one an SM (`tree_tc_items`
+# None): 28 rows, 20 sequences of up to 20 tokens 13.1 / 16.8, of up to 250 21.9 / 20.9, 32 of them 20.1 / 25.4 - or, in bfloat16, sequences of more than
+# `tree_tc_table` pages (32 of up to 1,000 tokens 39.3 / 39.4, of up to 2,500 60.5 / 51.1; 8 bits 30.9 / 47.7, 55.8 / 70.0); and in 8 bits no more than
+# `tree_tc_pages` pages in all (8 sequences of up to 16,000 70.0 / 97.2, 12 of up to 6,000 44.0 / 52.1: the codes of a page take the tcgen05 kernel as long for 20
+# rows as for 128).
+tree_tc_rows, tree_tc_items, tree_tc_table, tree_tc_pages = 17, None, 16, 4096
 _tree_parts = {}
 # source, entry point, whether it is compiled for a head size
 _TREE_FORMS = {"any": ("attention_tree.cu", "q3_attention_tree_any_", False), "mma": ("attention_tree_mma.cu", "q3_attention_tree_mma_", True),
@@ -1501,15 +1514,17 @@ def attention_tree_tiled(dtype: torch.dtype, d: int) -> bool:
     return dtype == torch.bfloat16 and d in (64, 128)
 
 
-def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int, eight_bit: bool, items: int, table: int) -> str:
-    """Which kernel takes a step of `rows` rows a kv head at most and of so many items (sequences x kv heads), with page tables of `table` pages, over a
+def _tree_form(dtype: torch.dtype, rows: int, d: int, scale: float, places: int, eight_bit: bool, items: int, table: int, device=None) -> str:
+    """Which kernel takes a step of `rows` rows a kv head at most and of so many items (sequences x kv heads), of sequences of up to `table` pages, over a
     cache of so many places (pages x kv heads x PAGE_TOKENS): `tc` and `mma` take bfloat16 queries and head sizes 64 and 128, `any` the others."""
     if not attention_tree_tiled(dtype, d):
         return "any"
     if rows < tree_tc_rows or scale <= 0 or places >= 2 ** 31:
         return "mma"
-    if rows <= 32 and (items > tree_tc_items or items * table > tree_tc_pages if eight_bit else items > tree_tc_items and table <= tree_tc_table):
-        return "mma"
+    if rows <= 32:
+        many = items > (tree_tc_items or sm_count(device))
+        if many or items * table > tree_tc_pages if eight_bit else many and table <= tree_tc_table:
+            return "mma"
     return "tc"
 
 
@@ -1535,13 +1550,14 @@ def attention_tree_scratch(n_seqs: int, max_new: int, nq: int, nkv: int, d: int,
 
 
 def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts: torch.Tensor, counters: torch.Tensor, seq_start, seq_pos0,
-                   page_table, max_new: int, nq: int, scale: float, tree: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   page_table, max_new: int, nq: int, scale: float, tree: Optional[torch.Tensor] = None, max_pages: Optional[int] = None) -> torch.Tensor:
     """Attention of the new tokens of every sequence - one, a run, or a tree of drafted ones - over the cache's pages, which hold
     their keys and values already (`cache_append`).  Sequence s brings tokens seq_start[s] .. seq_start[s + 1] - 1 (at most `max_new`),
     whose rows stand at places seq_pos0[s], seq_pos0[s] + 1, ... of its cache.  A token sees all earlier rows of its sequence
     and, of the new ones, number n where bit n % 64 of tree[token, n // 64] is set (`tree` int64 [tokens, words]); without `tree`
     those up to itself.  A token that sees nothing gets zeros.  q, out [tokens, nq * head size]; `parts` and `counters` as
-    `attention_tree_scratch` says."""
+    `attention_tree_scratch` says.  `max_pages`: the most pages that a sequence has after the step, where that is known and less than a row of
+    `page_table` has places; which kernel is taken hangs on it, not what comes out."""
     s, dtype, shape, d, nkv = _suffix(q), q.dtype, q.shape, cache.d, cache.kv_heads
     n_seqs, row_of = seq_pos0.numel(), page_table.shape
     if len(shape) != 2 or shape[1] != nq * d or out.shape != shape or nq <= 0 or nq % nkv or len(row_of) != 2 \
@@ -1553,7 +1569,8 @@ def attention_tree(q: torch.Tensor, cache: CachePages, out: torch.Tensor, parts:
             raise KernelError("attention_tree: the masks are int64 [tokens, words], with 64 new tokens a word")
         masks, words = _at(tree, "tree", torch.int64), tree.shape[1]
     q_at, rows, parts_at, counters_at, status = _at(q, "q", dtype), max_new * (nq // nkv), 0, 0, 0
-    form = _tree_form(dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS, cache.eight_bit, n_seqs * nkv, row_of[1])
+    form = _tree_form(dtype, rows, d, scale, cache.n_pages * nkv * PAGE_TOKENS, cache.eight_bit, n_seqs * nkv,
+                      row_of[1] if max_pages is None else min(max_pages, row_of[1]), q.device)
     if form != "any":
         if parts.numel() < _tree_parts_of(form, rows, d, q.device) or counters.numel() < n_seqs * nkv * -(-rows // 8):
             raise KernelError("attention_tree: parts or counters are too small (attention_tree_scratch)")

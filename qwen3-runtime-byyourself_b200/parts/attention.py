@@ -405,7 +405,7 @@ class GQAAttention(Part):
             parts = ctx.scratch.get("attn.tree_parts", (sizes.parts,), torch.float32)
             counters = ctx.scratch.counters("attn.tree_counters", sizes.counters)
             return ops.attention_tree(q, pages, attn, parts, counters, ctx.seq_start, ctx.seq_pos0, table, ctx.max_new, nq, self.scale,
-                                      tree=ctx.tree)
+                                      tree=ctx.tree, max_pages=-(-ctx.max_context // ops.PAGE_TOKENS))
         numbers, rows, read_table = ctx.read_back(cache.group)
         n_pages = numbers.shape[0]
         keys, values = (ctx.scratch.get(name, (n_pages, 1, nkv, ops.PAGE_TOKENS, d), ctx.dtype) for name in ("attn.read_keys", "attn.read_values"))
@@ -546,15 +546,7 @@ def _projection_pair_kernel(part, x, cache, q, ctx, table, q_norm_w, k_norm_w, e
     return True
 
 
-_sm_counts = {}
-
-
-def _sm_count(device) -> int:
-    device = torch.device(device)
-    count = _sm_counts.get(device)
-    if count is None:
-        count = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
-    return count
+_sm_count = ops.sm_count
 
 
 def _prefill_flash_kernel(part, q, cache, out, ctx, table) -> bool:

@@ -111,3 +111,24 @@ def test_a_step_reads_back_the_pages_that_it_holds(monkeypatch, name, dtype):
     # as the bound of the two ways over one sequence: a rounding of a layer's rows to the compute type, which can move a code by one of its steps
     bound = 0.06 if dtype == "bfloat16" else 0.02
     assert float((outs[0] - outs[1]).abs().max()) <= bound * float(outs[0].abs().max())
+
+
+@pytest.mark.parametrize("cache_dtype,sequences,positions,want", [(None, 80, 2048, "mma"), ("float8", 40, 8192, "tc"), (None, 40, 2048, "tc"), ("float8", 80, 8192, "mma")])
+def test_the_form_goes_by_the_steps_lengths(monkeypatch, cache_dtype, sequences, positions, want):
+    """Page tables of an engine are as wide as its longest sequence may become; which kernel takes a step of 20 rows a kv head goes by what the
+    sequences hold: 160 items of a page each are many for tcgen05 over bfloat16, 80 are not over 8 bits."""
+    from qwen3_b200.csrc import ops
+    config = q.config_from_dict(dict(tiny("D", max_position_embeddings=positions), torch_dtype="bfloat16"))
+    engine = q.Engine.from_random(config, 5, dtype="bfloat16", max_tokens=64 * max(sequences, positions // 64), n_slots=sequences, cache_dtype=cache_dtype)
+    assert engine.cache.pages_per_slot == positions // 64
+    slots, names, call = [engine.new_sequence() for _ in range(sequences)], [], ops._call_packed
+
+    def recorded(what, source, name, *a):
+        names.append(name)
+        return call(what, source, name, *a)
+    monkeypatch.setattr(ops, "_call_packed", recorded)
+    engine.step([q.StepEntry(s, [1 + s % 50, 2]) for s in slots])
+    names.clear()
+    engine.step_tree([q.TreeEntry(s, [3] * 10, list(range(-1, 9))) for s in slots])
+    engine.keep({s: [] for s in slots})
+    assert [n for n in names if "tree" in n] == [f"q3_attention_tree_{want}_bf16"] * 2
