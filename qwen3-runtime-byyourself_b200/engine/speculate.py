@@ -133,8 +133,9 @@ def generate_speculative(engine: Engine, prompts: Sequence[Sequence[int]], max_n
                     keep = keep[:max(room, 0)]
                     entries.append(TreeEntry(live[i], [text[-1]] + [int(tokens[n]) for n in keep],
                                              [-1] + [number[parents[n]] if parents[n] >= 0 else 0 for n in keep]))
-                # a tree that the pages have no room for, beside a page for each sequence, goes without its drafts
-                free = min(g.n_free for g in engine.cache.groups) - len(entries)
+                # a tree that the pages have no room for, beside the pages that the sequences' next tokens need, goes without its drafts
+                free = min(g.n_free for g in engine.cache.groups)
+                free -= sum(pages(engine.length(e.slot) + 1) - pages(engine.length(e.slot)) for e in entries)
                 for e in entries:
                     length = engine.length(e.slot)
                     need = pages(length + len(e.tokens)) - pages(length + 1)

@@ -75,3 +75,25 @@ def test_nothing_of_a_step_that_failed_is_taken(fails_at):
     with pytest.raises(ops.KernelError):
         q.generate_speculative(engine, [[5], [9, 10]], 9, draft=lambda text: ([text[-1] + 1], [-1]))
     assert len(engine.kept) == max(fails_at - 1, 0) and not engine.held       # of the prompts' step nothing has to be kept
+
+
+def test_drafts_that_need_no_page_run_where_none_is_free(monkeypatch):
+    """The sequences' pages have room for their drafts; no other page is free."""
+    monkeypatch.setattr(Group, "n_free", 0)
+    engine = Engine()
+    got = q.generate_speculative(engine, [[1] * 20, [2] * 30], 12, draft=lambda text: ([text[-1] + 1, text[-1] + 2], [-1, 0]))
+    assert [r.token_ids for r in got] == [list(range(2, 14)), list(range(3, 15))] and engine.steps == 5
+
+
+def test_drafts_leave_a_page_for_every_sequence(monkeypatch):
+    """Three sequences stand at the end of their pages and two pages more than they need are free: two of the trees that ask for one more get it."""
+    monkeypatch.setattr(Group, "n_free", 3 + 2)
+    engine, asked = Engine(), []
+    step_tree = engine.step_tree
+
+    def counted(entries):
+        asked.append([len(e.tokens) for e in entries])
+        return step_tree(entries)
+    engine.step_tree = counted
+    q.generate_speculative(engine, [[1] * 64] * 3, 80, draft=lambda text: ([0] * 70, [-1] * 70))
+    assert asked[0] == [71, 71, 1]
