@@ -114,11 +114,12 @@ class StepContext:
             first, total, most = np.cumsum(counts) - counts, int(counts.sum()), int(counts.max())
             seq = np.repeat(np.arange(self.n_seqs), counts)
             number = np.arange(total) - first[seq]
-            host = np.zeros(2 * total + self.n_seqs * most, dtype=np.int32)
+            pinned = torch.zeros(2 * total + self.n_seqs * most, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+            host = pinned.numpy()
             host[:total] = seq * self.page_tables[group].shape[1] + number
             host[total:2 * total] = np.minimum(lengths[seq] - PAGE_TOKENS * number, PAGE_TOKENS)
             host[2 * total:].reshape(self.n_seqs, most)[seq, number] = np.arange(total)        # (behind a sequence's last page: any page that there is)
-            dev = torch.from_numpy(host).to(self.device)
+            dev = pinned.to(self.device, non_blocking=True)                # (a copy that is waited for would stop the launches of the step's layers)
             self._read[-1] = dev[:total], dev[total:2 * total], dev[2 * total:].view(self.n_seqs, most)
         where, rows, table = self._read[-1]
         if group not in self._read:
