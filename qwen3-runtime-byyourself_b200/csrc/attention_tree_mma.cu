@@ -8,8 +8,8 @@
 //   - Products are mma.m16n8k16 with keys, then values, as the 16-row operand and the rows as its eight columns: S^T = K Q^T and O^T = V^T P^T, so 8 rows
 //     cost 8, not 16.  What a lane holds of keys and values are runs of 16 bytes, which fixes the order in which the products walk a
 //     head's values and the keys; the query is read in the same order.  The weights change from rows to columns by movmatrix.
-//   - 8 bits: a code is exact in half precision and becomes that in one conversion a pair (products of codes themselves are put together from the same
-//     conversions on this architecture).  Queries are divided by a power of two for each row, so that they fit, exactly, unless a value is below 2^-24 of its
+//   - 8 bits: a code is exact in half precision and becomes that in one conversion a pair (products of the codes themselves were tried and gained
+//     nothing).  Queries are divided by a power of two for each row, so that they fit, exactly, unless a value is below 2^-24 of its
 //     row's largest.  The key's scale multiplies the score.  The value's scale 2^v is part of the weight: w = 2^(x + v - M), x the score in log2 units
 //     and M the running maximum of x + v, so the largest weight is of the order of 1 whatever the scales are, and what half precision drops is
 //     below 2^-24 of the largest term; the sum of the softmax is that of w 2^-v, in 32 bits.
