@@ -7,9 +7,10 @@
 // of the query's type or codes of 8 bits with a scale a row (page8.cuh).
 // A block a (token, query head): each of its warps takes every eighth stretch of 32 keys, with a running maximum and sum of its own, and they meet at the
 // end.  The stretch's scores are made eight keys at a time, so that many loads are on their way; then its maximum and its weights, a key a lane; then
-// its values are added up, eight at a time again.  A key that is not seen is not read.  It is here for 32-bit queries and odd head sizes, and bound by the
-// latency of its loads: one token of 32 heads over 8 and 2,000 keys, 32-bit, 110 us (one key after the other 443), 8 sequences of them and 8 tokens each 877 (1,598); rows
-// that share a head's keys read them from the L2 again.
+// its values are added up, eight at a time again.  A key that is not seen is not read.  It is here for 32-bit queries and odd head sizes.  Its grid
+// bounds it: one token of 32 heads is 32 blocks on 148 SMs, each with a chain of loads over all keys, and rows that share a head's keys read them from the L2 again.
+// One token of 32 heads over 8 and 2,000 keys, 32-bit, 102 us (one key after the other 443; the floor is 2.5), 8 sequences of up to 2,000 and 8 tokens each 322
+// (floor 9.3); bfloat16 heads of 96 over 8 bits, 8 sequences of up to 4,000 and one token each 340 (floor 5.1), heads of 256 517 (7.7).
 #include "../include/qwen3/cache_args.h"
 #include "page8.cuh"
 

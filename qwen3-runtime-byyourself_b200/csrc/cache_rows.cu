@@ -2,9 +2,12 @@
 // read back, and moved after a step with drafted tokens.
 //
 // All three move bytes and compute next to nothing, so each is bound by memory; what each row costs:
-//   append   reads (nq + 2 nkv) d values of the projection and d / 2 angles a token, writes nq d values and 2 nkv rows: 8,000 tokens of 32 + 16 heads of 128
-//            40 us (4.6 TB/s; instructions share the bound: the norm, the rotation and the codes of a value), 8 tokens 2.7;
+//   append   reads (nq + 2 nkv) d values of the projection and d / 2 angles a token, writes nq d values and 2 nkv rows: 8,000 tokens of 32 + 16 heads of 128,
+//            bfloat16 to 8 bits, 39.7 us (4.6 TB/s) where a normed value is rounded once, 44.8 with Qwen3's roundings after each step of the norm: the same
+//            bytes, so instructions share the bound (the largest stall is memory all the same).  Into bfloat16 pages 41.4 and 43.8; 32-bit rows to 8 bits 62.6
+//            (5.6 TB/s), as they are 68.4.  8 tokens 2.4 to 2.9;
 //   read     reads d + 1 bytes a row and writes 2 d (bfloat16): 8 sequences of up to 8,000 rows and 8 heads of 128 in 43 us (6.0 TB/s), one of 2,000 3.7;
+//            float32, 4 d written, 99 (4.3 TB/s);
 //   keep     reads and writes the rows that move: 36 layers of 8 sequences 4.8 us, one sequence 3.5, which is a launch and a chain of three loads.
 // Norm and rotation as in attention.cu's qkv_prepare (src/model/self_attention.cpp:122-152): y = x / sqrt(mean(x^2) + eps) w
 // over a head, values i and i + r/2 of the first r turned by the angle of the token's position.  A token's place in the

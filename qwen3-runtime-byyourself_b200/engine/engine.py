@@ -220,7 +220,9 @@ class Engine:
                  cache_dtype: Optional[str] = None):
         """`guard_scratch` (tests): activation buffers of exact size between guard zones; see `scratch_violations`.
         `cache_dtype` "float8": keys and values are kept as 8-bit codes with a scale of a power of two for each row of a head (129 bytes
-        instead of 256 at head size 128), for models of plain attention over all keys; None: as they are computed."""
+        instead of 256 at head size 128), for models of plain attention over all keys; None: as they are computed.  The tensor-core kernels of
+        such a cache take bfloat16 engines with heads of 64 and 128; 32-bit engines and other head sizes decode over it with a general kernel (8 sequences
+        of up to 4,000 tokens, heads of 96: 340 us a layer, where a bfloat16 cache takes 20)."""
         if model.dtype is None:
             raise ValueError("the model has no weights bound")
         self.model, self.config, self.plan = model, config, model.plan

@@ -1,8 +1,13 @@
 """Greedy generation with drafted tokens: a drafter proposes how each sequence may go on, one step runs the whole tree of proposals
 over the cache, and the tokens that the model itself would have chosen are kept.
 
-The tokens are those of greedy generation one by one (up to ties and to what the order of 32-bit sums can turn), in fewer steps: a step
-reads weights and cache once for all tokens of its trees, and yields one token more than the drafted ones that stand.
+A step reads weights and cache once for all tokens of its trees, and yields one token more than the drafted ones that stand.  The tokens are those that
+greedy generation one by one chooses, but where the two largest logits lie within the arithmetic's rounding: a step of another shape takes other kernels, which
+add up in another order, in 32 bits and, in a bfloat16 engine, with roundings to 16 bits in other places (as steps of other batch sizes do).  A chosen token that
+differs changes all that follow.
+
+Drafts pay where enough of them stand: a tree step is launched kernel by kernel, where a decode step is replayed from a graph (8B shape, 8 sequences of
+4,096, bfloat16: 3.9 ms a decode step; 5.0, 5.3 and 6.0 with 4, 8 and 16 tokens a sequence).
 """
 from __future__ import annotations
 
@@ -20,7 +25,8 @@ class PromptLookup:
     """Drafts from the sequence's own text: where its last few tokens stood before, they were followed by what may follow now.
 
     `longest` to `shortest` tokens are looked for, the longest match first and the latest places first; up to `branches` different continuations
-    of up to `depth` tokens make a tree of at most `tokens` tokens."""
+    of up to `depth` tokens make a tree of at most `tokens` tokens.  The whole text is walked through on the host: without a match 1.5 ms for 4,096
+    tokens and 14 for 32,000, a sequence and step; long texts want a drafter that keeps an index."""
 
     def __init__(self, tokens: int = 15, depth: int = 8, branches: int = 3, longest: int = 4, shortest: int = 1):
         if tokens < 0 or depth < 1 or branches < 1 or not 1 <= shortest <= longest:

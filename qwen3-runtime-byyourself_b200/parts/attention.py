@@ -668,9 +668,11 @@ def _decode_capped_fused_kernel(part, qkv, cache, out, ctx, table, q_norm_w, k_n
 
 
 # Over a cache in 8 bits the sequences of a step that bring at most so many tokens attend to the pages as they are; with more the step reads its
-# sequences' pages back for the prompt kernels, which then share a head's keys among many tiles of rows.  A small layer with 32 heads of 128 over
-# 8, as they are / read back: 1 sequence of 2,000 tokens and 64 new ones 164 / 229 us, of 16,000 158 / 703; 8 of 4,000 and 64 197 / 395, 256 394 / 399, 512
-# 957 / 1,019, 1,024 2,420 / 2,362.  The general kernel (32-bit queries, other head sizes) is behind from two new tokens on (1 of 2,000: 329 / 237).
+# sequences' pages back for the prompt kernels, which then share a head's keys among many tiles of rows.  A layer of 32 heads of 128 over 8 and a hidden
+# size of 512 in a step of 12, as they are / read back: 1 sequence of 2,000 tokens and 256 new ones 136 / 174 us, 512 139 / 177, 1,024 181 / 180; of 16,000 and
+# 64 135 / 628, 256 178 / 311, 512 269 / 323, 1,024 455 / 390; 8 of 4,000 and 64 151 / 306, 256 317 / 300, 512 556 / 455, 1,024 1,115 / 794; 512 tokens beside ten
+# single ones of 4,000 325 / 413.  So the bound is a middle: many long runs are read back too late, one of a long sequence too soon.  The general kernel
+# (32-bit queries, other head sizes) is behind from two new tokens on.
 rows_at_once = 512
 long_context_keys = 4096  # a decode step whose sequences may be longer takes wider clusters (if they are few)
 # Rows (sequences x kv heads) an SM of a decode step beyond which its pages are shared out evenly: the other form has two blocks an SM,
