@@ -1609,6 +1609,112 @@ def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> torch.Te
     return out
 
 
+# ------------------------------------------------------------------ 8-bit integers with a scale a row
+_ROWS8_ARGS, _GEMM8_ARGS = struct.Struct("@7q5qd2i"), struct.Struct("@7q2q6i")
+INT8_MAX_WIDTH = 131071                # a sum of so many products of two codes stays below 2^31
+
+
+class Int8Rows:
+    """Rows [rows, width] in 8 bits: a code stands for code * scale of its row.  `codes` int8 with rows a multiple of 16 bytes apart (`Int8Rows.empty`
+    makes room for any width), `scales` float32 [rows].  Tokens and matrices [channels, width] alike."""
+
+    __slots__ = ("codes", "scales", "rows", "width", "stride", "shape", "at", "scales_at", "device")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dim() != 2 or codes.dtype != torch.int8 or scales.shape != codes.shape[:1]:
+            raise KernelError("int8 rows: codes are int8 [rows, width], scales float32 [rows]")
+        if not codes.is_cuda or scales.device != codes.device:
+            raise KernelError("int8 rows: codes and scales are CUDA tensors of one device (there is no CPU path)")
+        self.scales_at = _dev(scales, "scales", torch.float32)
+        self.rows, self.width = codes.shape
+        self.shape, self.device = (self.rows, self.width), codes.device
+        # (a tensor of one row, or without any, may have any stride)
+        self.stride = codes.stride(0) if self.rows > 1 else -(-self.width // 16) * 16
+        if (self.width > 1 and codes.stride(1) != 1) or self.stride % 16 or self.stride < self.width or codes.data_ptr() % 16:
+            raise KernelError("int8 rows: rows of codes are whole, begin at 16-byte boundaries and are a multiple of 16 bytes apart")
+        end = codes.storage_offset() + (self.rows - 1) * self.stride + -(-self.width // 16) * 16
+        if self.rows and end > codes.untyped_storage().nbytes():
+            raise KernelError("int8 rows: the memory of the last row ends inside its last 16 bytes")
+        self.codes, self.scales, self.at = codes, scales, codes.data_ptr()
+
+    @classmethod
+    def empty(cls, rows: int, width: int, device) -> "Int8Rows":
+        codes = torch.empty(rows, -(-width // 16) * 16, dtype=torch.int8, device=device)[:, :width]
+        return cls(codes, torch.empty(rows, dtype=torch.float32, device=device))
+
+    def float(self) -> torch.Tensor:
+        """The values that the codes stand for."""
+        return self.codes.float() * self.scales[:, None]
+
+
+def _strided(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device) -> int:
+    """Where rows lie that are whole but may be any distance apart."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise KernelError(f"{name} must be {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
+        raise KernelError(f"{name} must have contiguous rows that do not overlap")
+    return t.data_ptr()
+
+
+def _on_current(device, what: str) -> int:
+    """The stream to launch on; the tensors have to lie on its device."""
+    if device.index != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return _here()
+
+
+def quantize_rows(x: torch.Tensor, out: Int8Rows) -> Int8Rows:
+    """Rows of x [rows, width] (bfloat16 or float32, contiguous rows any distance apart) as 8-bit codes: with a = max |x| of a row, code = 127 x / a to
+    the nearest whole number, ties to even, and scale = a / 127.  A row of zeros gets the scale 0, one with a NaN or an infinity the
+    scale NaN and codes of 0."""
+    s = _suffix(x)
+    at = _strided(x, "x", x.dtype, out.shape, out.device)
+    _call_packed("quantize_rows", "int8_rows.cu", "q3_quantize_rows_" + s, _ROWS8_ARGS.pack(
+        at, 0, 0, 0, out.at, out.scales_at, _on_current(out.device, "quantize_rows"), out.rows, x.stride(0), 0, 0, out.stride, 0.0, out.width, 0))
+    return out
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Rows, delta: Optional[torch.Tensor] = None,
+                  total: Optional[torch.Tensor] = None) -> Int8Rows:
+    """The rows x / sqrt(mean x^2 + eps) * weight in 32 bits, as 8-bit codes (see `quantize_rows`); weight is float32 [width].
+
+    With `delta` the norm reads x + delta (32-bit sum, stored in x's type), which is written to `total`, by default to x itself.  A
+    row whose squares' sum 32 bits do not hold counts as one with an infinity.  x, delta and total: contiguous rows any distance apart."""
+    s, dtype, device, shape = _suffix(x), x.dtype, out.device, out.shape
+    at = _strided(x, "x", dtype, shape, device)
+    if delta is None:
+        if total is not None:
+            raise KernelError("rms_norm_int8: a total is that of x and delta")
+        delta_at = total_at = delta_stride = total_stride = 0
+    else:
+        delta_at, delta_stride = _strided(delta, "delta", dtype, shape, device), delta.stride(0)
+        total_at, total_stride = (at, x.stride(0)) if total is None else (_strided(total, "total", dtype, shape, device), total.stride(0))
+    if weight.numel() != out.width or weight.device != device:
+        raise KernelError("rms_norm_int8: the weight does not fit")
+    _call_packed("rms_norm_int8", "int8_rows.cu", "q3_rms_norm_int8_" + s, _ROWS8_ARGS.pack(
+        at, delta_at, _at(weight, "weight", _F32), total_at, out.at, out.scales_at, _on_current(device, "rms_norm_int8"), out.rows, x.stride(0),
+        delta_stride, total_stride, out.stride, float(eps), out.width, 0))
+    return out
+
+
+def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[str] = None) -> torch.Tensor:
+    """out[m, n] = (sum_k x.codes[m, k] w.codes[n, k]) x.scales[m] w.scales[n]: the sum in whole numbers, scaled in 32 bits and rounded once to
+    out's type, bfloat16 or float32.  With an `activation` ("silu", "gelu_tanh") w holds the gate and up rows interleaved in blocks of eight
+    (`interleave_gate_up`) and out [rows, channels / 2] = act(gate) * up, in 32 bits until it is rounded.  A row's result does not hang on the others."""
+    M, K, N = x.rows, x.width, w.rows
+    if w.width != K or out.shape != (M, N if activation is None else N // 2) or not 0 < K <= INT8_MAX_WIDTH or (activation is not None and N % 16):
+        raise KernelError(f"gemm_int8: shapes {x.shape} x {w.shape}^T -> {tuple(out.shape)}")
+    if activation is not None and activation not in ACTIVATIONS:
+        raise KernelError(f"gemm_int8: activation {activation!r}: one of {sorted(ACTIVATIONS)}")
+    if w.device != x.device or out.device != x.device:
+        raise KernelError("gemm_int8: the operands lie on different devices")
+    _suffix(out)
+    _call_packed("gemm_int8", "gemm_int8.cu", "q3_gemm_int8_few", _GEMM8_ARGS.pack(
+        x.at, x.scales_at, w.at, w.scales_at, _at(out, "out", out.dtype), _status_word(x.device).data_ptr(), _on_current(x.device, "gemm_int8"),
+        x.stride, w.stride, M, N, K, 1 if out.dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, 0))
+    return out
+
+
 # ------------------------------------------------------------------ bfloat16 prompt attention
 def attention_prefill(q, k_pages, v_pages, out, seq_start, seq_pos0, page_table, n_seqs: int, max_new: int, nq: int,
                       nkv: int, d: int, scale: float, window: Optional[int] = None):

@@ -24,6 +24,7 @@
 #include <stdint.h>
 
 #include "cache_args.h"
+#include "int8_args.h"
 
 #define Q3_ERR_BAD_SIZE 10001        /* a size the kernel does not take */
 #define Q3_ERR_TOO_LARGE 10002       /* more rows, heads or blocks than one launch takes */
@@ -516,6 +517,16 @@ int q3_attention_tree_mma_bf16(const q3_attention_tree_args* args);
 int q3_attention_tree_tc_head_dim(void);
 int64_t q3_attention_tree_tc_parts(void);
 int q3_attention_tree_tc_bf16(const q3_attention_tree_args* args);
+
+/* ---- int8_rows.cu: rows as 8-bit integers with a scale each, as they are or normed on the way (arguments: int8_args.h, read before the call
+   returns) ---- */
+int q3_quantize_rows_f32(const q3_int8_rows_args* args);
+int q3_quantize_rows_bf16(const q3_int8_rows_args* args);
+int q3_rms_norm_int8_f32(const q3_int8_rows_args* args);
+int q3_rms_norm_int8_bf16(const q3_int8_rows_args* args);
+
+/* ---- gemm_int8.cu: products of such rows, scaled by token and channel; all forms give the same bits ---- */
+int q3_gemm_int8_few(const q3_gemm_int8_args* args);
 
 /* ---- sampling.cu ------------------------------------------------------------------------------------------ */
 /* out[r] = index of the highest logit among the first `valid` (lowest id among equals, NaN as -inf) */

@@ -1,0 +1,146 @@
+"""Products of 8-bit integers with scales against the definition in 64 bits."""
+import pytest
+import torch
+
+import int8_cases as ic
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+U = 2.0 ** -24
+HALF = {"f32": U, "bf16": 2.0 ** -8}                       # half a step of the output
+
+
+def operands(M, N, K, seed):
+    """Codes of the whole range, with other memory full of other codes behind every row."""
+    from qwen3_b200.csrc import ops
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = []
+    for rows in (M, N):
+        memory = torch.randint(-128, 128, (rows, -(-K // 16) * 16 + 16), generator=g, device="cuda", dtype=torch.int64).to(torch.int8)
+        scales = torch.exp(0.3 * torch.randn(rows, generator=g, device="cuda")) / (74.0 * K ** 0.25)
+        out.append(ops.Int8Rows(memory[:, :K], scales))
+    return out
+
+
+def check(x, w, y, kind, activation):
+    """A sum of whole numbers has no error; it becomes 32 bits (half a unit) and is scaled twice (half a unit each); then the last rounding.  With a gate:
+    both errors, some units of the activation and a product, all beside |gate| |up|."""
+    want = ic.product(x.codes, x.scales, w.codes, w.scales, activation)
+    got = y.double()
+    if activation is None:
+        assert bool(((got - want).abs() <= want.abs() * (3.01 * U + HALF[kind] * (1 + 4 * U)) + 2.0 ** -140).all())
+    else:
+        want, gate, up = want
+        bound = 16 * U * gate.abs() * up.abs()
+        assert bool(((got - want).abs() <= bound + (want.abs() + bound) * HALF[kind] + 2.0 ** -120).all())
+
+
+SHAPES = [(1, 16, 64), (1, 64, 1), (2, 33, 15), (3, 100, 17), (7, 48, 100), (8, 4096, 4096), (8, 1000, 2050), (9, 160, 129), (16, 512, 1000), (17, 96, 640),
+          (31, 2000, 333), (33, 48, 4100), (64, 6144, 512), (65, 80, 63), (100, 272, 127), (128, 1024, 2048), (129, 1040, 500), (200, 4096, 1024),
+          (257, 272, 640), (300, 6144, 4096), (527, 1001, 777), (700, 512, 12288), (1024, 2048, 2048), (1500, 4096, 1008), (2100, 80, 96), (3001, 1072, 1500)]
+
+
+@pytest.mark.parametrize("kind,activation", [("bf16", None), ("f32", None), ("bf16", "silu"), ("f32", "silu"), ("bf16", "gelu_tanh")])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_product(M, N, K, kind, activation):
+    from qwen3_b200.csrc import ops
+    if activation:
+        N = -(-N // 16) * 16
+    x, w = operands(M, N, K, M + N + K)
+    columns = N // 2 if activation else N
+    memory = torch.full((M + 2, columns), 77.0, dtype=TYPES[kind], device="cuda")
+    y = memory[1:1 + M] if columns * memory.element_size() % 16 == 0 else memory[:M]
+    ops.gemm_int8(x, w, y, activation=activation)
+    assert ops.tcgen05_status("cuda") == 0
+    check(x, w, y, kind, activation)
+    rest = memory[M + 1:] if y.data_ptr() != memory.data_ptr() else memory[M:]
+    assert bool((rest == 77).all()) and (y.data_ptr() == memory.data_ptr() or bool((memory[0] == 77).all()))
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 150, 300, 1200])
+def test_a_token_does_not_hang_on_the_batch(M):
+    """Every form gives the same bits."""
+    from qwen3_b200.csrc import ops
+    x, w = operands(M, 528, 1111, 5)
+    for activation, columns in ((None, 528), ("silu", 264)):
+        y = ops.gemm_int8(x, w, torch.zeros(M, columns, device="cuda"), activation=activation)
+        for row in (0, M // 2, M - 1):
+            one = ops.Int8Rows(x.codes[row:row + 1], x.scales[row:row + 1])
+            assert torch.equal(ops.gemm_int8(one, w, torch.zeros(1, columns, device="cuda"), activation=activation)[0], y[row])
+
+
+@pytest.mark.parametrize("M", [1, 20, 140, 600])
+def test_largest_sums(M):
+    """-128 times -128 over the widest rows: 2^31 - 2^14; and the sum of opposite signs."""
+    from qwen3_b200.csrc import ops
+    K = ops.INT8_MAX_WIDTH
+    x, w = ops.Int8Rows.empty(M, K, "cuda"), ops.Int8Rows.empty(32, K, "cuda")
+    x.codes.fill_(-128), w.codes.fill_(-128)
+    w.codes[16:].fill_(127)
+    x.scales.fill_(0.5), w.scales.fill_(2.0)
+    y = ops.gemm_int8(x, w, torch.zeros(M, 32, device="cuda"))
+    assert bool((y[:, :16].double() == float(torch.tensor(float(K * 16384), dtype=torch.float32))).all())
+    assert bool((y[:, 16:].double() == float(torch.tensor(float(-K * 128 * 127), dtype=torch.float32))).all())
+
+
+@pytest.mark.parametrize("M", [1, 3, 50, 200, 600])
+def test_scales_that_are_no_numbers_and_zeros(M):
+    from qwen3_b200.csrc import ops
+    x, w = operands(M, 96, 200, 7)
+    x.scales[M - 1], w.scales[5], w.scales[6] = float("nan"), float("nan"), 0.0
+    y = ops.gemm_int8(x, w, torch.zeros(M, 96, dtype=torch.bfloat16, device="cuda"))
+    assert bool(y[M - 1].isnan().all()) and bool(y[:, 5].isnan().all()) and bool((y[:M - 1, 6] == 0).all())
+    assert not bool(y[:M - 1, :5].isnan().any())
+
+
+def test_no_rows():
+    from qwen3_b200.csrc import ops
+    x, w = operands(4, 32, 64, 1)
+    y = torch.full((4, 32), 77.0, device="cuda")
+    ops.gemm_int8(ops.Int8Rows(x.codes[:0], x.scales[:0]), w, y[:0])
+    ops.gemm_int8(x, ops.Int8Rows(w.codes[:0], w.scales[:0]), torch.zeros(4, 0, device="cuda"))
+    assert bool((y == 77).all())
+
+
+def test_on_another_stream_and_in_a_graph():
+    from qwen3_b200.csrc import ops
+    for M in (2, 100, 300, 900):
+        x, w = operands(M, 272, 500, M)
+        want = ops.gemm_int8(x, w, torch.zeros(M, 272, device="cuda"))
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            y = ops.gemm_int8(x, w, torch.zeros(M, 272, device="cuda"))
+        side.synchronize()
+        assert torch.equal(y, want)
+        graphs, outs = [], []
+        for _ in range(2):
+            graph, y = torch.cuda.CUDAGraph(), torch.zeros(M, 272, device="cuda")
+            with torch.cuda.graph(graph):
+                ops.gemm_int8(x, w, y)
+            graphs.append(graph), outs.append(y)
+        for _ in range(3):
+            for graph in graphs:
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for y in outs) and ops.tcgen05_status("cuda") == 0
+
+
+def test_refusals():
+    from qwen3_b200.csrc import ops
+    x, w = operands(4, 40, 64, 1)
+    good = torch.zeros(4, 40, device="cuda")
+    for out in (good[:3], good[:, :39], good.half(), good.cpu(), good.t().contiguous().t(), torch.zeros(4, 80, device="cuda")[:, ::2]):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int8(x, w, out)
+    with pytest.raises(ops.KernelError):                   # gates and ups in turns of eight
+        ops.gemm_int8(x, w, torch.zeros(4, 20, device="cuda"), activation="silu")
+    wide = operands(4, 48, 64, 1)[1]
+    for activation, out in (("relu", torch.zeros(4, 24, device="cuda")), ("silu", torch.zeros(4, 48, device="cuda"))):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int8(x, wide, out, activation=activation)
+    with pytest.raises(ops.KernelError):
+        ops.gemm_int8(x, operands(4, 40, 65, 1)[1], good)
+    a, b = ops.Int8Rows.empty(1, ops.INT8_MAX_WIDTH + 1, "cuda"), ops.Int8Rows.empty(4, ops.INT8_MAX_WIDTH + 1, "cuda")
+    with pytest.raises(ops.KernelError):
+        ops.gemm_int8(a, b, torch.zeros(1, 4, device="cuda"))
