@@ -3,7 +3,17 @@
 // The sum is taken in whole numbers, which 32 bits hold for K up to 131,071 (2^31 / 2^14), so it does not hang on the order: every form below gives
 // the same bits for a token, whatever the batch around it.  It becomes a 32-bit float, is scaled by the token's and then by the channel's scale and
 // rounded to the output type.  With a gate, gate and up stay in 32 bits until their product is rounded.
+//
+// Three forms: few tokens on mma.sync, W streamed through registers; up to some hundred on tcgen05 with W as the 128-row operand and K split over a
+// cluster; prompts on pairs of SMs.  A row of codes is 128 bytes of K a step, one swizzle row, and an instruction takes 32 of them.  Every wait on an
+// mbarrier is bounded: after Q3_WAIT_LIMIT polls the thread records where it gave up in `status` and the block winds down (tensor memory is
+// freed on every path, and the cluster barriers are reached by every thread on every path).
+#include <cuda.h>
+
 #include "common.cuh"
+#include "tcgen05.cuh"
+#include "tcgen05_pair.cuh"
+#include "tma.cuh"
 #include "../include/qwen3/int8_args.h"
 
 namespace {
@@ -150,6 +160,517 @@ template <int GATED, typename OutT> int few(const Product& p, cudaStream_t strea
     return launch_few<1, 8, 4, 3, GATED, OutT>(p, stream);
 }
 
+// ---------------------------------------------------------------------------------------------
+// Up to some hundred tokens, weights first: D[128 rows of W, MT tokens] = W tile . X tile^T on tcgen05, so that the 128-row operand is full whatever
+// the number of tokens.  Where W has few rows, K is split over the blocks of a cluster; their partial tiles meet in shared memory, and each block
+// adds up, scales and writes a share of the tokens.  Grid (tiles of 128 rows of W, K ranges, tiles of MT tokens), clusters (1, K ranges, 1).
+//   warp 0     TMA producer
+//   warp 1     allocates tensor memory; one elected thread issues the products and hands each stage back to the producer
+//   warps 2-5  bring the accumulator (a row of W a thread) into shared memory
+constexpr int BM = 128, BK = 128, UMMA_K = 32;
+constexpr int THREADS = 192;
+constexpr int PART_LD = BM + 4;         // words per token of the partial tile (rows stay 16-byte aligned)
+
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+template <typename OutT> __device__ __forceinline__ void store4(OutT* p, const float (&v)[4], bool whole, int valid) {
+    if (whole && valid >= 4) {
+        if constexpr (sizeof(OutT) == 4) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+            *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i < valid) p[i] = to_out<OutT>(v[i]);
+}
+
+template <int MT, int STAGES, int MINB, int GATED, typename OutT>
+__global__ void __launch_bounds__(THREADS, MINB)
+mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Product p, int* __restrict__ status) {
+    extern __shared__ unsigned char smem_raw[];
+    constexpr int A_BYTES = BM * BK, B_BYTES = MT * BK, STAGE_BYTES = A_BYTES + B_BYTES;   // multiples of 1024
+    constexpr uint32_t TMEM_COLS = MT < 32 ? 32 : MT;
+    static_assert(MT == 16 || (MT % 32 == 0 && MT <= 256), "token tile: the N of an M = 128 product of 8-bit integers");
+    // the partial tile reuses the stages (and what lies behind them, if it is the larger of the two)
+    constexpr int RING_BYTES = STAGES * STAGE_BYTES > MT * PART_LD * 4 ? STAGES * STAGE_BYTES : (MT * PART_LD * 4 + 1023) / 1024 * 1024;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;         // 128-byte swizzle wants 1024-byte tiles
+    const uint32_t bars = base + RING_BYTES;                              // full[STAGES], empty[STAGES], done, tmem slot
+    const uint32_t bar_done = bars + 2 * STAGES * 8, tmem_slot = bar_done + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n0 = blockIdx.x * BM, m0 = blockIdx.z * MT;
+    const uint32_t rank = cluster_rank(), ranks = gridDim.y;
+    const int nkb_all = (p.K + BK - 1) / BK;
+    const int kb_begin = (int)(((int64_t)rank * nkb_all) / ranks), kb_end = (int)(((int64_t)(rank + 1) * nkb_all) / ranks);
+    const int nkb = kb_end - kb_begin;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bars + s * 8, 1);
+            mbar_init(bars + (STAGES + s) * 8, 1);
+        }
+        mbar_init(bar_done, 1);
+        mbar_init_fence();
+    }
+    __syncthreads();
+    // the producer starts its stream now; tensor memory is handed out meanwhile and its address goes to the warps that use it
+    uint32_t tmem_base = 0;
+    if (warp >= 1) {
+        if (warp == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(THREADS - 32) : "memory");
+        tc_fence_after();
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+    }
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int i = 0; i < nkb; ++i) {
+                const int s = i % STAGES;
+                if (!mbar_wait(bars + (STAGES + s) * 8, ((uint32_t)(i / STAGES) & 1u) ^ 1u)) {      // the stage is free
+                    atomicExch(status, 1);
+                    break;
+                }
+                const uint32_t a = base + s * STAGE_BYTES, b = a + A_BYTES;
+                mbar_expect_tx(bars + s * 8, STAGE_BYTES);
+                tma_load_2d(a, &map_w, bars + s * 8, (kb_begin + i) * BK, n0);      // weights: independent of the
+                if (i == 0) pdl_wait();                                              // kernel before; X is not
+                tma_load_2d(b, &map_x, bars + s * 8, (kb_begin + i) * BK, m0);
+            }
+        }
+    } else if (warp == 1) {
+        // the whole warp walks the K steps and one elected thread issues, so that descriptors stay in uniform registers
+        constexpr uint32_t idesc = make_idesc_i8(BM, MT);
+        const uint64_t desc0 = desc_k_major(base);
+        const uint32_t acc = __shfl_sync(0xffffffffu, tmem_base, 0);
+        for (int i = 0; i < nkb; ++i) {
+            const uint32_t s = (uint32_t)i % STAGES;
+            if (!mbar_wait_warp(bars + s * 8, ((uint32_t)i / STAGES) & 1u)) {    // the tiles have landed
+                if (lane == 0) atomicExch(status, 2);
+                break;
+            }
+            tc_fence_after();
+            const uint64_t da = desc0 + (uint64_t)(s * (STAGE_BYTES >> 4)), db = da + (A_BYTES >> 4);
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k)                        // 32 bytes further along K per step
+                    tc_mma_i8(acc, da + (uint64_t)(k * 2), db + (uint64_t)(k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+                tc_commit(bars + (STAGES + s) * 8);                          // frees the stage when the products are done
+            }
+            __syncwarp();
+        }
+        if (elect_one()) tc_commit(bar_done);                                // accumulator complete (or abandoned)
+        __syncwarp();
+    } else {
+        // warps 2..5 own lanes 32 * (warp % 4) .. of tensor memory: accumulator -> part[token][row of W]
+        const bool ok = mbar_wait(bar_done, 0);                              // every load has landed and been consumed,
+        if (!ok && lane == 0) atomicExch(status, 3);                         // so the stages may be overwritten
+        tc_fence_after();
+        uint32_t* part = reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)));
+        const int lane_base = (warp & 3) * 32;
+#pragma unroll 1
+        for (int c = 0; c < MT; c += 16) {
+            uint32_t r[16];
+            if (ok && nkb > 0) {
+                tc_ld16(tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)c, r);
+                tc_wait_ld();
+            } else {                                                          // an empty K range adds nothing
+#pragma unroll
+                for (int j = 0; j < 16; ++j) r[j] = 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) part[(c + j) * PART_LD + lane_base + lane] = r[j];
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (ranks > 1) cluster_sync();                                            // every block's partial tile is in place
+    else __syncthreads();                                                     // (a block on its own: its own tile)
+
+    pdl_wait();                                                               // no global write before this
+    {
+        // this block finishes the tokens m with m % ranks == rank
+        OutT* Y = (OutT*)p.y;
+        const int out_n = GATED ? (p.N >> 1) : p.N;
+        const bool whole = (out_n % 4 == 0) && ((reinterpret_cast<uintptr_t>(Y) & 15u) == 0);
+        constexpr int GROUPS = GATED ? 16 : 32;                               // groups of four outputs per token and tile
+        const int my_tokens = (MT - (int)rank + (int)ranks - 1) / (int)ranks;
+        auto sum4 = [&](uint32_t addr) {
+            int4 sum = make_int4(0, 0, 0, 0);
+            for (uint32_t s = 0; s < ranks; ++s) {
+                const int4 v = ld_cluster_i4(map_to_rank(addr, s));
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+            }
+            return sum;
+        };
+        for (int idx = threadIdx.x; idx < my_tokens * GROUPS; idx += THREADS) {
+            const int local = (idx / GROUPS) * (int)ranks + (int)rank, g = idx % GROUPS;
+            const int m = m0 + local;
+            if (m >= p.M) continue;
+            const float sx = p.sx[m];
+            if constexpr (GATED == 0) {
+                const int n = n0 + 4 * g;
+                if (n >= p.N) continue;
+                const int4 sum = sum4(base + (uint32_t)(local * PART_LD + 4 * g) * 4u);
+                float v[4] = {scaled(sum.x, sx, p.sw[n]), 0.0f, 0.0f, 0.0f};
+                if (n + 1 < p.N) v[1] = scaled(sum.y, sx, p.sw[n + 1]);
+                if (n + 2 < p.N) v[2] = scaled(sum.z, sx, p.sw[n + 2]);
+                if (n + 3 < p.N) v[3] = scaled(sum.w, sx, p.sw[n + 3]);
+                store4<OutT>(Y + (int64_t)m * p.N + n, v, whole, p.N - n);
+            } else {
+                // rows 16t + 4h .. + 3 are gates, rows 16t + 8 + 4h .. + 3 the ups of features 8t + 4h .. + 3
+                const int t = g >> 1, h = g & 1, n = n0 + 16 * t + 4 * h;
+                if (n >= p.N) continue;
+                const uint32_t addr = base + (uint32_t)(local * PART_LD + 16 * t + 4 * h) * 4u;
+                const int4 gs = sum4(addr), us = sum4(addr + 32u);
+                const float* sw = p.sw + n;
+                const float v[4] = {gate_activation<GATED>(scaled(gs.x, sx, sw[0])) * scaled(us.x, sx, sw[8]),
+                                    gate_activation<GATED>(scaled(gs.y, sx, sw[1])) * scaled(us.y, sx, sw[9]),
+                                    gate_activation<GATED>(scaled(gs.z, sx, sw[2])) * scaled(us.z, sx, sw[10]),
+                                    gate_activation<GATED>(scaled(gs.w, sx, sw[3])) * scaled(us.w, sx, sw[11])};
+                store4<OutT>(Y + (int64_t)m * out_n + (n0 >> 1) + 8 * t + 4 * h, v, whole, 4);
+            }
+        }
+    }
+    __syncwarp();
+    if (ranks > 1) cluster_sync();                                            // nobody leaves while its tile is being read
+    else __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Prompts: persistent pairs of SMs (cta_group::2), W as the 256-row operand, `tile` tokens (a multiple of 32 up to 256) as the other one.  Each block of a
+// pair loads its own 128 rows of W and half of the tokens, the instruction reads both blocks' shared memory, and each block's tensor
+// memory receives the accumulator of its own rows of W, twice (a tile's drain runs under the next one's products).
+//   full[s]       in the leader (rank 0): both blocks' copies report their bytes there
+//   empty[s]      in each block: the leader's commit arrives at both
+//   acc_full[b]   in each block: likewise, when a tile's accumulator is complete
+//   acc_empty[b]  in the leader: the sixteen drain warps of both blocks arrive there
+constexpr int PAIR_THREADS = 320;       // producer, issuer, eight drain warps
+constexpr int PAIR_STAGES = 6;
+
+// The order of the tiles: bands of at most 16 tiles of tokens, all tiles of W inside a band, the tokens fastest, so that a band's tokens stay in the L2
+// while W passes.
+constexpr int BAND_TILES = 16;
+__device__ __forceinline__ void tile_place(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int bands = (tiles_m + BAND_TILES - 1) / BAND_TILES, high = (tiles_m + bands - 1) / bands;
+    const int band = tile / (high * tiles_n), inside = tile - band * high * tiles_n;
+    const int own = min(high, tiles_m - band * high);        // the last band may be lower
+    tn = inside / own;
+    tm = band * high + inside - tn * own;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+// Writes 32 tokens (from `m` on, `tokens` of them live) of the 32 rows of W that a warp's lanes own.  `v`: the lane's row, scaled by token and
+// channel.  bfloat16: lanes next to each other exchange, so that one takes both rows for the even token and the other for the odd one: 64
+// consecutive bytes a token and instruction (`words`: where a row of Y is whole 4-byte words).  GATED: the rows are gate[8] up[8] gate[8] up[8] of 16
+// features; a gate's lane and its up's, eight further, exchange first and take every other token each.
+template <int GATED, typename OutT>
+__device__ __forceinline__ void store_tokens(const float (&v)[32], OutT* Y, int m, int tokens, int row0, int lane, int N, bool words) {
+    if constexpr (GATED == 0) {
+        const int row = row0 + lane;
+        if (sizeof(OutT) == 4 || !words) {
+            if (row >= N) return;
+            OutT* to = Y + (int64_t)m * N + row;
+#pragma unroll
+            for (int t = 0; t < 32; ++t)
+                if (t < tokens) to[(int64_t)t * N] = to_out<OutT>(v[t]);
+        } else {
+            const int odd = lane & 1;
+            OutT* to = Y + (int64_t)(m + odd) * N + (row & ~1);
+#pragma unroll
+            for (int t = 0; t < 32; t += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, odd ? v[t] : v[t + 1], 1);
+                const uint32_t both = odd ? pack_bf16(got, v[t + 1]) : pack_bf16(v[t], got);
+                if (row < N && t + odd < tokens) *reinterpret_cast<uint32_t*>(to + (int64_t)t * N) = both;
+            }
+        }
+    } else {
+        const int out_n = N >> 1, feature = (row0 >> 1) + ((lane >> 4) << 3) + (lane & 7), up = (lane >> 3) & 1;
+        const bool live = row0 + (lane & 16) + 16 <= N;
+        float y[16];                                         // tokens 2 t + up
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[2 * t] : v[2 * t + 1], 8);
+            const float g = up ? got : v[2 * t], u = up ? v[2 * t + 1] : got;
+            y[t] = gate_activation<GATED>(g) * u;
+        }
+        if (sizeof(OutT) == 4 || !words) {
+            OutT* to = Y + (int64_t)(m + up) * out_n + feature;
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                if (live && 2 * t + up < tokens) to[(int64_t)(2 * t) * out_n] = to_out<OutT>(y[t]);
+        } else {
+            const int odd = lane & 1;
+            OutT* to = Y + (int64_t)(m + up + 2 * odd) * out_n + (feature & ~1);
+#pragma unroll
+            for (int t = 0; t < 16; t += 2) {
+                const float got = __shfl_xor_sync(0xffffffffu, odd ? y[t] : y[t + 1], 1);
+                const uint32_t both = odd ? pack_bf16(got, y[t + 1]) : pack_bf16(y[t], got);
+                if (live && 2 * (t + odd) + up < tokens) *reinterpret_cast<uint32_t*>(to + (int64_t)(2 * t) * out_n) = both;
+            }
+        }
+    }
+}
+
+template <int GATED, typename OutT>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Product p, int tile, int* __restrict__ status) {
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(16) float token_scales[8][128];      // of a drain warp's share of the tile
+    constexpr int STAGES = PAIR_STAGES, BN = 2 * BM;
+    constexpr int X_BYTES = BM * BK, W_BYTES = BM * BK, STAGE_BYTES = X_BYTES + W_BYTES;
+    constexpr uint32_t TMEM_COLS = 512;                       // two accumulators of 256 columns
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base + STAGES * STAGE_BYTES;       // full[S], empty[S], acc_full[2], acc_empty[2], slot
+    const uint32_t bar_acc_full = bars + 2 * STAGES * 8, bar_acc_empty = bar_acc_full + 16, tmem_slot = bar_acc_empty + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int tiles_m = (p.M + tile - 1) / tile, tiles_n = (p.N + BN - 1) / BN, tiles = tiles_m * tiles_n;
+    const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    const int nkb = (p.K + BK - 1) / BK;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bars + s * 8, 1);
+            mbar_init(bars + (STAGES + s) * 8, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_acc_full + b * 8, 1);
+            mbar_init(bar_acc_empty + b * 8, 16);            // one arrival per drain warp of the pair
+        }
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                           // the peer's barriers exist before anything signals them
+    tc_fence_after();
+    uint32_t tmem_base;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+
+    if (warp == 0) {
+        pdl_wait();                                           // X is the output of the kernel before
+        uint32_t it = 0;
+        bool ok = true;
+        for (int i = first; i < tiles && ok; i += stride) {
+            int tm, tn;
+            tile_place(i, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * tile + (int)rank * (tile / 2), n0 = tn * BN + (int)rank * BM;
+            for (int kb = 0; kb < nkb; ++kb, ++it) {
+                const uint32_t s = it % STAGES;
+                ok = mbar_wait_warp(bars + (STAGES + s) * 8, ((it / STAGES) & 1u) ^ 1u);
+                if (!ok) {
+                    if (lane == 0) atomicExch(status, 1);
+                    break;
+                }
+                const uint32_t x = base + s * STAGE_BYTES, w = x + X_BYTES;
+                const uint32_t full_in_leader = map_to_rank(bars + s * 8, 0);
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(bars + s * 8, 2 * (tile / 2 * BK + W_BYTES));       // both blocks' bytes
+                    tma_load_2d_pair(x, &map_x, full_in_leader, kb * BK, m0);
+                    tma_load_2d_pair(w, &map_w, full_in_leader, kb * BK, n0);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = make_idesc_i8(2 * BM, tile);
+            const uint64_t desc0 = desc_k_major(base);
+            uint32_t it = 0, local = 0;
+            bool ok = true;
+            tmem_base = __shfl_sync(0xffffffffu, tmem_base, 0);
+            for (int i = first; i < tiles && ok; i += stride, ++local) {
+                const uint32_t buf = local & 1u;
+                ok = mbar_wait_warp(bar_acc_empty + buf * 8, ((local >> 1) & 1u) ^ 1u);      // both blocks have drained it
+                if (!ok) {
+                    if (lane == 0) atomicExch(status, 4);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t acc = tmem_base + buf * 256u;
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    ok = mbar_wait_warp(bars + s * 8, (it / STAGES) & 1u);
+                    if (!ok) {
+                        if (lane == 0) atomicExch(status, 2);
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t dx = desc0 + (uint64_t)(s * (STAGE_BYTES >> 4)), dw = dx + (X_BYTES >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; ++k)
+                            tc_mma_pair_i8(acc, dw + (uint64_t)(k * 2), dx + (uint64_t)(k * 2), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        tc_commit_pair(bars + (STAGES + s) * 8);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one()) tc_commit_pair(bar_acc_full + buf * 8);
+                __syncwarp();
+            }
+        }
+    } else {
+        pdl_wait();
+        // 32 rows of W by the tokens of the tile's first or second half
+        const int lane_base = (warp & 3) * 32, set = (warp - 2) >> 2, half = tile / 2, c0 = set * half;
+        OutT* Y = (OutT*)p.y;
+        const bool words = (reinterpret_cast<uintptr_t>(Y) & 3u) == 0 && p.N % 2 == 0;      // (with a gate N / 2 is even, too)
+        float* sx = token_scales[warp - 2];
+        uint32_t local = 0;
+        for (int i = first; i < tiles; i += stride, ++local) {
+            const uint32_t buf = local & 1u;
+            int tm, tn;
+            tile_place(i, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * tile + c0, row0 = tn * BN + (int)rank * BM + lane_base;
+            const int tokens = min(half, p.M - m0);          // none or less where the tile's second half lies behind the last token
+            __syncwarp();
+            for (int t = lane; t < half; t += 32) sx[t] = t < tokens ? p.sx[m0 + t] : 0.0f;
+            const float sw = row0 + lane < p.N ? p.sw[row0 + lane] : 0.0f;
+            __syncwarp();
+            if (!mbar_wait(bar_acc_full + buf * 8, (local >> 1) & 1u)) {
+                if (lane == 0) atomicExch(status, 3);
+                break;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t acc = tmem_base + ((uint32_t)lane_base << 16) + buf * 256u + (uint32_t)c0;
+#pragma unroll 1
+            for (int c = 0; c < tokens; c += 32) {
+                uint32_t r[32];
+                tc_ld32(acc + (uint32_t)c, r);
+                tc_wait_ld();
+                float v[32];
+#pragma unroll
+                for (int t = 0; t < 32; t += 4) {
+                    const float4 x4 = *reinterpret_cast<const float4*>(sx + c + t);
+                    v[t] = scaled((int)r[t], x4.x, sw);
+                    v[t + 1] = scaled((int)r[t + 1], x4.y, sw);
+                    v[t + 2] = scaled((int)r[t + 2], x4.z, sw);
+                    v[t + 3] = scaled((int)r[t + 3], x4.w, sw);
+                }
+                store_tokens<GATED, OutT>(v, Y, m0 + c, tokens - c, row0, lane, p.N, words);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(bar_acc_empty + buf * 8, 0));
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync();                                           // the peer reads this block's memory and barriers until here
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// K ranges (blocks of a cluster) of the weights-first form: the largest power of two up to the portable cluster size that keeps the grid within
+// 2.6 blocks an SM (one an SM for tiles of 256 tokens) and leaves every block 8 K steps.
+int mid_splits(int M, int N, int K) {
+    const int token_tiles = M <= 128 ? 1 : (M + 255) / 256;
+    const int tiles = (N + BM - 1) / BM * token_tiles, nkb = (K + BK - 1) / BK;
+    const int limit = M > 128 ? q3_device_sm_count() : q3_device_sm_count() * 13 / 5;
+    int s = 1;
+    while (s < 8 && tiles * (2 * s) <= limit && nkb / (2 * s) >= 8) s *= 2;
+    return s;
+}
+
+template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid(const Product& p, int splits, int* status, cudaStream_t stream) {
+    constexpr int RING = STAGES * (BM * BK + MT * BK), PART = (MT * PART_LD * 4 + 1023) / 1024 * 1024;
+    constexpr int SMEM = (RING > PART ? RING : PART) + 1024 + 256;
+    static Q3PerDevice configured;
+    const cudaError_t e = q3_allow_shared_memory(mid_kernel<MT, STAGES, MINB, GATED, OutT>, SMEM, configured);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap map_w, map_x;
+    if (!q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM) || !q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, MT)) return Q3_ERR_BAD_SIZE;
+    const int64_t token_tiles = (p.M + MT - 1) / MT;
+    if (token_tiles > 65535) return Q3_ERR_TOO_LARGE;
+    return (int)q3_launch_cluster(mid_kernel<MT, STAGES, MINB, GATED, OutT>, dim3((p.N + BM - 1) / BM, splits, (unsigned)token_tiles), dim3(THREADS),
+                                  (size_t)SMEM, stream, dim3(1, splits, 1), map_w, map_x, p, status);
+}
+
+template <int GATED, typename OutT> int mid(const Product& p, int splits, int* status, cudaStream_t stream) {
+    const int nkb = (p.K + BK - 1) / BK;
+    if (splits == 0) splits = mid_splits(p.M, p.N, p.K);
+    if (splits > nkb) splits = nkb;
+    const bool waves = (int64_t)((p.N + BM - 1) / BM) * splits > 2 * q3_device_sm_count();
+#define Q3_MID(MT, ST, MB) return launch_mid<MT, ST, MB, GATED, OutT>(p, splits, status, stream)
+    if (p.M <= 16) { if (waves) Q3_MID(16, 4, 3); Q3_MID(16, 5, 2); }
+    if (p.M <= 32) { if (waves) Q3_MID(32, 3, 3); Q3_MID(32, 5, 2); }
+    if (p.M <= 64) { if (waves) Q3_MID(64, 3, 3); Q3_MID(64, 4, 2); }
+    if (p.M <= 128) { if (waves) Q3_MID(128, 2, 3); Q3_MID(128, 3, 2); }
+    Q3_MID(256, 4, 1);
+#undef Q3_MID
+}
+
+// Tokens of a tile of the pairs form: equal tiles of a multiple of 32, as many as whole 256s would make or one to three more, by what the tiles should
+// take: microseconds of a K step of 128 of a tile, at least what the copies take where it has few tokens, and of a tile's drain.
+struct PairTile {
+    int tile;
+    float us;
+};
+PairTile pair_tile(int M, int N, int K) {
+    const int pairs = q3_device_sm_count() / 2, whole = (M + 255) / 256;
+    PairTile best{256, 1e30f};
+    for (int cuts = whole; cuts <= whole + 3 && cuts <= (M + 31) / 32; ++cuts) {
+        const int tile = ((M + cuts - 1) / cuts + 31) / 32 * 32;
+        const int64_t tiles = (int64_t)((M + tile - 1) / tile) * ((N + 255) / 256);
+        const float step = fmaxf(0.224f, 0.343f * tile / 256.0f);
+        const float us = 6.0f + (float)((tiles + pairs - 1) / pairs) * (float)((K + BK - 1) / BK) * step;
+        if (us < best.us) best = PairTile{tile, us};
+    }
+    return best;
+}
+
+template <int GATED, typename OutT> int pair(const Product& p, int tile, int* status, cudaStream_t stream) {
+    constexpr int SMEM = PAIR_STAGES * (2 * BM * BK) + 1024 + 256;
+    const auto kernel = pair_kernel<GATED, OutT>;
+    static Q3PerDevice configured;
+    const cudaError_t e = q3_allow_shared_memory(kernel, SMEM, configured);
+    if (e != cudaSuccess) return (int)e;
+    if (tile == 0) tile = pair_tile(p.M, p.N, p.K).tile;
+    if (tile < 32 || tile > 256 || tile % 32 != 0) return Q3_ERR_BAD_SIZE;
+    CUtensorMap map_x, map_w;
+    if (!q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, tile / 2) || !q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM)) return Q3_ERR_BAD_SIZE;
+    const int64_t tiles = (int64_t)((p.M + tile - 1) / tile) * ((p.N + 255) / 256);
+    if (tiles > 0x3fffffff) return Q3_ERR_TOO_LARGE;
+    const int pairs = tiles < q3_device_sm_count() / 2 ? (int)tiles : q3_device_sm_count() / 2;
+    return (int)q3_launch_cluster(kernel, dim3(2 * pairs), dim3(PAIR_THREADS), (size_t)SMEM, stream, dim3(2, 1, 1), map_x, map_w, p, tile, status);
+}
+
 int product_of(const q3_gemm_int8_args& a, Product& p) {
     if (a.width <= 0 || a.width > 131071 || a.activation < 0 || a.activation > 2 || (a.activation != 0 && a.channels % 16 != 0)) return Q3_ERR_BAD_SIZE;
     if (a.x_stride < a.width || a.w_stride < a.width) return Q3_ERR_BAD_SIZE;
@@ -177,4 +698,27 @@ Q3_EXPORT int q3_gemm_int8_few(const q3_gemm_int8_args* a) {
 #define Q3_FEW(G, T) few<G, T>(p, (cudaStream_t)a->stream)
     Q3_BY_EPILOGUE(Q3_FEW);
 #undef Q3_FEW
+}
+
+// Up to some hundred tokens: weights first on tcgen05, `splits` K ranges in a cluster (0: chosen).
+Q3_EXPORT int q3_gemm_int8_mid(const q3_gemm_int8_args* a) {
+    if (a->rows <= 0 || a->channels <= 0) return 0;
+    Product p;
+    const int bad = product_of(*a, p);
+    if (bad) return bad;
+    if (a->splits < 0 || a->splits > 8) return Q3_ERR_BAD_SIZE;
+#define Q3_MIDDLE(G, T) mid<G, T>(p, a->splits, (int*)a->status, (cudaStream_t)a->stream)
+    Q3_BY_EPILOGUE(Q3_MIDDLE);
+#undef Q3_MIDDLE
+}
+
+// Prompts: pairs of SMs, tiles of `splits` tokens (a multiple of 32 up to 256; 0: chosen) by 256 rows of W.
+Q3_EXPORT int q3_gemm_int8_pair(const q3_gemm_int8_args* a) {
+    if (a->rows <= 0 || a->channels <= 0) return 0;
+    Product p;
+    const int bad = product_of(*a, p);
+    if (bad) return bad;
+#define Q3_PAIR(G, T) pair<G, T>(p, a->splits, (int*)a->status, (cudaStream_t)a->stream)
+    Q3_BY_EPILOGUE(Q3_PAIR);
+#undef Q3_PAIR
 }

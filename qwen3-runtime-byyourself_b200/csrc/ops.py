@@ -1697,10 +1697,21 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Ro
     return out
 
 
-def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[str] = None) -> torch.Tensor:
+_INT8_FORMS = {"few": "q3_gemm_int8_few", "mid": "q3_gemm_int8_mid", "pair": "q3_gemm_int8_pair"}
+
+
+def int8_form(M: int, N: int, K: int) -> str:
+    """Which kernel takes a product of M tokens with N channels of width K."""
+    return "few" if M <= 8 else "mid" if M <= 256 else "pair"
+
+
+def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[str] = None, form: Optional[str] = None, splits: int = 0) -> torch.Tensor:
     """out[m, n] = (sum_k x.codes[m, k] w.codes[n, k]) x.scales[m] w.scales[n]: the sum in whole numbers, scaled in 32 bits and rounded once to
     out's type, bfloat16 or float32.  With an `activation` ("silu", "gelu_tanh") w holds the gate and up rows interleaved in blocks of eight
-    (`interleave_gate_up`) and out [rows, channels / 2] = act(gate) * up, in 32 bits until it is rounded.  A row's result does not hang on the others."""
+    (`interleave_gate_up`) and out [rows, channels / 2] = act(gate) * up, in 32 bits until it is rounded.  A row's result does not hang on the others.
+
+    `form`: "few" (W streamed for eight tokens at a time), "mid" (weights first on tcgen05, K in `splits` ranges) or "pair" (pairs of SMs, tiles of `splits`
+    tokens); by default what the sizes ask for.  All give the same bits."""
     M, K, N = x.rows, x.width, w.rows
     if w.width != K or out.shape != (M, N if activation is None else N // 2) or not 0 < K <= INT8_MAX_WIDTH or (activation is not None and N % 16):
         raise KernelError(f"gemm_int8: shapes {x.shape} x {w.shape}^T -> {tuple(out.shape)}")
@@ -1709,9 +1720,12 @@ def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[
     if w.device != x.device or out.device != x.device:
         raise KernelError("gemm_int8: the operands lie on different devices")
     _suffix(out)
-    _call_packed("gemm_int8", "gemm_int8.cu", "q3_gemm_int8_few", _GEMM8_ARGS.pack(
+    name = _INT8_FORMS.get(int8_form(M, N, K) if form is None else form)
+    if name is None:
+        raise KernelError(f"gemm_int8: form {form!r}: one of {sorted(_INT8_FORMS)}")
+    _call_packed("gemm_int8", "gemm_int8.cu", name, _GEMM8_ARGS.pack(
         x.at, x.scales_at, w.at, w.scales_at, _at(out, "out", out.dtype), _status_word(x.device).data_ptr(), _on_current(x.device, "gemm_int8"),
-        x.stride, w.stride, M, N, K, 1 if out.dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, 0))
+        x.stride, w.stride, M, N, K, 1 if out.dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, splits))
     return out
 
 

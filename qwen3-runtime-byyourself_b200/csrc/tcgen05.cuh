@@ -35,6 +35,18 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 
+// The same on 8-bit integers (32 bytes along K) with a 32-bit integer accumulator.
+__device__ __forceinline__ void tc_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// Instruction descriptor of kind::i8: 32-bit integer accumulator [m, n], signed A and B, both K-major, no saturation.
+__host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
 // Shared-memory operand descriptors.  Bits: [0,14) address>>4, [16,30) leading offset>>4, [32,46) stride
 // offset>>4, [46,48) version 1, [61,64) layout 2 (128-byte swizzle).
 // K-major operand: rows of 128 bytes, groups of eight rows 1024 bytes apart (the leading offset is unused, 1).

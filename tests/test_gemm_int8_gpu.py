@@ -57,6 +57,36 @@ def test_product(M, N, K, kind, activation):
     assert bool((rest == 77).all()) and (y.data_ptr() == memory.data_ptr() or bool((memory[0] == 77).all()))
 
 
+@pytest.mark.parametrize("form,splits", [("few", 0), ("mid", 0), ("mid", 1), ("mid", 2), ("mid", 3), ("mid", 5), ("mid", 8), ("pair", 0)]
+                         + [("pair", tile) for tile in (32, 64, 96, 128, 160, 192, 224, 256)])
+@pytest.mark.parametrize("M,N,K", [(1, 272, 200), (31, 96, 1500), (130, 560, 1024), (417, 1056, 900)])
+def test_forms(M, N, K, form, splits):
+    """Whatever form takes a product: the same bits, written to rows that lie at whole words and beside them, and no others."""
+    from qwen3_b200.csrc import ops
+    x, w = operands(M, N, K, M)
+    for kind, activation, columns in (("bf16", None, N), ("f32", None, N), ("bf16", "silu", N // 2), ("f32", "gelu_tanh", N // 2)):
+        outs = []
+        for first, use in ((0, form), (1, form), (0, "few")):
+            memory = torch.full((M * columns + 9,), 77.0, dtype=TYPES[kind], device="cuda")
+            y = memory[first:first + M * columns].view(M, columns)
+            ops.gemm_int8(x, w, y, activation=activation, form=use, splits=splits if use == form else 0)
+            assert bool((memory[:first] == 77).all()) and bool((memory[first + M * columns:] == 77).all())
+            outs.append(y)
+        assert ops.tcgen05_status("cuda") == 0
+        check(x, w, outs[0], kind, activation)
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("form", ["few", "mid", "pair"])
+@pytest.mark.parametrize("M,N,K", [(40, 33, 100), (300, 1001, 300), (5, 7, 16)])
+def test_forms_of_odd_channels(M, N, K, form):
+    from qwen3_b200.csrc import ops
+    x, w = operands(M, N, K, M)
+    for kind in TYPES:
+        y = ops.gemm_int8(x, w, torch.zeros(M, N, dtype=TYPES[kind], device="cuda"), form=form)
+        check(x, w, y, kind, None)
+
+
 @pytest.mark.parametrize("M", [1, 5, 40, 150, 300, 1200])
 def test_a_token_does_not_hang_on_the_batch(M):
     """Every form gives the same bits."""
@@ -139,6 +169,9 @@ def test_refusals():
     for activation, out in (("relu", torch.zeros(4, 24, device="cuda")), ("silu", torch.zeros(4, 48, device="cuda"))):
         with pytest.raises(ops.KernelError):
             ops.gemm_int8(x, wide, out, activation=activation)
+    for form, splits in (("many", 0), ("mid", 9), ("mid", -1), ("pair", 16), ("pair", 48), ("pair", 288)):
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int8(x, w, good, form=form, splits=splits)
     with pytest.raises(ops.KernelError):
         ops.gemm_int8(x, operands(4, 40, 65, 1)[1], good)
     a, b = ops.Int8Rows.empty(1, ops.INT8_MAX_WIDTH + 1, "cuda"), ops.Int8Rows.empty(4, ops.INT8_MAX_WIDTH + 1, "cuda")
