@@ -1,9 +1,9 @@
 // Rows as 8-bit integers with a scale each: quantised as they are, or normed (after a residual sum) on the way.
 //
 // With a = max |x_k| of a row: code_k = 127 x_k / a to the nearest whole number, ties to even, and scale = a / 127.  The codes are those of the
-// exact ratio: a product with 127 / a decides unless it comes within 2^-15 of the middle between two codes, where the ratio is divided out in
-// 64 bits (127 x is exact there, and a quotient that is no tie is further from one than its rounding).  So every form, packet or thread layout gives the
-// same codes.
+// exact ratio: x_k is multiplied by the two 32-bit numbers next to 127 / a, below and above it, and where these round to different codes the middle
+// between the two is compared with the ratio exactly (127 x_k against (code + 1/2) a, in 64 bits).  So every form, packet or thread layout gives the
+// same codes, and a value that is not next to a tie costs two fused multiply-adds.
 //
 // The norm: t = x + delta (rounded to its type, and stored), y = t / sqrt(mean t^2 + eps) * w.  The root is common to a row, so it cancels
 // from the codes: they are those of u = t * w (32 bits), and the scale is max |u| / sqrt(mean t^2 + eps) / 127.  The sum and the maximum
@@ -12,13 +12,15 @@
 // A row with a NaN or an infinity (or whose squares' sum is none that 32 bits hold) gets the scale NaN and codes of zero: what is multiplied by it
 // becomes NaN.  A row of zeros gets the scale zero.  Scales below 2^-126 have fewer bits.
 //
-// Bound by memory: a row is read once, held in registers across the reduction, and written.
+// Bound by memory: a row is read once, in packets of 16 bytes, held in registers across the reduction, and written (8,000 rows, of the measured copy
+// rate: quantise 12,288 bfloat16 52.6 us, 0.86; 5,120 float32 36.2, 0.86; norm and sum 5,120 bfloat16 53.3, 0.82; 4,096 float32 65, 1.0).  Rows that do
+// not begin at such a boundary (an odd width, a slice) are read in the packets around them, each thread shifting two into its own values: 5,001
+// bfloat16 25.9 and 84.9 us where 5,120 takes 22.8 and 53.3.  Tried and slower: rows brought several ahead by bulk copies into a ring in shared
+// memory of blocks that stay (norm 5,120 126 us: barriers and a second pass over shared memory a row), 40 registers a thread for a third block (61.7).
 #include "common.cuh"
 #include "../include/qwen3/int8_args.h"
 
 namespace {
-
-constexpr int MOST = 32;               // values of a row that a thread holds
 
 struct Rows {
     const void *x, *delta;
@@ -33,101 +35,159 @@ struct Rows {
 
 // What a row's codes are made with.
 struct Grid {
-    float top, ratio;                  // max |u| (0: codes of zero) and 127 / max |u|
-    bool exact;                        // a maximum so small that the ratio may not be finite: all codes divided out
+    float top, ratio, below, above;    // max |u| (0: codes of zero), 127 / max |u| and the 32-bit numbers next to it
+    bool divide;                       // a maximum so small that the ratio may not be finite: all codes divided out
 };
 
-__device__ __forceinline__ int code_exact(float u, float top) { return __double2int_rn(__ddiv_rn(127.0 * (double)u, (double)top)); }
+__device__ __forceinline__ int code_exact(float u, const Grid& g) {
+    if (g.divide) return __double2int_rn(__ddiv_rn(127.0 * (double)u, (double)g.top));     // (a quotient that is no tie is further from one than its rounding)
+    const float low = floorf(u * g.below);
+    const double over = 127.0 * (double)u - ((double)low + 0.5) * (double)g.top;           // exact: 31 and 32 bits
+    const int k = (int)low;
+    return over > 0.0 ? k + 1 : over < 0.0 ? k : k + (k & 1);
+}
 
 // Codes of N values, a byte each; four to a word.
-template <int N> __device__ __forceinline__ void codes_of(const float (&u)[N], const Grid& g, uint32_t (&out)[(N + 3) / 4]) {
+template <int N> __device__ __forceinline__ void codes_of(const float (&u)[N], const Grid& g, uint32_t (&out)[N / 4]) {
     constexpr float MAGIC = 12582912.0f;                       // 1.5 * 2^23: adding it rounds to a whole number in the low bits
-    float f[N], worst = 0.0f;
+    uint32_t f[N], apart = 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float q = u[i] * g.ratio;
-        f[i] = q + MAGIC;
-        worst = fmaxf(worst, fabsf(q - (f[i] - MAGIC)));
+        f[i] = __float_as_uint(__fmaf_rn(u[i], g.below, MAGIC));
+        apart |= f[i] ^ __float_as_uint(__fmaf_rn(u[i], g.above, MAGIC));
     }
-    if (worst > 0.5f - 1.0f / 32768.0f || g.exact) {
+    if (apart != 0u || g.divide) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float q = u[i] * g.ratio;
-            if (g.exact || fabsf(q - (f[i] - MAGIC)) > 0.5f - 1.0f / 32768.0f) f[i] = MAGIC + (float)code_exact(u[i], g.top);
+        for (int i = 0; i < N; ++i)
+            if (g.divide || f[i] != __float_as_uint(__fmaf_rn(u[i], g.above, MAGIC))) f[i] = (uint32_t)code_exact(u[i], g);
+    }
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+        const uint32_t all = __byte_perm(__byte_perm(f[4 * w], f[4 * w + 1], 0x0040), __byte_perm(f[4 * w + 2], f[4 * w + 3], 0x0040), 0x5410);
+        out[w] = g.top == 0.0f ? 0u : all;
+    }
+}
+
+// The same for values of eight bits (bfloat16): a ratio 127 x / a of two such numbers that is no tie is at least 1 / (2 * 254 * 255) from one near 1/2, and
+// 2^n times as far near 2^n / 2, so rounding its magnitude to a multiple of 2^-17 (2^-16 beyond 32), as adding 96 to it does, moves no ratio onto a tie or
+// over it, and brings a tie that 127 / a's rounding has moved (by up to 2^-24 of itself) back onto it.
+template <int N> __device__ __forceinline__ void codes_of_bf16(const float (&u)[N], const Grid& g, uint32_t (&out)[N / 4]) {
+    if (g.divide) return codes_of<N>(u, g, out);
+    uint32_t f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float side = __uint_as_float((__float_as_uint(u[i]) & 0x80000000u) | 0x42c00000u);       // 96 on the value's side of zero
+        f[i] = __float_as_uint((__fmaf_rn(u[i], g.ratio, side) - side) + 12582912.0f);
+    }
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+        const uint32_t all = __byte_perm(__byte_perm(f[4 * w], f[4 * w + 1], 0x0040), __byte_perm(f[4 * w + 2], f[4 * w + 3], 0x0040), 0x5410);
+        out[w] = g.top == 0.0f ? 0u : all;
+    }
+}
+
+// `n` codes (of N) to a place that is a multiple of N bytes from the row's beginning.
+template <int N> __device__ __forceinline__ void store_codes(int8_t* to, const uint32_t (&w)[N / 4], int n) {
+    if (n >= N) {
+        if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(to) = w[0];
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < n) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+}
+
+template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[Pack<T>::N]) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+            v[i] = __uint_as_float(w[i]);
         }
     }
-#pragma unroll
-    for (int w = 0; w < (N + 3) / 4; ++w) {
-        uint32_t b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = 4 * w + i < N ? __float_as_uint(f[4 * w + i < N ? 4 * w + i : 0]) : 0u;
-        out[w] = g.top == 0.0f ? 0u : __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// The packets of a row's values c .., zeros behind its end.  APART: rows may begin anywhere, and a packet of values lies in two packets of memory.  The
+// first is asked for early (`fetch`) and held; the second is the next thread's first and is read when the two are shifted together (`whole`), from
+// the L1 then.  Both have to lie inside the row, else the values are fetched one by one.
+template <typename T, bool APART> struct Packet {
+    static constexpr int N = Pack<T>::N;
+    uint4 a;
+    __device__ __forceinline__ void fetch(const T* row, int c, int width) {
+        if constexpr (!APART) {
+            a = c < width ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
+        } else if (inside(c, width)) {
+            a = *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + c) & ~(uintptr_t)15);
+        }
     }
-}
-
-template <int VEC> __device__ __forceinline__ void store_codes(int8_t* to, const uint32_t (&w)[(VEC + 3) / 4]) {
-    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-    else if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(to) = w[0];
-    else to[0] = (int8_t)(w[0] & 0xffu);
-}
-
-template <typename T, int VEC> __device__ __forceinline__ void load_values(const T* p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = to_f32<T>(p[0]);
+    static __device__ __forceinline__ bool inside(int c, int width) { return c >= N && c + 2 * N <= width; }
+    __device__ __forceinline__ uint4 whole(const T* row, int c, int width) const {
+        if constexpr (!APART) return a;
+        uint4 b = make_uint4(0u, 0u, 0u, 0u);
+        if (inside(c, width)) b = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + c) & ~(uintptr_t)15)[1];
+        uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;       // the same for all of the row's packets
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = off & 8u ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = off & 4u ? w[i + 1] : w[i];
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t bits = (off & 2u) * 8u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+        }
+        if (!inside(c, width)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = 0u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (c + i >= width) continue;
+                if constexpr (sizeof(T) == 2) w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[c + i] << (16 * (i & 1));
+                else w[i] = reinterpret_cast<const uint32_t*>(row)[c + i];
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+__device__ __forceinline__ void load_weights(const float* w, int c, int width, bool whole, float (&v)[8]) {
+    if (whole) {
+        const float4 a = *reinterpret_cast<const float4*>(w + c), b = *reinterpret_cast<const float4*>(w + c + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
-        const Pack<T> k = load_pack<T>(p);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = k.get(i);
+        for (int i = 0; i < 8; ++i) v[i] = c + i < width ? w[c + i] : 0.0f;
     }
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_values(T* p, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        p[0] = from_f32<T>(v[0]);
-    } else {
-        Pack<T> k;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) k.set(i, v[i]);
-        store_pack<T>(p, k);
-    }
-}
-template <int VEC> __device__ __forceinline__ void load_weights(const float* p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = p[0];
+__device__ __forceinline__ void load_weights(const float* w, int c, int width, bool whole, float (&v)[4]) {
+    if (whole) {
+        const float4 a = *reinterpret_cast<const float4*>(w + c);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(p + i);
-            v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
-        }
+        for (int i = 0; i < 4; ++i) v[i] = c + i < width ? w[c + i] : 0.0f;
     }
 }
 
-// Values c .. c + VEC - 1 of a row as they go into the codes; adds to the sum of squares.
-template <typename T, int VEC, bool NORM>
-__device__ __forceinline__ void values_of(const Rows& a, int64_t row, int c, float (&u)[VEC], float& squares, bool store) {
-    load_values<T, VEC>((const T*)a.x + row * a.x_stride + c, u);
-    if constexpr (NORM) {
-        if (a.delta != nullptr) {
-            float d[VEC];
-            load_values<T, VEC>((const T*)a.delta + row * a.delta_stride + c, d);
+// The largest magnitude as bits: an infinity's or NaN's are above every finite number's.
+template <typename T> __device__ __forceinline__ uint32_t top_of(const uint4& raw, uint32_t top) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) u[i] = round_to<T>(u[i] + d[i]);
-            if (store) store_values<T, VEC>((T*)a.total + row * a.total_stride + c, u);
-        }
-        float w[VEC];
-        load_weights<VEC>(a.weight + c, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            squares += u[i] * u[i];
-            u[i] *= w[i];
-        }
-    }
+    for (int i = 0; i < 4; ++i) top = sizeof(T) == 2 ? __vmaxu2(top, w[i] & 0x7fff7fffu) : max(top, w[i] & 0x7fffffffu);
+    return top;
+}
+// (of two 16-bit halves the larger one, as 32 bits)
+template <typename T> __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
+    return sizeof(T) == 2 ? max(top << 16, top & 0xffff0000u) : top;
 }
 
-// The largest magnitude (as bits: above every finite number's where there is an infinity or NaN) and the sum of squares over a row's threads.
-template <bool WARP> __device__ __forceinline__ void reduce(uint32_t& top, float& squares, bool norm) {
+// The largest magnitude and the sum of squares over a row's threads.
+template <bool WARP, bool NORM> __device__ __forceinline__ void reduce(uint32_t& top, float& squares) {
     top = __reduce_max_sync(0xffffffffu, top);
-    if (norm) squares = warp_sum(squares);
+    if (NORM) squares = warp_sum(squares);
     if constexpr (!WARP) {
         __shared__ uint32_t tops[32];
         __shared__ float sums[32];
@@ -139,14 +199,14 @@ template <bool WARP> __device__ __forceinline__ void reduce(uint32_t& top, float
         __syncthreads();
         const bool in = lane < (int)(blockDim.x >> 5);
         top = __reduce_max_sync(0xffffffffu, in ? tops[lane] : 0u);
-        if (norm) squares = warp_sum(in ? sums[lane] : 0.0f);
+        if (NORM) squares = warp_sum(in ? sums[lane] : 0.0f);
     }
 }
 
-template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint32_t top_bits, float squares, float& scale) {
-    const float top = __uint_as_float(top_bits);
+template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint32_t bits, float squares, float& scale) {
+    const float top = __uint_as_float(bits);
     float mean = 0.0f;
-    bool fine = top_bits < 0x7f800000u;
+    bool fine = bits < 0x7f800000u;
     if constexpr (NORM) {
         mean = squares / (float)a.width;
         fine = fine && mean < INFINITY;
@@ -154,94 +214,210 @@ template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint3
     scale = !fine ? __uint_as_float(0x7fffffffu) : NORM ? top * rsqrtf(mean + a.eps) / 127.0f : top / 127.0f;
     Grid g;
     g.top = fine ? top : 0.0f;
-    g.exact = top < 7.9e-31f;                                  // 2^-100
+    g.divide = g.top != 0.0f && top < 7.9e-31f;                // 2^-100
     g.ratio = __fdiv_rn(127.0f, fmaxf(top, 7.9e-31f));
+    g.below = __uint_as_float(__float_as_uint(g.ratio) - 1u);
+    g.above = __uint_as_float(__float_as_uint(g.ratio) + 1u);
     return g;
 }
 
-// A row a block, or (WARP) a row a warp; a thread holds PER packets of VEC values.
-template <typename T, int VEC, int PER, bool NORM, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) rows_kernel(const Rows a) {
+// A packet of sums to where they are stored: at once, or, where rows may begin anywhere, through shared memory: a warp's 32 packets are consecutive
+// values, which go out side by side.
+template <typename T, bool APART> __device__ __forceinline__ void store_total(T* row, int c, int width, const uint4& k) {
+    constexpr int N = Pack<T>::N;
+    if constexpr (!APART) {
+        if (c < width) *reinterpret_cast<uint4*>(row + c) = k;
+    } else {
+        extern __shared__ __align__(16) unsigned char staged[];
+        const int lane = threadIdx.x & 31, first = c - lane * N;
+        T* mine = reinterpret_cast<T*>(staged) + (threadIdx.x >> 5) * (32 * N);
+        __syncwarp();
+        *reinterpret_cast<uint4*>(mine + lane * N) = k;
+        __syncwarp();
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (first + i * 32 + lane < width) row[first + i * 32 + lane] = mine[i * 32 + lane];
+        } else {                                               // words of two values where they lie on word boundaries
+            const int odd = (int)(reinterpret_cast<uintptr_t>(row) >> 1) & 1, live = min(32 * N, width - first);
+            const uint16_t* from = reinterpret_cast<const uint16_t*>(mine);
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const int at = 2 * (i * 32 + lane) + odd;
+                if (at + 1 < live) *reinterpret_cast<uint32_t*>(row + first + at) = (uint32_t)from[at] | (uint32_t)from[at + 1] << 16;
+                else if (at < live) row[first + at] = mine[at];
+            }
+            if (odd && lane == 0 && live > 0) row[first] = mine[0];
+        }
+    }
+}
+
+// x + delta of a packet, rounded to the type.
+template <typename T> __device__ __forceinline__ uint4 sum_of(const uint4& x, const uint4& d) {
+    const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {d.x, d.y, d.z, d.w};
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(a[i] << 16) + __uint_as_float(b[i] << 16),
+                                                           __uint_as_float(a[i] & 0xffff0000u) + __uint_as_float(b[i] & 0xffff0000u));
+            w[i] = *reinterpret_cast<const uint32_t*>(&t);
+        } else {
+            w[i] = __float_as_uint(__uint_as_float(a[i]) + __uint_as_float(b[i]));
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A row a block, or (WARP) a row a warp; a thread holds PER packets, as they are stored (a norm's products with the weights are made twice, which takes
+// fewer registers than holding them in 32 bits).
+template <typename T, int PER, bool NORM, bool APART, bool WARP, int MOST_THREADS>
+__global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) rows_kernel(const Rows a) {
+    constexpr int N = Pack<T>::N;
     pdl_launch_dependents();
     pdl_wait();
     const int threads = WARP ? 32 : blockDim.x, thread = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= a.rows) return;
-    float u[PER][VEC], squares = 0.0f;
+    const T* x = (const T*)a.x + row * a.x_stride;
+    const bool whole_weights = NORM && (reinterpret_cast<uintptr_t>(a.weight) & 15u) == 0;
+    Packet<T, APART> from_x[PER];
+#pragma unroll
+    for (int p = 0; p < PER; ++p) from_x[p].fetch(x, (p * threads + thread) * N, a.width);
+    uint4 raw[PER];
+    if (NORM && a.delta != nullptr) {
+        const T* delta = (const T*)a.delta + row * a.delta_stride;
+        T* total = (T*)a.total + row * a.total_stride;
+        Packet<T, APART> from_delta[PER];
+#pragma unroll
+        for (int p = 0; p < PER; ++p) from_delta[p].fetch(delta, (p * threads + thread) * N, a.width);
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const int c = (p * threads + thread) * N;
+            raw[p] = sum_of<T>(from_x[p].whole(x, c, a.width), from_delta[p].whole(delta, c, a.width));
+            store_total<T, APART>(total, c, a.width, raw[p]);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < PER; ++p) raw[p] = from_x[p].whole(x, (p * threads + thread) * N, a.width);
+    }
+    float squares = 0.0f;
     uint32_t top = 0u;
+    auto weighted = [&](int p, int c, float (&u)[N]) {         // what the codes are made of
+        unpack<T>(raw[p], u);
+        if constexpr (NORM) {
+            float w[N];
+            load_weights(a.weight, c, a.width, whole_weights && c + N <= a.width, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] *= w[i];
+        }
+    };
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-        const int c = (p * threads + thread) * VEC;
-        if (c < a.width) {
-            values_of<T, VEC, NORM>(a, row, c, u[p], squares, true);
-        } else {
+        const int c = (p * threads + thread) * N;
+        if constexpr (!NORM) {
+            top = top_of<T>(raw[p], top);
+        } else if (c < a.width) {
+            float t[N], u[N];
+            unpack<T>(raw[p], t);
+            weighted(p, c, u);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) u[p][i] = 0.0f;
+            for (int i = 0; i < N; ++i) {
+                squares += t[i] * t[i];
+                top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(u[p][i]) & 0x7fffffffu);
     }
-    reduce<WARP>(top, squares, NORM);
+    if (!NORM) top = top_bits<T>(top);
+    reduce<WARP, NORM>(top, squares);
     float scale;
     const Grid g = finish<NORM>(a, top, squares, scale);
     if (thread == 0) a.scales[row] = scale;
+    int8_t* codes = a.codes + row * a.codes_stride;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
-        const int c = (p * threads + thread) * VEC;
-        if (c < a.width) {
-            uint32_t w[(VEC + 3) / 4];
-            codes_of<VEC>(u[p], g, w);
-            store_codes<VEC>(a.codes + row * a.codes_stride + c, w);
-        }
+        const int c = (p * threads + thread) * N;
+        if (c >= a.width) continue;
+        uint32_t w[N / 4];
+        float u[N];
+        weighted(p, c, u);
+        if constexpr (sizeof(T) == 2 && !NORM) codes_of_bf16<N>(u, g, w);
+        else codes_of<N>(u, g, w);
+        store_codes<N>(codes + c, w, a.width - c);
     }
 }
 
-// A row that does not fit the registers of a block: read twice.
+// A row that does not fit the registers of a block: read twice, four values at a time.
 template <typename T, bool NORM> __global__ void __launch_bounds__(1024) long_rows_kernel(const Rows a) {
     pdl_launch_dependents();
     pdl_wait();
     const int64_t row = blockIdx.x;
-    float squares = 0.0f, u[1];
+    const T* x = (const T*)a.x + row * a.x_stride;
+    float squares = 0.0f, u[4];
     uint32_t top = 0u;
-    for (int c = threadIdx.x; c < a.width; c += 1024) {
-        values_of<T, 1, NORM>(a, row, c, u, squares, false);
-        top = max(top, __float_as_uint(u[0]) & 0x7fffffffu);
+    auto values = [&](int c, bool store) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = c + i < a.width ? to_f32<T>(x[c + i]) : 0.0f;
+            if constexpr (NORM) {
+                if (c + i >= a.width) continue;
+                if (a.delta != nullptr) {
+                    u[i] = round_to<T>(u[i] + to_f32<T>(((const T*)a.delta)[row * a.delta_stride + c + i]));
+                    if (store) ((T*)a.total)[row * a.total_stride + c + i] = from_f32<T>(u[i]);
+                }
+                squares += u[i] * u[i];
+                u[i] *= a.weight[c + i];
+            }
+        }
+    };
+    for (int c = threadIdx.x * 4; c < a.width; c += 4096) {
+        values(c, false);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
     }
-    reduce<false>(top, squares, NORM);
-    float scale, unused = 0.0f;
+    reduce<false, NORM>(top, squares);
+    float scale;
     const Grid g = finish<NORM>(a, top, squares, scale);
     if (threadIdx.x == 0) a.scales[row] = scale;
-    for (int c = threadIdx.x; c < a.width; c += 1024) {
-        values_of<T, 1, NORM>(a, row, c, u, unused, true);     // (the sum is stored now: `total` may be x)
+    for (int c = threadIdx.x * 4; c < a.width; c += 4096) {
+        values(c, true);                                       // (the sum is stored now: `total` may be x)
         uint32_t w[1];
-        codes_of<1>(u, g, w);
-        store_codes<1>(a.codes + row * a.codes_stride + c, w);
+        codes_of<4>(u, g, w);
+        store_codes<4>(a.codes + row * a.codes_stride + c, w, a.width - c);
     }
 }
 
-template <typename T, int VEC, int PER, bool NORM> int launch(const Rows& a, int threads, bool warp, cudaStream_t stream) {
+template <typename T, int PER, bool NORM, bool APART> int launch(const Rows& a, int threads, bool warp, cudaStream_t stream) {
+    const int block = warp ? 128 : threads;
+    const size_t staged = NORM && APART && a.delta != nullptr ? (size_t)block * 16 : 0;
     if (warp)
-        return (int)q3_launch(rows_kernel<T, VEC, PER, NORM, true>, dim3((unsigned)((a.rows + 3) / 4)), dim3(128), 0, stream, a);
-    return (int)q3_launch(rows_kernel<T, VEC, PER, NORM, false>, dim3((unsigned)a.rows), dim3(threads), 0, stream, a);
+        return (int)q3_launch(rows_kernel<T, PER, NORM, APART, true, 128>, dim3((unsigned)((a.rows + 3) / 4)), dim3(block), staged, stream, a);
+    if (threads <= 512) return (int)q3_launch(rows_kernel<T, PER, NORM, APART, false, 512>, dim3((unsigned)a.rows), dim3(block), staged, stream, a);
+    return (int)q3_launch(rows_kernel<T, PER, NORM, APART, false, 1024>, dim3((unsigned)a.rows), dim3(block), staged, stream, a);
 }
 
-template <typename T, int VEC, bool NORM> int pick(const Rows& a, cudaStream_t stream) {
-    const int packets = (a.width + VEC - 1) / VEC, most = MOST / VEC;
-    const bool many = a.rows >= 2 * q3_device_sm_count();
-    const bool warp = many && packets <= 32 * most;
-    int per = warp ? (packets + 31) / 32 : many ? (packets + 255) / 256 : (packets + 1023) / 1024;
-    if (per > most) per = most;
-    int p = VEC == 1 ? 4 : 1;                                  // packets a thread: the next power of two
-    while (p < per) p *= 2;
-    const int threads = ((packets + p - 1) / p + 31) / 32 * 32;
-    if (threads > 1024)
-        return (int)q3_launch(long_rows_kernel<T, NORM>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
-    switch (p * VEC) {
-        case 4: return launch<T, VEC, (4 / VEC > 0 ? 4 / VEC : 1), NORM>(a, threads, warp, stream);
-        case 8: return launch<T, VEC, 8 / VEC, NORM>(a, threads, warp, stream);
-        case 16: return launch<T, VEC, 16 / VEC, NORM>(a, threads, warp, stream);
-        default: return launch<T, VEC, 32 / VEC, NORM>(a, threads, warp, stream);
+template <typename T, bool NORM, bool APART> int pick(const Rows& a, cudaStream_t stream) {
+    constexpr int N = Pack<T>::N, MOST = 32 / N;               // packets that a thread may hold
+    const int packets = (a.width + N - 1) / N;
+    const int64_t sms = q3_device_sm_count();
+    // short rows, if they are many: a row a warp
+    const bool warp = a.rows >= 2 * sms && packets <= 32 * MOST;
+    // As few packets a thread as the SMs can hold threads for at once: few rows want threads, many want loads in flight while other rows of the SM are
+    // reduced.  (8,000 rows of 4,096, bfloat16, 4 / 2 / 1 packets a thread: norm 42.8 / 47.9 / 66 us, quantise 17.7 / 21.7 / 29.3; 527 rows 6.6 / 4.7 / 5.5
+    // and 3.2 / 2.6 / 2.7.  float32 8 / 4: quantise 8,000 rows of 5,120 36.2 / 41.4, norm 100 / 81.)
+    int per = 1;
+    if (warp) {
+        while (32 * per < packets) per *= 2;
+    } else {
+        while (per < (NORM ? 4 : MOST) && a.rows * ((packets + per - 1) / per) > 1200 * sms) per *= 2;
+        while (per < MOST && packets > 1024 * per) per *= 2;
     }
+    const int threads = ((packets + per - 1) / per + 31) / 32 * 32;
+    if (threads > 1024) return (int)q3_launch(long_rows_kernel<T, NORM>, dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+    if (per == 1) return launch<T, 1, NORM, APART>(a, threads, warp, stream);
+    if (per == 2) return launch<T, 2, NORM, APART>(a, threads, warp, stream);
+    if (per == 4) return launch<T, 4, NORM, APART>(a, threads, warp, stream);
+    return launch<T, MOST, NORM, APART>(a, threads, warp, stream);
 }
 
 template <typename T, bool NORM> int rows_launch(const q3_int8_rows_args& in) {
@@ -254,9 +430,8 @@ template <typename T, bool NORM> int rows_launch(const q3_int8_rows_args& in) {
     const Rows a{in.x, NORM ? in.delta : nullptr, NORM ? (const float*)in.weight : nullptr, NORM ? in.total : nullptr, (int8_t*)in.codes,
                  (float*)in.scales, in.rows, in.x_stride, in.delta_stride, in.total_stride, in.codes_stride, in.width, (float)in.eps};
     const bool packets = in.width % V == 0 && in.x_stride % V == 0 && aligned16(in.x) &&
-                         (!NORM || (aligned16(in.weight) && (in.delta == nullptr || (in.delta_stride % V == 0 && in.total_stride % V == 0 &&
-                                                                                      aligned16(in.delta) && aligned16(in.total)))));
-    return packets ? pick<T, V, NORM>(a, (cudaStream_t)in.stream) : pick<T, 1, NORM>(a, (cudaStream_t)in.stream);
+                         (a.delta == nullptr || (in.delta_stride % V == 0 && in.total_stride % V == 0 && aligned16(in.delta) && aligned16(in.total)));
+    return packets ? pick<T, NORM, false>(a, (cudaStream_t)in.stream) : pick<T, NORM, true>(a, (cudaStream_t)in.stream);
 }
 
 }  // namespace

@@ -175,3 +175,16 @@ def test_refusals():
     for weight in (w[:60], w.double(), w.cpu(), torch.zeros(128, device="cuda")[::2]):
         with pytest.raises(ops.KernelError):
             ops.rms_norm_int8(x, weight, 1e-6, out)
+
+
+def test_every_pair_of_bfloat16_magnitudes():
+    """Every largest magnitude of a binade beside every value of the eleven binades below it: ties, and what lies closest to them."""
+    from qwen3_b200.csrc import ops
+    tops = torch.arange(128, 256, device="cuda").double()
+    values = torch.cat([tops * 2.0 ** -e for e in range(11)])
+    for scale in (1.0, 2.0 ** -90, 2.0 ** 100):
+        x = torch.cat([tops[:, None], torch.where(values[None] <= tops[:, None], values[None], torch.zeros((), device="cuda").double())], dim=1) * scale
+        x = torch.cat([x, -x], dim=1).to(torch.bfloat16)
+        out, memory = rows_for(*x.shape)
+        ops.quantize_rows(x, out)
+        same_rows(out, memory, x.double(), 2.0 ** -24)
