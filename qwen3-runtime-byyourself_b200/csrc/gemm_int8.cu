@@ -22,6 +22,12 @@ template <typename OutT> __device__ __forceinline__ OutT to_out(float v);
 template <> __device__ __forceinline__ float to_out<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16 to_out<bf16>(float v) { return __float2bfloat16_rn(v); }
 
+// The activation of a value whose product with `up` is rounded to OutT.
+template <int GATED, typename OutT> __device__ __forceinline__ float activated(float z) {
+    if constexpr (GATED == 1) return silu_for<OutT>(z);
+    return gate_activation<GATED>(z);
+}
+
 __device__ __forceinline__ float scaled(int sum, float token, float channel) { return (float)sum * token * channel; }
 
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) few_kernel(const Product p) 
             if (m0 + m >= p.M || n0 + n >= p.N) continue;
             const float sx = p.sx[m0 + m];
             const float g = scaled(total(m, n), sx, p.sw[n0 + n]), u = scaled(total(m, n + 8), sx, p.sw[n0 + n + 8]);
-            ((OutT*)p.y)[(int64_t)(m0 + m) * (p.N >> 1) + (n0 >> 1) + n] = to_out<OutT>(gate_activation<GATED>(g) * u);
+            ((OutT*)p.y)[(int64_t)(m0 + m) * (p.N >> 1) + (n0 >> 1) + n] = to_out<OutT>(activated<GATED, OutT>(g) * u);
         }
     }
 }
@@ -343,10 +349,10 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 const uint32_t addr = base + (uint32_t)(local * PART_LD + 16 * t + 4 * h) * 4u;
                 const int4 gs = sum4(addr), us = sum4(addr + 32u);
                 const float* sw = p.sw + n;
-                const float v[4] = {gate_activation<GATED>(scaled(gs.x, sx, sw[0])) * scaled(us.x, sx, sw[8]),
-                                    gate_activation<GATED>(scaled(gs.y, sx, sw[1])) * scaled(us.y, sx, sw[9]),
-                                    gate_activation<GATED>(scaled(gs.z, sx, sw[2])) * scaled(us.z, sx, sw[10]),
-                                    gate_activation<GATED>(scaled(gs.w, sx, sw[3])) * scaled(us.w, sx, sw[11])};
+                const float v[4] = {activated<GATED, OutT>(scaled(gs.x, sx, sw[0])) * scaled(us.x, sx, sw[8]),
+                                    activated<GATED, OutT>(scaled(gs.y, sx, sw[1])) * scaled(us.y, sx, sw[9]),
+                                    activated<GATED, OutT>(scaled(gs.z, sx, sw[2])) * scaled(us.z, sx, sw[10]),
+                                    activated<GATED, OutT>(scaled(gs.w, sx, sw[3])) * scaled(us.w, sx, sw[11])};
                 store4<OutT>(Y + (int64_t)m * out_n + (n0 >> 1) + 8 * t + 4 * h, v, whole, 4);
             }
         }
@@ -367,8 +373,11 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
 //   full[s]       in the leader (rank 0): both blocks' copies report their bytes there
 //   empty[s]      in each block: the leader's commit arrives at both
 //   acc_full[b]   in each block: likewise, when a tile's accumulator is complete
-//   acc_empty[b]  in the leader: the sixteen drain warps of both blocks arrive there
-constexpr int PAIR_THREADS = 320;       // producer, issuer, eight drain warps
+//   acc_empty[b]  in the leader: the drain warps of both blocks arrive there
+#ifndef Q3_SETS
+#define Q3_SETS 4
+#endif
+constexpr int DRAIN_SETS = Q3_SETS, DRAIN_WARPS = 4 * DRAIN_SETS, PAIR_THREADS = 64 + 32 * DRAIN_WARPS;
 constexpr int PAIR_STAGES = 6;
 
 // The order of the tiles: bands of at most 16 tiles of tokens, all tiles of W inside a band, the tokens fastest, so that a band's tokens stay in the L2
@@ -386,53 +395,82 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
-// Writes 32 tokens (from `m` on, `tokens` of them live) of the 32 rows of W that a warp's lanes own.  `v`: the lane's row, scaled by token and
-// channel.  bfloat16: lanes next to each other exchange, so that one takes both rows for the even token and the other for the odd one: 64
-// consecutive bytes a token and instruction (`words`: where a row of Y is whole 4-byte words).  GATED: the rows are gate[8] up[8] gate[8] up[8] of 16
-// features; a gate's lane and its up's, eight further, exchange first and take every other token each.
-template <int GATED, typename OutT>
-__device__ __forceinline__ void store_tokens(const float (&v)[32], OutT* Y, int m, int tokens, int row0, int lane, int N, bool words) {
-    if constexpr (GATED == 0) {
-        const int row = row0 + lane;
-        if (sizeof(OutT) == 4 || !words) {
-            if (row >= N) return;
-            OutT* to = Y + (int64_t)m * N + row;
+// 16 lanes by 32 columns of tensor memory as the products' accumulators lie in registers: r[4 j], r[4 j + 1] of lane l are row l / 4, columns
+// 8 j + 2 (l % 4) and the next, r[4 j + 2], r[4 j + 3] the same columns eight rows further.
+__device__ __forceinline__ void tc_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+
+// What a warp of the drain does with 32 tokens (`live` of them there are, from `m` on, with scales `sx`) of its 32 rows of W at `row0`: columns of tensor
+// memory from `acc` on.  `words`: rows of Y are whole 4-byte words.
+//
+// Without a gate a lane reads its own row.  bfloat16: two tokens make a word; lanes next to each other exchange, and one takes both rows for the
+// even token, the other for the odd one: 64 consecutive bytes a token and instruction.
+template <typename OutT>
+__device__ __forceinline__ void drain_plain(uint32_t acc, const float* sx, float sw, OutT* Y, int64_t m, int live, int row0, int lane, int N, bool words) {
+    uint32_t r[32];
+    tc_ld32(acc, r);
+    tc_wait_ld();
+    float v[32];
 #pragma unroll
-            for (int t = 0; t < 32; ++t)
-                if (t < tokens) to[(int64_t)t * N] = to_out<OutT>(v[t]);
-        } else {
-            const int odd = lane & 1;
-            OutT* to = Y + (int64_t)(m + odd) * N + (row & ~1);
+    for (int t = 0; t < 32; t += 4) {
+        const float4 x4 = *reinterpret_cast<const float4*>(sx + t);
+        v[t] = scaled((int)r[t], x4.x, sw);
+        v[t + 1] = scaled((int)r[t + 1], x4.y, sw);
+        v[t + 2] = scaled((int)r[t + 2], x4.z, sw);
+        v[t + 3] = scaled((int)r[t + 3], x4.w, sw);
+    }
+    const int row = row0 + lane;
+    if (sizeof(OutT) == 4 || !words) {
+        if (row >= N) return;
+        OutT* to = Y + m * N + row;
 #pragma unroll
-            for (int t = 0; t < 32; t += 2) {
-                const float got = __shfl_xor_sync(0xffffffffu, odd ? v[t] : v[t + 1], 1);
-                const uint32_t both = odd ? pack_bf16(got, v[t + 1]) : pack_bf16(v[t], got);
-                if (row < N && t + odd < tokens) *reinterpret_cast<uint32_t*>(to + (int64_t)t * N) = both;
-            }
-        }
+        for (int t = 0; t < 32; ++t, to += N)
+            if (t < live) *to = to_out<OutT>(v[t]);
     } else {
-        const int out_n = N >> 1, feature = (row0 >> 1) + ((lane >> 4) << 3) + (lane & 7), up = (lane >> 3) & 1;
-        const bool live = row0 + (lane & 16) + 16 <= N;
-        float y[16];                                         // tokens 2 t + up
+        const int odd = lane & 1;
+        const uint32_t both = odd ? 0x3276u : 0x5410u;       // halves of the lane's word and the other's, the even row first
+        const int there = row < N ? live - odd : 0;
+        OutT* to = Y + (m + odd) * N + (row & ~1);
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const float got = __shfl_xor_sync(0xffffffffu, up ? v[2 * t] : v[2 * t + 1], 8);
-            const float g = up ? got : v[2 * t], u = up ? v[2 * t + 1] : got;
-            y[t] = gate_activation<GATED>(g) * u;
+        for (int t = 0; t < 32; t += 2, to += 2 * (int64_t)N) {
+            const uint32_t own = pack_bf16(v[t], v[t + 1]), other = __shfl_xor_sync(0xffffffffu, own, 1);
+            if (t < there) *reinterpret_cast<uint32_t*>(to) = __byte_perm(own, other, both);
         }
-        if (sizeof(OutT) == 4 || !words) {
-            OutT* to = Y + (int64_t)(m + up) * out_n + feature;
+    }
+}
+// With a gate the rows are gate[8] up[8] gate[8] up[8] of 16 features, and a lane reads a gate's row and its up's, of two tokens in eight.
+template <int GATED, typename OutT>
+__device__ __forceinline__ void drain_gated(uint32_t acc, const float* sx, const float (&sw)[4], OutT* Y, int64_t m, int live, int row0, int lane, int N,
+                                            bool words) {
+    const int64_t out_n = N >> 1;
+    const int quad = lane >> 2, odd = quad & 1, first = 2 * (lane & 3);
+    const uint32_t both = odd ? 0x3276u : 0x5410u;
+    uint32_t r[2][16];
+    tc_ld_16x32(acc, r[0]);
+    tc_ld_16x32(acc + (16u << 16), r[1]);
+    tc_wait_ld();
 #pragma unroll
-            for (int t = 0; t < 16; ++t)
-                if (live && 2 * t + up < tokens) to[(int64_t)(2 * t) * out_n] = to_out<OutT>(y[t]);
-        } else {
-            const int odd = lane & 1;
-            OutT* to = Y + (int64_t)(m + up + 2 * odd) * out_n + (feature & ~1);
+    for (int h = 0; h < 2; ++h) {
+        const bool whole = row0 + 16 * h + 16 <= N;
+        const int feature = (row0 >> 1) + 8 * h + quad;
+        OutT* to = Y + (m + first) * out_n + feature;
 #pragma unroll
-            for (int t = 0; t < 16; t += 2) {
-                const float got = __shfl_xor_sync(0xffffffffu, odd ? y[t] : y[t + 1], 1);
-                const uint32_t both = odd ? pack_bf16(got, y[t + 1]) : pack_bf16(y[t], got);
-                if (live && 2 * (t + odd) + up < tokens) *reinterpret_cast<uint32_t*>(to + (int64_t)(2 * t) * out_n) = both;
+        for (int j = 0; j < 4; ++j, to += 8 * out_n) {
+            const float2 s = *reinterpret_cast<const float2*>(sx + 8 * j + first);
+            const float y0 = activated<GATED, OutT>(scaled((int)r[h][4 * j], s.x, sw[2 * h])) * scaled((int)r[h][4 * j + 2], s.x, sw[2 * h + 1]);
+            const float y1 = activated<GATED, OutT>(scaled((int)r[h][4 * j + 1], s.y, sw[2 * h])) * scaled((int)r[h][4 * j + 3], s.y, sw[2 * h + 1]);
+            const int token = 8 * j + first;
+            if (sizeof(OutT) == 4 || !words) {
+                if (whole && token < live) to[0] = to_out<OutT>(y0);
+                if (whole && token + 1 < live) to[out_n] = to_out<OutT>(y1);
+            } else {
+                const uint32_t own = pack_bf16(y0, y1), other = __shfl_xor_sync(0xffffffffu, own, 4);
+                if (whole && token + odd < live) *reinterpret_cast<uint32_t*>(odd ? to + out_n - 1 : to) = __byte_perm(own, other, both);
             }
         }
     }
@@ -442,7 +480,7 @@ template <int GATED, typename OutT>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Product p, int tile, int* __restrict__ status) {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(16) float token_scales[8][128];      // of a drain warp's share of the tile
+    __shared__ __align__(16) float token_scales[DRAIN_WARPS][256 / DRAIN_SETS];       // of a drain warp's share of the tile
     constexpr int STAGES = PAIR_STAGES, BN = 2 * BM;
     constexpr int X_BYTES = BM * BK, W_BYTES = BM * BK, STAGE_BYTES = X_BYTES + W_BYTES;
     constexpr uint32_t TMEM_COLS = 512;                       // two accumulators of 256 columns
@@ -465,7 +503,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar_acc_full + b * 8, 1);
-            mbar_init(bar_acc_empty + b * 8, 16);            // one arrival per drain warp of the pair
+            mbar_init(bar_acc_empty + b * 8, 2 * DRAIN_WARPS);     // one arrival per drain warp of the pair
         }
         mbar_init_fence();
     }
@@ -544,8 +582,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
         }
     } else {
         pdl_wait();
-        // 32 rows of W by the tokens of the tile's first or second half
-        const int lane_base = (warp & 3) * 32, set = (warp - 2) >> 2, half = tile / 2, c0 = set * half;
+        // 32 rows of W by a share of the tile's tokens
+        const int lane_base = (warp & 3) * 32, set = (warp - 2) >> 2, share = tile / DRAIN_SETS, c0 = set * share;
         OutT* Y = (OutT*)p.y;
         const bool words = (reinterpret_cast<uintptr_t>(Y) & 3u) == 0 && p.N % 2 == 0;      // (with a gate N / 2 is even, too)
         float* sx = token_scales[warp - 2];
@@ -555,10 +593,15 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             int tm, tn;
             tile_place(i, tiles_m, tiles_n, tm, tn);
             const int m0 = tm * tile + c0, row0 = tn * BN + (int)rank * BM + lane_base;
-            const int tokens = min(half, p.M - m0);          // none or less where the tile's second half lies behind the last token
+            const int tokens = min(share, p.M - m0);         // none or less where the share lies behind the last token
             __syncwarp();
-            for (int t = lane; t < half; t += 32) sx[t] = t < tokens ? p.sx[m0 + t] : 0.0f;
-            const float sw = row0 + lane < p.N ? p.sw[row0 + lane] : 0.0f;
+            for (int t = lane; t < share; t += 32) sx[t] = t < tokens ? p.sx[m0 + t] : 0.0f;
+            float sw[4];                                     // of the rows that the lane reads
+#pragma unroll
+            for (int i = 0; i < (GATED ? 4 : 1); ++i) {
+                const int row = row0 + (GATED ? 8 * i + (lane >> 2) : lane);
+                sw[i] = row < p.N ? p.sw[row] : 0.0f;
+            }
             __syncwarp();
             if (!mbar_wait(bar_acc_full + buf * 8, (local >> 1) & 1u)) {
                 if (lane == 0) atomicExch(status, 3);
@@ -569,19 +612,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
             const uint32_t acc = tmem_base + ((uint32_t)lane_base << 16) + buf * 256u + (uint32_t)c0;
 #pragma unroll 1
             for (int c = 0; c < tokens; c += 32) {
-                uint32_t r[32];
-                tc_ld32(acc + (uint32_t)c, r);
-                tc_wait_ld();
-                float v[32];
-#pragma unroll
-                for (int t = 0; t < 32; t += 4) {
-                    const float4 x4 = *reinterpret_cast<const float4*>(sx + c + t);
-                    v[t] = scaled((int)r[t], x4.x, sw);
-                    v[t + 1] = scaled((int)r[t + 1], x4.y, sw);
-                    v[t + 2] = scaled((int)r[t + 2], x4.z, sw);
-                    v[t + 3] = scaled((int)r[t + 3], x4.w, sw);
-                }
-                store_tokens<GATED, OutT>(v, Y, m0 + c, tokens - c, row0, lane, p.N, words);
+                if constexpr (GATED != 0) drain_gated<GATED, OutT>(acc + (uint32_t)c, sx + c, sw, Y, m0 + c, tokens - c, row0, lane, p.N, words);
+                else drain_plain<OutT>(acc + (uint32_t)c, sx + c, sw[0], Y, m0 + c, tokens - c, row0, lane, p.N, words);
             }
             tc_fence_before();
             __syncwarp();
