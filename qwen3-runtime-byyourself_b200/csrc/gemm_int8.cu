@@ -162,8 +162,19 @@ template <int MT, int WARPS, int PF, int MINB, int GATED, typename OutT> int lau
                           WARPS * 8 * MT * 17 * 4, stream, p);
 }
 
+// Warps that share K, steps in flight and blocks an SM.  Up to eight tokens (16 warps, 2 steps, 2 blocks / 8, 4, 3 / 8, 2, 4, us): as long as all blocks
+// run at once, more warps (4,096 x 4,096 4.9 / 5.6 / 5.6, 4,096 x 12,288 10.1 / 11.2 / 12.8), then more steps where K is long (5,120 x 17,408 21.6 /
+// 16.7 / 18.9), else more blocks (6,144 x 4,096 7.3 / 6.6 / 6.1, gated 24,576 x 4,096 21.1 / 19.5 / 18.2).
 template <int GATED, typename OutT> int few(const Product& p, cudaStream_t stream) {
-    return launch_few<1, 8, 4, 3, GATED, OutT>(p, stream);
+    const int sms = q3_device_sm_count(), blocks = (p.N + 15) / 16;
+    if (p.M <= 8) {
+        if (blocks <= 2 * sms) return launch_few<1, 16, 2, 2, GATED, OutT>(p, stream);
+        if (blocks <= 3 * sms && p.K >= 8192) return launch_few<1, 8, 4, 3, GATED, OutT>(p, stream);
+        return launch_few<1, 8, 2, 4, GATED, OutT>(p, stream);
+    }
+    if (p.M <= 16)
+        return blocks <= 2 * sms ? launch_few<2, 16, 1, 2, GATED, OutT>(p, stream) : launch_few<2, 8, 2, 3, GATED, OutT>(p, stream);
+    return launch_few<4, 8, 2, 2, GATED, OutT>(p, stream);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -629,15 +640,62 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     }
 }
 
-// K ranges (blocks of a cluster) of the weights-first form: the largest power of two up to the portable cluster size that keeps the grid within
-// 2.6 blocks an SM (one an SM for tiles of 256 tokens) and leaves every block 8 K steps.
-int mid_splits(int M, int N, int K) {
-    const int token_tiles = M <= 128 ? 1 : (M + 255) / 256;
-    const int tiles = (N + BM - 1) / BM * token_tiles, nkb = (K + BK - 1) / BK;
-    const int limit = M > 128 ? q3_device_sm_count() : q3_device_sm_count() * 13 / 5;
-    int s = 1;
-    while (s < 8 && tiles * (2 * s) <= limit && nkb / (2 * s) >= 8) s *= 2;
-    return s;
+// ---------------------------------------------------------------------------------------------
+// Which form takes a product, in how many K ranges or tokens a tile: the one whose estimate is least.  Microseconds of a launch among others, W from
+// memory.  The constants are fitted to 5,500 times of 700 products of 1 to 8,000 tokens, 64 to 25,600 channels and widths, plain and gated; what they
+// choose is 3 % slower than the best of a product in the mean, 12 % for one in ten.
+inline int cuts(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// Steps of 64 a warp, as many blocks as run at once (see `few`); where a wave is not full what a step costs is latency.
+float few_us(int M, int N, int K) {
+    const int sms = q3_device_sm_count(), rows = cuts(N, 16), tiles = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+    const bool once = rows <= 2 * sms;
+    const int warps = tiles < 4 && once ? 16 : 8, slots = tiles == 4 || once ? 2 : tiles == 2 || (rows <= 3 * sms && K >= 8192) ? 3 : 4;
+    const float waves = (float)((int64_t)rows * cuts(M, 8 * tiles)) / (float)(slots * sms);
+    const float step = 0.28f + 0.37f * fminf(waves, 1.0f) * (float)(warps * slots) / 32.0f * (1.0f + 0.285f * (float)tiles);
+    return 1.14f + fmaxf(waves, 1.0f) * (0.38f * (float)tiles + 0.95f * (float)cuts(cuts(K, 64), warps) * step);
+}
+// Steps of 128 a block: latency, or the bytes of the blocks that share an SM.  Then the tile's way through shared memory and out.
+float mid_us(int M, int N, int K, int splits) {
+    const int sms = q3_device_sm_count(), tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    const int64_t blocks = (int64_t)cuts(N, BM) * splits * cuts(M, tile);
+    const int slots = tile == 256 ? 1 : (int64_t)cuts(N, BM) * splits > 2 * sms ? 3 : 2, waves = cuts(blocks, slots * sms);
+    const float shared = waves == 1 ? (float)blocks / (float)sms : (float)slots, t = (float)tile / 64.0f;
+    const float step = fmaxf(0.237f + 0.063f * t, shared * (16.0f + 8.0f * t) * 0.0171f);
+    const float around = 1.24f * t + 0.8f * shared + (splits > 1 ? 0.4f : 0.0f);
+    return 2.2f + (float)waves * ((float)cuts(cuts(K, BK), splits) * step + around);
+}
+// Steps of 128 a pair: the products, the copies of few tokens, or what the L2 gives all pairs; a tile's drain under the next one's steps, but for the last.
+float pair_us(int M, int N, int K, int tile) {
+    const int pairs = q3_device_sm_count() / 2;
+    const int64_t tiles = (int64_t)cuts(M, tile) * cuts(N, 256);
+    const float t = (float)tile / 256.0f, full = fminf((float)tiles / (float)pairs, 1.0f);
+    const float step = fmaxf(fmaxf(0.223f, 0.362f * t), 0.15f * full * (t + 1.0f)), drain = 1.77f + 1.63f * t;
+    return 1.05f * (0.75f + (float)cuts(tiles, pairs) * fmaxf((float)cuts(K, BK) * step, drain) + drain);
+}
+
+struct Choice {
+    int splits;
+    float us;
+};
+Choice mid_choice(int M, int N, int K) {
+    Choice best{1, mid_us(M, N, K, 1)};
+    for (int s : {2, 3, 4, 6, 8}) {
+        const float us = s <= cuts(K, BK) ? mid_us(M, N, K, s) : best.us;
+        if (us < best.us) best = Choice{s, us};
+    }
+    return best;
+}
+// Equal tiles of a multiple of 32 tokens: those that whole 256s, or one to three more, would make, and smaller ones where these fill the pairs.
+Choice pair_choice(int M, int N, int K) {
+    Choice best{256, 1e30f};
+    auto take = [&](int tile) {
+        const float us = pair_us(M, N, K, tile);
+        if (us < best.us) best = Choice{tile, us};
+    };
+    for (int n = cuts(M, 256); n < cuts(M, 256) + 4; ++n) take(cuts(cuts(M, n), 32) * 32);
+    for (int tile = 32; tile < 160 && tile < M + 32; tile += 32) take(tile);
+    return best;
 }
 
 template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid(const Product& p, int splits, int* status, cudaStream_t stream) {
@@ -656,7 +714,7 @@ template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid
 
 template <int GATED, typename OutT> int mid(const Product& p, int splits, int* status, cudaStream_t stream) {
     const int nkb = (p.K + BK - 1) / BK;
-    if (splits == 0) splits = mid_splits(p.M, p.N, p.K);
+    if (splits == 0) splits = mid_choice(p.M, p.N, p.K).splits;
     if (splits > nkb) splits = nkb;
     const bool waves = (int64_t)((p.N + BM - 1) / BM) * splits > 2 * q3_device_sm_count();
 #define Q3_MID(MT, ST, MB) return launch_mid<MT, ST, MB, GATED, OutT>(p, splits, status, stream)
@@ -668,32 +726,13 @@ template <int GATED, typename OutT> int mid(const Product& p, int splits, int* s
 #undef Q3_MID
 }
 
-// Tokens of a tile of the pairs form: equal tiles of a multiple of 32, as many as whole 256s would make or one to three more, by what the tiles should
-// take: microseconds of a K step of 128 of a tile, at least what the copies take where it has few tokens, and of a tile's drain.
-struct PairTile {
-    int tile;
-    float us;
-};
-PairTile pair_tile(int M, int N, int K) {
-    const int pairs = q3_device_sm_count() / 2, whole = (M + 255) / 256;
-    PairTile best{256, 1e30f};
-    for (int cuts = whole; cuts <= whole + 3 && cuts <= (M + 31) / 32; ++cuts) {
-        const int tile = ((M + cuts - 1) / cuts + 31) / 32 * 32;
-        const int64_t tiles = (int64_t)((M + tile - 1) / tile) * ((N + 255) / 256);
-        const float step = fmaxf(0.224f, 0.343f * tile / 256.0f);
-        const float us = 6.0f + (float)((tiles + pairs - 1) / pairs) * (float)((K + BK - 1) / BK) * step;
-        if (us < best.us) best = PairTile{tile, us};
-    }
-    return best;
-}
-
 template <int GATED, typename OutT> int pair(const Product& p, int tile, int* status, cudaStream_t stream) {
     constexpr int SMEM = PAIR_STAGES * (2 * BM * BK) + 1024 + 256;
     const auto kernel = pair_kernel<GATED, OutT>;
     static Q3PerDevice configured;
     const cudaError_t e = q3_allow_shared_memory(kernel, SMEM, configured);
     if (e != cudaSuccess) return (int)e;
-    if (tile == 0) tile = pair_tile(p.M, p.N, p.K).tile;
+    if (tile == 0) tile = pair_choice(p.M, p.N, p.K).splits;
     if (tile < 32 || tile > 256 || tile % 32 != 0) return Q3_ERR_BAD_SIZE;
     CUtensorMap map_x, map_w;
     if (!q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, tile / 2) || !q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM)) return Q3_ERR_BAD_SIZE;
@@ -721,7 +760,7 @@ int product_of(const q3_gemm_int8_args& a, Product& p) {
 
 }  // namespace
 
-// Few tokens, W streamed (any number of tokens is taken; W is read once for every eight).
+// Few tokens, W streamed (any number is taken; W is read once for every 8, 16 or 32 of them).
 Q3_EXPORT int q3_gemm_int8_few(const q3_gemm_int8_args* a) {
     if (a->rows <= 0 || a->channels <= 0) return 0;
     Product p;
@@ -753,4 +792,14 @@ Q3_EXPORT int q3_gemm_int8_pair(const q3_gemm_int8_args* a) {
 #define Q3_PAIR(G, T) pair<G, T>(p, a->splits, (int*)a->status, (cudaStream_t)a->stream)
     Q3_BY_EPILOGUE(Q3_PAIR);
 #undef Q3_PAIR
+}
+
+// The form that a product of these sizes should go to, and the `splits` of it: 0 few tokens, 1 weights first, 2 pairs of SMs.
+Q3_EXPORT int q3_gemm_int8_plan(int rows, int channels, int width, int* splits) {
+    *splits = 0;
+    if (rows <= 0 || channels <= 0 || width <= 0) return 0;
+    const Choice m = mid_choice(rows, channels, width), p = pair_choice(rows, channels, width);
+    if (rows <= 64 && few_us(rows, channels, width) <= fminf(m.us, p.us)) return 0;
+    *splits = m.us <= p.us ? m.splits : p.splits;
+    return m.us <= p.us ? 1 : 2;
 }

@@ -8,6 +8,7 @@ to a library: a CPU tensor or a missing compiler is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import struct
@@ -1700,9 +1701,12 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Ro
 _INT8_FORMS = {"few": "q3_gemm_int8_few", "mid": "q3_gemm_int8_mid", "pair": "q3_gemm_int8_pair"}
 
 
-def int8_form(M: int, N: int, K: int) -> str:
-    """Which kernel takes a product of M tokens with N channels of width K."""
-    return "few" if M <= 8 else "mid" if M <= 256 else "pair"
+@functools.lru_cache(maxsize=4096)
+def int8_plan(M: int, N: int, K: int) -> tuple:
+    """(form, splits): which kernel should take a product of M tokens with N channels of width K (`gemm_int8`), by its estimates of the times."""
+    lib, splits = load_library("gemm_int8.cu", ()), c_int(0)
+    form = lib.q3_gemm_int8_plan(c_int(M), c_int(N), c_int(K), ctypes.byref(splits))
+    return ("few", "mid", "pair")[form], splits.value
 
 
 def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[str] = None, form: Optional[str] = None, splits: int = 0) -> torch.Tensor:
@@ -1720,7 +1724,9 @@ def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[
     if w.device != x.device or out.device != x.device:
         raise KernelError("gemm_int8: the operands lie on different devices")
     _suffix(out)
-    name = _INT8_FORMS.get(int8_form(M, N, K) if form is None else form)
+    if form is None:
+        form, splits = int8_plan(M, N, K)
+    name = _INT8_FORMS.get(form)
     if name is None:
         raise KernelError(f"gemm_int8: form {form!r}: one of {sorted(_INT8_FORMS)}")
     _call_packed("gemm_int8", "gemm_int8.cu", name, _GEMM8_ARGS.pack(

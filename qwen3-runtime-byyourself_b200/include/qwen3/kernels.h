@@ -526,9 +526,11 @@ int q3_rms_norm_int8_f32(const q3_int8_rows_args* args);
 int q3_rms_norm_int8_bf16(const q3_int8_rows_args* args);
 
 /* ---- gemm_int8.cu: products of such rows, scaled by token and channel; all forms give the same bits ---- */
-int q3_gemm_int8_few(const q3_gemm_int8_args* args);
+int q3_gemm_int8_few(const q3_gemm_int8_args* args);    /* mma.sync, W streamed */
 int q3_gemm_int8_mid(const q3_gemm_int8_args* args);    /* tcgen05, weights first; splits: K ranges in a cluster (0: chosen) */
 int q3_gemm_int8_pair(const q3_gemm_int8_args* args);   /* tcgen05 on pairs of SMs; splits: tokens of a tile (0: chosen) */
+/* the form that should take a product (0, 1, 2 in this order), and its `splits` */
+int q3_gemm_int8_plan(int rows, int channels, int width, int* splits);
 
 /* ---- sampling.cu ------------------------------------------------------------------------------------------ */
 /* out[r] = index of the highest logit among the first `valid` (lowest id among equals, NaN as -inf) */
