@@ -6,6 +6,7 @@
                                    q.GenerationOptions(max_new_tokens=64, stop_token_ids=[eos]))
 
     engine = q.Engine.from_folder(model_dir, max_tokens=8 * 8192, cache_dtype="float8")    # keys and values in 8 bits
+    engine = q.Engine.from_folder(model_dir, max_tokens=8 * 8192, weight_dtype="int8")     # projections in 8 bits
     results = q.generate_speculative(engine, prompts, max_new_tokens=64)                   # greedy, with drafted tokens
 
 Names follow the reference where it has them: `generate_token_ids`, `GenerationOptions`

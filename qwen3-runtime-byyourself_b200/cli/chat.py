@@ -9,7 +9,7 @@ MODEL_DIRECTORY / --model, --gpu, --max-context (4096, at most max_position_embe
 extras (:830-843); a trailing stop token is dropped from what is printed (:1018-1021).
 
 Additions: raw token ids in and out without any tokenizer (--tokens, --tokens-file),
-several prompts of unequal length as one batch, --dtype, and --random-weights SEED with
+several prompts of unequal length as one batch, --dtype, --weight-dtype, and --random-weights SEED with
 --config for a model that exists only as a configuration.  Text chat needs tokenizer.json
 in the model folder.
 """
@@ -78,6 +78,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--tokens-file", metavar="PATH", help="A file with one prompt of token ids per line.")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default=None,
                     help="Compute type. Default: the checkpoint's torch_dtype")
+    ap.add_argument("--weight-dtype", choices=["int8"], default=None,
+                    help="Keep the layers' projections as 8-bit integers with a scale for each channel. Default: the compute type")
     ap.add_argument("--config", metavar="PATH", help="config.json for --random-weights.")
     ap.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                     help="Run the configuration of --config with seeded random weights instead of a checkpoint.")
@@ -131,9 +133,9 @@ def main(argv: Optional[List[str]] = None) -> int:
     def make_engine():
         if args.random_weights is not None:
             return q.Engine.from_random(config, args.random_weights, dtype=args.dtype, max_tokens=n_live * max_context,
-                                        max_seq_len=max_context, device=device)
+                                        max_seq_len=max_context, device=device, weight_dtype=args.weight_dtype)
         return q.Engine.from_folder(model_dir, dtype=args.dtype, max_tokens=n_live * max_context,
-                                    max_seq_len=max_context, device=device)
+                                    max_seq_len=max_context, device=device, weight_dtype=args.weight_dtype)
 
     if prompts:
         engine = make_engine()

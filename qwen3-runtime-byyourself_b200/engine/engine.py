@@ -264,14 +264,18 @@ class Engine:
     @classmethod
     def from_folder(cls, folder: str, dtype=None, max_tokens: int = 4096, max_seq_len: Optional[int] = None,
                     device="cuda:0", n_slots: Optional[int] = None, use_graphs: bool = True,
-                    guard_scratch: bool = False, cache_dtype: Optional[str] = None) -> "Engine":
-        """Load config.json and the safetensors of `folder`; the model class is chosen by config.json."""
+                    guard_scratch: bool = False, cache_dtype: Optional[str] = None, weight_dtype: Optional[str] = None) -> "Engine":
+        """Load config.json and the safetensors of `folder`; the model class is chosen by config.json.  `weight_dtype` "int8": the layers'
+        projections are kept as 8-bit integers with a scale for each output channel, and multiplied with activations in 8 bits with a scale
+        for each token (models of pre-norm blocks with attention and a gated feed-forward); None: as computed with."""
+        eight_bit = cls._eight_bit(weight_dtype)
         config = load_config(folder)
         model = build_model(config.plan())
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
         # every tensor goes from the mapped file to its final place on the device in one pass
-        source = open_upload(folder, model.weight_specs(), model.ignorable_names(), compute, device, model._warn_rounding)
-        model.bind(source, compute, device)
+        source = open_upload(folder, model.weight_specs(), model.ignorable_names(), compute, device, model._warn_rounding,
+                             apart=model.eight_bit_names() if eight_bit and model.takes_eight_bit() else ())
+        model.bind(source, compute, device, eight_bit)
         source.finish()
         engine = cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
         engine.weights_arena = source.arena                    # the parts' tensors are views of it
@@ -280,13 +284,20 @@ class Engine:
     @classmethod
     def from_random(cls, config, seed: int, dtype=None, max_tokens: int = 4096, max_seq_len: Optional[int] = None,
                     device="cuda:0", n_slots: Optional[int] = None, use_graphs: bool = True,
-                    guard_scratch: bool = False, cache_dtype: Optional[str] = None) -> "Engine":
+                    guard_scratch: bool = False, cache_dtype: Optional[str] = None, weight_dtype: Optional[str] = None) -> "Engine":
         """Seeded random weights drawn on the device (no folder is written)."""
+        eight_bit = cls._eight_bit(weight_dtype)
         model = build_model(config.plan())
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
         weights = random_weights(model.weight_specs(), seed, dtype=compute, device=device)
-        model.bind(weights, compute, device)
+        model.bind(weights, compute, device, eight_bit)
         return cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
+
+    @staticmethod
+    def _eight_bit(weight_dtype: Optional[str]) -> bool:
+        if weight_dtype not in (None, "int8"):
+            raise ValueError(f"weight_dtype {weight_dtype!r}: None (as computed with) or 'int8'")
+        return weight_dtype is not None
 
     # -- sequences
     def new_sequence(self) -> int:

@@ -55,7 +55,7 @@ from ..csrc import ops
 from ..weights.loader import WeightSpec
 from ..weights.upload import fuse_rows
 from .base import Part, build_part, register_part
-from .linear import linear
+from .linear import linear, quantized, quantized_weights
 
 # Hand-written bfloat16 kernels register themselves here: fn(part, q, cache, out, ctx, table) -> bool
 PREFILL_KERNELS = []
@@ -302,8 +302,19 @@ class GQAAttention(Part):
         if self.head_gate:
             gate = ctx.scratch.get("attn.head_gate", (ctx.n_tokens, self.num_heads), ctx.dtype)
             ops.head_gate(attn, linear(x, self.w_gate, gate), self.num_heads, self.value_dim)
-        linear(attn, self.w_o, out)
+        linear(quantized(attn, ctx, "attn.ctx8") if isinstance(self.w_o, ops.Int8Rows) else attn, self.w_o, out)
         return ops.add_bias(out, self.o_bias) if self.out_bias else out
+
+    def takes_eight_bit(self) -> bool:
+        """Whether weights in 8 bits can be had of this layer: it reads its input through the q/k/v projection alone (an output gate's is part of it)."""
+        return type(self).forward is GQAAttention.forward and type(self).mix is GQAAttention.mix and not self.head_gate
+
+    def eight_bit_names(self, prefix: str) -> list:
+        p, n = prefix + self.prefix, self.names
+        return [p + n[k] for k in ("q", "k", "v", "out_gate", "o") if p + n[k] in self.weight_specs(prefix)]
+
+    def to_eight_bit(self) -> None:
+        self.w_qkv, self.w_o = quantized_weights(self.w_qkv), quantized_weights(self.w_o)
 
     def mix(self, x: torch.Tensor, ctx, cache) -> torch.Tensor:
         """Everything before the output projection: [N, num_heads * value_dim] in the compute type (float32 with
@@ -534,7 +545,7 @@ def _projection_pair_kernel(part, x, cache, q, ctx, table, q_norm_w, k_norm_w, e
     from . import linear as linear_module
     nq, nkv, d = part.num_heads, part.num_kv_heads, part.head_dim
     N, K = ctx.n_tokens, part.hidden_size
-    if d not in ops.PAIR_QKV_HEAD_DIMS or K % 8 != 0 or N < fused_projection_rows:
+    if isinstance(getattr(part, "w_qkv", None), ops.Int8Rows) or d not in ops.PAIR_QKV_HEAD_DIMS or K % 8 != 0 or N < fused_projection_rows:
         return False
     if cos is not None and 2 * cos.shape[-1] != d:
         return False

@@ -20,6 +20,8 @@ from .base import Part, build_part, register_part
 
 
 class PreNormBlock(Part):
+    weights_in_eight_bit = False
+
     def __init__(self, mixer, feed_forward, norm: PartSpec, mixer_norm_name: str, feed_forward_norm_name: str):
         self.mixer, self.feed_forward = mixer, feed_forward
         self.mixer_norm = build_part("norm", norm)
@@ -40,7 +42,29 @@ class PreNormBlock(Part):
         self.mixer.bind(weights, prefix, dtype, device)
         self.feed_forward.bind(weights, prefix, dtype, device)
 
+    def parts(self):
+        return self.mixer_norm, self.mixer, self.feed_forward_norm, self.feed_forward
+
+    def takes_eight_bit(self) -> bool:
+        """Whether the products of this layer can be had with weights in 8 bits: its norms then write the sublayers' inputs in 8 bits."""
+        return all(getattr(part, "takes_eight_bit", lambda: False)() for part in self.parts())
+
+    def eight_bit_names(self, prefix: str) -> list:
+        return self.mixer.eight_bit_names(prefix) + self.feed_forward.eight_bit_names(prefix)
+
+    def to_eight_bit(self) -> None:
+        self.mixer.to_eight_bit()
+        self.feed_forward.to_eight_bit()
+        self.weights_in_eight_bit = True
+
     def forward(self, residual, delta, ctx, cache):
+        if self.weights_in_eight_bit:
+            from .linear import eight_bit_rows
+            normed = eight_bit_rows(ctx, "block.normed8", *residual.shape)
+            self.mixer_norm.eight_bit(residual, normed, delta)
+            mixed = self.mixer.forward(normed, ctx, cache)
+            self.feed_forward_norm.eight_bit(residual, normed, mixed)
+            return residual, self.feed_forward.forward(normed, ctx)
         normed = ctx.scratch.get("block.normed", residual.shape, ctx.dtype)
         self.mixer_norm(residual, normed, delta)
         mixed = self.mixer.forward(normed, ctx, cache)

@@ -8,6 +8,8 @@ tokens first and persistent on pairs of SMs for prompts); widths that are no mul
 with 32-bit accumulation.  No product goes to a library, where the reference's engine
 calls cublasGemmEx for every projection (src/ops/linear.cpp:165-193: bfloat16 in, 32-bit
 accumulate).  Another kernel can be registered for a shape (`set_bf16_kernel`).
+
+Where weights are 8-bit integers (`ops.Int8Rows`), so are the rows that they are multiplied with: a norm or `quantized` makes them.
 """
 from __future__ import annotations
 
@@ -106,8 +108,26 @@ def few_rows_weights_first(M: int, N: int, K: int) -> bool:
     return M >= 4 and 2 * N * K >= 150_000_000 and -(-N // 128) <= wave or K >= 4096 and wave < -(-N // 16) <= wave * 4 // 3
 
 
-def linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-    """out[M, N] = x[M, K] . w[N, K]^T; out is float32 or x's type."""
+def eight_bit_rows(ctx, name: str, rows: int, width: int) -> ops.Int8Rows:
+    """Room for a step's rows in 8 bits, in the scratch buffers of this name."""
+    codes = ctx.scratch.get(name, (rows, -(-width // 16) * 16), torch.int8)
+    return ops.Int8Rows(codes[:, :width], ctx.scratch.get(name + "_scales", (rows,), torch.float32))
+
+
+def quantized(x: torch.Tensor, ctx, name: str) -> ops.Int8Rows:
+    """The rows of x in 8 bits, for a product with weights in 8 bits."""
+    return ops.quantize_rows(x, eight_bit_rows(ctx, name, *x.shape))
+
+
+def quantized_weights(w: torch.Tensor) -> ops.Int8Rows:
+    """A matrix [out, in] in 8 bits, a scale for each output channel."""
+    return ops.quantize_rows(w, ops.Int8Rows.empty(*w.shape, w.device))
+
+
+def linear(x, w, out: torch.Tensor) -> torch.Tensor:
+    """out[M, N] = x[M, K] . w[N, K]^T; out is float32 or x's type.  Operands in 8 bits (`ops.Int8Rows`, both): out is float32 or bfloat16."""
+    if isinstance(w, ops.Int8Rows):
+        return ops.gemm_int8(x, w, out)
     if x.dtype == torch.float32:
         if out.dtype != torch.float32:
             raise ops.KernelError("a 32-bit product writes 32-bit output")

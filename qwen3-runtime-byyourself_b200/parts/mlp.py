@@ -48,11 +48,24 @@ class SwiGLU(Part):
         self.w_gate_up = fuse_interleaved(weights, gate, up, 8) if self.interleaved else fuse_rows(weights, [gate, up])
         self.w_down = weights.pop(p + self.names["down"]).contiguous()
 
+    def takes_eight_bit(self) -> bool:
+        return type(self) is SwiGLU
+
+    def eight_bit_names(self, prefix: str) -> list:
+        return [prefix + self.prefix + self.names[k] for k in ("gate", "up", "down")]
+
+    def to_eight_bit(self) -> None:
+        self.w_gate_up = linear_module.quantized_weights(self.w_gate_up)
+        self.w_down = linear_module.quantized_weights(self.w_down)
+
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         N, I = ctx.n_tokens, self.intermediate_size
         act = ctx.scratch.get("ff.act", (N, I), ctx.dtype)
-        fused = self.interleaved and ctx.dtype == torch.bfloat16 and self.hidden_size % 8 == 0 and self.activation != "clamped"
-        if fused and N <= linear_module.skinny_rows and not linear_module.few_rows_weights_first(N, 2 * I, self.hidden_size):
+        eight_bit = isinstance(self.w_gate_up, ops.Int8Rows)
+        fused = not eight_bit and self.interleaved and ctx.dtype == torch.bfloat16 and self.hidden_size % 8 == 0 and self.activation != "clamped"
+        if eight_bit and self.interleaved and self.activation != "clamped":
+            ops.gemm_int8(x, self.w_gate_up, act, self.activation)               # gate, up and the gating in 32 bits
+        elif fused and N <= linear_module.skinny_rows and not linear_module.few_rows_weights_first(N, 2 * I, self.hidden_size):
             ops.gemm_skinny_gated(x, self.w_gate_up, act, self.activation)   # product, activation and gating in one kernel
         elif fused and (N <= linear_module.skinny_rows or
                         linear_module.tcgen05_form(N, 2 * I, self.hidden_size, gated=True) == "weights_first"):
@@ -68,7 +81,7 @@ class SwiGLU(Part):
             else:
                 ops.silu_mul(gate_up, act, self.interleaved, self.activation)
         out = ctx.scratch.get("ff.out", (N, self.hidden_size), ctx.dtype)
-        return linear(act, self.w_down, out)
+        return linear(linear_module.quantized(act, ctx, "ff.act8") if eight_bit else act, self.w_down, out)
 
 
 class DenseMLP(Part):

@@ -61,16 +61,29 @@ class Model:
             names += list(getattr(block, "ignorable", lambda prefix: [])(spec.prefix))
         return names
 
-    def bind(self, weights, dtype: torch.dtype, device) -> None:
+    def takes_eight_bit(self) -> bool:
+        """Whether the layers' projections can be had in 8 bits (`bind`): every layer is a pre-norm block of attention and a gated feed-forward."""
+        return all(getattr(b, "takes_eight_bit", lambda: False)() for b in self.blocks)
+
+    def eight_bit_names(self) -> set:
+        """The tensors that `bind` with 8-bit weights quantises."""
+        return {name for spec, block in zip(self.plan.layers, self.blocks) for name in block.eight_bit_names(spec.prefix)}
+
+    def bind(self, weights, dtype: torch.dtype, device, eight_bit: bool = False) -> None:
         """Take the tensors (by checkpoint name) for computing in `dtype` on `device`.  `weights` is a dict of
         tensors, or a checkpoint that uploads on demand (`weights.loader.open_upload`).
 
         Matrices are used in the compute type: a bfloat16 checkpoint widens exactly for
         the 32-bit path; a 32-bit matrix is rounded to bfloat16 for a bfloat16 engine, with
-        one line on stderr saying so.  Scale vectors are always read as float32."""
+        one line on stderr saying so.  Scale vectors are always read as float32.
+
+        `eight_bit`: the layers' projections become 8-bit integers with a scale for each output channel, from what is stored (a 32-bit
+        matrix is not rounded to bfloat16 first); embedding and output projection stay as they are."""
         from ..weights.upload import TensorDict
+        if eight_bit and not self.takes_eight_bit():
+            raise ValueError("weights in 8 bits take a model whose layers are pre-norm blocks of attention and a gated feed-forward")
         if isinstance(weights, dict):
-            weights = TensorDict(weights, self.weight_specs(), dtype, device, self._warn_rounding)
+            weights = TensorDict(weights, self.weight_specs(), dtype, device, self._warn_rounding, self.eight_bit_names() if eight_bit else ())
         p = self.plan
         self.dtype, self.device = dtype, torch.device(device)
         self.embedding.bind(weights, p.embedding_prefix, dtype, device)
@@ -80,6 +93,9 @@ class Model:
         self.head.bind(weights, p.head_prefix, dtype, device)
         for spec, block in zip(p.layers, self.blocks):
             block.bind(weights, spec.prefix, dtype, device)
+            if eight_bit:
+                getattr(weights, "wait", lambda: None)()          # a streamed checkpoint: the tensors are in place now
+                block.to_eight_bit()                              # and are given back, layer by layer
 
     def _warn_rounding(self, name: str) -> None:
         if not self._warned_rounding:

@@ -46,6 +46,13 @@ class RMSNorm(Part):
             raise ops.KernelError("a norm in groups is applied on a float32 stream by sandwich_norm")
         return ops.rms_norm(x, self.weight, self.eps, out, delta)
 
+    def takes_eight_bit(self) -> bool:
+        return self.groups == 1
+
+    def eight_bit(self, x: torch.Tensor, out: ops.Int8Rows, delta=None) -> ops.Int8Rows:
+        """The same with the normed rows in 8 bits, rounded to these alone."""
+        return ops.rms_norm_int8(x, self.weight, self.eps, out, delta)
+
 
 class LayerNorm(Part):
     """y = (x - mean) / sqrt(variance + eps) * weight, without a bias, the variance being the mean of the squared deviations.

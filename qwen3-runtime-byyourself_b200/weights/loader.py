@@ -106,14 +106,14 @@ def load_weights(folder: str, specs: Dict[str, WeightSpec], ignorable: Iterable[
     return out
 
 
-def open_upload(folder: str, specs: Dict[str, WeightSpec], ignorable: Iterable[str], dtype: torch.dtype, device, warn=None):
+def open_upload(folder: str, specs: Dict[str, WeightSpec], ignorable: Iterable[str], dtype: torch.dtype, device, warn=None, apart=()):
     """The checkpoint of `folder`, checked against `specs`, as a source that a model binds from: every tensor goes
     from the mapped file to its final place on the device in one pass (weights/upload.py)."""
     from .upload import CheckpointUpload
     ckpt = Checkpoint(folder)
     specs = resolve_sizes(ckpt, specs)
     check_checkpoint(ckpt, folder, specs, ignorable)
-    return CheckpointUpload(ckpt, specs, dtype, device, warn)
+    return CheckpointUpload(ckpt, specs, dtype, device, warn, apart)
 
 
 def _stream_seed(seed: int, name: str) -> int:

@@ -57,12 +57,15 @@ class TensorDict(dict):
     """Tensors in memory (random weights, tests) prepared for a model: matrices in the compute type on the
     device, everything else moved as it is.  A 32-bit matrix that a bfloat16 engine rounds is announced once."""
 
-    def __init__(self, tensors: Dict[str, torch.Tensor], specs, dtype: torch.dtype, device, warn=None):
+    def __init__(self, tensors: Dict[str, torch.Tensor], specs, dtype: torch.dtype, device, warn=None, apart=()):
+        """`apart`: matrices that are quantised next, and therefore not rounded from 32-bit to bfloat16."""
         super().__init__()
         warned = False
         for name, t in tensors.items():
             spec = specs.get(name)
-            if spec is not None and spec.role == "matrix":
+            if name in apart and t.dtype == torch.float32:
+                t = t.to(device=device)
+            elif spec is not None and spec.role == "matrix":
                 if t.dtype == torch.float32 and dtype == torch.bfloat16 and not warned and warn is not None:
                     warned = True
                     warn(name)
@@ -75,13 +78,18 @@ class TensorDict(dict):
 class CheckpointUpload:
     """The tensors of a checkpoint, uploaded on demand into one device arena (see the top of the file)."""
 
-    def __init__(self, checkpoint: Checkpoint, specs, dtype: torch.dtype, device, warn=None):
+    def __init__(self, checkpoint: Checkpoint, specs, dtype: torch.dtype, device, warn=None, apart=()):
+        """`apart`: matrices that are quantised and given back before the next ones are read: each in memory of its own, in 32-bit if it is
+        stored so."""
+        self.apart = set(apart)
         self.ckpt, self.specs, self.dtype, self.device = checkpoint, specs, dtype, torch.device(device)
         if self.device.type != "cuda":
             raise ValueError("a checkpoint is uploaded to a CUDA device")
         self._warn, self._warned = warn, False
         total = 0
         for name, spec in specs.items():
+            if name in self.apart:
+                continue
             numel = 1
             for s in spec.shape:
                 numel *= s
@@ -105,9 +113,13 @@ class CheckpointUpload:
         t = self._done.get(name)
         if t is None:
             spec = self.specs[name]
-            t = self._carve(tuple(spec.shape), _role_dtype(spec.role, self.dtype))
+            if name in self.apart:
+                t = self._own([name], tuple(spec.shape))
+            else:
+                t = self._carve(tuple(spec.shape), _role_dtype(spec.role, self.dtype))
             self._place(name, t.view(-1, t.shape[-1]) if t.dim() > 1 else t.view(1, -1), 0, 0, 0)
-            self._done[name] = t
+            if name not in self.apart:
+                self._done[name] = t
         return t
 
     def get(self, name, default=None):
@@ -125,7 +137,8 @@ class CheckpointUpload:
         cols = shapes[0][1]
         if any(len(s) != 2 or s[1] != cols for s in shapes):
             raise ValueError(f"rows of {names} do not have one width")
-        out = self._carve((sum(s[0] for s in shapes), cols), self.dtype)
+        shape = (sum(s[0] for s in shapes), cols)
+        out = self._own(names, shape) if self.apart.issuperset(names) else self._carve(shape, self.dtype)
         row0 = 0
         for name, shape in zip(names, shapes):
             self._place(name, out, 0, 0, row0)
@@ -136,7 +149,8 @@ class CheckpointUpload:
         a, b = tuple(self.specs[first].shape), tuple(self.specs[second].shape)
         if a != b or len(a) != 2 or a[0] % block != 0:
             raise ValueError(f"{first} and {second} cannot be interleaved in blocks of {block} rows")
-        out = self._carve((2 * a[0], a[1]), self.dtype)
+        shape = (2 * a[0], a[1])
+        out = self._own([first, second], shape) if self.apart.issuperset((first, second)) else self._carve(shape, self.dtype)
         self._place(first, out, block, 2 * block, 0)
         self._place(second, out, block, 2 * block, block)
         return out
@@ -163,6 +177,12 @@ class CheckpointUpload:
         view = self.arena[self._used:self._used + nbytes].view(dtype).view(shape)
         self._used += -(-nbytes // ALIGN) * ALIGN
         return view
+
+    def _own(self, names: List[str], shape) -> torch.Tensor:
+        wide = any(self.ckpt.tensors[n].dtype == torch.float32 for n in names)
+        t = torch.empty(shape, dtype=torch.float32 if wide else self.dtype, device=self.device)
+        self._side.wait_stream(torch.cuda.current_stream(self.device))     # what used this memory before is done with it
+        return t
 
     # -- the stream of bytes
     def _place(self, name: str, dst: torch.Tensor, block_rows: int, dst_block_stride: int, dst_row0: int) -> None:
