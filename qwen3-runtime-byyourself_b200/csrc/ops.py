@@ -38,8 +38,9 @@ class KernelError(RuntimeError):
 # step at batch 16), while the few-row product loses (batch 8: chains of waiting blocks take the room that a kernel's
 # own later waves need) and the decode attention, which asks for its first pages before it waits, gains 0.5 % at batch
 # 16 and 32 and loses 0.3 % at batch 64; its form for many sequences, which stands between such products, gains 1.5 % at batch 64
-# (1526 -> 1503 us a step of 12 layers).  QWEN3_B200_PDL=1 / =0 turns it on / off for all.
-PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu", "attention_tree_tc.cu", "gemm_int8.cu", "int8_rows.cu")
+# (1526 -> 1503 us a step of 12 layers).  The products of 8-bit integers gain 2 to 4 % (8B shape, ms a step with / without: batch 1 2.37 / 2.46, 8
+# 3.03 / 3.09, 64 4.40 / 4.56), the rows in 8 bits between them lose (batch 8 3.76 with both).  QWEN3_B200_PDL=1 / =0 turns it on / off for all.
+PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu", "attention_tree_tc.cu", "gemm_int8.cu")
 _pdl_override = {"1": True, "0": False}.get(os.environ.get("QWEN3_B200_PDL", ""))
 _libs = {}
 
@@ -1612,6 +1613,7 @@ def gemm_skinny(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> torch.Te
 
 # ------------------------------------------------------------------ 8-bit integers with a scale a row
 _ROWS8_ARGS, _GEMM8_ARGS = struct.Struct("@7q5qd2i"), struct.Struct("@7q2q6i")
+_QUANTIZE, _NORM8 = ({d: name + s for d, s in _SUFFIX.items()} for name in ("q3_quantize_rows_", "q3_rms_norm_int8_"))
 INT8_MAX_WIDTH = 131071                # a sum of so many products of two codes stays below 2^31
 
 
@@ -1619,7 +1621,7 @@ class Int8Rows:
     """Rows [rows, width] in 8 bits: a code stands for code * scale of its row.  `codes` int8 with rows a multiple of 16 bytes apart (`Int8Rows.empty`
     makes room for any width), `scales` float32 [rows].  Tokens and matrices [channels, width] alike."""
 
-    __slots__ = ("codes", "scales", "rows", "width", "stride", "shape", "at", "scales_at", "device")
+    __slots__ = ("codes", "scales", "rows", "width", "stride", "shape", "at", "scales_at", "index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 2 or codes.dtype != torch.int8 or scales.shape != codes.shape[:1]:
@@ -1628,7 +1630,7 @@ class Int8Rows:
             raise KernelError("int8 rows: codes and scales are CUDA tensors of one device (there is no CPU path)")
         self.scales_at = _dev(scales, "scales", torch.float32)
         self.rows, self.width = codes.shape
-        self.shape, self.device = (self.rows, self.width), codes.device
+        self.shape, self.index = codes.shape, codes.get_device()
         # (a tensor of one row, or without any, may have any stride)
         self.stride = codes.stride(0) if self.rows > 1 else -(-self.width // 16) * 16
         if (self.width > 1 and codes.stride(1) != 1) or self.stride % 16 or self.stride < self.width or codes.data_ptr() % 16:
@@ -1648,30 +1650,35 @@ class Int8Rows:
         return self.codes.float() * self.scales[:, None]
 
 
-def _strided(t: torch.Tensor, name: str, dtype: torch.dtype, shape, device) -> int:
-    """Where rows lie that are whole but may be any distance apart."""
-    if t.shape != shape or t.dtype is not dtype or t.device != device:
-        raise KernelError(f"{name} must be {dtype} {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if (shape[1] > 1 and t.stride(1) != 1) or (shape[0] > 1 and t.stride(0) < shape[1]):
+def _strided(t: torch.Tensor, name: str, dtype: torch.dtype, shape, index: int):
+    """(address, values from row to row) of rows that are whole but may be any distance apart.  (Few calls: one into torch takes 0.1 to 0.5 us of the
+    host, a kernel of a decode step 2.)"""
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != index:
+        raise KernelError(f"{name} must be {dtype} {tuple(shape)} on cuda:{index}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), shape[1]
+    step, one = t.stride()
+    if (shape[1] > 1 and one != 1) or (shape[0] > 1 and step < shape[1]):
         raise KernelError(f"{name} must have contiguous rows that do not overlap")
-    return t.data_ptr()
+    return t.data_ptr(), step
 
 
-def _on_current(device, what: str) -> int:
+def _stream_on(index: int, what: str) -> int:
     """The stream to launch on; the tensors have to lie on its device."""
-    if device.index != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the tensors lie on {device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    return _here()
+    current = torch._C._cuda_getDevice()
+    if index != current:
+        raise KernelError(f"{what}: the tensors lie on cuda:{index}, the current device is cuda:{current}")
+    return _pinned_stream if _pinned_stream is not None else torch._C._cuda_getCurrentRawStream(current)
 
 
 def quantize_rows(x: torch.Tensor, out: Int8Rows) -> Int8Rows:
     """Rows of x [rows, width] (bfloat16 or float32, contiguous rows any distance apart) as 8-bit codes: with a = max |x| of a row, code = 127 x / a to
     the nearest whole number, ties to even, and scale = a / 127.  A row of zeros gets the scale 0, one with a NaN or an infinity the
     scale NaN and codes of 0."""
-    s = _suffix(x)
-    at = _strided(x, "x", x.dtype, out.shape, out.device)
-    _call_packed("quantize_rows", "int8_rows.cu", "q3_quantize_rows_" + s, _ROWS8_ARGS.pack(
-        at, 0, 0, 0, out.at, out.scales_at, _on_current(out.device, "quantize_rows"), out.rows, x.stride(0), 0, 0, out.stride, 0.0, out.width, 0))
+    dtype = x.dtype
+    at, step = _strided(x, "x", dtype, out.shape, out.index)
+    _call_packed("quantize_rows", "int8_rows.cu", _QUANTIZE.get(dtype) or "q3_quantize_rows_" + _suffix(x), _ROWS8_ARGS.pack(
+        at, 0, 0, 0, out.at, out.scales_at, _stream_on(out.index, "quantize_rows"), out.rows, step, 0, 0, out.stride, 0.0, out.width, 0))
     return out
 
 
@@ -1681,20 +1688,20 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Ro
 
     With `delta` the norm reads x + delta (32-bit sum, stored in x's type), which is written to `total`, by default to x itself.  A
     row whose squares' sum 32 bits do not hold counts as one with an infinity.  x, delta and total: contiguous rows any distance apart."""
-    s, dtype, device, shape = _suffix(x), x.dtype, out.device, out.shape
-    at = _strided(x, "x", dtype, shape, device)
+    dtype, index, shape = x.dtype, out.index, out.shape
+    at, step = _strided(x, "x", dtype, shape, index)
     if delta is None:
         if total is not None:
             raise KernelError("rms_norm_int8: a total is that of x and delta")
-        delta_at = total_at = delta_stride = total_stride = 0
+        delta_at = total_at = delta_step = total_step = 0
     else:
-        delta_at, delta_stride = _strided(delta, "delta", dtype, shape, device), delta.stride(0)
-        total_at, total_stride = (at, x.stride(0)) if total is None else (_strided(total, "total", dtype, shape, device), total.stride(0))
-    if weight.numel() != out.width or weight.device != device:
+        delta_at, delta_step = _strided(delta, "delta", dtype, shape, index)
+        total_at, total_step = (at, step) if total is None else _strided(total, "total", dtype, shape, index)
+    if weight.numel() != out.width or weight.get_device() != index:
         raise KernelError("rms_norm_int8: the weight does not fit")
-    _call_packed("rms_norm_int8", "int8_rows.cu", "q3_rms_norm_int8_" + s, _ROWS8_ARGS.pack(
-        at, delta_at, _at(weight, "weight", _F32), total_at, out.at, out.scales_at, _on_current(device, "rms_norm_int8"), out.rows, x.stride(0),
-        delta_stride, total_stride, out.stride, float(eps), out.width, 0))
+    _call_packed("rms_norm_int8", "int8_rows.cu", _NORM8.get(dtype) or "q3_rms_norm_int8_" + _suffix(x), _ROWS8_ARGS.pack(
+        at, delta_at, _at(weight, "weight", _F32), total_at, out.at, out.scales_at, _stream_on(index, "rms_norm_int8"), out.rows, step, delta_step,
+        total_step, out.stride, eps, out.width, 0))
     return out
 
 
@@ -1716,22 +1723,24 @@ def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[
 
     `form`: "few" (W streamed for eight tokens at a time), "mid" (weights first on tcgen05, K in `splits` ranges) or "pair" (pairs of SMs, tiles of `splits`
     tokens); by default what the sizes ask for.  All give the same bits."""
-    M, K, N = x.rows, x.width, w.rows
+    M, K, N, index, dtype = x.rows, x.width, w.rows, x.index, out.dtype
     if w.width != K or out.shape != (M, N if activation is None else N // 2) or not 0 < K <= INT8_MAX_WIDTH or (activation is not None and N % 16):
-        raise KernelError(f"gemm_int8: shapes {x.shape} x {w.shape}^T -> {tuple(out.shape)}")
+        raise KernelError(f"gemm_int8: shapes {tuple(x.shape)} x {tuple(w.shape)}^T -> {tuple(out.shape)}")
     if activation is not None and activation not in ACTIVATIONS:
         raise KernelError(f"gemm_int8: activation {activation!r}: one of {sorted(ACTIVATIONS)}")
-    if w.device != x.device or out.device != x.device:
-        raise KernelError("gemm_int8: the operands lie on different devices")
-    _suffix(out)
+    if w.index != index or out.get_device() != index or dtype not in _SUFFIX or not out.is_contiguous():
+        raise KernelError(f"gemm_int8: out must be contiguous, bfloat16 or float32, and on the operands' device, got {dtype} on {out.device}")
     if form is None:
         form, splits = int8_plan(M, N, K)
     name = _INT8_FORMS.get(form)
     if name is None:
         raise KernelError(f"gemm_int8: form {form!r}: one of {sorted(_INT8_FORMS)}")
+    status = _status_at.get(index)
+    if status is None:
+        status = _status_at[index] = _status_word(torch.device("cuda", index)).data_ptr()
     _call_packed("gemm_int8", "gemm_int8.cu", name, _GEMM8_ARGS.pack(
-        x.at, x.scales_at, w.at, w.scales_at, _at(out, "out", out.dtype), _status_word(x.device).data_ptr(), _on_current(x.device, "gemm_int8"),
-        x.stride, w.stride, M, N, K, 1 if out.dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, splits))
+        x.at, x.scales_at, w.at, w.scales_at, out.data_ptr(), status, _stream_on(index, "gemm_int8"), x.stride, w.stride, M, N, K,
+        1 if dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, splits))
     return out
 
 
@@ -1755,7 +1764,7 @@ def attention_prefill(q, k_pages, v_pages, out, seq_start, seq_pos0, page_table,
 
 
 # ------------------------------------------------------------------ bfloat16 tcgen05 product
-_tc_status = {}
+_tc_status, _status_at = {}, {}        # the word of a device, and where the word of a device's number lies
 
 
 def _status_word(device) -> torch.Tensor:
