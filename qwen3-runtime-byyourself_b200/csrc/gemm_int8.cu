@@ -331,12 +331,13 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         const bool whole = (out_n % 4 == 0) && ((reinterpret_cast<uintptr_t>(Y) & 15u) == 0);
         constexpr int GROUPS = GATED ? 16 : 32;                               // groups of four outputs per token and tile
         const int my_tokens = (MT - (int)rank + (int)ranks - 1) / (int)ranks;
-        auto sum4 = [&](uint32_t addr) {
-            int4 sum = make_int4(0, 0, 0, 0);
-            for (uint32_t s = 0; s < ranks; ++s) {
-                const int4 v = ld_cluster_i4(map_to_rank(addr, s));
-                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-            }
+        auto sum4 = [&](uint32_t addr) {                                      // all blocks' parts are asked for together
+            int4 v[8];
+#pragma unroll
+            for (uint32_t s = 0; s < 8; ++s) v[s] = s < ranks ? ld_cluster_i4(map_to_rank(addr, s)) : make_int4(0, 0, 0, 0);
+            int4 sum = v[0];
+#pragma unroll
+            for (int s = 1; s < 8; ++s) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
             return sum;
         };
         for (int idx = threadIdx.x; idx < my_tokens * GROUPS; idx += THREADS) {

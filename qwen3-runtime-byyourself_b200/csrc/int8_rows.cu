@@ -274,8 +274,8 @@ template <typename T> __device__ __forceinline__ uint4 sum_of(const uint4& x, co
 template <typename T, int PER, bool NORM, bool APART, bool WARP, int MOST_THREADS>
 __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) rows_kernel(const Rows a) {
     constexpr int N = Pack<T>::N;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int threads = WARP ? 32 : blockDim.x, thread = WARP ? threadIdx.x & 31 : threadIdx.x;
     const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (WARP && row >= a.rows) return;
@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
 
 // A row that does not fit the registers of a block: read twice, four values at a time.
 template <typename T, bool NORM> __global__ void __launch_bounds__(1024) long_rows_kernel(const Rows a) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const int64_t row = blockIdx.x;
     const T* x = (const T*)a.x + row * a.x_stride;
     float squares = 0.0f, u[4];
@@ -404,12 +404,12 @@ template <typename T, bool NORM, bool APART> int pick(const Rows& a, cudaStream_
     const bool warp = a.rows >= 2 * sms && packets <= 32 * MOST;
     // As few packets a thread as the SMs can hold threads for at once: few rows want threads, many want loads in flight while other rows of the SM are
     // reduced.  (8,000 rows of 4,096, bfloat16, 4 / 2 / 1 packets a thread: norm 42.8 / 47.9 / 66 us, quantise 17.7 / 21.7 / 29.3; 527 rows 6.6 / 4.7 / 5.5
-    // and 3.2 / 2.6 / 2.7.  float32 8 / 4: quantise 8,000 rows of 5,120 36.2 / 41.4, norm 100 / 81.)
+    // and 3.2 / 2.6 / 2.7.  float32 8 / 4: quantise 8,000 rows of 5,120 36.2 / 41.4, of 4,097 49.5 / 43.0, norm 100 / 81.)
     int per = 1;
     if (warp) {
         while (32 * per < packets) per *= 2;
     } else {
-        while (per < (NORM ? 4 : MOST) && a.rows * ((packets + per - 1) / per) > 1200 * sms) per *= 2;
+        while (per < (NORM || APART ? 4 : MOST) && a.rows * ((packets + per - 1) / per) > 1200 * sms) per *= 2;
         while (per < MOST && packets > 1024 * per) per *= 2;
     }
     const int threads = ((packets + per - 1) / per + 31) / 32 * 32;

@@ -38,9 +38,10 @@ class KernelError(RuntimeError):
 # step at batch 16), while the few-row product loses (batch 8: chains of waiting blocks take the room that a kernel's
 # own later waves need) and the decode attention, which asks for its first pages before it waits, gains 0.5 % at batch
 # 16 and 32 and loses 0.3 % at batch 64; its form for many sequences, which stands between such products, gains 1.5 % at batch 64
-# (1526 -> 1503 us a step of 12 layers).  The products of 8-bit integers gain 2 to 4 % (8B shape, ms a step with / without: batch 1 2.37 / 2.46, 8
-# 3.03 / 3.09, 64 4.40 / 4.56), the rows in 8 bits between them lose (batch 8 3.76 with both).  QWEN3_B200_PDL=1 / =0 turns it on / off for all.
-PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu", "attention_tree_tc.cu", "gemm_int8.cu")
+# (1526 -> 1503 us a step of 12 layers).  The products of 8-bit integers and the rows between them gain 2 to 4 % (8B shape, ms a step, both / the products /
+# none: batch 1 2.33 / 2.37 / 2.46, 8 2.99 / 3.03 / 3.09, 64 4.40 / 4.40 / 4.56) - the rows' kernels let the next one start after their own wait, not
+# before it, or the weights of a product are asked for while the one before still runs (batch 8 3.76).  QWEN3_B200_PDL=1 / =0 turns it on / off for all.
+PDL_SOURCES = ("gemm_tcgen05.cu", "attention_decode_flat.cu", "attention_tree_tc.cu", "gemm_int8.cu", "int8_rows.cu")
 _pdl_override = {"1": True, "0": False}.get(os.environ.get("QWEN3_B200_PDL", ""))
 _libs = {}
 
