@@ -183,9 +183,9 @@ template <int GATED, typename OutT> int few(const Product& p, cudaStream_t strea
 // adds up, scales and writes a share of the tokens.  Grid (tiles of 128 rows of W, K ranges, tiles of MT tokens), clusters (1, K ranges, 1).
 //   warp 0     TMA producer
 //   warp 1     allocates tensor memory; one elected thread issues the products and hands each stage back to the producer
-//   warps 2-5  bring the accumulator (a row of W a thread) into shared memory
+//   warps 2-9  bring the accumulator (a row of W a thread, every other 16 tokens) into shared memory, and the scales
 constexpr int BM = 128, BK = 128, UMMA_K = 32;
-constexpr int THREADS = 192;
+constexpr int MID_SETS = 2, THREADS = 64 + 128 * MID_SETS;    // drain warps: twice the four quarters of tensor memory
 constexpr int PART_LD = BM + 4;         // words per token of the partial tile (rows stay 16-byte aligned)
 
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -219,6 +219,7 @@ template <int MT, int STAGES, int MINB, int GATED, typename OutT>
 __global__ void __launch_bounds__(THREADS, MINB)
 mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Product p, int* __restrict__ status) {
     extern __shared__ unsigned char smem_raw[];
+    __shared__ float channel_scales[BM], token_scales[MT];
     constexpr int A_BYTES = BM * BK, B_BYTES = MT * BK, STAGE_BYTES = A_BYTES + B_BYTES;   // multiples of 1024
     constexpr uint32_t TMEM_COLS = MT < 32 ? 32 : MT;
     static_assert(MT == 16 || (MT % 32 == 0 && MT <= 256), "token tile: the N of an M = 128 product of 8-bit integers");
@@ -298,14 +299,19 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         if (elect_one()) tc_commit(bar_done);                                // accumulator complete (or abandoned)
         __syncwarp();
     } else {
-        // warps 2..5 own lanes 32 * (warp % 4) .. of tensor memory: accumulator -> part[token][row of W]
+        // warps own lanes 32 * (warp % 4) .. of tensor memory: accumulator -> part[token][row of W].  The scales are there before they are needed: fetched
+        // in the end they are the longest step of it.
+        const int t = threadIdx.x - 64;
+        if (t < BM) channel_scales[t] = n0 + t < p.N ? p.sw[n0 + t] : 0.0f;
+        pdl_wait();
+        if (t < MT) token_scales[t] = m0 + t < p.M ? p.sx[m0 + t] : 0.0f;
         const bool ok = mbar_wait(bar_done, 0);                              // every load has landed and been consumed,
         if (!ok && lane == 0) atomicExch(status, 3);                         // so the stages may be overwritten
         tc_fence_after();
         uint32_t* part = reinterpret_cast<uint32_t*>(smem_raw + (base - smem_u32(smem_raw)));
         const int lane_base = (warp & 3) * 32;
 #pragma unroll 1
-        for (int c = 0; c < MT; c += 16) {
+        for (int c = 16 * ((warp - 2) >> 2); c < MT; c += 16 * MID_SETS) {
             uint32_t r[16];
             if (ok && nkb > 0) {
                 tc_ld16(tmem_base + ((uint32_t)lane_base << 16) + (uint32_t)c, r);
@@ -344,15 +350,13 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
             const int local = (idx / GROUPS) * (int)ranks + (int)rank, g = idx % GROUPS;
             const int m = m0 + local;
             if (m >= p.M) continue;
-            const float sx = p.sx[m];
+            const float sx = token_scales[local];
             if constexpr (GATED == 0) {
                 const int n = n0 + 4 * g;
                 if (n >= p.N) continue;
                 const int4 sum = sum4(base + (uint32_t)(local * PART_LD + 4 * g) * 4u);
-                float v[4] = {scaled(sum.x, sx, p.sw[n]), 0.0f, 0.0f, 0.0f};
-                if (n + 1 < p.N) v[1] = scaled(sum.y, sx, p.sw[n + 1]);
-                if (n + 2 < p.N) v[2] = scaled(sum.z, sx, p.sw[n + 2]);
-                if (n + 3 < p.N) v[3] = scaled(sum.w, sx, p.sw[n + 3]);
+                const float* sw = channel_scales + 4 * g;
+                const float v[4] = {scaled(sum.x, sx, sw[0]), scaled(sum.y, sx, sw[1]), scaled(sum.z, sx, sw[2]), scaled(sum.w, sx, sw[3])};
                 store4<OutT>(Y + (int64_t)m * p.N + n, v, whole, p.N - n);
             } else {
                 // rows 16t + 4h .. + 3 are gates, rows 16t + 8 + 4h .. + 3 the ups of features 8t + 4h .. + 3
@@ -360,7 +364,7 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 if (n >= p.N) continue;
                 const uint32_t addr = base + (uint32_t)(local * PART_LD + 16 * t + 4 * h) * 4u;
                 const int4 gs = sum4(addr), us = sum4(addr + 32u);
-                const float* sw = p.sw + n;
+                const float* sw = channel_scales + 16 * t + 4 * h;
                 const float v[4] = {activated<GATED, OutT>(scaled(gs.x, sx, sw[0])) * scaled(us.x, sx, sw[8]),
                                     activated<GATED, OutT>(scaled(gs.y, sx, sw[1])) * scaled(us.y, sx, sw[9]),
                                     activated<GATED, OutT>(scaled(gs.z, sx, sw[2])) * scaled(us.z, sx, sw[10]),
