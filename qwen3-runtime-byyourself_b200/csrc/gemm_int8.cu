@@ -645,10 +645,40 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
     }
 }
 
+// Tokens of a tile, stages and blocks an SM: more blocks with shorter rings where two an SM do not hold all.
+#define Q3_BY_TILE(M, N, SPLITS, CALL)                                                            \
+    do {                                                                                          \
+        const bool more = (int64_t)(((N) + BM - 1) / BM) * (SPLITS) > 2 * q3_device_sm_count();   \
+        if ((M) <= 16) { if (more) CALL(16, 4, 3); CALL(16, 5, 2); }                              \
+        if ((M) <= 32) { if (more) CALL(32, 3, 3); CALL(32, 5, 2); }                              \
+        if ((M) <= 64) { if (more) CALL(64, 3, 3); CALL(64, 4, 2); }                              \
+        if ((M) <= 128) { if (more) CALL(128, 2, 3); CALL(128, 3, 2); }                           \
+        CALL(256, 4, 1);                                                                          \
+    } while (0)
+
+constexpr int mid_shared(int tile, int stages) {
+    const int ring = stages * (BM * BK + tile * BK), part = (tile * PART_LD * 4 + 1023) / 1024 * 1024;
+    return (ring > part ? ring : part) + 1024 + 256;
+}
+
+template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid(const Product& p, int splits, int* status, cudaStream_t stream) {
+    constexpr int SMEM = mid_shared(MT, STAGES);
+    static Q3PerDevice configured;
+    const cudaError_t e = q3_allow_shared_memory(mid_kernel<MT, STAGES, MINB, GATED, OutT>, SMEM, configured);
+    if (e != cudaSuccess) return (int)e;
+    CUtensorMap map_w, map_x;
+    if (!q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM) || !q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, MT)) return Q3_ERR_BAD_SIZE;
+    const int64_t token_tiles = (p.M + MT - 1) / MT;
+    if (token_tiles > 65535) return Q3_ERR_TOO_LARGE;
+    return (int)q3_launch_cluster(mid_kernel<MT, STAGES, MINB, GATED, OutT>, dim3((p.N + BM - 1) / BM, splits, (unsigned)token_tiles), dim3(THREADS),
+                                  (size_t)SMEM, stream, dim3(1, splits, 1), map_w, map_x, p, status);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Which form takes a product, in how many K ranges or tokens a tile: the one whose estimate is least.  Microseconds of a launch among others, W from
-// memory.  The constants are fitted to 5,500 times of 700 products of 1 to 8,000 tokens, 64 to 25,600 channels and widths, plain and gated; what they
-// choose is 3 % slower than the best of a product in the mean, 12 % for one in ten.
+// memory, but for a constant that all have.  The other constants are fitted so that what they choose of 7,900 times of 1,000 products (1 to 8,000 tokens, 64
+// to 25,600 channels and widths, plain and gated) is near the best of each product: 1.9 % slower in the mean, 7 % or more for one in ten (2.1 and 8 %
+// for 700 other products).
 inline int cuts(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Steps of 64 a warp, as many blocks as run at once (see `few`); where a wave is not full what a step costs is latency.
@@ -657,26 +687,29 @@ float few_us(int M, int N, int K) {
     const bool once = rows <= 2 * sms;
     const int warps = tiles < 4 && once ? 16 : 8, slots = tiles == 4 || once ? 2 : tiles == 2 || (rows <= 3 * sms && K >= 8192) ? 3 : 4;
     const float waves = (float)((int64_t)rows * cuts(M, 8 * tiles)) / (float)(slots * sms);
-    const float step = 0.28f + 0.37f * fminf(waves, 1.0f) * (float)(warps * slots) / 32.0f * (1.0f + 0.285f * (float)tiles);
-    return 1.14f + fmaxf(waves, 1.0f) * (0.38f * (float)tiles + 0.95f * (float)cuts(cuts(K, 64), warps) * step);
+    const float step = 0.273f + fminf(waves, 1.0f) * (float)(warps * slots) / 32.0f * (tiles == 1 ? 0.146f : tiles == 2 ? 0.47f : 0.82f);
+    return -0.53f + fmaxf(waves, 1.0f) * (0.35f * (float)tiles + (float)cuts(cuts(K, 64), warps) * step);
 }
-// Steps of 128 a block: latency, or the bytes of the blocks that share an SM.  Then the tile's way through shared memory and out.
+// Steps of 128 a block: latency, or the bytes of the blocks that share an SM.  Then the tile's way through shared memory and out.  Not all places are
+// taken by clusters: the SMs come in groups, and a group whose places are no multiple of a cluster leaves some empty.
 float mid_us(int M, int N, int K, int splits) {
-    const int sms = q3_device_sm_count(), tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    const int64_t blocks = (int64_t)cuts(N, BM) * splits * cuts(M, tile);
-    const int slots = tile == 256 ? 1 : (int64_t)cuts(N, BM) * splits > 2 * sms ? 3 : 2, waves = cuts(blocks, slots * sms);
-    const float shared = waves == 1 ? (float)blocks / (float)sms : (float)slots, t = (float)tile / 64.0f;
-    const float step = fmaxf(0.237f + 0.063f * t, shared * (16.0f + 8.0f * t) * 0.0171f);
-    const float around = 1.24f * t + 0.8f * shared + (splits > 1 ? 0.4f : 0.0f);
-    return 2.2f + (float)waves * ((float)cuts(cuts(K, BK), splits) * step + around);
+    const int sms = q3_device_sm_count(), tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256, rows = cuts(N, BM);
+    const int tokens = cuts(M, tile), an_sm = tile == 256 ? 1 : (int64_t)rows * splits > 2 * sms ? 3 : 2;
+    const float taken = splits <= 2 ? 1.0f : tile == 256 ? (splits == 3 ? 0.91f : splits <= 6 ? 0.89f : 0.81f) : splits <= 4 ? 0.96f : 0.89f;
+    const int64_t blocks = (int64_t)rows * splits * tokens;
+    const int slots = (int)((float)(an_sm * sms) * taken), waves = cuts(blocks, slots);
+    const float shared = (float)(waves == 1 ? (int)blocks : slots) / (float)sms, t = (float)tile / 64.0f;
+    const float step = fmaxf(0.214f + 0.03f * t, shared * (16.0f + 8.0f * t) * 0.0085f);
+    const float around = 1.34f * t + 1.21f * shared + (splits > 1 ? 0.08f : 0.0f);
+    return 0.24f + fmaxf((float)waves * ((float)cuts(cuts(K, BK), splits) * step + around), (float)N * (float)K * (float)tokens / 14e6f);
 }
 // Steps of 128 a pair: the products, the copies of few tokens, or what the L2 gives all pairs; a tile's drain under the next one's steps, but for the last.
 float pair_us(int M, int N, int K, int tile) {
     const int pairs = q3_device_sm_count() / 2;
     const int64_t tiles = (int64_t)cuts(M, tile) * cuts(N, 256);
     const float t = (float)tile / 256.0f, full = fminf((float)tiles / (float)pairs, 1.0f);
-    const float step = fmaxf(fmaxf(0.223f, 0.362f * t), 0.15f * full * (t + 1.0f)), drain = 1.77f + 1.63f * t;
-    return 1.05f * (0.75f + (float)cuts(tiles, pairs) * fmaxf((float)cuts(K, BK) * step, drain) + drain);
+    const float step = fmaxf(fmaxf(0.1835f, 0.335f * t), 0.1525f * full * (t + 1.0f)), drain = 1.23f + 0.77f * t;
+    return 0.03f * t + (float)cuts(tiles, pairs) * fmaxf((float)cuts(K, BK) * step, drain) + drain;
 }
 
 struct Choice {
@@ -703,31 +736,12 @@ Choice pair_choice(int M, int N, int K) {
     return best;
 }
 
-template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid(const Product& p, int splits, int* status, cudaStream_t stream) {
-    constexpr int RING = STAGES * (BM * BK + MT * BK), PART = (MT * PART_LD * 4 + 1023) / 1024 * 1024;
-    constexpr int SMEM = (RING > PART ? RING : PART) + 1024 + 256;
-    static Q3PerDevice configured;
-    const cudaError_t e = q3_allow_shared_memory(mid_kernel<MT, STAGES, MINB, GATED, OutT>, SMEM, configured);
-    if (e != cudaSuccess) return (int)e;
-    CUtensorMap map_w, map_x;
-    if (!q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM) || !q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, MT)) return Q3_ERR_BAD_SIZE;
-    const int64_t token_tiles = (p.M + MT - 1) / MT;
-    if (token_tiles > 65535) return Q3_ERR_TOO_LARGE;
-    return (int)q3_launch_cluster(mid_kernel<MT, STAGES, MINB, GATED, OutT>, dim3((p.N + BM - 1) / BM, splits, (unsigned)token_tiles), dim3(THREADS),
-                                  (size_t)SMEM, stream, dim3(1, splits, 1), map_w, map_x, p, status);
-}
-
 template <int GATED, typename OutT> int mid(const Product& p, int splits, int* status, cudaStream_t stream) {
     const int nkb = (p.K + BK - 1) / BK;
     if (splits == 0) splits = mid_choice(p.M, p.N, p.K).splits;
     if (splits > nkb) splits = nkb;
-    const bool waves = (int64_t)((p.N + BM - 1) / BM) * splits > 2 * q3_device_sm_count();
 #define Q3_MID(MT, ST, MB) return launch_mid<MT, ST, MB, GATED, OutT>(p, splits, status, stream)
-    if (p.M <= 16) { if (waves) Q3_MID(16, 4, 3); Q3_MID(16, 5, 2); }
-    if (p.M <= 32) { if (waves) Q3_MID(32, 3, 3); Q3_MID(32, 5, 2); }
-    if (p.M <= 64) { if (waves) Q3_MID(64, 3, 3); Q3_MID(64, 4, 2); }
-    if (p.M <= 128) { if (waves) Q3_MID(128, 2, 3); Q3_MID(128, 3, 2); }
-    Q3_MID(256, 4, 1);
+    Q3_BY_TILE(p.M, p.N, splits, Q3_MID);
 #undef Q3_MID
 }
 

@@ -13,10 +13,12 @@
 // becomes NaN.  A row of zeros gets the scale zero.  Scales below 2^-126 have fewer bits.
 //
 // Bound by memory: a row is read once, in packets of 16 bytes, held in registers across the reduction, and written (8,000 rows, of the measured copy
-// rate: quantise 12,288 bfloat16 52.6 us, 0.86; 5,120 float32 36.2, 0.86; norm and sum 5,120 bfloat16 53.3, 0.82; 4,096 float32 65, 1.0).  Rows that do
-// not begin at such a boundary (an odd width, a slice) are read in the packets around them, each thread shifting two into its own values: 5,001
-// bfloat16 25.9 and 84.9 us where 5,120 takes 22.8 and 53.3.  Tried and slower: rows brought several ahead by bulk copies into a ring in shared
-// memory of blocks that stay (norm 5,120 126 us: barriers and a second pass over shared memory a row), 40 registers a thread for a third block (61.7).
+// rate: quantise 12,288 bfloat16 48.3 us, 0.93; 5,120 float32 35.0, 0.89; norm and sum 5,120 bfloat16 50.9, 0.86; 5,120 float32 78.5, 1.0).  What a value
+// costs in instructions comes next (seven in ten issue slots were taken where these times were 55 and 57): three-way maxima of packed halves, no
+// fallbacks compiled into rows that need none and one rounding less took 8 and 5 %.  Rows that do not begin at a packet's boundary (an odd width, a
+// slice) are read in the packets around them, each thread shifting two into its own values: 5,001 bfloat16 24.3 and 77 us where 5,120 takes 20.8
+// and 50.9.  Tried and slower: rows brought several ahead by bulk copies into a ring in shared memory of blocks that stay (norm 5,120 126 us: barriers and
+// a second pass over shared memory a row), 40 registers a thread for a third block (61.7), loads that are evicted first (1 to 2 %).
 #include "common.cuh"
 #include "../include/qwen3/int8_args.h"
 
@@ -68,17 +70,14 @@ template <int N> __device__ __forceinline__ void codes_of(const float (&u)[N], c
     }
 }
 
-// The same for values of eight bits (bfloat16): a ratio 127 x / a of two such numbers that is no tie is at least 1 / (2 * 254 * 255) from one near 1/2, and
-// 2^n times as far near 2^n / 2, so rounding its magnitude to a multiple of 2^-17 (2^-16 beyond 32), as adding 96 to it does, moves no ratio onto a tie or
-// over it, and brings a tie that 127 / a's rounding has moved (by up to 2^-24 of itself) back onto it.
+// The same for values of eight bits (bfloat16).  A ratio 127 x / a of two such numbers that is no tie is at least 1 / (256 * 253) from one at 1/2 and further
+// from the others (every pair is in the tests), so rounding it to a multiple of 2^-15, as adding 384 does on either side of zero, moves no ratio onto a
+// tie or over it, and brings a tie that the rounding of 127 / a has moved (by up to 2^-24 of itself) back onto it.
 template <int N> __device__ __forceinline__ void codes_of_bf16(const float (&u)[N], const Grid& g, uint32_t (&out)[N / 4]) {
     if (g.divide) return codes_of<N>(u, g, out);
     uint32_t f[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float side = __uint_as_float((__float_as_uint(u[i]) & 0x80000000u) | 0x42c00000u);       // 96 on the value's side of zero
-        f[i] = __float_as_uint((__fmaf_rn(u[i], g.ratio, side) - side) + 12582912.0f);
-    }
+    for (int i = 0; i < N; ++i) f[i] = __float_as_uint(__fmaf_rn(u[i], g.ratio, 384.0f) + (12582912.0f - 384.0f));
 #pragma unroll
     for (int w = 0; w < N / 4; ++w) {
         const uint32_t all = __byte_perm(__byte_perm(f[4 * w], f[4 * w + 1], 0x0040), __byte_perm(f[4 * w + 2], f[4 * w + 3], 0x0040), 0x5410);
@@ -87,8 +86,8 @@ template <int N> __device__ __forceinline__ void codes_of_bf16(const float (&u)[
 }
 
 // `n` codes (of N) to a place that is a multiple of N bytes from the row's beginning.
-template <int N> __device__ __forceinline__ void store_codes(int8_t* to, const uint32_t (&w)[N / 4], int n) {
-    if (n >= N) {
+template <int N, bool WHOLE> __device__ __forceinline__ void store_codes(int8_t* to, const uint32_t (&w)[N / 4], int n) {
+    if (WHOLE || n >= N) {
         if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(to) = w[0];
         return;
@@ -153,31 +152,25 @@ template <typename T, bool APART> struct Packet {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
-__device__ __forceinline__ void load_weights(const float* w, int c, int width, bool whole, float (&v)[8]) {
+// The norm's weights of values c .. (`whole`: all are there, at a 16-byte boundary).
+template <int N> __device__ __forceinline__ void load_weights(const float* w, int c, int width, bool whole, float (&v)[N]) {
     if (whole) {
-        const float4 a = *reinterpret_cast<const float4*>(w + c), b = *reinterpret_cast<const float4*>(w + c + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(w + c + i);
+            v[i] = a.x; v[i + 1] = a.y; v[i + 2] = a.z; v[i + 3] = a.w;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < width ? w[c + i] : 0.0f;
-    }
-}
-__device__ __forceinline__ void load_weights(const float* w, int c, int width, bool whole, float (&v)[4]) {
-    if (whole) {
-        const float4 a = *reinterpret_cast<const float4*>(w + c);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = c + i < width ? w[c + i] : 0.0f;
+        for (int i = 0; i < N; ++i) v[i] = c + i < width ? w[c + i] : 0.0f;
     }
 }
 
 // The largest magnitude as bits: an infinity's or NaN's are above every finite number's.
 template <typename T> __device__ __forceinline__ uint32_t top_of(const uint4& raw, uint32_t top) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = sizeof(T) == 2 ? __vmaxu2(top, w[i] & 0x7fff7fffu) : max(top, w[i] & 0x7fffffffu);
-    return top;
+    constexpr uint32_t M = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+    if constexpr (sizeof(T) == 2) return __vimax3_u16x2(__vimax3_u16x2(top, raw.x & M, raw.y & M), raw.z & M, raw.w & M);
+    else return __vimax3_u32(__vimax3_u32(top, raw.x & M, raw.y & M), raw.z & M, raw.w & M);
 }
 // (of two 16-bit halves the larger one, as 32 bits)
 template <typename T> __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
@@ -269,8 +262,9 @@ template <typename T> __device__ __forceinline__ uint4 sum_of(const uint4& x, co
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A row a block, or (WARP) a row a warp; a thread holds PER packets, as they are stored (a norm's products with the weights are made twice, which takes
-// fewer registers than holding them in 32 bits).
+// A row a block, or (WARP) a row a warp; a thread holds PER packets.  Of a norm it holds the products with the weights, or (rows of bfloat16 at packet
+// boundaries) the sums as they are stored, in half the registers, and makes the products twice (the other way round / so: 8,000 rows of 5,120
+// bfloat16 51.9 / 50.8 us, of 5,001 77.0 / 84.8, of 4,097 float32 103.8 / 111.6).
 template <typename T, int PER, bool NORM, bool APART, bool WARP, int MOST_THREADS>
 __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) rows_kernel(const Rows a) {
     constexpr int N = Pack<T>::N;
@@ -284,7 +278,9 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
     Packet<T, APART> from_x[PER];
 #pragma unroll
     for (int p = 0; p < PER; ++p) from_x[p].fetch(x, (p * threads + thread) * N, a.width);
+    constexpr bool HOLD = NORM && (APART || sizeof(T) == 4);
     uint4 raw[PER];
+    float held[HOLD ? PER : 1][N];
     if (NORM && a.delta != nullptr) {
         const T* delta = (const T*)a.delta + row * a.delta_stride;
         T* total = (T*)a.total + row * a.total_stride;
@@ -307,7 +303,7 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
         unpack<T>(raw[p], u);
         if constexpr (NORM) {
             float w[N];
-            load_weights(a.weight, c, a.width, whole_weights && c + N <= a.width, w);
+            load_weights<N>(a.weight, c, a.width, !APART || (whole_weights && c + N <= a.width), w);
 #pragma unroll
             for (int i = 0; i < N; ++i) u[i] *= w[i];
         }
@@ -321,10 +317,15 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
             float t[N], u[N];
             unpack<T>(raw[p], t);
             weighted(p, c, u);
+            if constexpr (HOLD) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+                for (int i = 0; i < N; ++i) held[p][i] = u[i];
+            }
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
                 squares += t[i] * t[i];
-                top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
+                squares += t[i + 1] * t[i + 1];
+                top = __vimax3_u32(top, __float_as_uint(u[i]) & 0x7fffffffu, __float_as_uint(u[i + 1]) & 0x7fffffffu);
             }
         }
     }
@@ -340,10 +341,15 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
         if (c >= a.width) continue;
         uint32_t w[N / 4];
         float u[N];
-        weighted(p, c, u);
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] = held[p][i];
+        } else {
+            weighted(p, c, u);
+        }
         if constexpr (sizeof(T) == 2 && !NORM) codes_of_bf16<N>(u, g, w);
         else codes_of<N>(u, g, w);
-        store_codes<N>(codes + c, w, a.width - c);
+        store_codes<N, !APART>(codes + c, w, a.width - c);
     }
 }
 
@@ -383,7 +389,7 @@ template <typename T, bool NORM> __global__ void __launch_bounds__(1024) long_ro
         values(c, true);                                       // (the sum is stored now: `total` may be x)
         uint32_t w[1];
         codes_of<4>(u, g, w);
-        store_codes<4>(a.codes + row * a.codes_stride + c, w, a.width - c);
+        store_codes<4, false>(a.codes + row * a.codes_stride + c, w, a.width - c);
     }
 }
 
@@ -403,8 +409,8 @@ template <typename T, bool NORM, bool APART> int pick(const Rows& a, cudaStream_
     // short rows, if they are many: a row a warp
     const bool warp = a.rows >= 2 * sms && packets <= 32 * MOST;
     // As few packets a thread as the SMs can hold threads for at once: few rows want threads, many want loads in flight while other rows of the SM are
-    // reduced.  (8,000 rows of 4,096, bfloat16, 4 / 2 / 1 packets a thread: norm 42.8 / 47.9 / 66 us, quantise 17.7 / 21.7 / 29.3; 527 rows 6.6 / 4.7 / 5.5
-    // and 3.2 / 2.6 / 2.7.  float32 8 / 4: quantise 8,000 rows of 5,120 36.2 / 41.4, of 4,097 49.5 / 43.0, norm 100 / 81.)
+    // reduced.  (8,000 rows of 4,096, bfloat16, 4 / 2 / 1 packets a thread, when it was measured: norm 42.8 / 47.9 / 66 us, quantise 17.7 / 21.7 / 29.3; 527 rows
+    // 6.6 / 4.7 / 5.5 and 3.2 / 2.6 / 2.7.  float32 8 / 4: quantise 8,000 rows of 5,120 36.2 / 41.4, of 4,097 49.5 / 43.0, norm 100 / 81.)
     int per = 1;
     if (warp) {
         while (32 * per < packets) per *= 2;
@@ -423,13 +429,13 @@ template <typename T, bool NORM, bool APART> int pick(const Rows& a, cudaStream_
 template <typename T, bool NORM> int rows_launch(const q3_int8_rows_args& in) {
     constexpr int V = Pack<T>::N;
     if (in.rows <= 0 || in.width <= 0) return in.rows < 0 || in.width < 0 ? Q3_ERR_BAD_SIZE : 0;
-    if (in.rows > 0x7fffffff) return Q3_ERR_TOO_LARGE;
+    if (in.rows > 0x7fffffff || in.width > 1 << 30) return Q3_ERR_TOO_LARGE;
     if (in.codes_stride < in.width || in.x == nullptr || (NORM && (in.weight == nullptr || (in.delta != nullptr && in.total == nullptr))))
         return Q3_ERR_BAD_SIZE;
     if (in.codes_stride % 16 != 0 || !aligned16(in.codes)) return Q3_ERR_MISALIGNED;
     const Rows a{in.x, NORM ? in.delta : nullptr, NORM ? (const float*)in.weight : nullptr, NORM ? in.total : nullptr, (int8_t*)in.codes,
                  (float*)in.scales, in.rows, in.x_stride, in.delta_stride, in.total_stride, in.codes_stride, in.width, (float)in.eps};
-    const bool packets = in.width % V == 0 && in.x_stride % V == 0 && aligned16(in.x) &&
+    const bool packets = in.width % V == 0 && in.x_stride % V == 0 && aligned16(in.x) && aligned16(a.weight) &&
                          (a.delta == nullptr || (in.delta_stride % V == 0 && in.total_stride % V == 0 && aligned16(in.delta) && aligned16(in.total)));
     return packets ? pick<T, NORM, false>(a, (cudaStream_t)in.stream) : pick<T, NORM, true>(a, (cudaStream_t)in.stream);
 }
