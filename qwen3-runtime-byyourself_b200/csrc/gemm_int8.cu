@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) few_kernel(const Product p) 
             }
         }
     };
+    pdl_wait();                          // (for W, too: the caller may just have quantised it)
 #pragma unroll
     for (int s = 0; s < PF; ++s) load_w(s, kb_begin + s);
-    pdl_wait();
 #pragma unroll
     for (int s = 0; s < PF; ++s) load_x(s, kb_begin + s);
     for (int kb = kb_begin; kb < kb_end; kb += PF) {
@@ -262,6 +262,7 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
 
     if (warp == 0) {
         if (lane == 0) {
+            pdl_wait();              // (for W, too: the caller may just have quantised it; asking for it earlier gained nothing to 4 %)
             for (int i = 0; i < nkb; ++i) {
                 const int s = i % STAGES;
                 if (!mbar_wait(bars + (STAGES + s) * 8, ((uint32_t)(i / STAGES) & 1u) ^ 1u)) {      // the stage is free
@@ -270,8 +271,7 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 }
                 const uint32_t a = base + s * STAGE_BYTES, b = a + A_BYTES;
                 mbar_expect_tx(bars + s * 8, STAGE_BYTES);
-                tma_load_2d(a, &map_w, bars + s * 8, (kb_begin + i) * BK, n0);      // weights: independent of the
-                if (i == 0) pdl_wait();                                              // kernel before; X is not
+                tma_load_2d(a, &map_w, bars + s * 8, (kb_begin + i) * BK, n0);
                 tma_load_2d(b, &map_x, bars + s * 8, (kb_begin + i) * BK, m0);
             }
         }
@@ -302,8 +302,8 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
         // warps own lanes 32 * (warp % 4) .. of tensor memory: accumulator -> part[token][row of W].  The scales are there before they are needed: fetched
         // in the end they are the longest step of it.
         const int t = threadIdx.x - 64;
-        if (t < BM) channel_scales[t] = n0 + t < p.N ? p.sw[n0 + t] : 0.0f;
         pdl_wait();
+        if (t < BM) channel_scales[t] = n0 + t < p.N ? p.sw[n0 + t] : 0.0f;
         if (t < MT) token_scales[t] = m0 + t < p.M ? p.sx[m0 + t] : 0.0f;
         const bool ok = mbar_wait(bar_done, 0);                              // every load has landed and been consumed,
         if (!ok && lane == 0) atomicExch(status, 3);                         // so the stages may be overwritten

@@ -177,3 +177,24 @@ def test_refusals():
     a, b = ops.Int8Rows.empty(1, ops.INT8_MAX_WIDTH + 1, "cuda"), ops.Int8Rows.empty(4, ops.INT8_MAX_WIDTH + 1, "cuda")
     with pytest.raises(ops.KernelError):
         ops.gemm_int8(a, b, torch.zeros(1, 4, device="cuda"))
+
+
+@pytest.mark.parametrize("M", [1, 16, 64, 200, 700])
+def test_weights_that_were_written_just_before(M):
+    """Quantised one launch before the product, over and over into the same memory: a product that starts before the kernel ahead of it has ended
+    may not read its weights until then."""
+    from qwen3_b200.csrc import ops
+    N, K = 2048, 1000
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = operands(M, N, K, M)[0]
+    matrices = [torch.randn(N, K, generator=g, device="cuda") for _ in range(3)]
+    settled = [ops.quantize_rows(m, ops.Int8Rows.empty(N, K, "cuda")) for m in matrices]
+    torch.cuda.synchronize()
+    want = [ops.gemm_int8(x, w, torch.zeros(M, N, device="cuda")) for w in settled]
+    w, outs = ops.Int8Rows.empty(N, K, "cuda"), [torch.zeros(M, N, device="cuda") for _ in range(30)]
+    torch.cuda.synchronize()
+    for i, y in enumerate(outs):
+        ops.quantize_rows(matrices[i % 3], w)
+        ops.gemm_int8(x, w, y)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(outs))
