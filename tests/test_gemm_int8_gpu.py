@@ -198,3 +198,22 @@ def test_weights_that_were_written_just_before(M):
         ops.gemm_int8(x, w, y)
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(outs))
+
+
+@pytest.mark.parametrize("form", ["few", "mid", "pair"])
+def test_offsets_beyond_32_bits(form):
+    """Codes of 2.2 GB, and 2.3 billion outputs: the last rows are those of the rows alone."""
+    from qwen3_b200.csrc import ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for M, N, K in ((270000, 16, 8192), (143000, 16400, 64)):
+        x, w = ops.Int8Rows.empty(M, K, "cuda"), ops.Int8Rows.empty(N, K, "cuda")
+        x.codes.random_(-127, 128, generator=g), w.codes.random_(-127, 128, generator=g)
+        x.scales.fill_(0.01), w.scales.fill_(0.02)
+        y = ops.gemm_int8(x, w, torch.zeros(M, N, dtype=torch.bfloat16, device="cuda"), form=form)
+        assert ops.tcgen05_status("cuda") == 0
+        for first in (0, M // 2, M - 40):
+            some = ops.Int8Rows(x.codes[first:first + 40], x.scales[first:first + 40])
+            assert torch.equal(ops.gemm_int8(some, w, torch.zeros(40, N, dtype=torch.bfloat16, device="cuda")), y[first:first + 40])
+            check(some, w, y[first:first + 40], "bf16", None)
+        del x, w, y
+        torch.cuda.empty_cache()

@@ -188,3 +188,23 @@ def test_every_pair_of_bfloat16_magnitudes():
         out, memory = rows_for(*x.shape)
         ops.quantize_rows(x, out)
         same_rows(out, memory, x.double(), 2.0 ** -24)
+
+
+@pytest.mark.parametrize("width", [8192, 8191])
+def test_offsets_beyond_32_bits(width):
+    """2.2 billion values: the last rows as by themselves."""
+    from qwen3_b200.csrc import ops
+    rows = 270000
+    x = torch.randn(1000, width, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(torch.bfloat16).repeat(rows // 1000, 1)
+    w, out = torch.rand(width, device="cuda") + 0.5, ops.Int8Rows.empty(rows, width, "cuda")
+    ops.quantize_rows(x, out)
+    codes, scales = ic.quantised(x[:1000])
+    for first in (0, 135000, 269000):
+        assert torch.equal(out.codes[first:first + 1000].long(), codes)
+    ops.rms_norm_int8(x, w, 1e-6, out, delta=x, total=x)
+    stored = (2 * x[:1000].float() / 2).to(torch.bfloat16)           # (x was doubled, which rounds nothing)
+    codes = ic.quantised(ic.normed(stored, w))[0]
+    for first in (0, 135000, 269000):
+        assert torch.equal(x[first:first + 1000], stored) and torch.equal(out.codes[first:first + 1000].long(), codes)
+    del x, out
+    torch.cuda.empty_cache()
