@@ -204,7 +204,7 @@ template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint3
         mean = squares / (float)a.width;
         fine = fine && mean < INFINITY;
     }
-    scale = !fine ? __uint_as_float(0x7fffffffu) : NORM ? top * rsqrtf(mean + a.eps) / 127.0f : top / 127.0f;
+    scale = !fine ? __uint_as_float(0x7fffffffu) : NORM && top != 0.0f ? top * rsqrtf(mean + a.eps) / 127.0f : top / 127.0f;
     Grid g;
     g.top = fine ? top : 0.0f;
     g.divide = g.top != 0.0f && top < 7.9e-31f;                // 2^-100

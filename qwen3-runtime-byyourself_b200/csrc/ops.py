@@ -1640,6 +1640,9 @@ class Int8Rows:
         if self.rows and end > codes.untyped_storage().nbytes():
             raise KernelError("int8 rows: the memory of the last row ends inside its last 16 bytes")
         self.codes, self.scales, self.at = codes, scales, codes.data_ptr()
+        if self.index not in _status_at and not torch.cuda.is_current_stream_capturing():
+            # the word that a product notes a wait in: made here, because one that is made inside a capture is zero only where the graph runs
+            _status_at[self.index] = _status_word(codes.device).data_ptr()
 
     @classmethod
     def empty(cls, rows: int, width: int, device) -> "Int8Rows":
@@ -1738,7 +1741,7 @@ def gemm_int8(x: Int8Rows, w: Int8Rows, out: torch.Tensor, activation: Optional[
         raise KernelError(f"gemm_int8: form {form!r}: one of {sorted(_INT8_FORMS)}")
     status = _status_at.get(index)
     if status is None:
-        status = _status_at[index] = _status_word(torch.device("cuda", index)).data_ptr()
+        raise KernelError("gemm_int8: operands that were all made inside a capture, in a process without any others")
     _call_packed("gemm_int8", "gemm_int8.cu", name, _GEMM8_ARGS.pack(
         x.at, x.scales_at, w.at, w.scales_at, out.data_ptr(), status, _stream_on(index, "gemm_int8"), x.stride, w.stride, M, N, K,
         1 if dtype is _F32 else 0, 0 if activation is None else ACTIVATIONS[activation] + 1, splits))

@@ -217,3 +217,44 @@ def test_offsets_beyond_32_bits(form):
             check(some, w, y[first:first + 40], "bf16", None)
         del x, w, y
         torch.cuda.empty_cache()
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from qwen3_b200.csrc import ops
+x, w = torch.randn({M}, 200, device="cuda"), torch.randn(272, 200, device="cuda")
+x8, w8, y = ops.Int8Rows.empty({M}, 200, "cuda"), ops.Int8Rows.empty(272, 200, "cuda"), torch.zeros({M}, 272, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.quantize_rows(x, x8), ops.quantize_rows(w, w8)
+    ops.gemm_int8(x8, w8, y)
+assert ops.tcgen05_status("cuda") == 0
+graph.replay()
+torch.cuda.synchronize()
+want = ops.gemm_int8(x8, w8, torch.zeros({M}, 272, device="cuda"))
+assert torch.equal(y, want) and bool(y.any()) and ops.tcgen05_status("cuda") == 0
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("M", [3, 100, 700])
+def test_first_call_of_a_process_inside_a_capture(M):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root, M=M)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+def test_another_current_device_is_refused(monkeypatch):
+    from qwen3_b200.csrc import ops
+    x, w = operands(4, 32, 64, 1)
+    a = torch.zeros(4, 64, device="cuda")
+    y = torch.zeros(4, 32, device="cuda")
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 1)
+    for call in (lambda: ops.gemm_int8(x, w, y), lambda: ops.quantize_rows(a, x), lambda: ops.rms_norm_int8(a, a[0].contiguous(), 1e-6, x)):
+        with pytest.raises(ops.KernelError, match="current device"):
+            call()

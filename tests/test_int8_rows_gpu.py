@@ -208,3 +208,14 @@ def test_offsets_beyond_32_bits(width):
         assert torch.equal(x[first:first + 1000], stored) and torch.equal(out.codes[first:first + 1000].long(), codes)
     del x, out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,width", [(3, 64), (3, 65), (700, 65), (2, 40000)])
+def test_rows_of_zeros_without_an_epsilon(rows, width):
+    from qwen3_b200.csrc import ops
+    x = torch.zeros(rows, width, device="cuda")
+    x[0, 0] = 3.0
+    out, _ = rows_for(rows, width)
+    ops.rms_norm_int8(x, torch.ones(width, device="cuda"), 0.0, out)
+    assert int(out.codes[0, 0]) == 127 and abs(float(out.scales[0]) * 127 / width ** 0.5 - 1) < 1e-6
+    assert not bool(out.codes[1:].any()) and bool((out.scales[1:] == 0).all())
