@@ -35,6 +35,13 @@ def _role_dtype(role: str, compute: torch.dtype) -> torch.dtype:
     return {"matrix": compute, "norm": torch.float32, "bias": torch.float32, "int_table": torch.int32}[role]
 
 
+def _numel(shape) -> int:
+    numel = 1
+    for s in shape:
+        numel *= s
+    return numel
+
+
 def fuse_rows(weights, names: Sequence[str]) -> torch.Tensor:
     """One matrix whose rows are those of `names`, one tensor after the other."""
     rows = getattr(weights, "rows", None)
@@ -97,6 +104,10 @@ class CheckpointUpload:
             total += -(-numel * item // ALIGN) * ALIGN
         self.arena = torch.empty(total + ALIGN, dtype=torch.uint8, device=self.device)
         self._used = (-self.arena.data_ptr()) % ALIGN
+        if self.apart:
+            # What these will take in 8 bits, and some of them as they are read, from the device at once: the allocator cuts it up (each piece by itself
+            # would make the copies wait).
+            torch.empty(sum(_numel(specs[n].shape) for n in self.apart) * 9 // 8 + (1 << 28), dtype=torch.uint8, device=self.device)
         self._done: Dict[str, torch.Tensor] = {}
         self._side = torch.cuda.Stream(self.device)
         self._host = [torch.empty(STAGE_BYTES, dtype=torch.uint8).pin_memory() for _ in range(2)]
