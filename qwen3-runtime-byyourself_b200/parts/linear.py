@@ -110,7 +110,7 @@ def few_rows_weights_first(M: int, N: int, K: int) -> bool:
 
 def eight_bit_rows(ctx, name: str, rows: int, width: int) -> ops.Int8Rows:
     """Room for a step's rows in 8 bits, in the scratch buffers of this name."""
-    codes = ctx.scratch.get(name, (rows, -(-width // 16) * 16), torch.int8)
+    codes = ctx.scratch.get(name, (rows, -(-width // ops.INT8_ROW_BYTES) * ops.INT8_ROW_BYTES), torch.int8)
     return ops.Int8Rows(codes[:, :width], ctx.scratch.get(name + "_scales", (rows,), torch.float32))
 
 
