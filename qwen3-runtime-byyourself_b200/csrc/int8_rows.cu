@@ -13,9 +13,10 @@
 // becomes NaN.  A row of zeros gets the scale zero.  Scales below 2^-126 have fewer bits.
 //
 // Bound by memory: a row is read once, in packets of 16 bytes, held in registers across the reduction, and written (8,000 rows, of the measured copy
-// rate: quantise 12,288 bfloat16 48.3 us, 0.93; 5,120 float32 35.0, 0.89; norm and sum 5,120 bfloat16 50.9, 0.86; 5,120 float32 78.5, 1.0).  What a value
+// rate: quantise 12,288 bfloat16 47.2 us, 0.95; 10,240 of 5,120 float32 42.5, 0.94; norm and sum 5,120 bfloat16 50.9, 0.86; in long runs, at the clocks that
+// they settle at, 50.0, 48.2 and 56.1).  What a value
 // costs in instructions comes next (seven in ten issue slots were taken where these times were 55 and 57): three-way maxima of packed halves, no
-// fallbacks compiled into rows that need none and one rounding less took 8 and 5 %.  Rows that do not begin at a packet's boundary (an odd width, a
+// fallbacks compiled into rows that need none, one rounding less and the scale's divisions in one thread took 10 and 6 %.  Rows that do not begin at a packet's boundary (an odd width, a
 // slice) are read in the packets around them, each thread shifting two into its own values: 5,001 bfloat16 24.3 and 77 us where 5,120 takes 20.8
 // and 50.9.  Tried and slower: rows brought several ahead by bulk copies into a ring in shared memory of blocks that stay (norm 5,120 126 us: barriers and
 // a second pass over shared memory a row), 40 registers a thread for a third block (61.7), loads that are evicted first (1 to 2 %).
@@ -110,6 +111,13 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, f
     }
 }
 
+// Where value c of a row lies; of 32-bit rows by a 32-bit offset from the row (in a row, with / without: 10,240 rows of 5,120 float32 quantised 47.4 / 49.5
+// us, normed 101 / 103.5; bfloat16 rows normed 56.7 / 54).
+template <typename T> __device__ __forceinline__ T* value_at(T* row, int c) {
+    if constexpr (sizeof(T) == 4) return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(row) + (uint32_t)(c * 4));
+    else return row + c;
+}
+
 // The packets of a row's values c .., zeros behind its end.  APART: rows may begin anywhere, and a packet of values lies in two packets of memory.  The
 // first is asked for early (`fetch`) and held; the second is the next thread's first and is read when the two are shifted together (`whole`), from
 // the L1 then.  Both have to lie inside the row, else the values are fetched one by one.
@@ -118,7 +126,7 @@ template <typename T, bool APART> struct Packet {
     uint4 a;
     __device__ __forceinline__ void fetch(const T* row, int c, int width) {
         if constexpr (!APART) {
-            a = c < width ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
+            a = c < width ? *reinterpret_cast<const uint4*>(value_at(row, c)) : make_uint4(0u, 0u, 0u, 0u);
         } else if (inside(c, width)) {
             a = *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(row + c) & ~(uintptr_t)15);
         }
@@ -157,7 +165,7 @@ template <int N> __device__ __forceinline__ void load_weights(const float* w, in
     if (whole) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(w + c + i);
+            const float4 a = *reinterpret_cast<const float4*>(N == 4 ? value_at(w, c) : w + c + i);        // (N 4: rows of 32 bits)
             v[i] = a.x; v[i + 1] = a.y; v[i + 2] = a.z; v[i + 3] = a.w;
         }
     } else {
@@ -196,15 +204,13 @@ template <bool WARP, bool NORM> __device__ __forceinline__ void reduce(uint32_t&
     }
 }
 
-template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint32_t bits, float squares, float& scale) {
+// What the codes are made with; the row's first thread writes the scale, whose root and divisions the others do without.
+template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, int64_t row, bool first, uint32_t bits, float squares) {
     const float top = __uint_as_float(bits);
-    float mean = 0.0f;
     bool fine = bits < 0x7f800000u;
-    if constexpr (NORM) {
-        mean = squares / (float)a.width;
-        fine = fine && mean < INFINITY;
-    }
-    scale = !fine ? __uint_as_float(0x7fffffffu) : NORM && top != 0.0f ? top * rsqrtf(mean + a.eps) / 127.0f : top / 127.0f;
+    if constexpr (NORM) fine = fine && squares < INFINITY;
+    if (first)
+        a.scales[row] = !fine ? __uint_as_float(0x7fffffffu) : NORM && top != 0.0f ? top * rsqrtf(squares / (float)a.width + a.eps) / 127.0f : top / 127.0f;
     Grid g;
     g.top = fine ? top : 0.0f;
     g.divide = g.top != 0.0f && top < 7.9e-31f;                // 2^-100
@@ -219,7 +225,7 @@ template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, uint3
 template <typename T, bool APART> __device__ __forceinline__ void store_total(T* row, int c, int width, const uint4& k) {
     constexpr int N = Pack<T>::N;
     if constexpr (!APART) {
-        if (c < width) *reinterpret_cast<uint4*>(row + c) = k;
+        if (c < width) *reinterpret_cast<uint4*>(value_at(row, c)) = k;
     } else {
         extern __shared__ __align__(16) unsigned char staged[];
         const int lane = threadIdx.x & 31, first = c - lane * N;
@@ -331,9 +337,7 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
     }
     if (!NORM) top = top_bits<T>(top);
     reduce<WARP, NORM>(top, squares);
-    float scale;
-    const Grid g = finish<NORM>(a, top, squares, scale);
-    if (thread == 0) a.scales[row] = scale;
+    const Grid g = finish<NORM>(a, row, thread == 0, top, squares);
     int8_t* codes = a.codes + row * a.codes_stride;
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(MOST_THREADS, MOST_THREADS == 512 ? 2 : 1) row
         }
         if constexpr (sizeof(T) == 2 && !NORM) codes_of_bf16<N>(u, g, w);
         else codes_of<N>(u, g, w);
-        store_codes<N, !APART>(codes + c, w, a.width - c);
+        store_codes<N, !APART>(codes + (uint32_t)c, w, a.width - c);
     }
 }
 
@@ -382,9 +386,7 @@ template <typename T, bool NORM> __global__ void __launch_bounds__(1024) long_ro
         for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
     }
     reduce<false, NORM>(top, squares);
-    float scale;
-    const Grid g = finish<NORM>(a, top, squares, scale);
-    if (threadIdx.x == 0) a.scales[row] = scale;
+    const Grid g = finish<NORM>(a, row, threadIdx.x == 0, top, squares);
     for (int c = threadIdx.x * 4; c < a.width; c += 4096) {
         values(c, true);                                       // (the sum is stored now: `total` may be x)
         uint32_t w[1];
