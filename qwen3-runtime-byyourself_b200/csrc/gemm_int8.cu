@@ -390,10 +390,7 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
 //   empty[s]      in each block: the leader's commit arrives at both
 //   acc_full[b]   in each block: likewise, when a tile's accumulator is complete
 //   acc_empty[b]  in the leader: the drain warps of both blocks arrive there
-#ifndef Q3_SETS
-#define Q3_SETS 4
-#endif
-constexpr int DRAIN_SETS = Q3_SETS, DRAIN_WARPS = 4 * DRAIN_SETS, PAIR_THREADS = 64 + 32 * DRAIN_WARPS;
+constexpr int DRAIN_SETS = 4, DRAIN_WARPS = 4 * DRAIN_SETS, PAIR_THREADS = 64 + 32 * DRAIN_WARPS;
 constexpr int PAIR_STAGES = 6;
 
 // The order of the tiles: bands of at most 16 tiles of tokens, all tiles of W inside a band, the tokens fastest, so that a band's tokens stay in the L2

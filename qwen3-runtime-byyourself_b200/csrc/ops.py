@@ -1782,7 +1782,7 @@ def _status_word(device) -> torch.Tensor:
         device = torch.device(device.type, torch.cuda.current_device())
     word = _tc_status.get(device)
     if word is None:
-        word = _tc_status[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        word = _tc_status.setdefault(device, torch.zeros(1, dtype=torch.int32, device=device))      # (another thread may have been first)
     return word
 
 
