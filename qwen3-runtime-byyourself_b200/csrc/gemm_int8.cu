@@ -30,9 +30,11 @@ template <int GATED, typename OutT> __device__ __forceinline__ float activated(f
 
 __device__ __forceinline__ float scaled(int sum, float token, float channel) { return (float)sum * token * channel; }
 
+// Read once, past the L1.  W may have been written by the kernel ahead, which a dependent launch overlaps: so the load is neither one of memory that
+// stays as it is for the whole kernel (.nc), nor may it be moved over the wait for that kernel (volatile, with its memory).
 __device__ __forceinline__ uint4 ld_stream16(const void* p) {
-    uint4 v;   // not volatile: the compiler may hoist and batch these loads
-    asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

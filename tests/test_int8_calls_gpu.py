@@ -1,0 +1,41 @@
+"""Calls of the 8-bit operators as programs make them: one kernel right behind the other, forms that the sizes alone would not ask for, edges of the sizes."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def drawn(rows, width, seed):
+    return torch.randn(rows, width, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("activation", [None, "silu", "gelu_tanh"])
+@pytest.mark.parametrize("form,M,N,K", [("few", 1, 2048, 1000), ("few", 8, 6144, 8200), ("few", 5, 9600, 500), ("few", 16, 2048, 1000), ("few", 12, 6144, 500),
+                                        ("few", 32, 2048, 1000), ("few", 70, 4000, 200), ("mid", 16, 2048, 1000), ("mid", 64, 4096, 4096),
+                                        ("mid", 200, 1024, 640), ("pair", 40, 2048, 512), ("pair", 700, 2048, 1000)])
+def test_weights_and_tokens_written_just_before(form, M, N, K, activation, kind):
+    """Weights and tokens are quantised one and two launches before the product, over and over into the same memory: what a product reads before the kernel
+    ahead has ended is the round before's.  All variants of the form for few tokens, every output and gate."""
+    from qwen3_b200.csrc import ops
+    columns = N // 2 if activation else N
+    matrices, tokens = [drawn(N, K, 3 + i) for i in range(3)], [drawn(M, K, 13 + i) for i in range(3)]
+    want = []
+    for w, x in zip(matrices, tokens):
+        w8, x8 = ops.quantize_rows(w, ops.Int8Rows.empty(N, K, "cuda")), ops.quantize_rows(x, ops.Int8Rows.empty(M, K, "cuda"))
+        torch.cuda.synchronize()
+        want.append(ops.gemm_int8(x8, w8, torch.zeros(M, columns, dtype=kind, device="cuda"), activation=activation, form="mid" if form != "mid" else "pair"))
+        torch.cuda.synchronize()
+    w8, x8 = ops.Int8Rows.empty(N, K, "cuda"), ops.Int8Rows.empty(M, K, "cuda")
+    outs = [torch.zeros(M, columns, dtype=kind, device="cuda") for _ in range(12)]
+    torch.cuda.synchronize()
+    for i, y in enumerate(outs):
+        for which in ((0, 1), (1, 0))[i % 2]:              # either of them last
+            if which:
+                ops.quantize_rows(matrices[i % 3], w8)
+            else:
+                ops.quantize_rows(tokens[i % 3], x8)
+        ops.gemm_int8(x8, w8, y, activation=activation, form=form)
+    torch.cuda.synchronize()
+    assert ops.tcgen05_status("cuda") == 0
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(outs))
