@@ -10,7 +10,8 @@
 // go through one reduction, and a code does not hang on the order of the sum.
 //
 // A row with a NaN or an infinity (or whose squares' sum is none that 32 bits hold) gets the scale NaN and codes of zero: what is multiplied by it
-// becomes NaN.  A row of zeros gets the scale zero.  Scales below 2^-126 have fewer bits.
+// becomes NaN.  A row of zeros gets the scale zero.  Scales below 2^-126 have fewer bits.  An eps below 2^-126 (32 bits; zero, say) does not cover what
+// squares of small values lose: rows whose mean square is below that are finished by a kernel of their own.
 //
 // Bound by memory: a row is read once, in packets of 16 bytes, held in registers across the reduction, and written (8,000 rows, of the measured copy
 // rate: quantise 12,288 bfloat16 47.2 us, 0.95; 10,240 of 5,120 float32 42.5, 0.94; norm and sum 5,120 bfloat16 50.9, 0.86; in long runs, at the clocks that
@@ -33,7 +34,7 @@ struct Rows {
     float* scales;
     int64_t rows, x_stride, delta_stride, total_stride, codes_stride;
     int width;
-    float eps;
+    float eps, lost;                   // lost: a norm's sums of squares below this are taken again (0: none)
 };
 
 // What a row's codes are made with.
@@ -210,7 +211,10 @@ template <bool NORM> __device__ __forceinline__ Grid finish(const Rows& a, int64
     bool fine = bits < 0x7f800000u;
     if constexpr (NORM) fine = fine && squares < INFINITY;
     if (first)
-        a.scales[row] = !fine ? __uint_as_float(0x7fffffffu) : NORM && top != 0.0f ? top * rsqrtf(squares / (float)a.width + a.eps) / 127.0f : top / 127.0f;
+        a.scales[row] = !fine ? __uint_as_float(0x7fffffffu)
+                        : !NORM || top == 0.0f ? top / 127.0f
+                        : squares < a.lost ? -top              // (for `small_rows_kernel`)
+                                           : top * rsqrtf(squares / (float)a.width + a.eps) / 127.0f;
     Grid g;
     g.top = fine ? top : 0.0f;
     g.divide = g.top != 0.0f && top < 7.9e-31f;                // 2^-100
@@ -395,6 +399,27 @@ template <typename T, bool NORM> __global__ void __launch_bounds__(1024) long_ro
     }
 }
 
+// The scales of normed rows whose squares 32 bits lose, after one of the kernels above has noted -max |u| in their place: a row a warp, sums in 64 bits, which
+// hold the square of every 32-bit number.
+template <typename T> __global__ void __launch_bounds__(256) small_rows_kernel(const Rows a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= a.rows) return;
+    const float noted = a.scales[row];
+    if (!(noted < 0.0f)) return;
+    const T* t = a.delta != nullptr ? (const T*)a.total + row * a.total_stride : (const T*)a.x + row * a.x_stride;
+    double squares = 0.0;
+    for (int64_t c = lane; c < a.width; c += 32) {
+        const double v = (double)to_f32<T>(t[c]);
+        squares += v * v;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    if (lane == 0) a.scales[row] = (float)(-(double)noted / sqrt(squares / (double)a.width + (double)a.eps) / 127.0);
+}
+
 template <typename T, int PER, bool NORM, bool APART> int launch(const Rows& a, int threads, bool warp, cudaStream_t stream) {
     const int block = warp ? 128 : threads;
     const size_t staged = NORM && APART && a.delta != nullptr ? (size_t)block * 16 : 0;
@@ -436,10 +461,15 @@ template <typename T, bool NORM> int rows_launch(const q3_int8_rows_args& in) {
         return Q3_ERR_BAD_SIZE;
     if (in.codes_stride % 16 != 0 || !aligned16(in.codes)) return Q3_ERR_MISALIGNED;
     const Rows a{in.x, NORM ? in.delta : nullptr, NORM ? (const float*)in.weight : nullptr, NORM ? in.total : nullptr, (int8_t*)in.codes,
-                 (float*)in.scales, in.rows, in.x_stride, in.delta_stride, in.total_stride, in.codes_stride, in.width, (float)in.eps};
+                 (float*)in.scales, in.rows, in.x_stride, in.delta_stride, in.total_stride, in.codes_stride, in.width, (float)in.eps,
+                 NORM && (float)in.eps < 0x1p-126f ? (float)in.width * 0x1p-126f : 0.0f};
     const bool packets = in.width % V == 0 && in.x_stride % V == 0 && aligned16(in.x) && aligned16(a.weight) &&
                          (a.delta == nullptr || (in.delta_stride % V == 0 && in.total_stride % V == 0 && aligned16(in.delta) && aligned16(in.total)));
-    return packets ? pick<T, NORM, false>(a, (cudaStream_t)in.stream) : pick<T, NORM, true>(a, (cudaStream_t)in.stream);
+    const cudaStream_t stream = (cudaStream_t)in.stream;
+    const int failed = packets ? pick<T, NORM, false>(a, stream) : pick<T, NORM, true>(a, stream);
+    if constexpr (NORM)
+        if (failed == 0 && a.lost > 0.0f) return (int)q3_launch(small_rows_kernel<T>, dim3((unsigned)((a.rows + 7) / 8)), dim3(256), 0, stream, a);
+    return failed;
 }
 
 }  // namespace

@@ -1618,6 +1618,7 @@ _QUANTIZE, _NORM8 = ({d: name + s for d, s in _SUFFIX.items()} for name in ("q3_
 # Rows of codes begin at multiples of 16 bytes; made here, of lines of the L2, which the copies of a product's tiles then take whole (width 4,099, rows 4,112
 # / 4,224 bytes apart: 2,000 x 5,120 42.5 / 31.6 us, 300 14.7 / 11.6, 40 9.2 / 8.5).
 INT8_ROW_BYTES = 128
+_LEAST_NORMAL = 2.0 ** -126            # (of 32 bits)
 INT8_MAX_WIDTH = 131071                # a sum of so many products of two codes stays below 2^31
 
 
@@ -1696,7 +1697,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Ro
     """The rows x / sqrt(mean x^2 + eps) * weight in 32 bits, as 8-bit codes (see `quantize_rows`); weight is float32 [width].
 
     With `delta` the norm reads x + delta (32-bit sum, stored in x's type), which is written to `total`, by default to x itself.  A
-    row whose squares' sum 32 bits do not hold counts as one with an infinity.  x, delta and total: contiguous rows any distance apart."""
+    row whose squares' sum 32 bits do not hold counts as one with an infinity.  eps is a 32-bit number; where it is below 2^-126 (0, say), a second kernel
+    finishes rows with squares so small that 32 bits lose them.  x, delta and total: contiguous rows any distance apart."""
     dtype, index, shape = x.dtype, out.index, out.shape
     at, step = _strided(x, "x", dtype, shape, index)
     if delta is None:
@@ -1711,6 +1713,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Int8Ro
     _call_packed("rms_norm_int8", "int8_rows.cu", _NORM8.get(dtype) or "q3_rms_norm_int8_" + _suffix(x), _ROWS8_ARGS.pack(
         at, delta_at, _at(weight, "weight", _F32), total_at, out.at, out.scales_at, _stream_on(index, "rms_norm_int8"), out.rows, step, delta_step,
         total_step, out.stride, eps, out.width, 0))
+    if eps < _LEAST_NORMAL and out.rows and out.width:
+        _count_extra(1)
     return out
 
 

@@ -39,3 +39,33 @@ def test_weights_and_tokens_written_just_before(form, M, N, K, activation, kind)
     torch.cuda.synchronize()
     assert ops.tcgen05_status("cuda") == 0
     assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(outs))
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("rows,width", [(6, 1), (12, 64), (13, 65), (1, 4096), (700, 1000), (400, 1001), (13, 5001), (12, 40000)])
+def test_norm_of_small_rows_without_an_epsilon(rows, width, delta, kind):
+    """Squares that 32 bits lose, wholly or in part, between rows that they hold: beside an eps of 0 the scale is that of 64 bits but for the rounding of
+    some sums of at most 110 terms in a row, a root, a product and a division (2^-18), and a step of the smallest scales."""
+    import int8_cases as ic
+    from qwen3_b200.csrc import ops
+    x = drawn(rows, width, rows + width)
+    for i in range(rows):
+        x[i] *= (1.0, 1e-10, 1e-18, 1e-20, 1e-22, 1e-25, 1e-30, 1e-36, 1e-38, 1e-40)[i % 10]
+    x[rows // 2] = 0
+    x, w = x.to(kind), 1 + 0.3 * drawn(1, width, 7)[0]
+    d = (0.5 * x.float().roll(1, 1)).to(kind) if delta else None
+    stored = (x.float() + d.float()).to(kind) if delta else x.clone()
+    u = ic.normed(stored, w)
+    codes, tops = ic.quantised(u)
+    for eps in (0.0, 1e-42, 2.0 ** -127):
+        mean = stored.double().square().mean(-1) + float(torch.tensor(eps, dtype=torch.float32))
+        want = torch.where(tops > 0, tops / mean.sqrt(), torch.zeros_like(tops))
+        t, total, out = x.clone(), torch.full_like(x, 77.0), ops.Int8Rows.empty(rows, width, "cuda")
+        ops.rms_norm_int8(t, w, eps, out, **({"delta": d, "total": total} if delta else {}))
+        assert torch.equal(out.codes.long(), codes)
+        assert bool(((out.scales.double() - want).abs() <= 2.0 ** -18 * want + 2.0 ** -149).all()), (eps, out.scales, want)
+        if delta:
+            assert torch.equal(total, stored) and torch.equal(t, x)
+            ops.rms_norm_int8(t, w, eps, out, delta=d)     # in place
+            assert torch.equal(t, stored) and bool(((out.scales.double() - want).abs() <= 2.0 ** -18 * want + 2.0 ** -149).all())
