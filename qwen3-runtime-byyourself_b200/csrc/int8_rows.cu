@@ -455,7 +455,8 @@ template <typename T, bool NORM, bool APART> int pick(const Rows& a, cudaStream_
 
 template <typename T, bool NORM> int rows_launch(const q3_int8_rows_args& in) {
     constexpr int V = Pack<T>::N;
-    if (in.rows <= 0 || in.width <= 0) return in.rows < 0 || in.width < 0 ? Q3_ERR_BAD_SIZE : 0;
+    if (in.rows <= 0 || in.width < 0) return in.rows < 0 || in.width < 0 ? Q3_ERR_BAD_SIZE : 0;
+    if (in.width == 0) return (int)cudaMemsetAsync(in.scales, 0, (size_t)in.rows * sizeof(float), (cudaStream_t)in.stream);     // as a row of zeros
     if (in.rows > 0x7fffffff || in.width > 1 << 30) return Q3_ERR_TOO_LARGE;
     if (in.codes_stride < in.width || in.x == nullptr || (NORM && (in.weight == nullptr || (in.delta != nullptr && in.total == nullptr))))
         return Q3_ERR_BAD_SIZE;

@@ -1636,8 +1636,8 @@ class Int8Rows:
         self.scales_at = _dev(scales, "scales", torch.float32)
         self.rows, self.width = codes.shape
         self.shape, self.index = codes.shape, codes.get_device()
-        # (a tensor of one row, or without any, may have any stride)
-        self.stride = codes.stride(0) if self.rows > 1 else -(-self.width // 16) * 16
+        # (a tensor of one row, or without any values, may have any stride)
+        self.stride = codes.stride(0) if codes.numel() > self.width else -(-self.width // 16) * 16
         if self.rows > 0x7FFFFFFF:
             raise KernelError(f"int8 rows: {self.rows} rows, more than one launch takes")
         if (self.width > 1 and codes.stride(1) != 1) or self.stride % 16 or self.stride < self.width or codes.data_ptr() % 16:
@@ -1683,7 +1683,7 @@ def _stream_on(index: int, what: str) -> int:
 
 def quantize_rows(x: torch.Tensor, out: Int8Rows) -> Int8Rows:
     """Rows of x [rows, width] (bfloat16 or float32, contiguous rows any distance apart) as 8-bit codes: with a = max |x| of a row, code = 127 x / a to
-    the nearest whole number, ties to even, and scale = a / 127.  A row of zeros gets the scale 0, one with a NaN or an infinity the
+    the nearest whole number, ties to even, and scale = a / 127.  A row of zeros (or of no values) gets the scale 0, one with a NaN or an infinity the
     scale NaN and codes of 0."""
     dtype = x.dtype
     at, step = _strided(x, "x", dtype, out.shape, out.index)

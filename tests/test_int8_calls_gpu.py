@@ -69,3 +69,20 @@ def test_norm_of_small_rows_without_an_epsilon(rows, width, delta, kind):
             assert torch.equal(total, stored) and torch.equal(t, x)
             ops.rms_norm_int8(t, w, eps, out, delta=d)     # in place
             assert torch.equal(t, stored) and bool(((out.scales.double() - want).abs() <= 2.0 ** -18 * want + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 5, 700])
+def test_rows_of_no_values(rows, kind):
+    """As rows of zeros: the scale 0.  A product over no values is refused."""
+    from qwen3_b200.csrc import ops
+    x, w = torch.zeros(rows, 0, dtype=kind, device="cuda"), torch.zeros(0, device="cuda")
+    memory = torch.full((rows, 16), 77, dtype=torch.int8, device="cuda")
+    for out in (ops.Int8Rows(memory[:, :0], torch.full((rows,), 77.0, device="cuda")), ops.Int8Rows.empty(rows, 0, "cuda")):
+        for call in (lambda: ops.quantize_rows(x, out), lambda: ops.rms_norm_int8(x, w, 1e-6, out), lambda: ops.rms_norm_int8(x, w, 0.0, out, delta=x)):
+            out.scales.fill_(77.0)
+            call()
+            assert bool((out.scales == 0).all()) and out.float().shape == (rows, 0)
+        with pytest.raises(ops.KernelError):
+            ops.gemm_int8(out, out, torch.zeros(rows, rows, device="cuda"))
+    assert bool((memory == 77).all())
