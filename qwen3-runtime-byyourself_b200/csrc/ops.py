@@ -1624,9 +1624,10 @@ INT8_MAX_WIDTH = 131071                # a sum of so many products of two codes 
 
 class Int8Rows:
     """Rows [rows, width] in 8 bits: a code stands for code * scale of its row.  `codes` int8 with rows a multiple of 16 bytes apart (`Int8Rows.empty`
-    makes room for any width), `scales` float32 [rows].  Tokens and matrices [channels, width] alike."""
+    makes room for any width), `scales` float32 [rows].  Tokens and matrices [channels, width] alike.
+    The tensors are those that it was made with, whose addresses the kernels get; their values may change."""
 
-    __slots__ = ("codes", "scales", "rows", "width", "stride", "shape", "at", "scales_at", "index")
+    __slots__ = ("_codes", "_scales", "rows", "width", "stride", "shape", "at", "scales_at", "index")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dim() != 2 or codes.dtype != torch.int8 or scales.shape != codes.shape[:1]:
@@ -1645,7 +1646,7 @@ class Int8Rows:
         end = codes.storage_offset() + (self.rows - 1) * self.stride + -(-self.width // 16) * 16
         if self.rows and end > codes.untyped_storage().nbytes():
             raise KernelError("int8 rows: the memory of the last row ends inside its last 16 bytes")
-        self.codes, self.scales, self.at = codes, scales, codes.data_ptr()
+        self._codes, self._scales, self.at = codes, scales, codes.data_ptr()
         if self.index not in _status_at and not torch.cuda.is_current_stream_capturing():
             # the word that a product notes a wait in: made here, because one that is made inside a capture is zero only where the graph runs
             _status_at[self.index] = _status_word(codes.device).data_ptr()
@@ -1654,6 +1655,9 @@ class Int8Rows:
     def empty(cls, rows: int, width: int, device) -> "Int8Rows":
         codes = torch.empty(rows, -(-width // INT8_ROW_BYTES) * INT8_ROW_BYTES, dtype=torch.int8, device=device)[:, :width]
         return cls(codes, torch.empty(rows, dtype=torch.float32, device=device))
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
 
     def float(self) -> torch.Tensor:
         """The values that the codes stand for."""

@@ -86,3 +86,16 @@ def test_rows_of_no_values(rows, kind):
         with pytest.raises(ops.KernelError):
             ops.gemm_int8(out, out, torch.zeros(rows, rows, device="cuda"))
     assert bool((memory == 77).all())
+
+
+def test_tensors_of_rows_stay_those_they_were_made_with():
+    """Other tensors in their place would not reach the kernels: assigning them is an error."""
+    from qwen3_b200.csrc import ops
+    a, b = (ops.quantize_rows(drawn(4, 64, seed), ops.Int8Rows.empty(4, 64, "cuda")) for seed in (1, 2))
+    before = a.float()
+    for name in ("codes", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(a, name, getattr(b, name))
+    assert torch.equal(a.float(), before)
+    a.scales.mul_(2)                                       # (values in place are felt)
+    assert torch.equal(a.float(), 2 * before)
