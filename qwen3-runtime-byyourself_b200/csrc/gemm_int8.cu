@@ -42,6 +42,8 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+inline int most(int a, int b) { return a > b ? a : b; }
+
 struct Product {
     const int8_t *x, *w;
     const float *sx, *sw;
@@ -693,10 +695,11 @@ float few_us(int M, int N, int K) {
 // taken by clusters: the SMs come in groups, and a group whose places are no multiple of a cluster leaves some empty.
 float mid_us(int M, int N, int K, int splits) {
     const int sms = q3_device_sm_count(), tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256, rows = cuts(N, BM);
-    const int tokens = cuts(M, tile), an_sm = tile == 256 ? 1 : (int64_t)rows * splits > 2 * sms ? 3 : 2;
+    const int tokens = cuts(M, tile);
+    const int an_sm = tile == 256 ? 1 : (int64_t)rows * splits > 2 * sms ? 3 : 2;
     const float taken = splits <= 2 ? 1.0f : tile == 256 ? (splits == 3 ? 0.91f : splits <= 6 ? 0.89f : 0.81f) : splits <= 4 ? 0.96f : 0.89f;
     const int64_t blocks = (int64_t)rows * splits * tokens;
-    const int slots = (int)((float)(an_sm * sms) * taken), waves = cuts(blocks, slots);
+    const int slots = most((int)((float)(an_sm * sms) * taken), 1), waves = cuts(blocks, slots);
     const float shared = (float)(waves == 1 ? (int)blocks : slots) / (float)sms, t = (float)tile / 64.0f;
     const float step = fmaxf(0.214f + 0.03f * t, shared * (16.0f + 8.0f * t) * 0.0085f);
     const float around = 1.34f * t + 1.21f * shared + (splits > 1 ? 0.08f : 0.0f);
@@ -704,7 +707,7 @@ float mid_us(int M, int N, int K, int splits) {
 }
 // Steps of 128 a pair: the products, the copies of few tokens, or what the L2 gives all pairs; a tile's drain under the next one's steps, but for the last.
 float pair_us(int M, int N, int K, int tile) {
-    const int pairs = q3_device_sm_count() / 2;
+    const int pairs = most(q3_device_sm_count() / 2, 1);
     const int64_t tiles = (int64_t)cuts(M, tile) * cuts(N, 256);
     const float t = (float)tile / 256.0f, full = fminf((float)tiles / (float)pairs, 1.0f);
     const float step = fmaxf(fmaxf(0.1835f, 0.335f * t), 0.1525f * full * (t + 1.0f)), drain = 1.23f + 0.77f * t;
@@ -731,7 +734,7 @@ Choice pair_choice(int M, int N, int K) {
         if (us < best.us) best = Choice{tile, us};
     };
     for (int n = cuts(M, 256); n < cuts(M, 256) + 4; ++n) take(cuts(cuts(M, n), 32) * 32);
-    for (int tile = 32; tile < 160 && tile < M + 32; tile += 32) take(tile);
+    for (int tile = 32; tile < 160 && tile - 32 < M; tile += 32) take(tile);
     return best;
 }
 
@@ -756,7 +759,7 @@ template <int GATED, typename OutT> int pair(const Product& p, int tile, int* st
     if (!q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, tile / 2) || !q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM)) return Q3_ERR_BAD_SIZE;
     const int64_t tiles = (int64_t)((p.M + tile - 1) / tile) * ((p.N + 255) / 256);
     if (tiles > 0x3fffffff) return Q3_ERR_TOO_LARGE;
-    const int pairs = tiles < q3_device_sm_count() / 2 ? (int)tiles : q3_device_sm_count() / 2;
+    const int most_pairs = most(q3_device_sm_count() / 2, 1), pairs = tiles < most_pairs ? (int)tiles : most_pairs;
     return (int)q3_launch_cluster(kernel, dim3(2 * pairs), dim3(PAIR_THREADS), (size_t)SMEM, stream, dim3(2, 1, 1), map_x, map_w, p, tile, status);
 }
 

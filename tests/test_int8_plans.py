@@ -1,0 +1,23 @@
+"""Sizes at the ends of what the products in 8 bits take: their plan, and what is refused before a launch."""
+import os
+import subprocess
+import sys
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+CALLS = """
+import ctypes, sys
+sys.path.insert(0, {root!r})
+from qwen3_b200.csrc import ops
+lib = ops.load_library("gemm_int8.cu", ())
+splits = ctypes.c_int(0)
+for rows, channels, width in ((1, 1, 1), (64, 4096, 4096), (527, 5120, 17408), (0x7fffffff, 0x7fffffff, 131071), (0x7fffffff, 16, 1), (16, 0x7fffffff, 64), (0, 4, 4)):
+    assert lib.q3_gemm_int8_plan(rows, channels, width, ctypes.byref(splits)) in (0, 1, 2)
+print("done")
+"""
+
+
+def test_plans_and_sizes_without_a_device():
+    """In a process of its own: without a device, whose SMs the plan counts, it once divided by zero."""
+    done = subprocess.run([sys.executable, "-c", CALLS.format(root=ROOT)], capture_output=True, text=True, timeout=600, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""))
+    assert done.returncode == 0 and "done" in done.stdout, (done.returncode, done.stderr[-2000:])
