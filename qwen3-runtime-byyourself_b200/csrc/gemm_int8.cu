@@ -763,7 +763,10 @@ template <int GATED, typename OutT> int pair(const Product& p, int tile, int* st
     return (int)q3_launch_cluster(kernel, dim3(2 * pairs), dim3(PAIR_THREADS), (size_t)SMEM, stream, dim3(2, 1, 1), map_x, map_w, p, tile, status);
 }
 
+// The kernels' 32-bit row numbers run on to the end of a tile of at most 256.
+constexpr int MOST_ROWS = 0x7fffffff - 256;
 int product_of(const q3_gemm_int8_args& a, Product& p) {
+    if (a.rows > MOST_ROWS || a.channels > MOST_ROWS) return Q3_ERR_TOO_LARGE;
     if (a.width <= 0 || a.width > 131071 || a.activation < 0 || a.activation > 2 || (a.activation != 0 && a.channels % 16 != 0)) return Q3_ERR_BAD_SIZE;
     if (a.x_stride < a.width || a.w_stride < a.width) return Q3_ERR_BAD_SIZE;
     if (!aligned16(a.x) || !aligned16(a.w) || a.x_stride % 16 != 0 || a.w_stride % 16 != 0) return Q3_ERR_MISALIGNED;

@@ -13,11 +13,16 @@ lib = ops.load_library("gemm_int8.cu", ())
 splits = ctypes.c_int(0)
 for rows, channels, width in ((1, 1, 1), (64, 4096, 4096), (527, 5120, 17408), (0x7fffffff, 0x7fffffff, 131071), (0x7fffffff, 16, 1), (16, 0x7fffffff, 64), (0, 4, 4)):
     assert lib.q3_gemm_int8_plan(rows, channels, width, ctypes.byref(splits)) in (0, 1, 2)
+for rows, channels in ((0x7fffffff, 16), (16, 0x7fffffff), (0x7fffffff - 255, 16)):
+    for form in ("few", "mid", "pair"):
+        args = ops._GEMM8_ARGS.pack(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 0, 16, 16, rows, channels, 16, 0, 0, 0)
+        code = getattr(lib, "q3_gemm_int8_" + form)(args)
+        assert code == 10002, (form, rows, channels, code)
 print("done")
 """
 
 
 def test_plans_and_sizes_without_a_device():
-    """In a process of its own: without a device, whose SMs the plan counts, it once divided by zero."""
+    """In a process of its own: without a device, whose SMs the plan counts, it once divided by zero.  Sizes that 32 bits do not count to are refused before a launch."""
     done = subprocess.run([sys.executable, "-c", CALLS.format(root=ROOT)], capture_output=True, text=True, timeout=600, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""))
     assert done.returncode == 0 and "done" in done.stdout, (done.returncode, done.stderr[-2000:])
