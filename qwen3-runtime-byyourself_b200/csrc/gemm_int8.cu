@@ -43,6 +43,7 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 }
 
 inline int most(int a, int b) { return a > b ? a : b; }
+constexpr int GRID_YZ = 65535;         // blocks along a grid's second and third axis
 
 struct Product {
     const int8_t *x, *w;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(WARPS * 32, MINB) few_kernel(const Product p) 
 
 template <int MT, int WARPS, int PF, int MINB, int GATED, typename OutT> int launch_few(const Product& p, cudaStream_t stream) {
     const int64_t tokens = (p.M + 8 * MT - 1) / (8 * MT);
-    if (tokens > 65535) return Q3_ERR_TOO_LARGE;
+    if (tokens > GRID_YZ) return Q3_ERR_TOO_LARGE;
     return (int)q3_launch(few_kernel<MT, WARPS, PF, MINB, GATED, OutT>, dim3((unsigned)((p.N + 15) / 16), (unsigned)tokens), dim3(WARPS * 32),
                           WARPS * 8 * MT * 17 * 4, stream, p);
 }
@@ -670,7 +671,7 @@ template <int MT, int STAGES, int MINB, int GATED, typename OutT> int launch_mid
     CUtensorMap map_w, map_x;
     if (!q3_make_map_bytes(&map_w, p.w, p.N, p.K, p.ldw, BM) || !q3_make_map_bytes(&map_x, p.x, p.M, p.K, p.ldx, MT)) return Q3_ERR_BAD_SIZE;
     const int64_t token_tiles = (p.M + MT - 1) / MT;
-    if (token_tiles > 65535) return Q3_ERR_TOO_LARGE;
+    if (token_tiles > GRID_YZ) return Q3_ERR_TOO_LARGE;
     return (int)q3_launch_cluster(mid_kernel<MT, STAGES, MINB, GATED, OutT>, dim3((p.N + BM - 1) / BM, splits, (unsigned)token_tiles), dim3(THREADS),
                                   (size_t)SMEM, stream, dim3(1, splits, 1), map_w, map_x, p, status);
 }
@@ -696,6 +697,7 @@ float few_us(int M, int N, int K) {
 float mid_us(int M, int N, int K, int splits) {
     const int sms = q3_device_sm_count(), tile = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256, rows = cuts(N, BM);
     const int tokens = cuts(M, tile);
+    if (tokens > GRID_YZ) return 1e30f;                        // more tiles of tokens than a grid takes
     const int an_sm = tile == 256 ? 1 : (int64_t)rows * splits > 2 * sms ? 3 : 2;
     const float taken = splits <= 2 ? 1.0f : tile == 256 ? (splits == 3 ? 0.91f : splits <= 6 ? 0.89f : 0.81f) : splits <= 4 ? 0.96f : 0.89f;
     const int64_t blocks = (int64_t)rows * splits * tokens;

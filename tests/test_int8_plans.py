@@ -3,6 +3,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 CALLS = """
@@ -26,3 +28,17 @@ def test_plans_and_sizes_without_a_device():
     """In a process of its own: without a device, whose SMs the plan counts, it once divided by zero.  Sizes that 32 bits do not count to are refused before a launch."""
     done = subprocess.run([sys.executable, "-c", CALLS.format(root=ROOT)], capture_output=True, text=True, timeout=600, env=dict(os.environ, CUDA_VISIBLE_DEVICES=""))
     assert done.returncode == 0 and "done" in done.stdout, (done.returncode, done.stderr[-2000:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,channels,width", [(17_000_000, 64, 8192), (16_777_000, 128, 4096), (20_000_000, 16, 4096), (1, 25600, 131071), (64, 64, 64),
+                                                 (0x7ffffeff, 16, 16), (8000, 24576, 4096)])
+def test_plans_can_be_launched(rows, channels, width):
+    """A grid takes 65,535 tiles of tokens along an axis; `splits` are K ranges of a cluster, or a tile's tokens."""
+    from qwen3_b200.csrc import ops
+    form, splits = ops.int8_plan(rows, channels, width)
+    assert form in ("few", "mid", "pair")
+    if form == "mid":
+        assert -(-rows // 256) <= 65535 and 1 <= splits <= 8
+    elif form == "pair":
+        assert splits % 32 == 0 and 32 <= splits <= 256 and -(-rows // splits) * -(-channels // 256) <= 0x3FFFFFFF
