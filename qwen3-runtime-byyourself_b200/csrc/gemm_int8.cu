@@ -220,6 +220,12 @@ template <typename OutT> __device__ __forceinline__ void store4(OutT* p, const f
         if (i < valid) p[i] = to_out<OutT>(v[i]);
 }
 
+// A producer's end: the copies of its `issued` steps have landed and been read (every stage has been handed back), or the limit has run out.  No block goes
+// while its copies are under way, also where another role has given up; otherwise the accumulator that its last warps wait for is later than this.
+template <int STAGES> __device__ __forceinline__ void wait_for_stages(uint32_t empty, uint32_t issued) {
+    for (uint32_t i = issued; i < issued + STAGES; ++i) mbar_wait(empty + i % STAGES * 8, ((i / STAGES) & 1u) ^ 1u);
+}
+
 template <int MT, int STAGES, int MINB, int GATED, typename OutT>
 __global__ void __launch_bounds__(THREADS, MINB)
 mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Product p, int* __restrict__ status) {
@@ -268,7 +274,8 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
     if (warp == 0) {
         if (lane == 0) {
             pdl_wait();              // (for W, too: the caller may just have quantised it; asking for it earlier gained nothing to 4 %)
-            for (int i = 0; i < nkb; ++i) {
+            int i = 0;
+            for (; i < nkb; ++i) {
                 const int s = i % STAGES;
                 if (!mbar_wait(bars + (STAGES + s) * 8, ((uint32_t)(i / STAGES) & 1u) ^ 1u)) {      // the stage is free
                     atomicExch(status, 1);
@@ -279,6 +286,7 @@ mid_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CU
                 tma_load_2d(a, &map_w, bars + s * 8, (kb_begin + i) * BK, n0);
                 tma_load_2d(b, &map_x, bars + s * 8, (kb_begin + i) * BK, m0);
             }
+            wait_for_stages<STAGES>(bars + STAGES * 8, (uint32_t)i);
         }
     } else if (warp == 1) {
         // the whole warp walks the K steps and one elected thread issues, so that descriptors stay in uniform registers
@@ -561,6 +569,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ C
                 __syncwarp();
             }
         }
+        wait_for_stages<STAGES>(bars + STAGES * 8, it);
+        __syncwarp();
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t idesc = make_idesc_i8(2 * BM, tile);

@@ -22,3 +22,14 @@ def test_loads_stay_behind_the_wait_for_the_kernel_ahead(name):
     for volatile, body in loads:
         assert volatile and '"memory"' in body and ".nc" not in body, body
     assert "__ldg(" not in text
+
+
+def test_a_block_waits_for_its_copies_before_it_goes():
+    """Also where another role of the block has given up: each producer's last step is to wait until every stage has been handed back."""
+    text = source("gemm_int8.cu")
+    kernels = re.split(r"__global__", text)[1:]
+    producers = [k for k in kernels if "tma_load_2d" in k]
+    assert len(producers) == 2
+    for kernel in producers:
+        role = kernel[kernel.index("if (warp == 0) {"):kernel.index("else if (warp == 1) {", kernel.index("if (warp == 0) {"))]
+        assert role.rindex("wait_for_stages<STAGES>(bars + STAGES * 8,") > role.rindex("tma_load_2d")
