@@ -313,8 +313,8 @@ class GQAAttention(Part):
         p, n = prefix + self.prefix, self.names
         return [p + n[k] for k in ("q", "k", "v", "out_gate", "o") if p + n[k] in self.weight_specs(prefix)]
 
-    def to_eight_bit(self) -> None:
-        self.w_qkv, self.w_o = quantized_weights(self.w_qkv), quantized_weights(self.w_o)
+    def to_eight_bit(self, weights=None) -> None:
+        self.w_qkv, self.w_o = quantized_weights(self.w_qkv, weights), quantized_weights(self.w_o, weights)
 
     def mix(self, x: torch.Tensor, ctx, cache) -> torch.Tensor:
         """Everything before the output projection: [N, num_heads * value_dim] in the compute type (float32 with

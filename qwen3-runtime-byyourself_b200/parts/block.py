@@ -52,9 +52,10 @@ class PreNormBlock(Part):
     def eight_bit_names(self, prefix: str) -> list:
         return self.mixer.eight_bit_names(prefix) + self.feed_forward.eight_bit_names(prefix)
 
-    def to_eight_bit(self) -> None:
-        self.mixer.to_eight_bit()
-        self.feed_forward.to_eight_bit()
+    def to_eight_bit(self, weights=None) -> None:
+        """The projections in 8 bits, after `bind`; `weights`: what they were bound from, which may have room for them."""
+        self.mixer.to_eight_bit(weights)
+        self.feed_forward.to_eight_bit(weights)
         self.weights_in_eight_bit = True
 
     def forward(self, residual, delta, ctx, cache):

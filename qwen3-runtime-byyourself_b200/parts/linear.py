@@ -119,9 +119,10 @@ def quantized(x: torch.Tensor, ctx, name: str) -> ops.Int8Rows:
     return ops.quantize_rows(x, eight_bit_rows(ctx, name, *x.shape))
 
 
-def quantized_weights(w: torch.Tensor) -> ops.Int8Rows:
-    """A matrix [out, in] in 8 bits, a scale for each output channel."""
-    return ops.quantize_rows(w, ops.Int8Rows.empty(*w.shape, w.device))
+def quantized_weights(w: torch.Tensor, weights=None) -> ops.Int8Rows:
+    """A matrix [out, in] in 8 bits, a scale for each output channel, in the arena of the checkpoint that it comes from (`weights`), if it comes from one."""
+    room = getattr(weights, "int8_rows", None)
+    return ops.quantize_rows(w, room(*w.shape) if room is not None else ops.Int8Rows.empty(*w.shape, w.device))
 
 
 def linear(x, w, out: torch.Tensor) -> torch.Tensor:

@@ -54,9 +54,9 @@ class SwiGLU(Part):
     def eight_bit_names(self, prefix: str) -> list:
         return [prefix + self.prefix + self.names[k] for k in ("gate", "up", "down")]
 
-    def to_eight_bit(self) -> None:
-        self.w_gate_up = linear_module.quantized_weights(self.w_gate_up)
-        self.w_down = linear_module.quantized_weights(self.w_down)
+    def to_eight_bit(self, weights=None) -> None:
+        self.w_gate_up = linear_module.quantized_weights(self.w_gate_up, weights)
+        self.w_down = linear_module.quantized_weights(self.w_down, weights)
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         N, I = ctx.n_tokens, self.intermediate_size

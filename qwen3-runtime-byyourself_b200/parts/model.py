@@ -95,7 +95,7 @@ class Model:
             block.bind(weights, spec.prefix, dtype, device)
             if eight_bit:
                 getattr(weights, "wait", lambda: None)()          # a streamed checkpoint: the tensors are in place now
-                block.to_eight_bit()                              # and are given back, layer by layer
+                block.to_eight_bit(weights)                       # and are given back, layer by layer
 
     def _warn_rounding(self, name: str) -> None:
         if not self._warned_rounding:

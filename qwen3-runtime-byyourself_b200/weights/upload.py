@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import mmap
 import sys
-from typing import Dict, Iterable, List, Optional, Sequence
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -35,11 +35,10 @@ def _role_dtype(role: str, compute: torch.dtype) -> torch.dtype:
     return {"matrix": compute, "norm": torch.float32, "bias": torch.float32, "int_table": torch.int32}[role]
 
 
-def _numel(shape) -> int:
-    numel = 1
-    for s in shape:
-        numel *= s
-    return numel
+def _int8_bytes(rows: int, width: int) -> Tuple[int, int]:
+    """Of the codes and of the scales of a matrix."""
+    from ..csrc import ops
+    return rows * (-(-width // ops.INT8_ROW_BYTES) * ops.INT8_ROW_BYTES), rows * 4
 
 
 def fuse_rows(weights, names: Sequence[str]) -> torch.Tensor:
@@ -86,8 +85,8 @@ class CheckpointUpload:
     """The tensors of a checkpoint, uploaded on demand into one device arena (see the top of the file)."""
 
     def __init__(self, checkpoint: Checkpoint, specs, dtype: torch.dtype, device, warn=None, apart=()):
-        """`apart`: matrices that are quantised and given back before the next ones are read: each in memory of its own, in 32-bit if it is
-        stored so."""
+        """`apart`: matrices that are quantised, into rows of the arena (`int8_rows`), and given back before the next ones are read: each in memory of
+        its own, in 32-bit if it is stored so."""
         self.apart = set(apart)
         self.ckpt, self.specs, self.dtype, self.device = checkpoint, specs, dtype, torch.device(device)
         if self.device.type != "cuda":
@@ -95,7 +94,8 @@ class CheckpointUpload:
         self._warn, self._warned = warn, False
         total = 0
         for name, spec in specs.items():
-            if name in self.apart:
+            if name in self.apart:                       # what `int8_rows` will be asked for: no more where matrices become one
+                total += sum(-(-n // ALIGN) * ALIGN for n in _int8_bytes(*spec.shape))
                 continue
             numel = 1
             for s in spec.shape:
@@ -104,10 +104,6 @@ class CheckpointUpload:
             total += -(-numel * item // ALIGN) * ALIGN
         self.arena = torch.empty(total + ALIGN, dtype=torch.uint8, device=self.device)
         self._used = (-self.arena.data_ptr()) % ALIGN
-        if self.apart:
-            # What these will take in 8 bits, and some of them as they are read, from the device at once: the allocator cuts it up (each piece by itself
-            # would make the copies wait).
-            torch.empty(sum(_numel(specs[n].shape) for n in self.apart) * 9 // 8 + (1 << 28), dtype=torch.uint8, device=self.device)
         self._done: Dict[str, torch.Tensor] = {}
         self._side = torch.cuda.Stream(self.device)
         self._host = [torch.empty(STAGE_BYTES, dtype=torch.uint8).pin_memory() for _ in range(2)]
@@ -165,6 +161,12 @@ class CheckpointUpload:
         self._place(first, out, block, 2 * block, 0)
         self._place(second, out, block, 2 * block, block)
         return out
+
+    def int8_rows(self, rows: int, width: int):
+        """Room in the arena for a matrix in 8 bits."""
+        from ..csrc import ops
+        codes = self._carve((rows, _int8_bytes(1, width)[0]), torch.int8)
+        return ops.Int8Rows(codes[:, :width], self._carve((rows,), torch.float32))
 
     def wait(self) -> None:
         """Work on the current stream that follows sees every tensor handed out so far in place (a part that
