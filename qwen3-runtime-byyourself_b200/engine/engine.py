@@ -270,11 +270,11 @@ class Engine:
         for each token (models of pre-norm blocks with attention and a gated feed-forward); None: as computed with."""
         eight_bit = cls._eight_bit(weight_dtype)
         config = load_config(folder)
-        model = build_model(config.plan())
+        model = cls._model(config, eight_bit)
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
         # every tensor goes from the mapped file to its final place on the device in one pass
         source = open_upload(folder, model.weight_specs(), model.ignorable_names(), compute, device, model._warn_rounding,
-                             apart=model.eight_bit_names() if eight_bit and model.takes_eight_bit() else ())
+                             apart=model.eight_bit_names() if eight_bit else ())
         model.bind(source, compute, device, eight_bit)
         source.finish()
         engine = cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
@@ -287,7 +287,7 @@ class Engine:
                     guard_scratch: bool = False, cache_dtype: Optional[str] = None, weight_dtype: Optional[str] = None) -> "Engine":
         """Seeded random weights drawn on the device (no folder is written)."""
         eight_bit = cls._eight_bit(weight_dtype)
-        model = build_model(config.plan())
+        model = cls._model(config, eight_bit)
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
         weights = random_weights(model.weight_specs(), seed, dtype=compute, device=device)
         model.bind(weights, compute, device, eight_bit)
@@ -298,6 +298,13 @@ class Engine:
         if weight_dtype not in (None, "int8"):
             raise ValueError(f"weight_dtype {weight_dtype!r}: None (as computed with) or 'int8'")
         return weight_dtype is not None
+
+    @staticmethod
+    def _model(config, eight_bit: bool) -> Model:
+        model = build_model(config.plan())
+        if eight_bit:
+            model.check_eight_bit()                            # before anything is read or drawn for it
+        return model
 
     # -- sequences
     def new_sequence(self) -> int:

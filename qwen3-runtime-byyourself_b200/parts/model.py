@@ -65,6 +65,11 @@ class Model:
         """Whether the layers' projections can be had in 8 bits (`bind`): every layer is a pre-norm block of attention and a gated feed-forward."""
         return all(getattr(b, "takes_eight_bit", lambda: False)() for b in self.blocks)
 
+    def check_eight_bit(self) -> None:
+        """Raise if the layers' projections cannot be had in 8 bits."""
+        if not self.takes_eight_bit():
+            raise ValueError("weights in 8 bits take a model whose layers are pre-norm blocks of attention and a gated feed-forward")
+
     def eight_bit_names(self) -> set:
         """The tensors that `bind` with 8-bit weights quantises."""
         return {name for spec, block in zip(self.plan.layers, self.blocks) for name in block.eight_bit_names(spec.prefix)}
@@ -80,8 +85,8 @@ class Model:
         `eight_bit`: the layers' projections become 8-bit integers with a scale for each output channel, from what is stored (a 32-bit
         matrix is not rounded to bfloat16 first); embedding and output projection stay as they are."""
         from ..weights.upload import TensorDict
-        if eight_bit and not self.takes_eight_bit():
-            raise ValueError("weights in 8 bits take a model whose layers are pre-norm blocks of attention and a gated feed-forward")
+        if eight_bit:
+            self.check_eight_bit()
         if isinstance(weights, dict):
             weights = TensorDict(weights, self.weight_specs(), dtype, device, self._warn_rounding, self.eight_bit_names() if eight_bit else ())
         p = self.plan

@@ -1,0 +1,26 @@
+"""Models whose projections are not to be had in 8 bits are refused before anything is read, drawn or allocated for them."""
+import pytest
+
+import qwen3_b200 as q
+from helpers import tiny
+
+
+def not_reached(*args, **kwargs):
+    raise AssertionError("weights were asked for")
+
+
+def test_refused_before_weights_are_asked_for(tmp_path, monkeypatch):
+    from dozazen_cases import case
+    from qwen3_b200.engine import engine as engine_module
+    config = q.config_from_dict(case("A"))
+    folder = str(tmp_path / "model")
+    q.write_random_model(folder, config, 1)
+    for name in ("open_upload", "random_weights"):
+        monkeypatch.setattr(engine_module, name, not_reached)
+    with pytest.raises(ValueError, match="8 bits"):
+        q.Engine.from_folder(folder, max_tokens=64, weight_dtype="int8")
+    with pytest.raises(ValueError, match="8 bits"):
+        q.Engine.from_random(config, 1, max_tokens=64, weight_dtype="int8")
+    for taken, weight_dtype in ((q.config_from_dict(tiny("A")), "int8"), (config, None)):
+        with pytest.raises(AssertionError, match="asked for"):           # (others go on to their weights)
+            q.Engine.from_random(taken, 1, max_tokens=64, weight_dtype=weight_dtype)
