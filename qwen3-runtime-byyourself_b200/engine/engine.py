@@ -289,8 +289,10 @@ class Engine:
         eight_bit = cls._eight_bit(weight_dtype)
         model = cls._model(config, eight_bit)
         compute = DTYPES[dtype] if dtype is not None else DTYPES[getattr(config, "torch_dtype", "bfloat16")]
-        weights = random_weights(model.weight_specs(), seed, dtype=compute, device=device)
-        model.bind(weights, compute, device, eight_bit)
+        # the source is the drawn tensors' only holder: what the model makes others of is given back while it is bound
+        source = model.source_of(random_weights(model.weight_specs(), seed, dtype=compute, device=device), compute, device, eight_bit)
+        model.bind(source, compute, device, eight_bit)
+        del source
         return cls(model, config, max_tokens, max_seq_len, n_slots, use_graphs, guard_scratch, cache_dtype)
 
     @staticmethod

@@ -74,6 +74,11 @@ class Model:
         """The tensors that `bind` with 8-bit weights quantises."""
         return {name for spec, block in zip(self.plan.layers, self.blocks) for name in block.eight_bit_names(spec.prefix)}
 
+    def source_of(self, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device, eight_bit: bool = False):
+        """A dict of tensors as what `bind` takes them from, one by one: a tensor that no one else holds is given back once the model has made others of it."""
+        from ..weights.upload import TensorDict
+        return TensorDict(tensors, self.weight_specs(), dtype, device, self._warn_rounding, self.eight_bit_names() if eight_bit else ())
+
     def bind(self, weights, dtype: torch.dtype, device, eight_bit: bool = False) -> None:
         """Take the tensors (by checkpoint name) for computing in `dtype` on `device`.  `weights` is a dict of
         tensors, or a checkpoint that uploads on demand (`weights.loader.open_upload`).
@@ -83,12 +88,13 @@ class Model:
         one line on stderr saying so.  Scale vectors are always read as float32.
 
         `eight_bit`: the layers' projections become 8-bit integers with a scale for each output channel, from what is stored (a 32-bit
-        matrix is not rounded to bfloat16 first); embedding and output projection stay as they are."""
+        matrix is not rounded to bfloat16 first); embedding and output projection stay as they are.  Of a checkpoint, or a source made by
+        `source_of`, a layer's matrices are given back when they are quantised; a dict of the caller's keeps what it holds."""
         from ..weights.upload import TensorDict
         if eight_bit:
             self.check_eight_bit()
-        if isinstance(weights, dict):
-            weights = TensorDict(weights, self.weight_specs(), dtype, device, self._warn_rounding, self.eight_bit_names() if eight_bit else ())
+        if isinstance(weights, dict) and not isinstance(weights, TensorDict):
+            weights = self.source_of(weights, dtype, device, eight_bit)
         p = self.plan
         self.dtype, self.device = dtype, torch.device(device)
         self.embedding.bind(weights, p.embedding_prefix, dtype, device)

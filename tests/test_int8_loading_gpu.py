@@ -58,3 +58,26 @@ def test_codes_in_the_arena_are_those_of_the_stored_matrices(tmp_path, name, sto
     for a, b in zip(matrices(got), matrices(plain)):
         want = ops.quantize_rows(b, ops.Int8Rows.empty(*b.shape, "cuda"))
         assert torch.equal(a.codes, want.codes) and torch.equal(a.scales, want.scales)
+
+
+def test_drawn_weights_are_given_back_while_they_are_quantised(monkeypatch):
+    """When the engine's own memory is taken, the device holds the codes and the embeddings; at no time much more than all matrices as drawn."""
+    config = q.config_from_dict(tiny("B", **WIDE))
+    held = []
+    built = q.Engine.__init__
+
+    def init(self, model, *args, **kwargs):
+        held.append((torch.cuda.memory_allocated(), torch.cuda.max_memory_allocated()))
+        built(self, model, *args, **kwargs)
+    monkeypatch.setattr(q.Engine, "__init__", init)
+    q.Engine.from_random(config, 3, dtype="bfloat16", max_tokens=64, max_seq_len=64, weight_dtype="int8")
+    settle()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    engine = q.Engine.from_random(config, 3, dtype="bfloat16", max_tokens=64, max_seq_len=64, weight_dtype="int8")
+    codes = sum(w.rows * (w.stride + 4) for w in matrices(engine.model))
+    drawn = 2 * sum(w.rows * w.width for w in matrices(engine.model))
+    embeddings = 2 * 2 * config.vocab_size * config.hidden_size
+    now, peak = held[-1]
+    assert now - before <= codes + embeddings + (8 << 20)
+    assert peak - before <= drawn + embeddings + drawn // 4 + (32 << 20)

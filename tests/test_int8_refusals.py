@@ -24,3 +24,20 @@ def test_refused_before_weights_are_asked_for(tmp_path, monkeypatch):
     for taken, weight_dtype in ((q.config_from_dict(tiny("A")), "int8"), (config, None)):
         with pytest.raises(AssertionError, match="asked for"):           # (others go on to their weights)
             q.Engine.from_random(taken, 1, max_tokens=64, weight_dtype=weight_dtype)
+
+
+def test_drawn_weights_are_held_by_the_model_alone(monkeypatch):
+    """When the engine's own memory is taken, a matrix that was made into another one is gone."""
+    import weakref
+    from qwen3_b200.engine import engine as engine_module
+    drawn, alive = {}, []
+    plain = engine_module.random_weights
+
+    def draw(*args, **kwargs):
+        tensors = plain(*args, **kwargs)
+        drawn.update({name: weakref.ref(t) for name, t in tensors.items()})
+        return tensors
+    monkeypatch.setattr(engine_module, "random_weights", draw)
+    monkeypatch.setattr(q.Engine, "__init__", lambda self, *args: alive.extend(n for n, t in drawn.items() if t() is not None))
+    q.Engine.from_random(q.config_from_dict(tiny("A")), 1, dtype="bfloat16", max_tokens=64, device="cpu")
+    assert len(drawn) > 10 and not [n for n in alive if any(part in n for part in ("q_proj", "k_proj", "v_proj", "gate_proj", "up_proj"))]
