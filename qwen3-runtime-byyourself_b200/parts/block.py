@@ -47,7 +47,7 @@ class PreNormBlock(Part):
 
     def takes_eight_bit(self) -> bool:
         """Whether the products of this layer can be had with weights in 8 bits: its norms then write the sublayers' inputs in 8 bits."""
-        return all(getattr(part, "takes_eight_bit", lambda: False)() for part in self.parts())
+        return type(self).forward is PreNormBlock.forward and all(getattr(part, "takes_eight_bit", lambda: False)() for part in self.parts())
 
     def eight_bit_names(self, prefix: str) -> list:
         return self.mixer.eight_bit_names(prefix) + self.feed_forward.eight_bit_names(prefix)

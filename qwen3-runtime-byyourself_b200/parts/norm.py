@@ -47,7 +47,8 @@ class RMSNorm(Part):
         return ops.rms_norm(x, self.weight, self.eps, out, delta)
 
     def takes_eight_bit(self) -> bool:
-        return self.groups == 1
+        """Whether `eight_bit` norms as this part does (a part that is built on this one and norms in another way says so by itself)."""
+        return self.groups == 1 and type(self).__call__ is RMSNorm.__call__
 
     def eight_bit(self, x: torch.Tensor, out: ops.Int8Rows, delta=None) -> ops.Int8Rows:
         """The same with the normed rows in 8 bits, rounded to these alone."""

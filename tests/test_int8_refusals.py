@@ -41,3 +41,29 @@ def test_drawn_weights_are_held_by_the_model_alone(monkeypatch):
     monkeypatch.setattr(q.Engine, "__init__", lambda self, *args: alive.extend(n for n, t in drawn.items() if t() is not None))
     q.Engine.from_random(q.config_from_dict(tiny("A")), 1, dtype="bfloat16", max_tokens=64, device="cpu")
     assert len(drawn) > 10 and not [n for n in alive if any(part in n for part in ("q_proj", "k_proj", "v_proj", "gate_proj", "up_proj"))]
+
+
+def test_parts_that_do_something_else_are_not_taken_for_those_they_are_built_on():
+    """A norm or a block of another formula would otherwise run with the formula of its base, without an error."""
+    from qwen3_b200.parts.block import PreNormBlock
+    from qwen3_b200.parts.norm import RMSNorm
+
+    class HalvedNorm(RMSNorm):
+        def __call__(self, x, out, delta=None):
+            return super().__call__(x, out, delta).mul_(0.5)
+
+    class Renamed(RMSNorm):
+        pass
+
+    class OtherBlock(PreNormBlock):
+        def forward(self, residual, delta, ctx, cache):
+            return super().forward(residual, delta, ctx, cache)
+    model = q.build_model(q.config_from_dict(tiny("A")).plan())
+    assert model.takes_eight_bit() and Renamed(64, 1e-6).takes_eight_bit()
+    assert not HalvedNorm(64, 1e-6).takes_eight_bit()
+    block = model.blocks[0]
+    kept = block.mixer_norm
+    block.mixer_norm = HalvedNorm(64, 1e-6)
+    assert not model.takes_eight_bit()
+    block.mixer_norm, block.__class__ = kept, OtherBlock
+    assert not model.takes_eight_bit()
