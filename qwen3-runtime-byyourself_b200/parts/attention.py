@@ -306,8 +306,10 @@ class GQAAttention(Part):
         return ops.add_bias(out, self.o_bias) if self.out_bias else out
 
     def takes_eight_bit(self) -> bool:
-        """Whether weights in 8 bits can be had of this layer: it reads its input through the q/k/v projection alone (an output gate's is part of it)."""
-        return type(self).forward is GQAAttention.forward and type(self).mix is GQAAttention.mix and not self.head_gate
+        """Whether weights in 8 bits can be had of this layer: it reads its input through the q/k/v projection alone (an output gate's is part of it),
+        and its products' sums fit 32 bits."""
+        return (type(self).forward is GQAAttention.forward and type(self).mix is GQAAttention.mix and not self.head_gate
+                and max(self.hidden_size, self.output_width()) <= ops.INT8_MAX_WIDTH)
 
     def eight_bit_names(self, prefix: str) -> list:
         p, n = prefix + self.prefix, self.names

@@ -49,7 +49,7 @@ class SwiGLU(Part):
         self.w_down = weights.pop(p + self.names["down"]).contiguous()
 
     def takes_eight_bit(self) -> bool:
-        return type(self) is SwiGLU
+        return type(self) is SwiGLU and max(self.hidden_size, self.intermediate_size) <= ops.INT8_MAX_WIDTH
 
     def eight_bit_names(self, prefix: str) -> list:
         return [prefix + self.prefix + self.names[k] for k in ("gate", "up", "down")]

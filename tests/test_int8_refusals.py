@@ -67,3 +67,14 @@ def test_parts_that_do_something_else_are_not_taken_for_those_they_are_built_on(
     assert not model.takes_eight_bit()
     block.mixer_norm, block.__class__ = kept, OtherBlock
     assert not model.takes_eight_bit()
+
+
+def test_widths_whose_sums_do_not_fit_32_bits():
+    """Refused with the model, not by its first step."""
+    from qwen3_b200.csrc import ops
+    from qwen3_b200.parts.attention import GQAAttention
+    from qwen3_b200.parts.mlp import SwiGLU
+    most = ops.INT8_MAX_WIDTH
+    assert SwiGLU(64, most).takes_eight_bit() and not SwiGLU(64, most + 1).takes_eight_bit() and not SwiGLU(most + 1, 64).takes_eight_bit()
+    assert GQAAttention(most, 4, 2, 16, 1.0).takes_eight_bit() and not GQAAttention(most + 1, 4, 2, 16, 1.0).takes_eight_bit()
+    assert not GQAAttention(64, 1024, 2, 128, 1.0).takes_eight_bit()
