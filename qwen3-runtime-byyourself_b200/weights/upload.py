@@ -66,6 +66,7 @@ class TensorDict(dict):
     def __init__(self, tensors: Dict[str, torch.Tensor], specs, dtype: torch.dtype, device, warn=None, apart=()):
         """`apart`: matrices that are quantised next, and therefore not rounded from 32-bit to bfloat16."""
         super().__init__()
+        self.apart = set(apart)
         warned = False
         for name, t in tensors.items():
             spec = specs.get(name)

@@ -78,3 +78,17 @@ def test_widths_whose_sums_do_not_fit_32_bits():
     assert SwiGLU(64, most).takes_eight_bit() and not SwiGLU(64, most + 1).takes_eight_bit() and not SwiGLU(most + 1, 64).takes_eight_bit()
     assert GQAAttention(most, 4, 2, 16, 1.0).takes_eight_bit() and not GQAAttention(most + 1, 4, 2, 16, 1.0).takes_eight_bit()
     assert not GQAAttention(64, 1024, 2, 128, 1.0).takes_eight_bit()
+
+
+def test_sources_that_round_before_they_are_quantised():
+    """A source of tensors that was not told of the 8 bits hands out 32-bit matrices rounded to bfloat16."""
+    import types
+    import torch
+    model = q.build_model(q.config_from_dict(tiny("A")).plan())
+    tensors = q.random_weights(model.weight_specs(), 1, dtype=torch.float32)
+    for source in (types.SimpleNamespace(apart=set()), types.SimpleNamespace(apart=set(list(model.eight_bit_names())[1:])),
+                   model.source_of(tensors, torch.bfloat16, "cpu")):
+        with pytest.raises(ValueError, match="rounded"):
+            model.bind(source, torch.bfloat16, "cpu", eight_bit=True)
+    kept = model.source_of(tensors, torch.bfloat16, "cpu", eight_bit=True)
+    assert {n for n, t in kept.items() if t.dtype == torch.float32} >= model.eight_bit_names()
