@@ -107,6 +107,7 @@ class CheckpointUpload:
         self._used = (-self.arena.data_ptr()) % ALIGN
         self._done: Dict[str, torch.Tensor] = {}
         self._side = torch.cuda.Stream(self.device)
+        self._side.wait_stream(torch.cuda.current_stream(self.device))       # what used the arena's memory before is done with it
         self._host = [torch.empty(STAGE_BYTES, dtype=torch.uint8).pin_memory() for _ in range(2)]
         self._dev: List[Optional[torch.Tensor]] = [None, None]
         self._events: List[Optional[torch.cuda.Event]] = [None, None]

@@ -81,3 +81,31 @@ def test_drawn_weights_are_given_back_while_they_are_quantised(monkeypatch):
     now, peak = held[-1]
     assert now - before <= codes + embeddings + (8 << 20)
     assert peak - before <= drawn + embeddings + drawn // 4 + (32 << 20)
+
+
+@pytest.mark.parametrize("weight_dtype", [None, "int8"])
+def test_memory_that_is_still_being_written_when_the_arena_gets_it(tmp_path, weight_dtype):
+    """A kernel that is queued before the load writes a tensor of the arena's size, which the program has given up: the arena is likely to be its memory."""
+    from helpers import make_folder
+    folder, _ = make_folder(tmp_path, tiny("B", num_hidden_layers=4, hidden_size=256, intermediate_size=1024), seed=5)
+    load = lambda: q.Engine.from_folder(folder, dtype="bfloat16", max_tokens=64, max_seq_len=64, weight_dtype=weight_dtype)  # noqa: E731
+    first = load()
+    torch.cuda.synchronize()
+    size = first.weights_arena.numel()
+    for _ in range(3):
+        memory = torch.empty(size, dtype=torch.uint8, device="cuda")
+        torch.cuda._sleep(200_000_000)                     # 0.1 s
+        memory.fill_(255)
+        del memory
+        engine = load()
+        torch.cuda.synchronize()
+        for (name, a), (_, b) in zip(parameters(first.model), parameters(engine.model)):
+            assert torch.equal(a, b), name
+        del engine
+
+
+def parameters(model):
+    out = [("embedding", model.embedding.table), ("head", model.head.weight), ("norm", model.final_norm.weight)]
+    for i, w in enumerate(matrices(model)):
+        out += [(f"{i} codes", w.codes), (f"{i} scales", w.scales)] if hasattr(w, "codes") else [(str(i), w)]
+    return out
