@@ -110,6 +110,8 @@ def main(argv: Optional[List[str]] = None) -> int:
 
     config = q.load_config(args.config if args.random_weights is not None else model_dir)
     plan = config.plan()                 # sizes and stop tokens as every architecture states them
+    if args.weight_dtype is not None and not q.build_model(plan).takes_eight_bit():
+        ap.error(f"--weight-dtype {args.weight_dtype} is not to be had with this model: its layers are no pre-norm blocks of attention and a gated feed-forward")
     max_context = args.max_context if args.max_context is not None else min(4096, plan.max_positions)
     if not 0 < max_context <= plan.max_positions:
         ap.error(f"--max-context must be in 1..{plan.max_positions} (the model's longest sequence)")
