@@ -133,6 +133,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     n_live = max(1, len(prompts))
 
     def make_engine():
+        import torch
+        torch.cuda.set_device(args.gpu)            # kernels are launched on the current device
         if args.random_weights is not None:
             return q.Engine.from_random(config, args.random_weights, dtype=args.dtype, max_tokens=n_live * max_context,
                                         max_seq_len=max_context, device=device, weight_dtype=args.weight_dtype)

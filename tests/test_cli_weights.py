@@ -22,6 +22,15 @@ def made(*args, **kwargs):
     raise Made(kwargs)
 
 
+@pytest.fixture(autouse=True)
+def current(monkeypatch):
+    """The devices that were made the current one."""
+    import torch
+    seen = []
+    monkeypatch.setattr(torch.cuda, "set_device", seen.append)
+    return seen
+
+
 def test_a_model_that_takes_no_8_bit_weights_is_a_usage_error(tmp_path, monkeypatch, capsys):
     from dozazen_cases import case
     monkeypatch.setattr(q.Engine, "from_random", made)
@@ -34,3 +43,12 @@ def test_a_model_that_takes_no_8_bit_weights_is_a_usage_error(tmp_path, monkeypa
     with pytest.raises(Made) as asked:
         chat.main(args + [config_file(tmp_path, tiny("A")), "--weight-dtype", "int8"])
     assert asked.value.args[0]["weight_dtype"] == "int8"
+
+
+@pytest.mark.parametrize("gpu", [0, 1, 3])
+def test_the_device_asked_for_is_the_current_one_when_the_engine_is_made(tmp_path, monkeypatch, current, gpu):
+    """Kernels go to the current device's streams, wherever the tensors lie."""
+    monkeypatch.setattr(q.Engine, "from_random", lambda *args, **kwargs: made(current=list(current), **kwargs))
+    with pytest.raises(Made) as asked:
+        chat.main(["--random-weights", "1", "--tokens", "1,2", "--max-context", "64", "--gpu", str(gpu), "--config", config_file(tmp_path, tiny("A"))])
+    assert asked.value.args[0]["current"] == [gpu] and asked.value.args[0]["device"] == f"cuda:{gpu}"
