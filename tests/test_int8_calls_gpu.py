@@ -99,3 +99,41 @@ def test_tensors_of_rows_stay_those_they_were_made_with():
     assert torch.equal(a.float(), before)
     a.scales.mul_(2)                                       # (values in place are felt)
     assert torch.equal(a.float(), 2 * before)
+
+
+@pytest.mark.parametrize("width,apart", [(8192, True), (8191, False)])
+def test_scales_and_sums_beyond_32_bit_offsets(width, apart):
+    """2.2 billion values of x, delta and total: three runs of rows, of their own values each, against 64 bits: codes, scales (rounded once; under the norm as in the
+    tests of widths, 2^-18) and sums; and the rows between them, which are zeros."""
+    import int8_cases as ic
+    from qwen3_b200.csrc import ops
+    rows, runs = 270000, (0, 135000, 269000)
+    x, d = (torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    for i, first in enumerate(runs):
+        x[first:first + 1000] = (drawn(1000, width, 3 + i) * (1 + i)).to(torch.bfloat16)
+        d[first:first + 1000] = (drawn(1000, width, 33 + i) * 0.5).to(torch.bfloat16)
+    w, out = 0.5 + drawn(1, width, 9)[0].abs(), ops.Int8Rows.empty(rows, width, "cuda")
+    out.codes.fill_(77), out.scales.fill_(77.0)
+    ops.quantize_rows(x, out)
+    for first in runs:
+        part = slice(first, first + 1000)
+        codes, scales = ic.quantised(x[part])
+        assert torch.equal(out.codes[part].long(), codes)
+        assert bool(((out.scales[part].double() - scales).abs() <= 2.0 ** -24 * scales).all())
+        assert bool((out.scales[first + 1000:first + 1010] == 0).all()) and not bool(out.codes[first + 1000:first + 1010].any())
+    stored = [(x[f:f + 1000].float() + d[f:f + 1000].float()).to(torch.bfloat16) for f in runs]
+    before = [x[f:f + 1000].clone() for f in runs]
+    total = torch.full_like(x, 77.0) if apart else x
+    out.codes.fill_(77), out.scales.fill_(77.0)
+    ops.rms_norm_int8(x, w, 1e-6, out, delta=d, **({"total": total} if apart else {}))
+    for first, sums, old in zip(runs, stored, before):
+        part = slice(first, first + 1000)
+        assert not torch.equal(sums, old) and torch.equal(total[part], sums) and (not apart or torch.equal(x[part], old))
+        u = ic.normed(sums, w)
+        codes, tops = ic.quantised(u)
+        scales = tops / (sums.double().square().mean(-1) + 1e-6).sqrt()
+        assert torch.equal(out.codes[part].long(), codes)
+        assert bool(((out.scales[part].double() - scales).abs() <= 2.0 ** -18 * scales).all())
+        assert bool((out.scales[first + 1000:first + 1010] == 0).all()) and not bool(total[first + 1000:first + 1010].any())
+    del x, d, total, out
+    torch.cuda.empty_cache()
