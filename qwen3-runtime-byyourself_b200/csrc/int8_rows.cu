@@ -89,14 +89,16 @@ template <int N> __device__ __forceinline__ void codes_of_bf16(const float (&u)[
 
 // `n` codes (of N) to a place that is a multiple of N bytes from the row's beginning.
 template <int N, bool WHOLE> __device__ __forceinline__ void store_codes(int8_t* to, const uint32_t (&w)[N / 4], int n) {
-    if (WHOLE || n >= N) {
-        if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(to) = w[0];
-        return;
-    }
+    if constexpr (!WHOLE) {
+        if (n < N) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i < n) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+            for (int i = 0; i < N; ++i)
+                if (i < n) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+            return;
+        }
+    }
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(to) = w[0];
 }
 
 template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[Pack<T>::N]) {
