@@ -54,9 +54,12 @@ static inline cudaError_t q3_allow_shared_memory(Kernel kernel, int bytes, Q3Per
 // attribute, a kernel may start while its predecessor drains: it does what needs no input
 // of the predecessor (address arithmetic, fetching weights) and then waits in `pdl_wait()`,
 // which returns once the predecessor has completed and its writes are visible.  Rules that
-// every kernel here keeps: `pdl_launch_dependents()` first thing, and no read of an
-// activation and no write to global memory before `pdl_wait()`.  Without the attribute
-// both calls do nothing.
+// every kernel here keeps: no read of an activation and no write to global memory before
+// `pdl_wait()` (nor, for operands in 8 bits, of weights, which may have been quantised one launch
+// before), and `pdl_launch_dependents()` first thing - but for the kernels of 8-bit rows, which
+// call it after their own wait, and the few-token product in 8 bits, after its loads: the next kernel
+// would otherwise take their place while the one before them runs (ops.PDL_SOURCES has the times).
+// Without the attribute both calls do nothing.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

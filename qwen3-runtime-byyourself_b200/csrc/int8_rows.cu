@@ -14,13 +14,17 @@
 // squares of small values lose: rows whose mean square is below that are finished by a kernel of their own.
 //
 // Bound by memory: a row is read once, in packets of 16 bytes, held in registers across the reduction, and written (8,000 rows, of the measured copy
-// rate: quantise 12,288 bfloat16 47.2 us, 0.95; 10,240 of 5,120 float32 42.5, 0.94; norm and sum 5,120 bfloat16 50.9, 0.86; in long runs, at the clocks that
+// rate: quantise 12,288 bfloat16 47.1 us, 0.95; 10,240 of 5,120 float32 42.5, 0.94; norm and sum 5,120 bfloat16 51, 0.86; in long runs, at the clocks that
 // they settle at, 50.0, 48.2 and 56.1).  What a value
 // costs in instructions comes next (seven in ten issue slots were taken where these times were 55 and 57): three-way maxima of packed halves, no
-// fallbacks compiled into rows that need none, one rounding less and the scale's divisions in one thread took 10 and 6 %.  Rows that do not begin at a packet's boundary (an odd width, a
-// slice) are read in the packets around them, each thread shifting two into its own values: 5,001 bfloat16 24.3 and 77 us where 5,120 takes 20.8
-// and 50.9.  Tried and slower: rows brought several ahead by bulk copies into a ring in shared memory of blocks that stay (norm 5,120 126 us: barriers and
-// a second pass over shared memory a row), 40 registers a thread for a third block (61.7), loads that are evicted first (1 to 2 %).
+// fallbacks compiled into rows that need none, one rounding less and the scale's divisions in one thread took 10 and 6 %.  Blocks of up to 512 threads are bound to 64
+// registers a thread, so that two fit an SM whatever their size; the variants that hold most (four packets of a norm, eight of float32 rows) spill 32 to 168 bytes a
+// thread there, among them those that run the norm and the float32 rows above, in blocks of 160 threads; what they would take with more registers was not measured.
+// Rows that do not begin at a packet's boundary (an odd width, a
+// slice) are read in the packets around them, each thread shifting two into its own values: 5,001 bfloat16 24.4 and 76 us where 5,120 takes 20.8
+// and 51.  Rows wider than 1,024 threads hold (32,768) are read twice, value by value: 400 of 70,001 bfloat16 45 us quantised and 135 normed, 3.5 and 4.5 times
+// what their bytes take (no model here has them).  Tried and slower: rows brought several ahead by bulk copies into a ring in shared memory of blocks that stay (norm 5,120
+// 126 us: barriers and a second pass over shared memory a row), 40 registers a thread for a third block (61.7), loads that are evicted first (1 to 2 %).
 #include "common.cuh"
 #include "../include/qwen3/int8_args.h"
 
