@@ -137,3 +137,84 @@ def test_scales_and_sums_beyond_32_bit_offsets(width, apart):
         assert bool((out.scales[first + 1000:first + 1010] == 0).all()) and not bool(total[first + 1000:first + 1010].any())
     del x, d, total, out
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,width", [(3, 4096), (700, 65), (20, 40000)])
+def test_norm_of_small_rows_on_another_stream_and_in_graphs(rows, width):
+    """Two launches: the second reads what the first has noted, also from a graph, and where a product follows."""
+    from qwen3_b200.csrc import ops
+    x = drawn(rows, width, 5).mul_(1e-30)
+    x[::2] *= 1e30
+    w, matrix = 1 + 0.3 * drawn(1, width, 7)[0], ops.quantize_rows(drawn(48, width, 6), ops.Int8Rows.empty(48, width, "cuda"))
+    want = ops.rms_norm_int8(x.clone(), w, 0.0, ops.Int8Rows.empty(rows, width, "cuda"))
+    torch.cuda.synchronize()
+    product = ops.gemm_int8(want, matrix, torch.zeros(rows, 48, device="cuda"))
+    assert bool(product.isfinite().all()) and bool((want.scales > 0).all())
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        out = ops.rms_norm_int8(x, w, 0.0, ops.Int8Rows.empty(rows, width, "cuda"))
+        y = ops.gemm_int8(out, matrix, torch.zeros(rows, 48, device="cuda"))
+    side.synchronize()
+    assert torch.equal(out.codes, want.codes) and torch.equal(out.scales, want.scales) and torch.equal(y, product)
+    graph, out, y = torch.cuda.CUDAGraph(), ops.Int8Rows.empty(rows, width, "cuda"), torch.zeros(rows, 48, device="cuda")
+    with torch.cuda.graph(graph):
+        ops.rms_norm_int8(x, w, 0.0, out)
+        ops.gemm_int8(out, matrix, y)
+    for _ in range(3):
+        out.scales.fill_(77.0), y.fill_(77.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.scales, want.scales) and torch.equal(y, product)
+
+
+def test_graphs_replayed_at_once_and_threads():
+    """Products on the same weights from graphs on two streams at once, and from two threads, each with outputs of its own."""
+    import threading
+    from qwen3_b200.csrc import ops
+    w = ops.quantize_rows(drawn(2048, 1000, 1), ops.Int8Rows.empty(2048, 1000, "cuda"))
+    tokens = [ops.quantize_rows(drawn(M, 1000, M), ops.Int8Rows.empty(M, 1000, "cuda")) for M in (4, 60, 200, 700)]
+    want = [ops.gemm_int8(x, w, torch.zeros(x.rows, 2048, device="cuda")) for x in tokens]
+    torch.cuda.synchronize()
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for _ in streams:
+        graph, ys = torch.cuda.CUDAGraph(), [torch.zeros_like(y) for y in want]
+        with torch.cuda.graph(graph):
+            for x, y in zip(tokens, ys):
+                ops.gemm_int8(x, w, y)
+        graphs.append(graph), outs.append(ys)
+    for _ in range(10):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, z) for ys in outs for y, z in zip(ys, want))
+    failed = []
+
+    def work(stream):
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                ys = [ops.gemm_int8(x, w, torch.empty(x.rows, 2048, device="cuda")) for x in tokens]
+                stream.synchronize()
+                if not all(torch.equal(y, z) for y, z in zip(ys, want)):
+                    failed.append(stream)
+    threads = [threading.Thread(target=work, args=(s,)) for s in streams]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and ops.tcgen05_status("cuda") == 0
+
+
+@pytest.mark.parametrize("form", ["few", "mid", "pair"])
+@pytest.mark.parametrize("rows,width", [(37, 100), (300, 1000)])
+def test_rows_multiplied_with_themselves_and_slices_of_rows(rows, width, form):
+    from qwen3_b200.csrc import ops
+    x = ops.quantize_rows(drawn(rows, width, 2), ops.Int8Rows.empty(rows, width, "cuda"))
+    y = ops.gemm_int8(x, x, torch.zeros(rows, rows, device="cuda"), form=form)
+    want = (x.codes.double() @ x.codes.double().t() * x.scales.double()[:, None] * x.scales.double())
+    assert bool(((y.double() - want).abs() <= 3.01 * 2.0 ** -24 * want.abs()).all())
+    a, b = (ops.Int8Rows(x.codes[s], x.scales[s].contiguous()) for s in (slice(3, 20), slice(1, None, 2)))
+    assert b.stride == 2 * x.stride
+    part = ops.gemm_int8(a, b, torch.zeros(a.rows, b.rows, device="cuda"), form=form)
+    assert torch.equal(part, y[3:20, 1::2])
