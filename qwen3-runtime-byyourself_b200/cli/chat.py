@@ -79,7 +79,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default=None,
                     help="Compute type. Default: the checkpoint's torch_dtype")
     ap.add_argument("--weight-dtype", choices=["int8"], default=None,
-                    help="Keep the layers' projections as 8-bit integers with a scale for each channel. Default: the compute type")
+                    help="Keep the layers' projections as 8-bit integers with a scale for each channel (Qwen3 models). Default: the compute type")
     ap.add_argument("--config", metavar="PATH", help="config.json for --random-weights.")
     ap.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                     help="Run the configuration of --config with seeded random weights instead of a checkpoint.")
