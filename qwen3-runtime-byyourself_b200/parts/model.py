@@ -95,7 +95,7 @@ class Model:
             self.check_eight_bit()
         if isinstance(weights, dict) and not isinstance(weights, TensorDict):
             weights = self.source_of(weights, dtype, device, eight_bit)
-        if eight_bit and not self.eight_bit_names() <= set(weights.apart):
+        if eight_bit and not self.eight_bit_names() <= set(getattr(weights, "apart", ())):
             raise ValueError("weights in 8 bits: the source was made without them (`source_of(..., eight_bit=True)`, `open_upload(..., apart=model.eight_bit_names())`), "
                              "so that matrices would be rounded before they are quantised")
         p = self.plan

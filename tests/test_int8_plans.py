@@ -42,3 +42,12 @@ def test_plans_can_be_launched(rows, channels, width):
         assert -(-rows // 256) <= 65535 and 1 <= splits <= 8
     elif form == "pair":
         assert splits % 32 == 0 and 32 <= splits <= 256 and -(-rows // splits) * -(-channels // 256) <= 0x3FFFFFFF
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,channels,width,form", [(1, 4096, 4096, "few"), (8, 4096, 12288, "few"), (8, 24576, 4096, "few"), (64, 6144, 4096, "mid"),
+                                                      (1024, 4096, 4096, "pair"), (2048, 24576, 4096, "pair"), (8000, 4096, 12288, "pair")])
+def test_forms_of_sizes_where_the_others_are_far_behind(rows, channels, width, form):
+    """A token alone streams W; some dozen share it in tensor memory, K split over a cluster; a thousand and more fill the pairs of SMs."""
+    from qwen3_b200.csrc import ops
+    assert ops.int8_plan(rows, channels, width)[0] == form

@@ -86,7 +86,7 @@ def test_sources_that_round_before_they_are_quantised():
     import torch
     model = q.build_model(q.config_from_dict(tiny("A")).plan())
     tensors = q.random_weights(model.weight_specs(), 1, dtype=torch.float32)
-    for source in (types.SimpleNamespace(apart=set()), types.SimpleNamespace(apart=set(list(model.eight_bit_names())[1:])),
+    for source in (types.SimpleNamespace(), types.SimpleNamespace(apart=set()), types.SimpleNamespace(apart=set(list(model.eight_bit_names())[1:])),
                    model.source_of(tensors, torch.bfloat16, "cpu")):
         with pytest.raises(ValueError, match="rounded"):
             model.bind(source, torch.bfloat16, "cpu", eight_bit=True)
